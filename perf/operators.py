@@ -181,7 +181,7 @@ def _prepare_prompt(case, g, dtype):
          "longest": max(lengths)}
     if own:
         s["ctx"] = _context()
-        s["plan"] = s["ctx"].prompt_plan(lengths, causal=case["causal"])
+        s["plan"] = s["ctx"].prompt_plan(lengths, h, kv, causal=case["causal"])
     return s
 
 
@@ -205,7 +205,7 @@ def _prepare_step(case, g, dtype):
         cache.extend(seqs, lengths)
         plan = cache.plan(seqs, lengths)
         cache.write_async(plan, s["k_own"], s["v_own"])
-        s["cache"], s["plan"] = cache, cache.plan(seqs, [new] * n)
+        s["cache"], s["plan"] = cache, cache.plan(seqs, [new] * n, heads=h)
     return s
 
 
