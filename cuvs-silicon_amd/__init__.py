@@ -137,6 +137,42 @@ _SIGNATURES["cvs_cagra_replay_gathers"] = (c_int, [c_void_p, c_void_p, c_void_p,
                                                    c_int, POINTER(c_double)])
 _SIGNATURES["cvs_context_bf_escalations"] = (c_int, [c_void_p, POINTER(c_uint64), POINTER(c_uint64), c_int])
 
+
+
+class Heads(ctypes.Structure):
+    """cvs_heads (include/cvs_hip.h)."""
+    _fields_ = [("data", c_void_p), ("tokens", c_int64), ("token_stride", c_int64), ("head_stride", c_int64),
+                ("heads", c_int), ("head_dim", c_int), ("type", c_int)]
+
+
+FP16, BF16 = 0, 1
+ATTN_MAX_DIM = 128
+
+_HEADS = POINTER(Heads)
+_SIGNATURES["cvs_context_create_on_stream"] = (c_int, [c_int, c_void_p, POINTER(c_void_p)])
+_SIGNATURES["cvs_prompt_plan_create"] = (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int,
+                                                 POINTER(c_void_p)])
+_SIGNATURES["cvs_prompt_plan_destroy"] = (c_int, [c_void_p])
+_SIGNATURES["cvs_prompt_attention_async"] = (c_int, [c_void_p, c_void_p, _HEADS, _HEADS, _HEADS, _HEADS, c_void_p,
+                                                     c_float])
+_SIGNATURES["cvs_kv_cache_create"] = (c_int, [c_void_p, c_int, c_int64, c_int, c_int, c_int, c_int,
+                                              POINTER(c_void_p)])
+_SIGNATURES["cvs_kv_cache_destroy"] = (c_int, [c_void_p])
+_SIGNATURES["cvs_kv_cache_pages"] = (c_int, [c_void_p, POINTER(c_int64), POINTER(c_int64)])
+_SIGNATURES["cvs_kv_sequence_create"] = (c_int, [c_void_p, c_int64, c_void_p])
+_SIGNATURES["cvs_kv_sequence_fork"] = (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p])
+_SIGNATURES["cvs_kv_sequence_extend"] = (c_int, [c_void_p, c_void_p, c_void_p, c_int64])
+_SIGNATURES["cvs_kv_sequence_truncate"] = (c_int, [c_void_p, c_int64, c_int64])
+_SIGNATURES["cvs_kv_sequence_free"] = (c_int, [c_void_p, c_void_p, c_int64])
+_SIGNATURES["cvs_kv_sequence_pages"] = (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+                                                POINTER(c_int64)])
+_SIGNATURES["cvs_kv_cache_compact"] = (c_int, [c_void_p, POINTER(c_int64)])
+_SIGNATURES["cvs_kv_plan_create"] = (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, POINTER(c_void_p)])
+_SIGNATURES["cvs_kv_plan_destroy"] = (c_int, [c_void_p])
+_SIGNATURES["cvs_kv_write_async"] = (c_int, [c_void_p, c_void_p, c_int, c_int, _HEADS, c_int64, _HEADS, c_int64])
+_SIGNATURES["cvs_kv_read_async"] = (c_int, [c_void_p, c_void_p, c_int, c_int, _HEADS, c_int64, _HEADS, c_int64])
+_SIGNATURES["cvs_kv_attention_async"] = (c_int, [c_void_p, c_void_p, c_int, _HEADS, _HEADS, c_void_p, c_float])
+
 # The bucketing permutation seed of the reference (src/metal_context.mm:803).
 DEFAULT_BUILD_SEED = 0xFEDCBA9876543210
 
@@ -262,16 +298,81 @@ class DeviceArray:
             pass
 
 
-class Context:
-    """One device + one HIP stream (C: cvs_context)."""
+# Element types of attention operands by the name of their dtype (numpy's and
+# torch's); numpy has no bfloat16, so a DeviceArray of uint16 holds those.
+_HEAD_TYPES = {"float16": FP16, "torch.float16": FP16, "fp16": FP16, "half": FP16, "uint16": BF16, "bf16": BF16,
+               "bfloat16": BF16, "torch.bfloat16": BF16}
 
-    def __init__(self, device: int = 0):
+
+def _head_type(dtype) -> int:
+    t = _HEAD_TYPES.get(str(dtype))
+    if t is None:
+        raise ValueError(f"type {dtype}: attention takes float16 or bfloat16")
+    return t
+
+
+def _heads(ctx: "Context", x, what: str, layered: bool = False):
+    """The cvs_heads view of a (tokens, heads, head_dim) device array, a
+    DeviceArray or a torch tensor on the context's device, whose last axis is
+    contiguous; with layered, of (layers, tokens, heads, head_dim) as well.
+    Returns (view, layers, layer stride)."""
+    shape = x.shape
+    nd = len(shape)
+    if nd != 3 and not (layered and nd == 4):
+        raise ValueError(f"{what} must be (tokens, heads, head_dim)" + (" or (layers, ...)" if layered else ""))
+    if isinstance(x, DeviceArray):
+        ptr, stride = x.ptr.value, (shape[-2] * shape[-1], shape[-1])
+        layer = shape[-3] * stride[0] if nd == 4 else 0
+    elif hasattr(x, "data_ptr"):
+        if not x.is_cuda or x.device.index != ctx.device:
+            raise ValueError(f"{what} must be on the context's device")
+        st = x.stride()
+        if st[-1] != 1 and shape[-1] > 1:
+            raise ValueError(f"{what}: the last axis must be contiguous")
+        ptr, stride, layer = x.data_ptr(), st[-3:-1], st[0] if nd == 4 else 0
+    else:
+        raise ValueError(f"{what} must be a DeviceArray or a torch tensor")
+    view = Heads(ptr, shape[-3], stride[0], stride[1], shape[-2], shape[-1], _head_type(x.dtype))
+    return view, (shape[0] if nd == 4 else 1), layer
+
+
+def _lse(ctx: "Context", lse, heads: int, tokens: int):
+    """Device address of a (heads, tokens) float32 array, or None."""
+    if lse is None:
+        return None
+    if tuple(lse.shape) != (heads, tokens) or str(lse.dtype) not in ("float32", "torch.float32"):
+        raise ValueError(f"lse must be a float32 device array of shape {(heads, tokens)}")
+    if isinstance(lse, DeviceArray):
+        return lse.ptr
+    if not lse.is_cuda or lse.device.index != ctx.device or not lse.is_contiguous():
+        raise ValueError("lse must be contiguous and on the context's device")
+    return lse.data_ptr()
+
+
+def _i64(a, n=None):
+    """A list of whole numbers as a C array."""
+    if n is not None and len(a) != n:
+        raise ValueError(f"{n} values are needed, {len(a)} given")
+    return (c_int64 * len(a))(*a)
+
+
+class Context:
+    """One device + one HIP stream (C: cvs_context).  stream: None for a
+    stream of its own, or the address of a HIP stream of the caller's (a torch
+    stream's cuda_stream) that the context works on, in order with the
+    caller's own work there."""
+
+    def __init__(self, device: int = 0, stream: int = None):
         h = c_void_p()
-        _check(load().cvs_context_create(int(device), byref(h)))
+        if stream is None:
+            _check(load().cvs_context_create(int(device), byref(h)))
+        else:
+            _check(load().cvs_context_create_on_stream(int(device), c_void_p(int(stream)), byref(h)))
         self.handle = h
-        # Datasets and graph indexes made on this context: the C library
-        # refuses to destroy a context that still owns any, so close() closes
-        # the live ones first.
+        self.device = int(device)
+        # What was made on this context (datasets, graph indexes, caches,
+        # prompt plans): the C library refuses to destroy a context that still
+        # owns any, so close() closes the live ones first.
         self._children = weakref.WeakSet()
 
     def _adopt(self, child) -> None:
@@ -354,6 +455,22 @@ class Context:
 
     def dataset(self, rows) -> "Dataset":
         return Dataset(self, rows)
+
+    def prompt_plan(self, q_lengths, heads: int, kv_heads: int, k_lengths=None, causal: bool = True) -> "PromptPlan":
+        return PromptPlan(self, q_lengths, heads, kv_heads, k_lengths, causal)
+
+    def prompt_attention_async(self, plan: "PromptPlan", q, k, v, out, lse=None, scale: float = 0.0) -> None:
+        """Attention over packed sequences (C: cvs_prompt_attention_async):
+        q, out (query tokens, heads, head_dim), k, v (key tokens, kv_heads,
+        head_dim); lse, when given, (heads, query tokens) float32; scale 0:
+        1 / sqrt(head_dim)."""
+        hq, hk, hv, ho = (_heads(self, x, w)[0] for x, w in ((q, "q"), (k, "k"), (v, "v"), (out, "out")))
+        _check(load().cvs_prompt_attention_async(self.handle, plan.handle, hq, hk, hv, ho,
+                                                 _lse(self, lse, hq.heads, hq.tokens), scale))
+
+    def kv_cache(self, layers: int, pages: int, page_tokens: int, kv_heads: int, head_dim: int,
+                 dtype="bf16") -> "KvCache":
+        return KvCache(self, layers, pages, page_tokens, kv_heads, head_dim, dtype)
 
     def cagra_index(self, rows, graph, seeds=None, traversal_bits: int = 32) -> "CagraIndex":
         return CagraIndex(self, rows, graph, seeds, traversal_bits)
@@ -669,6 +786,173 @@ class CagraIndex:
         _check(load().cvs_cagra_search_async(self.ctx.handle, self.handle, queries.ptr, queries.shape[0], int(k),
                                              int(itopk_size), int(search_width), int(max_iterations), nbr.ptr,
                                              dist.ptr, stats.ptr if stats is not None else None))
+
+
+class PromptPlan:
+    """How a batch of packed sequences is worked on, for every layer of a
+    model (C: cvs_prompt_plan)."""
+
+    def __init__(self, ctx: Context, q_lengths, heads: int, kv_heads: int, k_lengths=None, causal: bool = True):
+        self.ctx = ctx
+        self.handle = None
+        n = len(q_lengths)
+        h = c_void_p()
+        _check(load().cvs_prompt_plan_create(ctx.handle, _i64(q_lengths),
+                                             None if k_lengths is None else _i64(k_lengths, n), n, int(heads),
+                                             int(kv_heads), 1 if causal else 0, byref(h)))
+        self.handle = h
+        ctx._adopt(self)
+
+    def close(self) -> None:
+        # A plan dies with its context (Context.close closes it first).
+        if self.handle is not None and self.ctx.handle is not None:
+            _check(load().cvs_prompt_plan_destroy(self.handle))
+        self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class KvCache:
+    """Paged cache of attention keys and values whose sequences share pages
+    (C: cvs_kv_cache).  Sequences are ids; plans name the newest tokens of
+    some of them."""
+
+    def __init__(self, ctx: Context, layers: int, pages: int, page_tokens: int, kv_heads: int, head_dim: int,
+                 dtype="bf16"):
+        self.ctx = ctx
+        self.handle = None
+        h = c_void_p()
+        _check(load().cvs_kv_cache_create(ctx.handle, int(layers), int(pages), int(page_tokens), int(kv_heads),
+                                          int(head_dim), _head_type(dtype), byref(h)))
+        self.handle = h
+        self.layers, self.kv_heads, self.head_dim = int(layers), int(kv_heads), int(head_dim)
+        self.page_tokens = int(page_tokens)
+        self._plans = weakref.WeakSet()
+        ctx._adopt(self)
+
+    def close(self) -> None:
+        # A cache dies with its context (Context.close closes it first), its plans with it.
+        if self.handle is not None and self.ctx.handle is not None:
+            for plan in list(self._plans):
+                plan.close()
+            _check(load().cvs_kv_cache_destroy(self.handle))
+        self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def free_pages(self) -> int:
+        free = c_int64(0)
+        _check(load().cvs_kv_cache_pages(self.handle, None, byref(free)))
+        return free.value
+
+    def sequences(self, n: int) -> list:
+        """n new sequences without tokens."""
+        ids = (c_int64 * n)()
+        _check(load().cvs_kv_sequence_create(self.handle, n, ids))
+        return list(ids)
+
+    def sequence(self) -> int:
+        return self.sequences(1)[0]
+
+    def fork(self, parent: int, n: int, length: int = -1) -> list:
+        """n new sequences of the parent's first `length` tokens (-1: all), on
+        its pages."""
+        ids = (c_int64 * n)()
+        _check(load().cvs_kv_sequence_fork(self.handle, int(parent), int(length), n, ids))
+        return list(ids)
+
+    def extend(self, seqs, tokens) -> None:
+        """Room for tokens[i] more tokens in seqs[i]; RuntimeError and no change
+        when the free pages do not suffice."""
+        n = len(seqs)
+        _check(load().cvs_kv_sequence_extend(self.handle, _i64(seqs), _i64(tokens, n), n))
+
+    def truncate(self, seq: int, length: int) -> None:
+        _check(load().cvs_kv_sequence_truncate(self.handle, int(seq), int(length)))
+
+    def free(self, seqs) -> None:
+        _check(load().cvs_kv_sequence_free(self.handle, _i64(seqs), len(seqs)))
+
+    def lengths(self, seqs) -> list:
+        out = (c_int64 * len(seqs))()
+        _check(load().cvs_kv_sequence_pages(self.handle, _i64(seqs), len(seqs), out, None, 0, None))
+        return list(out)
+
+    def pages(self, seqs) -> np.ndarray:
+        """The sequences' page ids, one list behind another."""
+        ids, n, count = _i64(seqs), len(seqs), c_int64(0)
+        _check(load().cvs_kv_sequence_pages(self.handle, ids, n, None, None, 0, byref(count)))
+        out = np.empty(count.value, np.uint32)
+        _check(load().cvs_kv_sequence_pages(self.handle, ids, n, None, out.ctypes.data, count.value, None))
+        return out
+
+    def compact(self) -> int:
+        """Moves the live pages to the front; returns their number."""
+        live = c_int64(0)
+        _check(load().cvs_kv_cache_compact(self.handle, byref(live)))
+        return live.value
+
+    def plan(self, seqs, tokens, heads: int = 0) -> "KvPlan":
+        """The newest tokens[i] tokens of seqs[i] as rows to write, read and,
+        with a number of query heads, query."""
+        return KvPlan(self, seqs, tokens, heads)
+
+    def _move(self, call, plan, k, v, layer: int) -> None:
+        (hk, nk, lk), (hv, nv, lv) = _heads(self.ctx, k, "k", True), _heads(self.ctx, v, "v", True)
+        if nk != nv:
+            raise ValueError("k and v must have the same layers")
+        if nk:
+            _check(call(self.handle, plan.handle, layer, nk, hk, lk, hv, lv))
+
+    def write_async(self, plan: "KvPlan", k, v, layer: int = 0) -> None:
+        """Writes the plan's tokens: k, v (tokens, kv_heads, head_dim) of one
+        layer, or (layers, tokens, kv_heads, head_dim) of `layer` and on."""
+        self._move(load().cvs_kv_write_async, plan, k, v, layer)
+
+    def read_async(self, plan: "KvPlan", k, v, layer: int = 0) -> None:
+        """Reads the plan's tokens into k, v (shapes as write_async)."""
+        self._move(load().cvs_kv_read_async, plan, k, v, layer)
+
+    def attention_async(self, plan: "KvPlan", q, out, layer: int = 0, lse=None, scale: float = 0.0) -> None:
+        """Attention of the plan's tokens over a layer (C:
+        cvs_kv_attention_async): q, out (tokens, heads, head_dim); lse, when
+        given, (heads, tokens) float32; scale 0: 1 / sqrt(head_dim)."""
+        hq, ho = _heads(self.ctx, q, "q")[0], _heads(self.ctx, out, "out")[0]
+        _check(load().cvs_kv_attention_async(self.handle, plan.handle, layer, hq, ho,
+                                             _lse(self.ctx, lse, hq.heads, hq.tokens), scale))
+
+
+class KvPlan:
+    """The newest tokens of some sequences of a cache (C: cvs_kv_plan)."""
+
+    def __init__(self, cache: KvCache, seqs, tokens, heads: int = 0):
+        self.cache = cache
+        self.handle = None
+        n = len(seqs)
+        h = c_void_p()
+        _check(load().cvs_kv_plan_create(cache.handle, _i64(seqs), _i64(tokens, n), n, int(heads), byref(h)))
+        self.handle = h
+        cache._plans.add(self)
+
+    def close(self) -> None:
+        # A plan dies with its cache (KvCache.close closes it first).
+        if self.handle is not None and self.cache.handle is not None and self.cache.ctx.handle is not None:
+            _check(load().cvs_kv_plan_destroy(self.handle))
+        self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 # ---- synthetic data (lib/libcvs_synth.so) ---------------------------------

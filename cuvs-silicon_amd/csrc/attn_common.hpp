@@ -1,0 +1,267 @@
+// Definitions shared by the attention kernels (attn_prompt.hip, attn_cached.hip)
+// and the paged cache (kv_cache.hip).
+//
+// All attention kernels compute, for a tile of 32 query rows a wave and 32
+// keys, S^T = K Q^T and O^T += V^T P^T with v_mfma_f32_32x32x16.  A query row
+// is a column of both accumulators, so everything that belongs to a row (its
+// maximum, its sum, its rescaling) is a per-lane value shared by lanes l and
+// l + 32, and the probabilities that leave the first product are the B operand
+// of the second without moving between lanes: accumulator register r of lane l
+// is key 8 (r / 4) + 4 (l / 32) + r % 4 of column l % 32, and the eight
+// consecutive registers 8 s .. 8 s + 7 are the lane's B operand of the s-th 16
+// keys when the A operand (V^T) orders its keys the same way.
+#pragma once
+
+#include <cmath>
+#include <cstdint>
+#include <memory>
+#include <vector>
+
+#include "bf_common.hpp"
+#include "cvs_internal.hpp"
+#include "device_util.hpp"
+#include "kv_pages.hpp"
+
+namespace cvs {
+namespace attn {
+
+using bf::f32x16;
+using bf::lds_addr;
+using bf::lds_dma;
+using bf::make_rsrc;
+using bf::rsrc4;
+using bf::u32x4;
+
+constexpr int kMaxDim = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// One 16-byte MFMA operand: 8 elements of fp16 or bf16.
+template <bool kBf>
+__device__ CVS_INLINE f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (kBf) {
+    typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(bf::half8, a), __builtin_bit_cast(bf::half8, b),
+                                                  c, 0, 0, 0);
+  }
+}
+
+// Two floats rounded to nearest even, packed.
+template <bool kBf>
+__device__ CVS_INLINE uint32_t pack2(float a, float b) {
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  const f32x2_t f = {a, b};
+  if constexpr (kBf) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2));
+  } else {
+    typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, half2_t));
+  }
+}
+
+template <bool kBf>
+__device__ CVS_INLINE float to_float(uint16_t x) {
+  if constexpr (kBf) return __uint_as_float(uint32_t(x) << 16);
+  return float(__builtin_bit_cast(_Float16, x));
+}
+
+// Bits 15 and 31 set where the half-word is an infinity or NaN (all exponent
+// bits set: adding one unit of the exponent to the magnitude carries into
+// bit 15, and never past it).
+template <bool kBf>
+__device__ CVS_INLINE uint32_t nonfinite(uint32_t x) {
+  return ((x & 0x7fff7fffu) + (kBf ? 0x00800080u : 0x04000400u)) & 0x80008000u;
+}
+
+// Zeroes the infinities and NaNs of an operand; `bad` collects whether there were any.
+template <bool kBf>
+__device__ CVS_INLINE u32x4 clean(u32x4 v, uint32_t& bad) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t f = nonfinite<kBf>(v[i]);
+    bad |= f;
+    v[i] &= ~((f >> 15) * 0xffffu);
+  }
+  return v;
+}
+
+// Running softmax of a lane's query row over the keys seen so far: m the
+// largest log2-scaled score, l this lane's share (its half of the keys) of
+// the sum of 2^(score - m), o the weighted values.  All in fp32.
+template <int NB>
+struct RowState {
+  f32x16 o[NB];
+  float m, l;
+  __device__ CVS_INLINE void init() {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) o[b] = f32x16{};
+    m = -INFINITY;
+    l = 0.f;
+  }
+};
+
+// The largest of a row's two lanes.
+__device__ CVS_INLINE float both_max(float x) { return fmaxf(x, xor_lanes_f(x, 32)); }
+__device__ CVS_INLINE float both_sum(float x) { return x + xor_lanes_f(x, 32); }
+
+// Scores of NT 32-key tiles -> probabilities 2^(c s - m), with the state
+// rescaled to the new maximum.  Masked scores come in as -inf and leave as 0.
+// While a row has seen nothing its maximum is -inf; 0 stands in for it then,
+// so that -inf - (-inf) does not arise.
+template <int NB, int NT>
+__device__ CVS_INLINE void softmax_step(f32x16 (&s)[NT], RowState<NB>& st, float c) {
+  float top = s[0][0];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
+  const float m = fmaxf(st.m, both_max(top) * c);
+  const float base = m == -INFINITY ? 0.f : m;
+  if (__ballot(m != st.m)) {
+    const float alpha = __builtin_amdgcn_exp2f(st.m - base);
+    st.l *= alpha;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st.o[b][r] *= alpha;
+    st.m = m;
+  }
+  float sum = 0.f;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], c, -base));
+      sum += s[t][r];
+    }
+  st.l += sum;
+}
+
+// B operand of the 16 keys `step` (0 or 1) of a probability tile.  The
+// probabilities are rounded to the values' type here, the product's operand
+// type: each is off by at most half a unit of its own last place, which the
+// sum over keys averages; the sum l keeps them unrounded.
+template <bool kBf>
+__device__ CVS_INLINE u32x4 prob_operand(const f32x16& p, int step) {
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = pack2<kBf>(p[8 * step + 2 * i], p[8 * step + 2 * i + 1]);
+  return r;
+}
+
+// Adds what `clean` took out of a tile's values for the rows that do see
+// them: 32 keys from `key0`, seen by a lane's row below `limit`.  value(j, d)
+// is element d of key key0 + j.  Only for tiles with infinities or NaNs in
+// keys that some row of the wave does not see: there 0 * inf in the matrix
+// product would reach rows the key is masked from.
+template <bool kBf, int NB, typename Value>
+__device__ CVS_INLINE void add_nonfinite(RowState<NB>& st, const f32x16& p, int key0, int limit, int dim,
+                                         const Value& value) {
+  const int half = __lane_id() >> 5;
+#pragma unroll 1
+  for (int j = 0; j < 32; ++j) {
+    const int reg = 4 * (j / 8) + j % 4;
+    float own = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) own = r == reg ? p[r] : own;
+    const float other = xor_lanes_f(own, 32);
+    const float pj = half == ((j >> 2) & 1) ? own : other;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int d = 32 * b + 8 * (r / 4) + 4 * half + r % 4;
+        const uint16_t x = d < dim ? value(j, d) : uint16_t(0);
+        if (nonfinite<kBf>(x) != 0 && key0 + j < limit) st.o[b][r] += pj * to_float<kBf>(x);
+      }
+  }
+}
+
+// Writes a lane's half of a row's 32 NB outputs, scaled.  Lanes l and l + 32
+// hold alternate groups of 4 elements; the pair exchanges them so that each
+// stores 16 bytes at a time.
+template <bool kBf, int NB>
+__device__ CVS_INLINE void store_row(const RowState<NB>& st, float scale, uint16_t* out, int dim, bool there) {
+  const int half = __lane_id() >> 5;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+      uint32_t w[2][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          w[i][k] = pack2<kBf>(st.o[b][4 * (j + i) + 2 * k] * scale, st.o[b][4 * (j + i) + 2 * k + 1] * scale);
+      // Upper lanes take their partner's group j + 1, lower lanes their partner's group j.
+      const auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+      const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+      const int d = 32 * b + 8 * (j + half);
+      if (there && d < dim) *reinterpret_cast<u32x4*>(out + d) = u32x4{x[0], y[0], x[1], y[1]};
+    }
+}
+
+// A heads view as the kernels take it: strides in elements.
+struct View {
+  char* p;
+  int64_t token, head;
+};
+
+// Checks a view's geometry; `what` names it in messages.
+void check_view(const cvs_heads* x, const char* what);
+inline View view_of(const cvs_heads* x) { return {static_cast<char*>(x->data), x->token_stride, x->head_stride}; }
+
+// The softmax scale in log2 units: 0 stands for 1 / sqrt(dim).
+float scale_log2(float scale, int dim);
+
+// Copies host bytes to device memory as arguments of kernels, kUploadBytes a
+// launch: the host buffer is free on return and nothing is pinned, staged or
+// waited for.
+constexpr size_t kUploadBytes = 3840;
+void upload(cvs_context* ctx, void* dst, const void* src, size_t bytes);
+
+}  // namespace attn
+}  // namespace cvs
+
+// A cache of key and value rows in pages, kv_cache.hip.
+struct cvs_kv_cache {
+  cvs_context* ctx = nullptr;
+  int layers = 0, kv_heads = 0, dim = 0, type = 0;
+  int nb = 0;                  // 32-element blocks of a padded row
+  int64_t head_bytes = 0;      // one head's keys (and, behind them, values) of a page: 2 * page_tokens * 64 nb
+  int64_t page_bytes = 0;      // kv_heads * head_bytes
+  int64_t layer_bytes = 0;     // pages * page_bytes
+  char* pool = nullptr;
+  std::unique_ptr<cvs::kv::PageBook> book;
+  int live_plans = 0;
+  std::vector<cvs::DeviceBuffer> blobs;  // device memory of destroyed plans, for the next ones
+};
+
+struct cvs_kv_plan {
+  cvs_kv_cache* cache = nullptr;
+  std::vector<int64_t> seqs;
+  std::vector<uint64_t> versions;
+  std::vector<int32_t> written;  // the pages that the plan's tokens lie in
+  int64_t tokens = 0;            // of all sequences
+  int heads = 0;                 // query heads; 0: for reading and writing alone
+  cvs::DeviceBuffer blob;
+  // Offsets into the blob, in bytes.
+  int spans = 0;       // of tokens, a page each (kv_cache.hip, Span)
+  size_t at_spans = 0;
+  int items = 0;       // of attention work (attn_cached.hip, Item)
+  int64_t slots = 0;   // rows of partial results a kv head; 0: every row has one part
+  size_t at_items = 0, at_pages = 0, at_limits = 0, at_rows = 0, at_leaves = 0, at_runs = 0;
+};
+
+namespace cvs {
+namespace attn {
+// The attention part of a plan's blob, appended to `blob`.
+void plan_attention(cvs_kv_plan* plan, const int64_t* lengths, const int64_t* tokens, std::vector<char>& blob);
+// The plan is the cache's and its sequences are as they were when it was made.
+void check_plan(const cvs_kv_plan* plan);
+}  // namespace attn
+}  // namespace cvs

@@ -82,6 +82,7 @@ struct cvs_context {
   // of them uses the context's stream and device at its own destruction.
   int live_children = 0;
   hipStream_t stream = nullptr;
+  bool owns_stream = true;  // false: the caller's (cvs_context_create_on_stream)
   int compute_units = 0;
   int64_t total_mem = 0;
   std::string name;
@@ -91,6 +92,7 @@ struct cvs_context {
   cvs::DeviceBuffer ws_search;    // brute force: query tiles, thresholds, candidate lists
   cvs::DeviceBuffer ws_io;        // staging of host queries / results
   cvs::DeviceBuffer ws_teams;     // per-team lists of multi-team graph search
+  cvs::DeviceBuffer ws_attn;      // attention over a cache: partial results of split rows
   // Pinned host memory of kPinnedIoBytes for small blocking calls (host_call);
   // made by the first one.
   char* pinned_io = nullptr;

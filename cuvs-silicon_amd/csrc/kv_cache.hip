@@ -1,0 +1,470 @@
+// A paged cache of attention keys and values: sequences as lists of pages
+// that they may share, and the device work on pages - writing new tokens,
+// reading tokens back, copying pages.
+//
+// Layout of the pool: layer, page, kv head, then the head's keys and its
+// values, each in tiles of 32 tokens.  A tile is a run of 1 KiB blocks that
+// are operands of v_mfma_f32_32x32x16 as they stand, 16 bytes a lane, as the
+// datasets' tiles are, so that attention streams whole blocks from memory
+// into operand registers:
+//   keys:   block s holds columns [16 s, 16 s + 16); lane l has token l % 32, columns 16 s + 8 (l / 32) + [0, 8);
+//   values: block 2 b + s holds columns [32 b, 32 b + 32) of tokens [16 s, 16 s + 16); lane l has column 32 b + l % 32
+//           of tokens 16 s + 4 (l / 32) + {0, 1, 2, 3, 8, 9, 10, 11}, the order in which the first product leaves
+//           its probabilities (attn_common.hpp).
+// Rows are padded to whole 32-column blocks with zeros.
+#include <cstring>
+
+#include "attn_common.hpp"
+
+namespace cvs {
+namespace attn {
+namespace {
+
+struct Upload {
+  uint32_t words[kUploadBytes / 4];
+};
+
+__global__ __launch_bounds__(256) void upload_kernel(uint32_t* __restrict__ dst, const Upload u, int words) {
+  for (int i = threadIdx.x; i < words; i += 256) dst[i] = u.words[i];
+}
+
+// Up to kCopies page copies of a launch, passed as arguments.
+constexpr int kCopies = 448;
+struct Copies {
+  kv::PageCopy c[kCopies];
+};
+
+constexpr int kCopyBytes = 16384;  // of a workgroup: 4 loads of 16 bytes a thread in flight
+
+__global__ __launch_bounds__(256) void copy_pages_kernel(char* __restrict__ pool, int64_t layer_bytes,
+                                                         int64_t page_bytes, const Copies copies) {
+  const kv::PageCopy c = copies.c[blockIdx.x];
+  char* const layer = pool + int64_t(blockIdx.y) * layer_bytes;
+  const int64_t at = int64_t(blockIdx.z) * kCopyBytes + threadIdx.x * 16;
+  const char* const src = layer + c.src * page_bytes;
+  char* const dst = layer + c.dst * page_bytes;
+  u32x4 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (at + i * 4096 < page_bytes) v[i] = *reinterpret_cast<const u32x4*>(src + at + i * 4096);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (at + i * 4096 < page_bytes) *reinterpret_cast<u32x4*>(dst + at + i * 4096) = v[i];
+}
+
+void copy_pages(cvs_kv_cache* cache, const std::vector<kv::PageCopy>& copies) {
+  for (size_t at = 0; at < copies.size(); at += kCopies) {
+    const size_t n = std::min(copies.size() - at, size_t(kCopies));
+    Copies c;
+    std::memcpy(c.c, copies.data() + at, n * sizeof(kv::PageCopy));
+    const unsigned chunks = unsigned((cache->page_bytes + kCopyBytes - 1) / kCopyBytes);
+    hipLaunchKernelGGL(copy_pages_kernel, dim3(unsigned(n), unsigned(cache->layers), chunks), dim3(256), 0,
+                       cache->ctx->stream, cache->pool, cache->layer_bytes, cache->page_bytes, c);
+    after_launch("copy_pages_kernel");
+  }
+}
+
+// Tokens [begin, end) of a page, rows row0 and on of the caller's arrays.
+struct Span {
+  int32_t page, begin, end, row0;
+};
+
+struct MoveArgs {
+  char* pool;  // of the first layer
+  int64_t layer_bytes, page_bytes, head_bytes;
+  const Span* spans;
+  View k, v;
+  int64_t k_layer, v_layer;  // strides of the caller's arrays from layer to layer
+  int page_tokens, dim, kv_heads;
+};
+
+// Between rows of the caller's arrays and tiles of the pool, one workgroup a
+// tile of 32 tokens, kv head and layer, through LDS: rows are read and
+// written 16 bytes at a time along the row, tiles along their blocks.  A
+// tile whose tokens the span does not cover keeps its other tokens; a span's
+// tiles belong to one sequence, so no other workgroup touches them.
+template <int NB, bool kWrite>
+__global__ __launch_bounds__(256) void move_tokens_kernel(const MoveArgs a) {
+  constexpr int D = 32 * NB;
+  __shared__ __align__(16) uint16_t s[2][32][D];
+  const int tiles = a.page_tokens / 32;
+  const Span sp = a.spans[blockIdx.x / tiles];
+  const int tile = blockIdx.x % tiles;
+  const int lo = max(sp.begin - 32 * tile, 0), hi = min(sp.end - 32 * tile, 32);
+  if (lo >= hi) return;
+  const int g = blockIdx.y;
+  char* const head = a.pool + blockIdx.z * a.layer_bytes + sp.page * a.page_bytes + g * a.head_bytes;
+  char* const kt = head + int64_t(tile) * 2048 * NB;
+  char* const vt = kt + a.head_bytes / 2;
+  const int64_t row = int64_t(sp.row0) + 32 * tile - sp.begin;  // of the tile's token 0
+  char* const ks = a.k.p + 2 * (blockIdx.z * a.k_layer + row * a.k.token + g * a.k.head);
+  char* const vs = a.v.p + 2 * (blockIdx.z * a.v_layer + row * a.v.token + g * a.v.head);
+  if constexpr (kWrite) {
+    for (int i = threadIdx.x; i < 2 * 32 * 4 * NB; i += 256) {
+      const int which = i / (32 * 4 * NB), t = i / (4 * NB) % 32, p = i % (4 * NB);
+      u32x4 x{};
+      if (t >= lo && t < hi && 8 * p < a.dim)
+        x = which ? *reinterpret_cast<const u32x4*>(vs + 2 * (t * a.v.token + 8 * p))
+                  : *reinterpret_cast<const u32x4*>(ks + 2 * (t * a.k.token + 8 * p));
+      *reinterpret_cast<u32x4*>(&s[which][t][8 * p]) = x;
+    }
+    __syncthreads();
+  }
+  // Keys.
+  for (int i = threadIdx.x; i < 2 * NB * 64; i += 256) {
+    const int t = i & 31, col = 16 * (i >> 6) + 8 * ((i >> 5) & 1);
+    if (t < lo || t >= hi) continue;
+    if constexpr (kWrite)
+      *reinterpret_cast<u32x4*>(kt + 16 * i) = *reinterpret_cast<const u32x4*>(&s[0][t][col]);
+    else
+      *reinterpret_cast<u32x4*>(&s[0][t][col]) = *reinterpret_cast<const u32x4*>(kt + 16 * i);
+  }
+  // Values: 8 tokens of a column.
+  for (int i = threadIdx.x; i < 2 * NB * 64; i += 256) {
+    const int l = i & 63, col = 32 * (i >> 7) + (l & 31), t0 = 16 * ((i >> 6) & 1) + 4 * (l >> 5);
+    if (t0 + 11 < lo || t0 >= hi) continue;
+    const bool whole = t0 >= lo && t0 + 11 < hi;
+    uint16_t x[8] = {};
+    if (!kWrite || !whole) {
+      const u32x4 old = *reinterpret_cast<const u32x4*>(vt + 16 * i);
+      __builtin_memcpy(x, &old, 16);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int t = t0 + 8 * (j / 4) + j % 4;
+      if (t < lo || t >= hi) continue;
+      if constexpr (kWrite) x[j] = s[1][t][col];
+      else s[1][t][col] = x[j];
+    }
+    if constexpr (kWrite) {
+      u32x4 packed;
+      __builtin_memcpy(&packed, x, 16);
+      *reinterpret_cast<u32x4*>(vt + 16 * i) = packed;
+    }
+  }
+  if constexpr (!kWrite) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * 32 * 4 * NB; i += 256) {
+      const int which = i / (32 * 4 * NB), t = i / (4 * NB) % 32, p = i % (4 * NB);
+      if (t < lo || t >= hi || 8 * p >= a.dim) continue;
+      const u32x4 x = *reinterpret_cast<const u32x4*>(&s[which][t][8 * p]);
+      if (which) *reinterpret_cast<u32x4*>(vs + 2 * (t * a.v.token + 8 * p)) = x;
+      else *reinterpret_cast<u32x4*>(ks + 2 * (t * a.k.token + 8 * p)) = x;
+    }
+  }
+}
+
+void move_tokens(cvs_kv_plan* plan, int first_layer, int layers, const cvs_heads* k, int64_t k_layer,
+                 const cvs_heads* v, int64_t v_layer, bool write) {
+  check_plan(plan);
+  cvs_kv_cache* const c = plan->cache;
+  if (first_layer < 0 || layers < 1 || first_layer > c->layers - layers)
+    fail(CVS_ERR_INVALID_ARGUMENT, "layers outside the cache's " + std::to_string(c->layers));
+  for (const cvs_heads* x : {k, v}) {
+    const char* const what = x == k ? "k" : "v";
+    check_view(x, what);
+    if (x->tokens != plan->tokens)
+      fail(CVS_ERR_INVALID_ARGUMENT, std::string(what) + " must have the plan's " + std::to_string(plan->tokens) +
+                                         " tokens");
+    if (x->heads != c->kv_heads || x->head_dim != c->dim || x->type != c->type)
+      fail(CVS_ERR_INVALID_ARGUMENT, std::string(what) + " must have the cache's heads, head_dim and type");
+  }
+  if (layers > 1 && (k_layer % 8 != 0 || v_layer % 8 != 0 || k_layer < 0 || v_layer < 0))
+    fail(CVS_ERR_UNSUPPORTED, "layer strides must be non-negative multiples of 8 elements");
+  if (write)
+    for (const int32_t pg : plan->written)
+      if (c->book->refs(pg) > 1)
+        fail(CVS_ERR_INVALID_ARGUMENT, "the plan's tokens lie in a page that sequences share: extend first");
+  if (plan->spans == 0) return;
+  const MoveArgs a{c->pool + first_layer * c->layer_bytes, c->layer_bytes, c->page_bytes, c->head_bytes,
+                   reinterpret_cast<const Span*>(plan->blob.as<char>() + plan->at_spans), view_of(k), view_of(v),
+                   k_layer, v_layer, int(c->book->page_tokens()), c->dim, c->kv_heads};
+  const dim3 grid(unsigned(plan->spans * (c->book->page_tokens() / 32)), unsigned(c->kv_heads), unsigned(layers));
+  const TimerSpan ts = timer_span(c->ctx, write ? "kv_write" : "kv_read");
+  auto go = [&](auto kernel) {
+    hipExtLaunchKernelGGL(kernel, grid, dim3(256), 0, c->ctx->stream, ts.start, ts.stop, 0, a);
+  };
+  switch (c->nb) {
+    case 1: write ? go(move_tokens_kernel<1, true>) : go(move_tokens_kernel<1, false>); break;
+    case 2: write ? go(move_tokens_kernel<2, true>) : go(move_tokens_kernel<2, false>); break;
+    case 3: write ? go(move_tokens_kernel<3, true>) : go(move_tokens_kernel<3, false>); break;
+    default: write ? go(move_tokens_kernel<4, true>) : go(move_tokens_kernel<4, false>); break;
+  }
+  after_launch("move_tokens_kernel");
+}
+
+// Runs fn on the cache's bookkeeping with its errors as status codes.
+template <typename Fn>
+int on_book(cvs_kv_cache* cache, Fn&& fn) {
+  return guarded([&] {
+    if (!cache) fail(CVS_ERR_INVALID_ARGUMENT, "null cache");
+    try {
+      fn();
+    } catch (const kv::PageError& e) {
+      fail(e.full ? CVS_ERR_OUT_OF_MEMORY : CVS_ERR_INVALID_ARGUMENT, e.what);
+    }
+  });
+}
+
+void need(const void* p, const char* what) {
+  if (!p) fail(CVS_ERR_INVALID_ARGUMENT, std::string("null ") + what);
+}
+
+void need_list(const void* p, int64_t n, const char* what) {
+  if (n < 0) fail(CVS_ERR_INVALID_ARGUMENT, std::string("negative count of ") + what);
+  if (n > 0) need(p, what);
+}
+
+// The blob of a destroyed plan that fits, or a new one.
+DeviceBuffer take_blob(cvs_kv_cache* cache, size_t bytes) {
+  auto& pool = cache->blobs;
+  size_t best = pool.size();
+  for (size_t i = 0; i < pool.size(); ++i)
+    if (pool[i].bytes >= bytes && (best == pool.size() || pool[i].bytes < pool[best].bytes)) best = i;
+  DeviceBuffer b;
+  if (best < pool.size()) {
+    b = pool[best];
+    pool.erase(pool.begin() + int64_t(best));
+    return b;
+  }
+  cache->blobs.reserve(cache->blobs.size() + size_t(cache->live_plans) + 1);  // destroying a plan does not allocate
+  b.reserve(std::max(bytes, size_t(65536)));
+  return b;
+}
+
+}  // namespace
+
+void upload(cvs_context* ctx, void* dst, const void* src, size_t bytes) {
+  for (size_t at = 0; at < bytes; at += kUploadBytes) {
+    const size_t n = std::min(bytes - at, kUploadBytes);
+    Upload u;
+    std::memcpy(u.words, static_cast<const char*>(src) + at, n);
+    hipLaunchKernelGGL(upload_kernel, dim3(1), dim3(256), 0, ctx->stream,
+                       reinterpret_cast<uint32_t*>(static_cast<char*>(dst) + at), u, int(n / 4));
+    after_launch("upload_kernel");
+  }
+}
+
+void check_plan(const cvs_kv_plan* plan) {
+  if (!plan) fail(CVS_ERR_INVALID_ARGUMENT, "null plan");
+  try {
+    for (size_t i = 0; i < plan->seqs.size(); ++i)
+      if (plan->cache->book->at(plan->seqs[i]).version != plan->versions[i])
+        fail(CVS_ERR_INVALID_ARGUMENT, "sequence " + std::to_string(plan->seqs[i]) +
+                                           " has changed since the plan was made: make a new one");
+  } catch (const kv::PageError& e) {
+    fail(CVS_ERR_INVALID_ARGUMENT, e.what);
+  }
+}
+
+}  // namespace attn
+}  // namespace cvs
+
+using namespace cvs;
+using namespace cvs::attn;
+
+extern "C" {
+
+int cvs_kv_cache_create(cvs_context* ctx, int layers, int64_t pages, int page_tokens, int kv_heads, int head_dim,
+                        int type, cvs_kv_cache** out_cache) {
+  return guarded([&] {
+    bind(ctx);
+    need(out_cache, "out_cache");
+    *out_cache = nullptr;
+    if (type != CVS_FP16 && type != CVS_BF16) fail(CVS_ERR_UNSUPPORTED, "a cache holds fp16 or bf16");
+    if (layers < 1 || pages < 1 || kv_heads < 1)
+      fail(CVS_ERR_INVALID_ARGUMENT, "a cache needs at least one layer, page and kv head");
+    if (layers > 65535 || kv_heads > 65535 || pages > (int64_t(1) << 30))
+      fail(CVS_ERR_UNSUPPORTED, "too many layers, pages or heads");
+    if (page_tokens < 32 || page_tokens > 4096 || (page_tokens & (page_tokens - 1)) != 0)
+      fail(CVS_ERR_UNSUPPORTED, "page_tokens must be a power of two from 32 to 4096");
+    if (head_dim < 8 || head_dim % 8 != 0 || head_dim > kMaxDim)
+      fail(CVS_ERR_UNSUPPORTED, "head_dim must be a multiple of 8 from 8 to " + std::to_string(kMaxDim));
+    auto c = std::make_unique<cvs_kv_cache>();
+    c->ctx = ctx;
+    c->layers = layers;
+    c->kv_heads = kv_heads;
+    c->dim = head_dim;
+    c->type = type;
+    c->nb = (head_dim + 31) / 32;
+    c->head_bytes = int64_t(2) * page_tokens * 64 * c->nb;
+    c->page_bytes = c->head_bytes * kv_heads;
+    if (c->page_bytes > (int64_t(1) << 29)) fail(CVS_ERR_UNSUPPORTED, "a page of a layer must not exceed 512 MiB");
+    c->layer_bytes = c->page_bytes * pages;
+    if (c->layer_bytes > (int64_t(1) << 50) / layers) fail(CVS_ERR_OUT_OF_MEMORY, "the pages exceed the memory");
+    c->book = std::make_unique<kv::PageBook>(pages, page_tokens);
+    CVS_HIP(hipMalloc(reinterpret_cast<void**>(&c->pool), size_t(c->layer_bytes) * size_t(layers)));
+    ++ctx->live_children;
+    *out_cache = c.release();
+  });
+}
+
+int cvs_kv_cache_destroy(cvs_kv_cache* cache) {
+  return guarded([&] {
+    if (!cache) return;
+    if (cache->live_plans > 0)
+      fail(CVS_ERR_INVALID_ARGUMENT, "cache still has " + std::to_string(cache->live_plans) +
+                                         " plan(s): destroy them first");
+    bind(cache->ctx);
+    (void)hipStreamSynchronize(cache->ctx->stream);
+    for (auto& b : cache->blobs) b.release();
+    (void)hipFree(cache->pool);
+    --cache->ctx->live_children;
+    delete cache;
+  });
+}
+
+int cvs_kv_cache_pages(cvs_kv_cache* cache, int64_t* out_pages, int64_t* out_free) {
+  return on_book(cache, [&] {
+    if (out_pages) *out_pages = cache->book->pages();
+    if (out_free) *out_free = cache->book->free_pages();
+  });
+}
+
+int cvs_kv_sequence_create(cvs_kv_cache* cache, int64_t n, int64_t* out_seqs) {
+  return on_book(cache, [&] {
+    need_list(out_seqs, n, "sequences");
+    for (int64_t i = 0; i < n; ++i) out_seqs[i] = cache->book->create();
+  });
+}
+
+int cvs_kv_sequence_fork(cvs_kv_cache* cache, int64_t parent, int64_t length, int64_t n, int64_t* out_seqs) {
+  return on_book(cache, [&] {
+    need_list(out_seqs, n, "sequences");
+    const int64_t len = length < 0 ? cache->book->at(parent).length : length;
+    for (int64_t i = 0; i < n; ++i) out_seqs[i] = cache->book->fork(parent, len);
+  });
+}
+
+int cvs_kv_sequence_extend(cvs_kv_cache* cache, const int64_t* seqs, const int64_t* tokens, int64_t n) {
+  return on_book(cache, [&] {
+    need_list(seqs, n, "sequences");
+    need_list(tokens, n, "tokens");
+    bind(cache->ctx);
+    copy_pages(cache, cache->book->extend(seqs, tokens, n));
+  });
+}
+
+int cvs_kv_sequence_truncate(cvs_kv_cache* cache, int64_t seq, int64_t length) {
+  return on_book(cache, [&] { cache->book->truncate(seq, length); });
+}
+
+int cvs_kv_sequence_free(cvs_kv_cache* cache, const int64_t* seqs, int64_t n) {
+  return on_book(cache, [&] {
+    need_list(seqs, n, "sequences");
+    cache->book->release(seqs, n);
+  });
+}
+
+int cvs_kv_sequence_pages(cvs_kv_cache* cache, const int64_t* seqs, int64_t n, int64_t* out_lengths,
+                          uint32_t* out_pages, int64_t room, int64_t* out_count) {
+  return on_book(cache, [&] {
+    need_list(seqs, n, "sequences");
+    int64_t total = 0;
+    for (int64_t i = 0; i < n; ++i) {
+      const kv::Sequence& s = cache->book->at(seqs[i]);
+      if (out_lengths) out_lengths[i] = s.length;
+      for (const int32_t pg : s.pages) {
+        if (out_pages && total < room) out_pages[total] = uint32_t(pg);
+        ++total;
+      }
+    }
+    if (out_count) *out_count = total;
+    if (out_pages && total > room) fail(CVS_ERR_INVALID_ARGUMENT, "room for fewer pages than the sequences have");
+  });
+}
+
+int cvs_kv_cache_compact(cvs_kv_cache* cache, int64_t* out_live) {
+  return on_book(cache, [&] {
+    bind(cache->ctx);
+    copy_pages(cache, cache->book->compact());
+    if (out_live) *out_live = cache->book->pages() - cache->book->free_pages();
+  });
+}
+
+int cvs_kv_plan_create(cvs_kv_cache* cache, const int64_t* seqs, const int64_t* tokens, int64_t n, int heads,
+                       cvs_kv_plan** out_plan) {
+  return on_book(cache, [&] {
+    need(out_plan, "out_plan");
+    *out_plan = nullptr;
+    need_list(seqs, n, "sequences");
+    need_list(tokens, n, "tokens");
+    if (heads < 0 || heads % cache->kv_heads != 0)
+      fail(CVS_ERR_INVALID_ARGUMENT, "heads must be a multiple of the cache's kv heads (0: no attention)");
+    bind(cache->ctx);
+    kv::PageBook& book = *cache->book;
+    book.check_ids(seqs, n);
+    auto plan = std::make_unique<cvs_kv_plan>();
+    plan->cache = cache;
+    plan->heads = heads;
+    std::vector<int64_t> lengths;
+    std::vector<Span> spans;
+    const int64_t pt = book.page_tokens();
+    for (int64_t i = 0; i < n; ++i) {
+      const kv::Sequence& s = book.at(seqs[i]);
+      if (tokens[i] < 0 || tokens[i] > s.length)
+        fail(CVS_ERR_INVALID_ARGUMENT, "sequence " + std::to_string(seqs[i]) + " has " + std::to_string(s.length) +
+                                           " tokens, the plan asks for " + std::to_string(tokens[i]));
+      if (plan->tokens + tokens[i] > kv::PageBook::kMaxTokens) fail(CVS_ERR_UNSUPPORTED, "tokens must fit 31 bits");
+      plan->seqs.push_back(seqs[i]);
+      plan->versions.push_back(s.version);
+      lengths.push_back(s.length);
+      for (int64_t t = s.length - tokens[i]; t < s.length;) {
+        const int64_t in = t % pt, end = std::min(pt, in + s.length - t);
+        const int32_t pg = s.pages[size_t(t / pt)];
+        spans.push_back({pg, int32_t(in), int32_t(end), int32_t(plan->tokens)});
+        plan->written.push_back(pg);
+        plan->tokens += end - in;
+        t += end - in;
+      }
+    }
+    if (int64_t(spans.size()) * (pt / 32) > (int64_t(1) << 31) - 1) fail(CVS_ERR_UNSUPPORTED, "too many tokens");
+    plan->spans = int(spans.size());
+    std::vector<char> blob(spans.size() * sizeof(Span));
+    if (!spans.empty()) std::memcpy(blob.data(), spans.data(), blob.size());
+    if (heads > 0) plan_attention(plan.get(), lengths.data(), tokens, blob);
+    if (!blob.empty()) {
+      plan->blob = take_blob(cache, blob.size());
+      try {
+        upload(cache->ctx, plan->blob.ptr, blob.data(), blob.size());
+      } catch (...) {
+        cache->blobs.push_back(plan->blob);
+        throw;
+      }
+    }
+    ++cache->live_plans;
+    *out_plan = plan.release();
+  });
+}
+
+int cvs_kv_plan_destroy(cvs_kv_plan* plan) {
+  return guarded([&] {
+    if (!plan) return;
+    // Later plans use the memory on the same stream, after whatever still reads it.
+    if (plan->blob.ptr) plan->cache->blobs.push_back(plan->blob);
+    --plan->cache->live_plans;
+    delete plan;
+  });
+}
+
+int cvs_kv_write_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int first_layer, int layers, const cvs_heads* k,
+                       int64_t k_layer_stride, const cvs_heads* v, int64_t v_layer_stride) {
+  return on_book(cache, [&] {
+    need(plan, "plan");
+    if (plan->cache != cache) fail(CVS_ERR_INVALID_ARGUMENT, "the plan belongs to another cache");
+    bind(cache->ctx);
+    move_tokens(plan, first_layer, layers, k, k_layer_stride, v, v_layer_stride, true);
+  });
+}
+
+int cvs_kv_read_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int first_layer, int layers, const cvs_heads* k,
+                      int64_t k_layer_stride, const cvs_heads* v, int64_t v_layer_stride) {
+  return on_book(cache, [&] {
+    need(plan, "plan");
+    if (plan->cache != cache) fail(CVS_ERR_INVALID_ARGUMENT, "the plan belongs to another cache");
+    bind(cache->ctx);
+    move_tokens(plan, first_layer, layers, k, k_layer_stride, v, v_layer_stride, false);
+  });
+}
+
+}  // extern "C"

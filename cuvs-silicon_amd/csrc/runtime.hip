@@ -421,6 +421,45 @@ __global__ __launch_bounds__(256) void gather_read_kernel(const stream_vec* __re
   if (acc == 0x9E3779B9u) sink[blockIdx.x * 256 + threadIdx.x] = acc;
 }
 
+namespace {
+// A context on a stream of its own, or on the caller's (null: the default stream).
+void create_context(int device, bool own_stream, hipStream_t stream, cvs_context** out_ctx) {
+  if (!out_ctx) fail(CVS_ERR_INVALID_ARGUMENT, "null out_ctx");
+  *out_ctx = nullptr;
+  int count = 0;
+  if (hipGetDeviceCount(&count) != hipSuccess || count <= 0)
+    fail(CVS_ERR_NO_DEVICE, "no HIP device available");
+  if (device < 0 || device >= count)
+    fail(CVS_ERR_INVALID_ARGUMENT, "device index out of range");
+  hipDeviceProp_t prop;
+  CVS_HIP(hipGetDeviceProperties(&prop, device));
+  if (std::strncmp(prop.gcnArchName, "gfx950", 6) != 0)
+    fail(CVS_ERR_NO_DEVICE, std::string("kernels are built for gfx950, device is ") +
+                                prop.gcnArchName);
+  auto* ctx = new cvs_context();
+  ctx->owns_stream = own_stream;
+  ctx->device = device;
+  ctx->compute_units = prop.multiProcessorCount;
+  ctx->total_mem = static_cast<int64_t>(prop.totalGlobalMem);
+  ctx->name = prop.name[0] ? std::string(prop.name) + " (" + prop.gcnArchName + ")"
+                           : std::string(prop.gcnArchName);
+  try {
+    CVS_HIP(hipSetDevice(device));
+    if (own_stream) CVS_HIP(hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking));
+    else ctx->stream = stream;
+    CVS_HIP(hipMalloc(&ctx->bf_counters, 2 * sizeof(unsigned long long)));
+    CVS_HIP(hipMemsetAsync(ctx->bf_counters, 0, 2 * sizeof(unsigned long long), ctx->stream));
+    CVS_HIP(hipStreamSynchronize(ctx->stream));
+  } catch (...) {
+    if (ctx->bf_counters) (void)hipFree(ctx->bf_counters);
+    if (own_stream && ctx->stream) (void)hipStreamDestroy(ctx->stream);
+    delete ctx;
+    throw;
+  }
+  *out_ctx = ctx;
+}
+}  // namespace
+
 }  // namespace cvs
 
 using namespace cvs;
@@ -491,39 +530,11 @@ int cvs_device_count(int* out_count) {
 }
 
 int cvs_context_create(int device, cvs_context** out_ctx) {
-  return guarded([&] {
-    if (!out_ctx) fail(CVS_ERR_INVALID_ARGUMENT, "null out_ctx");
-    *out_ctx = nullptr;
-    int count = 0;
-    if (hipGetDeviceCount(&count) != hipSuccess || count <= 0)
-      fail(CVS_ERR_NO_DEVICE, "no HIP device available");
-    if (device < 0 || device >= count)
-      fail(CVS_ERR_INVALID_ARGUMENT, "device index out of range");
-    hipDeviceProp_t prop;
-    CVS_HIP(hipGetDeviceProperties(&prop, device));
-    if (std::strncmp(prop.gcnArchName, "gfx950", 6) != 0)
-      fail(CVS_ERR_NO_DEVICE, std::string("kernels are built for gfx950, device is ") +
-                                  prop.gcnArchName);
-    auto* ctx = new cvs_context();
-    ctx->device = device;
-    ctx->compute_units = prop.multiProcessorCount;
-    ctx->total_mem = static_cast<int64_t>(prop.totalGlobalMem);
-    ctx->name = prop.name[0] ? std::string(prop.name) + " (" + prop.gcnArchName + ")"
-                             : std::string(prop.gcnArchName);
-    try {
-      CVS_HIP(hipSetDevice(device));
-      CVS_HIP(hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking));
-      CVS_HIP(hipMalloc(&ctx->bf_counters, 2 * sizeof(unsigned long long)));
-      CVS_HIP(hipMemsetAsync(ctx->bf_counters, 0, 2 * sizeof(unsigned long long), ctx->stream));
-      CVS_HIP(hipStreamSynchronize(ctx->stream));
-    } catch (...) {
-      if (ctx->bf_counters) (void)hipFree(ctx->bf_counters);
-      if (ctx->stream) (void)hipStreamDestroy(ctx->stream);
-      delete ctx;
-      throw;
-    }
-    *out_ctx = ctx;
-  });
+  return guarded([&] { create_context(device, true, nullptr, out_ctx); });
+}
+
+int cvs_context_create_on_stream(int device, void* stream, cvs_context** out_ctx) {
+  return guarded([&] { create_context(device, false, static_cast<hipStream_t>(stream), out_ctx); });
 }
 
 int cvs_context_destroy(cvs_context* ctx) {
@@ -531,9 +542,9 @@ int cvs_context_destroy(cvs_context* ctx) {
     if (!ctx) return;
     if (ctx->live_children > 0)
       fail(CVS_ERR_INVALID_ARGUMENT, "context still owns " + std::to_string(ctx->live_children) +
-                                         " dataset(s) or graph index(es): destroy them first");
+                                         " dataset(s) or graph index(es), cache(s) or plan(s): destroy them first");
     (void)hipSetDevice(ctx->device);
-    if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
+    (void)hipStreamSynchronize(ctx->stream);
     for (auto& kv : ctx->timers) {
       for (auto& p : kv.second.pending) {
         (void)hipEventDestroy(p.first);
@@ -544,9 +555,10 @@ int cvs_context_destroy(cvs_context* ctx) {
     ctx->ws_search.release();
     ctx->ws_io.release();
     ctx->ws_teams.release();
+    ctx->ws_attn.release();
     if (ctx->pinned_io) (void)hipHostFree(ctx->pinned_io);
     if (ctx->bf_counters) (void)hipFree(ctx->bf_counters);
-    if (ctx->stream) (void)hipStreamDestroy(ctx->stream);
+    if (ctx->owns_stream) (void)hipStreamDestroy(ctx->stream);
     delete ctx;
   });
 }

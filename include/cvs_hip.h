@@ -80,6 +80,11 @@ int cvs_device_count(int* out_count);
 /* Create a context on `device` (replaces MetalContext::instance(),
  * metal_context.hpp:15, and is_available(), metal_context.hpp:19). */
 int cvs_context_create(int device, cvs_context** out_ctx);
+/* The same on a stream of the caller's (a hipStream_t; null: the default
+ * stream), which the context does not destroy: its calls then run in order
+ * with the caller's own work on that stream, and arrays that work makes or
+ * reads need no synchronization in between. */
+int cvs_context_create_on_stream(int device, void* stream, cvs_context** out_ctx);
 int cvs_context_destroy(cvs_context* ctx);
 int cvs_context_synchronize(cvs_context* ctx);
 
@@ -94,7 +99,8 @@ int cvs_context_device_info(cvs_context* ctx, char* name, size_t name_len,
  * ends it), so timing inserts nothing between kernels on the stream.
  * cvs_context_kernel_time() synchronizes and returns the summed elapsed
  * milliseconds and the number of spans for `kernel` ("bf_prep", "bf_sample",
- * "bf_scan", "bf_merge", "cagra_search", "cagra_edge_distances"), then
+ * "bf_scan", "bf_merge", "cagra_search", "cagra_edge_distances",
+ * "prompt_attention", "kv_attention", "kv_join", "kv_write", "kv_read"), then
  * clears them. */
 int cvs_context_set_timing(cvs_context* ctx, int enable);
 int cvs_context_kernel_time(cvs_context* ctx, const char* kernel,
@@ -480,6 +486,139 @@ int cvs_cagra_build_reference(cvs_context* ctx, const float* rows, int64_t n, in
 int cvs_cagra_build_reference_ex(cvs_context* ctx, const float* rows, int64_t n, int64_t d, int rows_on_device,
                                  uint32_t graph_degree, int64_t exact_limit, int64_t pq_limit, uint32_t* out_graph,
                                  int graph_on_device, cvs_ref_build_stats* stats);
+
+/* ---- attention over the passages a search found -------------------------- */
+
+/* No counterpart in the reference: what a program does on the same card
+ * around a search.  Passages and questions go through a model's attention
+ * (cvs_prompt_attention_async); the keys and values of the passages that were
+ * found are kept in a cache (cvs_kv_cache) whose pages several questions'
+ * sequences share; each step's new tokens attend to it, what the sequences
+ * share being read once for all of them (cvs_kv_attention_async).  Forward
+ * only: the library trains nothing.
+ *
+ * With x_ij = scale * q_i . k_j over the keys j that query i sees,
+ *   lse_i = ln sum_j exp(x_ij),  out_i = sum_j exp(x_ij - lse_i) v_j;
+ * a query that sees no key gets zeros and lse = -inf.  Products take fp16 or
+ * bf16 operands and accumulate in fp32, the softmax's maxima and sums are
+ * fp32, probabilities are rounded to the operands' type for the second
+ * product and the output once.  Keys and values a query does not see do not
+ * reach its result, infinities and NaNs included. */
+
+#define CVS_FP16 0 /* IEEE half */
+#define CVS_BF16 1 /* bfloat16 */
+
+/* A device array of tokens x heads x head_dim 16-bit elements: element (t, h,
+ * i) at data + t * token_stride + h * head_stride + i (strides in elements),
+ * so q, k and v may be views of one projection, and a batch's sequences lie
+ * one behind another.  data 16-byte aligned, strides multiples of 8
+ * (CVS_ERR_UNSUPPORTED otherwise), token_stride at most 2^23, head_dim a
+ * multiple of 8 from 8 to CVS_ATTN_MAX_DIM.  Outputs must not overlap. */
+#define CVS_ATTN_MAX_DIM 128
+typedef struct cvs_heads {
+  void* data;
+  int64_t tokens;
+  int64_t token_stride;
+  int64_t head_stride;
+  int heads;
+  int head_dim;
+  int type; /* CVS_FP16 or CVS_BF16 */
+} cvs_heads;
+
+/* How a batch of n sequences of q_lengths[i] query tokens and k_lengths[i]
+ * key tokens (null: as many), packed one behind another, is worked on; made
+ * once for a batch and used for every layer.  Lengths may be 0.  `causal` =
+ * 1: query i of a sequence sees its keys up to i + k_length - q_length (the
+ * last query sees all); 0: every key of its sequence.  heads query heads,
+ * kv_heads key/value heads (heads a multiple of them; query head h reads
+ * kv head h / (heads / kv_heads)).  Lengths are host arrays. */
+typedef struct cvs_prompt_plan cvs_prompt_plan;
+int cvs_prompt_plan_create(cvs_context* ctx, const int64_t* q_lengths, const int64_t* k_lengths, int64_t n, int heads,
+                           int kv_heads, int causal, cvs_prompt_plan** out_plan);
+int cvs_prompt_plan_destroy(cvs_prompt_plan* plan);
+
+/* Attention of a plan's batch.  q, out: the plan's query tokens x heads; k,
+ * v: its key tokens x kv_heads.  scale: finite and positive, or 0 for 1 /
+ * sqrt(head_dim).  lse (may be null): heads x query tokens floats.  Device
+ * memory; enqueued on the context stream. */
+int cvs_prompt_attention_async(cvs_context* ctx, const cvs_prompt_plan* plan, const cvs_heads* q, const cvs_heads* k,
+                               const cvs_heads* v, const cvs_heads* out, float* lse, float scale);
+
+/* A cache of keys and values: `layers` layers of `pages` pages of
+ * page_tokens tokens (a power of two from 32 to 4096), each token kv_heads x
+ * head_dim elements of keys and of values.  Allocated once, in the layout
+ * the attention's matrix instructions read; 4 * kv_heads * (head_dim rounded
+ * up to 32) * page_tokens bytes a page and layer.
+ *
+ * Sequences are lists of pages, the same in every layer, and may share
+ * pages: forking one copies nothing, and a page several sequences hold is
+ * never written - extending a sequence whose last page is partly filled and
+ * shared first copies that page (on the GPU, all layers).  Free pages are
+ * taken lowest id first.  Page bookkeeping is on the host, in the order of
+ * the calls; all device work is on the context stream, in the same order, so
+ * a page freed by one call may be reused by the next.  Like a context, a
+ * cache serves one host thread at a time. */
+typedef struct cvs_kv_cache cvs_kv_cache;
+typedef struct cvs_kv_plan cvs_kv_plan;
+int cvs_kv_cache_create(cvs_context* ctx, int layers, int64_t pages, int page_tokens, int kv_heads, int head_dim,
+                        int type, cvs_kv_cache** out_cache);
+/* Refused while plans made on it are alive. */
+int cvs_kv_cache_destroy(cvs_kv_cache* cache);
+int cvs_kv_cache_pages(cvs_kv_cache* cache, int64_t* out_pages, int64_t* out_free);
+
+/* n new sequences without tokens; their ids (host) to out_seqs. */
+int cvs_kv_sequence_create(cvs_kv_cache* cache, int64_t n, int64_t* out_seqs);
+/* n new sequences of the first `length` tokens of `parent` (-1: all of
+ * them), on the parent's pages. */
+int cvs_kv_sequence_fork(cvs_kv_cache* cache, int64_t parent, int64_t length, int64_t n, int64_t* out_seqs);
+/* Room for tokens[i] more tokens in sequence seqs[i], in this order, no
+ * sequence twice; CVS_ERR_OUT_OF_MEMORY and no change when the free pages do
+ * not suffice.  The new tokens hold nothing until written. */
+int cvs_kv_sequence_extend(cvs_kv_cache* cache, const int64_t* seqs, const int64_t* tokens, int64_t n);
+/* Keeps the first `length` tokens. */
+int cvs_kv_sequence_truncate(cvs_kv_cache* cache, int64_t seq, int64_t length);
+/* Ends n sequences; pages that no other sequence holds are free again. */
+int cvs_kv_sequence_free(cvs_kv_cache* cache, const int64_t* seqs, int64_t n);
+/* Lengths of n sequences (may be null) and their pages, one list behind
+ * another, into out_pages (null: only counted; `room` entries); *out_count
+ * (may be null) is the number of pages in all. */
+int cvs_kv_sequence_pages(cvs_kv_cache* cache, const int64_t* seqs, int64_t n, int64_t* out_lengths,
+                          uint32_t* out_pages, int64_t room, int64_t* out_count);
+/* Moves pages so that the live ones are pages 0 to *out_live - 1 (may be
+ * null): those at or past that number, lowest id first, into the free ones
+ * below it, lowest id first. */
+int cvs_kv_cache_compact(cvs_kv_cache* cache, int64_t* out_live);
+
+/* The newest tokens[i] tokens of sequence seqs[i], no sequence twice, as the
+ * rows that the calls below write, read or query: packed, in the order given.
+ * heads: query heads, a multiple of the cache's kv heads, or 0 for a plan
+ * that only reads and writes.  Made once for a step and used for every
+ * layer; calls with it fail once one of its sequences has changed
+ * (extended, truncated, freed, or moved by compaction). */
+int cvs_kv_plan_create(cvs_kv_cache* cache, const int64_t* seqs, const int64_t* tokens, int64_t n, int heads,
+                       cvs_kv_plan** out_plan);
+int cvs_kv_plan_destroy(cvs_kv_plan* plan);
+
+/* Writes the plan's tokens into, or reads them out of, layers [first_layer,
+ * first_layer + layers): k, v are the plan's tokens x the cache's kv heads of
+ * the first layer, the next layers' at multiples of the layer strides (in
+ * elements).  Writing into a page that sequences share is refused (extend
+ * makes the newest tokens' pages a sequence's own).  Device memory; enqueued
+ * on the context stream. */
+int cvs_kv_write_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int first_layer, int layers, const cvs_heads* k,
+                       int64_t k_layer_stride, const cvs_heads* v, int64_t v_layer_stride);
+int cvs_kv_read_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int first_layer, int layers, const cvs_heads* k,
+                      int64_t k_layer_stride, const cvs_heads* v, int64_t v_layer_stride);
+
+/* Attention of the plan's tokens over a layer of the cache: a sequence's
+ * last token sees all of it, the one before all but the last, and so on.
+ * Pages that sequences of the plan share from their beginnings on are read
+ * once for all of them.  q, out: the plan's tokens x its heads; scale and
+ * lse (heads x tokens) as in cvs_prompt_attention_async.  Device memory;
+ * enqueued on the context stream.  Partial results of long sequences go
+ * through a workspace that the context keeps. */
+int cvs_kv_attention_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int layer, const cvs_heads* q,
+                           const cvs_heads* out, float* lse, float scale);
 
 #ifdef __cplusplus
 }

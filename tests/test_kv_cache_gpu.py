@@ -1,0 +1,457 @@
+"""The paged cache (cvs_kv_*) and attention over it: pages against a model of
+their bookkeeping, contents bit for bit, attention against 64 bits (bounds:
+attention_oracle.py)."""
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from attention_oracle import TORCH, assert_within, attention, f64
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def tctx(cvs):
+    c = cvs.Context(0, stream=torch.cuda.current_stream().cuda_stream)
+    yield c
+    c.close()
+
+
+def rand(seed, *shape, dtype, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * spread).to(TORCH[dtype]).cuda()
+
+
+def bits(x):
+    return x.contiguous().view(torch.int16)
+
+
+class Filled:
+    """A cache and what it should hold: each sequence's keys and values, (layers, tokens, kv_heads, dim) on the GPU."""
+
+    def __init__(self, ctx, layers, pages, page, kv, dim, dtype, seed=0):
+        self.cache = ctx.kv_cache(layers, pages, page, kv, dim, dtype)
+        self.layers, self.kv, self.dim, self.dtype, self.seed = layers, kv, dim, dtype, seed
+        self.held = {}
+
+    def new(self, n=1):
+        ids = self.cache.sequences(n)
+        for i in ids:
+            self.held[i] = [torch.zeros(self.layers, 0, self.kv, self.dim, dtype=TORCH[self.dtype], device="cuda")
+                            for _ in "kv"]
+        return ids
+
+    def fork(self, parent, n, length=-1):
+        ids = self.cache.fork(parent, n, length)
+        for i in ids:
+            self.held[i] = [x if length < 0 else x[:, :length] for x in self.held[parent]]
+        return ids
+
+    def append(self, seqs, tokens, make=None):
+        """Extends and writes, in one call each."""
+        self.cache.extend(seqs, tokens)
+        self.seed += 2
+        make = make or (lambda s, *shape: rand(s, *shape, dtype=self.dtype))
+        k, v = (make(self.seed + i, self.layers, sum(tokens), self.kv, self.dim) for i in (0, 1))
+        plan = self.cache.plan(seqs, tokens)
+        self.cache.write_async(plan, k, v)
+        at = 0
+        for s, t in zip(seqs, tokens):
+            self.held[s] = [torch.cat([old, new[:, at:at + t]], dim=1) for old, new in zip(self.held[s], (k, v))]
+            at += t
+
+    def check(self, seqs=None):
+        """Reads everything back."""
+        seqs = list(self.held) if seqs is None else seqs
+        lengths = [self.held[s][0].shape[1] for s in seqs]
+        assert self.cache.lengths(seqs) == lengths
+        t = sum(lengths)
+        k, v = (torch.full((self.layers, t, self.kv, self.dim), 9.0, dtype=TORCH[self.dtype], device="cuda")
+                for _ in "kv")
+        self.cache.read_async(self.cache.plan(seqs, lengths), k, v)
+        at = 0
+        for s, n in zip(seqs, lengths):
+            for got, want in zip((k, v), self.held[s]):
+                assert torch.equal(bits(got[:, at:at + n]), bits(want)), f"sequence {s}"
+            at += n
+
+    def free(self, seqs):
+        self.cache.free(seqs)
+        for s in seqs:
+            del self.held[s]
+
+
+class Model:
+    """The pages' bookkeeping in a few lines: lowest free id first, copy on write, moves to the front."""
+
+    def __init__(self, pages, page):
+        self.free, self.page, self.seqs = set(range(pages)), page, {}
+
+    def take(self):
+        p = min(self.free)
+        self.free.remove(p)
+        return p
+
+    def refs(self, p):
+        return sum(p in pages for pages, _ in self.seqs.values())
+
+    def need(self, n):
+        return -(-n // self.page)
+
+    def extend(self, s, t):
+        pages, n = self.seqs[s]
+        if t and n % self.page and self.refs(pages[-1]) > 1:
+            pages[-1] = self.take()
+        while len(pages) < self.need(n + t):
+            pages.append(self.take())
+        self.seqs[s] = (pages, n + t)
+
+    def fork(self, s, child, n):
+        self.seqs[child] = (self.seqs[s][0][:self.need(n)], n)
+
+    def cut(self, s, n):
+        pages = self.seqs[s][0]
+        gone = pages[self.need(n):]
+        self.seqs[s] = (pages[:self.need(n)], n)
+        self.free |= {p for p in gone if not self.refs(p)}
+
+    def drop(self, s):
+        pages, _ = self.seqs.pop(s)
+        self.free |= {p for p in pages if not self.refs(p)}
+
+    def compact(self, total):
+        live = total - len(self.free)
+        src = sorted(set(range(live, total)) - self.free)
+        to = dict(zip(src, sorted(p for p in self.free if p < live)))
+        for s, (pages, n) in self.seqs.items():
+            self.seqs[s] = ([to.get(p, p) for p in pages], n)
+        self.free = set(range(live, total))
+
+
+@pytest.mark.parametrize("page,dim,dtype,seed", [(32, 64, "fp16", 1), (32, 80, "bf16", 2), (64, 128, "bf16", 3),
+                                                 (128, 24, "fp16", 4)])
+def test_any_order_of_calls(tctx, cvs, page, dim, dtype, seed):
+    """Random calls: page ids as the model's, contents as written, through forks, copies, cuts and compaction."""
+    r = random.Random(seed)
+    total = 40
+    f, m = Filled(tctx, 2, total, page, 2, dim, dtype, 100 * seed), Model(total, page)
+    for s in f.new(2):
+        m.seqs[s] = ([], 0)
+    for step in range(120):
+        seqs = list(f.held)
+        do = r.choice(["append", "append", "append", "fork", "cut", "free", "compact", "new"])
+        if do == "new" or not seqs:
+            for s in f.new(1):
+                m.seqs[s] = ([], 0)
+        elif do == "append":
+            some = r.sample(seqs, r.randint(1, min(4, len(seqs))))
+            tokens = [r.choice([0, 1, 2, page - 1, page, page + 1, r.randint(0, 3 * page)]) for _ in some]
+            try:
+                f.append(some, tokens)
+            except RuntimeError as e:
+                assert "free pages" in str(e)
+                assert len(m.free) < sum(m.need(m.seqs[s][1] + t) - len(m.seqs[s][0]) + 1 for s, t in zip(some, tokens))
+                continue
+            for s, t in zip(some, tokens):
+                m.extend(s, t)
+        elif do == "fork" and len(seqs) < 12:
+            p = r.choice(seqs)
+            n = r.randint(0, m.seqs[p][1])
+            for c in f.fork(p, 2, n):
+                m.fork(p, c, n)
+        elif do == "cut":
+            s = r.choice(seqs)
+            n = r.randint(0, m.seqs[s][1])
+            f.cache.truncate(s, n)
+            f.held[s] = [x[:, :n] for x in f.held[s]]
+            m.cut(s, n)
+        elif do == "free" and len(seqs) > 3:
+            some = r.sample(seqs, 2)
+            f.free(some)
+            for s in some:
+                m.drop(s)
+        elif do == "compact":
+            assert f.cache.compact() == total - len(m.free)
+            m.compact(total)
+        assert f.cache.free_pages() == len(m.free)
+        seqs = list(f.held)
+        want = [p for s in seqs for p in m.seqs[s][0]]
+        assert f.cache.pages(seqs).tolist() == want, (step, do)
+        if step % 10 == 9 or do == "compact":
+            f.check()
+    f.check()
+    f.cache.close()
+
+
+@pytest.mark.parametrize("dim,page", [(8, 32), (32, 64), (40, 32), (64, 128), (96, 32), (104, 64), (128, 4096)])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_written_tokens_come_back(tctx, dim, page, dtype):
+    """One token, tiles and pages begun in the middle, several layers at once and one at a time, strided arrays."""
+    f = Filled(tctx, 3, 64 if page < 4096 else 4, page, 3, dim, dtype, 7)
+    a, b = f.new(2)
+    for tokens in ([1, 0], [30, 5], [2, 33], [page, 1], [7, page - 1]):
+        f.append([a, b], tokens)
+        f.check()
+    # One layer at a time, keys and values as views of one array.
+    f.cache.extend([a], [9])
+    plan = f.cache.plan([a], [9])
+    x = rand(5, 3, 9, 8, dim, dtype=dtype)
+    for layer in range(3):
+        f.cache.write_async(plan, x[layer, :, 2:5], x[layer, :, 5:], layer=layer)
+    f.held[a] = [torch.cat([h, x[:, :, o:o + 3]], dim=1) for h, o in zip(f.held[a], (2, 5))]
+    f.check()
+    f.cache.close()
+
+
+def attend(f, seqs, tokens, heads, layer=0, seed=50, spread=1.0, scale=None, q=None):
+    """Attention of the newest tokens against 64 bits; returns the output."""
+    plan = f.cache.plan(seqs, tokens, heads=heads)
+    t = sum(tokens)
+    q = rand(seed, t, heads, f.dim, dtype=f.dtype, spread=spread) if q is None else q
+    out = torch.full_like(q, 7.0)
+    lse = torch.full((heads, t), 7.0, device="cuda")
+    f.cache.attention_async(plan, q, out, layer, lse, 0.0 if scale is None else scale)
+    got, got_lse, at = f64(out), f64(lse), 0
+    for s, n in zip(seqs, tokens):
+        k, v = (f64(x[layer]) for x in f.held[s])
+        limits = [len(k) - n + i + 1 for i in range(n)]
+        want, tol, l, l_tol = attention(f64(q[at:at + n]), k, v, limits, f.dtype, scale)
+        assert_within(got[at:at + n], want, tol, f"sequence {s}")
+        assert_within(got_lse[:, at:at + n], l, l_tol, f"lse of {s}")
+        at += n
+    return out
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim,page", [(4, 4, 64, 32), (8, 2, 128, 64), (5, 1, 80, 32), (3, 3, 24, 128),
+                                               (40, 2, 96, 32), (12, 4, 40, 64)])
+@pytest.mark.parametrize("new", [1, 5])
+def test_sequences_of_many_lengths(tctx, dtype, heads, kv, dim, page, new):
+    """Lengths from the new tokens alone on, at and around ends of tiles and pages; one sequence with no new token."""
+    lengths = [new, new + 1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 200, 17]
+    f = Filled(tctx, 2, 80, page, kv, dim, dtype, 11)
+    seqs = f.new(len(lengths))
+    f.append(seqs, lengths)
+    tokens = [new] * (len(seqs) - 1) + [0]
+    attend(f, seqs, tokens, heads, layer=1)
+    f.cache.close()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_shared_prefixes(tctx, dtype, new):
+    """A tree of forks: of the whole, in the middle of a page and of a tile, at a page's end, two levels deep, and
+    sequences of their own beside it, in an order that mixes them."""
+    f = Filled(tctx, 1, 200, 32, 2, 64, dtype, 13)
+    (root,) = f.new()
+    f.append([root], [203])
+    first = f.fork(root, 4) + f.fork(root, 2, 100) + f.fork(root, 2, 96) + f.fork(root, 1, 1)
+    f.append(first, [new, new + 3, 70, new, new, 45, new, 90, new])
+    second = f.fork(first[2], 3) + f.fork(first[7], 2, 100)
+    f.append(second, [new, new + 1, 33 + new, new, new + 64])
+    alone = f.new(2)
+    f.append(alone, [new, 400])
+    seqs = [second[1], alone[0], first[3], first[0], second[4], first[8], alone[1], first[5], second[0], first[1],
+            second[3], first[6], first[4], second[2]]
+    attend(f, seqs, [new] * len(seqs), 8)
+    attend(f, seqs, [1 + i % new for i in range(len(seqs))], 8)
+    # Forks that have nothing of their own: equal page lists, one a prefix of the other, a page's part.
+    same = f.fork(root, 3) + f.fork(root, 1, 64) + f.fork(root, 2, 50)
+    attend(f, [root] + same, [min(new, 50)] * 7, 8)
+    f.check()
+    f.cache.close()
+
+
+@pytest.mark.parametrize("dtype,heads", [("fp16", 8), ("bf16", 64)])
+def test_long_prefix_split_over_workgroups(tctx, dtype, heads):
+    """Thousands of keys for few rows: parts of a row joined, some of them empty for the rows of earlier tokens."""
+    f = Filled(tctx, 1, 400, 64, 4, 64, dtype, 17)
+    (root,) = f.new()
+    f.append([root], [9001])
+    seqs = f.fork(root, 3)
+    f.append(seqs, [1, 700, 65])
+    attend(f, seqs, [1, 1, 1], heads)
+    attend(f, seqs, [1, 3, 2], heads, spread=6.0)
+    f.cache.close()
+
+
+def test_scores_of_any_size(tctx):
+    for spread in (1e-3, 8.0, 40.0):
+        f = Filled(tctx, 1, 40, 32, 2, 64, "bf16", 19)
+        seqs = f.new(3)
+        f.append(seqs, [1, 300, 77], make=lambda s, *shape: rand(s, *shape, dtype="bf16", spread=spread))
+        attend(f, seqs, [1, 2, 3], 4, spread=spread)
+        attend(f, seqs, [1, 2, 3], 4, spread=spread, scale=0.3)
+        f.cache.close()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_what_pages_held_before(tctx, dtype):
+    """Pages full of NaN and infinities from sequences that ended do not reach later ones, whose last pages they fill up."""
+    f = Filled(tctx, 1, 24, 64, 2, 80, dtype, 23)
+    for fill in (float("nan"), float("inf"), -float("inf")):
+        (s,) = f.new()
+        f.append([s], [24 * 64], make=lambda seed, *shape: torch.full(shape, fill, dtype=TORCH[dtype], device="cuda"))
+        f.free([s])
+        seqs = f.new(5)
+        f.append(seqs, [1, 33, 64, 70, 100])
+        out = attend(f, seqs, [1] * 5, 4)
+        assert torch.isfinite(out.float()).all()
+        out = attend(f, seqs, [1, 33, 5, 7, 40], 4)
+        assert torch.isfinite(out.float()).all()
+        kids = f.fork(seqs[4], 2, 90)  # the page's rest is the parent's
+        attend(f, kids + [seqs[4]], [2, 1, 1], 4)
+        f.append(kids, [1, 3])
+        attend(f, kids + [seqs[4]], [2, 4, 1], 4)
+        f.check()
+        f.free(seqs + kids)
+    f.cache.close()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan"), "lowest"])
+def test_values_in_keys_not_seen(tctx, dtype, value):
+    """Tokens before a key do not see it: the same bits whatever it holds; the tokens after it see what it holds."""
+    x = torch.finfo(TORCH[dtype]).min if value == "lowest" else value
+    got = {}
+    for at in (70, 80, 95, 96, 108):  # of 110 tokens, the last 40 of them new
+        for fill in (0.0, x):
+            def make(seed, *shape):
+                t = rand(seed, *shape, dtype=dtype)
+                t[:, at] = fill
+                return t
+            f = Filled(tctx, 1, 8, 32, 2, 64, dtype, 29)
+            (s,) = f.new()
+            f.append([s], [110], make=make)
+            plan = f.cache.plan([s], [40], heads=4)
+            q, out = rand(3, 40, 4, 64, dtype=dtype), torch.zeros(40, 4, 64, dtype=TORCH[dtype], device="cuda")
+            f.cache.attention_async(plan, q, out)
+            got[fill] = out[:at - 70].clone()
+            f.cache.close()
+        assert torch.equal(bits(got[0.0]), bits(got[x])), at
+        assert torch.isfinite(got[x].float()).all()
+    if value == "lowest":
+        return
+
+    def one_value(seed, *shape):
+        t = rand(seed, *shape, dtype=dtype)
+        if seed % 2 == 0:  # Filled.append makes the values with the even seed after the keys' odd one
+            t[:, 90, :, 3] = x
+        return t
+
+    f = Filled(tctx, 1, 8, 32, 2, 64, dtype, 29)
+    (s,) = f.new()
+    f.append([s], [110], make=one_value)
+    out = torch.zeros(40, 4, 64, dtype=TORCH[dtype], device="cuda")
+    f.cache.attention_async(f.cache.plan([s], [40], heads=4), rand(3, 40, 4, 64, dtype=dtype), out)
+    seen = out[20:, :, 3].float()
+    assert torch.isnan(seen).all() if x != x else (seen == x).all()
+    assert torch.isfinite(out[:20].float()).all() and torch.isfinite(out[..., 4:].float()).all()
+    f.cache.close()
+
+
+def test_layers_past_4_gib(tctx):
+    """Pages whose offsets pass 32 bits, in every kernel: written, copied, read and attended to."""
+    page, kv, dim = 4096, 8, 128
+    f = Filled(tctx, 2, 320, page, kv, dim, "bf16", 31)  # 16 MiB a page, 5 GiB a layer
+    (low,) = f.new()
+    f.cache.extend([low], [318 * page])
+    (s,) = f.new()
+    f.append([s], [100])
+    assert f.cache.pages([s]).tolist() == [318]
+    del f.held[low]
+    (kid,) = f.fork(s, 1)
+    f.append([kid], [40])
+    assert f.cache.pages([kid]).tolist() == [319]
+    attend(f, [s, kid], [1, 2], 16, layer=1)
+    f.check()
+    f.cache.free([low])
+    assert f.cache.compact() == 2
+    assert f.cache.pages([s, kid]).tolist() == [0, 1]
+    f.check()
+    attend(f, [s, kid], [1, 2], 16, layer=0)
+    f.cache.close()
+
+
+def test_same_bits_again(tctx):
+    f = Filled(tctx, 1, 200, 64, 2, 128, "bf16", 37)
+    (root,) = f.new()
+    f.append([root], [5000])
+    seqs = f.fork(root, 5)
+    f.append(seqs, [1, 20, 300, 4, 90])
+    q = rand(3, 5, 16, 128, dtype="bf16")
+    outs = [attend(f, seqs, [1] * 5, 16, q=q) for _ in range(3)]
+    assert all(torch.equal(bits(outs[0]), bits(o)) for o in outs)
+    f.cache.close()
+
+
+def test_refusals(tctx, cvs):
+    for bad, match in (((0, 4, 32, 2, 64), "at least one"), ((1, 0, 32, 2, 64), "at least one"),
+                       ((1, 4, 48, 2, 64), "power of two"), ((1, 4, 16, 2, 64), "power of two"),
+                       ((1, 4, 32, 2, 60), "multiple of 8"), ((1, 4, 32, 2, 136), "multiple of 8"),
+                       ((1, 4, 4096, 512, 128), "512 MiB")):
+        with pytest.raises(ValueError, match=match):
+            tctx.kv_cache(*bad)
+    with pytest.raises(ValueError, match="attention takes"):
+        tctx.kv_cache(1, 4, 32, 2, 64, "float32")
+    with pytest.raises(RuntimeError):
+        tctx.kv_cache(4096, 1 << 20, 4096, 8, 128)
+    f = Filled(tctx, 2, 6, 32, 2, 64, "fp16", 41)
+    c = f.cache
+    a, b = f.new(2)
+    f.append([a, b], [40, 10])
+    for call, match in ((lambda: c.extend([a, a], [1, 1]), "given twice"), (lambda: c.extend([a], [-1]), "cannot grow"),
+                        (lambda: c.extend([99], [1]), "no sequence 99"), (lambda: c.extend([a], [1 << 31]), "grow"),
+                        (lambda: c.fork(a, 1, 41), "fork at 41"), (lambda: c.truncate(a, 41), "truncate to 41"),
+                        (lambda: c.free([a, a]), "given twice"), (lambda: c.free([99]), "no sequence"),
+                        (lambda: c.plan([a], [41]), "has 40 tokens"), (lambda: c.plan([a], [-1]), "tokens"),
+                        (lambda: c.plan([a, a], [1, 1]), "given twice"), (lambda: c.plan([a], [1], heads=3), "multiple"),
+                        (lambda: c.plan([a], [1, 2]), "values are needed")):
+        with pytest.raises(ValueError, match=match):
+            call()
+    with pytest.raises(RuntimeError, match="3 free pages, 4 are needed"):
+        c.extend([a, b], [60, 60])
+    assert c.lengths([a, b]) == [40, 10] and c.free_pages() == 3
+    k = rand(1, 40, 2, 64, dtype="fp16")
+    plan = c.plan([a], [40])
+    for call, match in ((lambda: c.write_async(plan, k[:39], k), "plan's 40 tokens"),
+                        (lambda: c.write_async(plan, k[:, :1], k), "cache's heads"),
+                        (lambda: c.write_async(plan, k.bfloat16(), k), "type"),
+                        (lambda: c.write_async(plan, k, k, layer=2), "layers outside"),
+                        (lambda: c.write_async(plan, k[None].expand(3, -1, -1, -1), k[None].expand(3, -1, -1, -1)),
+                         "layers outside"),
+                        (lambda: c.write_async(plan, k[None], k[None].expand(2, -1, -1, -1)), "same layers"),
+                        (lambda: c.attention_async(plan, k, k.clone()), "without query heads")):
+        with pytest.raises(ValueError, match=match):
+            call()
+    step = c.plan([a, b], [1, 1], heads=4)
+    q = rand(2, 2, 4, 64, dtype="fp16")
+    for call, match in ((lambda: c.attention_async(step, q[:1], q), "plan's 2 tokens"),
+                        (lambda: c.attention_async(step, q[:, :2], q), "plan's heads"),
+                        (lambda: c.attention_async(step, q, q.clone(), layer=2), "layer outside"),
+                        (lambda: c.attention_async(step, q, q.clone(), scale=-1.0), "scale")):
+        with pytest.raises(ValueError, match=match):
+            call()
+    (kid,) = f.fork(a, 1)
+    with pytest.raises(ValueError, match="sequences share"):
+        c.write_async(c.plan([kid], [1]), k[:1], k[:1])
+    with pytest.raises(ValueError, match="sequences share"):
+        c.write_async(plan, k, k)
+    c.extend([a], [1])
+    with pytest.raises(ValueError, match="has changed"):
+        c.attention_async(step, q, q.clone())
+    late = c.plan([kid], [1], heads=4)
+    c.free([b, kid])
+    with pytest.raises(ValueError, match="no sequence"):
+        c.attention_async(late, q[:1], q[:1].clone())
+    other = tctx.kv_cache(1, 4, 32, 2, 64, "fp16")
+    with pytest.raises(ValueError, match="another cache"):
+        other.read_async(plan, k, k)
+    lib = cvs.load()
+    assert lib.cvs_kv_cache_destroy(c.handle) == cvs.CVS_ERR_INVALID_ARGUMENT
+    assert b"plan(s)" in lib.cvs_last_error()
+    other.close()
+    c.close()
+    assert plan.handle is None and c.handle is None
