@@ -98,6 +98,7 @@ __global__ __launch_bounds__(256, 2) void cached_attn_kernel(const CachedArgs a)
 
   RowState<NB> st;
   st.init();
+  uint32_t bad = 0;
   if (wave < it.tiles) {
     const char* p = tile_at(wave);
     load_keys(p);
@@ -106,7 +107,6 @@ __global__ __launch_bounds__(256, 2) void cached_attn_kernel(const CachedArgs a)
       f32x16 s[1] = {f32x16{}};
 #pragma unroll
       for (int k = 0; k < 2 * NB; ++k) s[0] = mfma<kBf>(kf[k], q[k], s[0]);
-      const char* const cur = p;
       p = tile_at(i + kWaves < it.tiles ? i + kWaves : i);
       load_keys(p);
       const int key0 = it.key0 + kTile * (it.tile0 + i);
@@ -117,7 +117,6 @@ __global__ __launch_bounds__(256, 2) void cached_attn_kernel(const CachedArgs a)
           if (key0 + 8 * (r / 4) + 4 * half + r % 4 >= limit) s[0][r] = -INFINITY;
       }
       softmax_step<NB, 1>(s, st, a.c);
-      uint32_t bad = 0;
       if (mixed) {
         // Past the largest limit the page holds whatever was there: zeros instead.  Infinities and NaNs in keys that
         // some rows see go around the product.
@@ -138,20 +137,13 @@ __global__ __launch_bounds__(256, 2) void cached_attn_kernel(const CachedArgs a)
 #pragma unroll
         for (int b = 0; b < NB; ++b) st.o[b] = mfma<kBf>(vf[2 * b + h], pr, st.o[b]);
       }
-      if (mixed && __ballot(bad != 0)) {
-        const char* const v = cur - lane * 16 + a.head_bytes / 2;
-        add_nonfinite<kBf, NB>(st, s[0], key0, limit, a.dim, [&](int j, int d) CVS_INLINE {
-          const int l = (d & 31) + 32 * ((j >> 2) & 1), e = 4 * ((j >> 3) & 1) + (j & 3);
-          return *reinterpret_cast<const uint16_t*>(v + (2 * (d >> 5) + (j >> 4)) * 1024 + 16 * l + 2 * e);
-        });
-      }
       load_values(p);
     }
   }
 
   // The waves' states joined, in the order 0 + 2, 1 + 3, then both.
   s_m[wave][lane] = st.m;
-  __syncthreads();
+  const bool met = __syncthreads_or(bad != 0);  // infinities or NaNs that some rows do not see
   float m = s_m[0][lane];
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_m[w][lane]);
@@ -180,23 +172,38 @@ __global__ __launch_bounds__(256, 2) void cached_attn_kernel(const CachedArgs a)
   }
   if (wave != 0) return;
   const float l = both_sum((s_l[0][lane] + s_l[2][lane]) + (s_l[1][lane] + s_l[3][lane]));
+  auto value = [&](int key, int d) CVS_INLINE {
+    const int rel = key - it.key0, j = rel & 31, t = rel / kTile;
+    const int64_t page = a.pages[it.page_first + (t >> a.page_shift)];
+    const char* const v = a.pool + page * a.page_bytes + g * a.head_bytes + a.head_bytes / 2 +
+                          (t & page_mask) * (2048 * NB);
+    const int at = (d & 31) + 32 * ((j >> 2) & 1), e = 4 * ((j >> 3) & 1) + (j & 3);
+    return *reinterpret_cast<const uint16_t*>(v + (2 * (d >> 5) + (j >> 4)) * 1024 + 16 * at + 2 * e);
+  };
+  const int first = it.key0 + kTile * it.tile0;
+  const int last = there && l == l ? min(first + kTile * it.tiles, limit) : 0;
   if (a.slots == 0) {
-    store_row<kBf, NB>(st, 1.f / l, reinterpret_cast<uint16_t*>(a.out.p) + q_row * a.out.token + head * a.out.head,
-                       a.dim, there);
+    uint16_t* const out = reinterpret_cast<uint16_t*>(a.out.p) + q_row * a.out.token + head * a.out.head;
+    store_row<kBf, NB>(st, 1.f / l, out, a.dim, there);
+    if (met)
+      store_nonfinite<kBf>(first, last, a.dim, value,
+                           [&](int d, float x) CVS_INLINE { out[d] = uint16_t(pack2<kBf>(x, x)); });
     if (a.lse && there && half == 0)
       a.lse[int64_t(head) * a.q_tokens + q_row] = (m + __builtin_amdgcn_logf(l)) * kLn2;
     return;
   }
-  if (!there) return;
   const int64_t slot = g * a.slots + it.slot0 + col;
-  float* const o = a.part_o + slot * (32 * NB) + 4 * half;
+  float* const o = a.part_o + slot * (32 * NB);
+  if (there) {
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<float4*>(o + 32 * b + 8 * j) =
-          float4{st.o[b][4 * j], st.o[b][4 * j + 1], st.o[b][4 * j + 2], st.o[b][4 * j + 3]};
-  if (half == 0) a.part_ml[slot] = float2{m, l};
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<float4*>(o + 32 * b + 8 * j + 4 * half) =
+            float4{st.o[b][4 * j], st.o[b][4 * j + 1], st.o[b][4 * j + 2], st.o[b][4 * j + 3]};
+    if (half == 0) a.part_ml[slot] = float2{m, l};
+  }
+  if (met) store_nonfinite<kBf>(first, last, a.dim, value, [&](int d, float x) CVS_INLINE { o[d] = x; });
 }
 
 struct JoinArgs {

@@ -153,34 +153,6 @@ __device__ CVS_INLINE u32x4 prob_operand(const f32x16& p, int step) {
   return r;
 }
 
-// Adds what `clean` took out of a tile's values for the rows that do see
-// them: 32 keys from `key0`, seen by a lane's row below `limit`.  value(j, d)
-// is element d of key key0 + j.  Only for tiles with infinities or NaNs in
-// keys that some row of the wave does not see: there 0 * inf in the matrix
-// product would reach rows the key is masked from.
-template <bool kBf, int NB, typename Value>
-__device__ CVS_INLINE void add_nonfinite(RowState<NB>& st, const f32x16& p, int key0, int limit, int dim,
-                                         const Value& value) {
-  const int half = __lane_id() >> 5;
-#pragma unroll 1
-  for (int j = 0; j < 32; ++j) {
-    const int reg = 4 * (j / 8) + j % 4;
-    float own = 0.f;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) own = r == reg ? p[r] : own;
-    const float other = xor_lanes_f(own, 32);
-    const float pj = half == ((j >> 2) & 1) ? own : other;
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int d = 32 * b + 8 * (r / 4) + 4 * half + r % 4;
-        const uint16_t x = d < dim ? value(j, d) : uint16_t(0);
-        if (nonfinite<kBf>(x) != 0 && key0 + j < limit) st.o[b][r] += pj * to_float<kBf>(x);
-      }
-  }
-}
-
 // Writes a lane's half of a row's 32 NB outputs, scaled.  Lanes l and l + 32
 // hold alternate groups of 4 elements; the pair exchanges them so that each
 // stores 16 bytes at a time.
@@ -203,6 +175,28 @@ __device__ CVS_INLINE void store_row(const RowState<NB>& st, float scale, uint16
       const int d = 32 * b + 8 * (j + half);
       if (there && d < dim) *reinterpret_cast<u32x4*>(out + d) = u32x4{x[0], y[0], x[1], y[1]};
     }
+}
+
+// Puts right the outputs of a wave whose values had infinities or NaNs in keys
+// that some of its rows do not see (`clean` took them out of the product: 0 *
+// inf there would reach those rows), after its rows have been stored: an
+// infinity or NaN of any positive weight is its element's result, so the
+// weights are not needed.  value(j, d) is element d of key j, a lane's row
+// sees keys [first, last), store(d, x) writes its element d.  Such a wave
+// reads its values again, one element at a time; no other wave comes here.
+template <bool kBf, typename Value, typename Store>
+__device__ CVS_INLINE void store_nonfinite(int first, int last, int dim, const Value& value, const Store& store) {
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the rows' stores come first
+#pragma unroll 1
+  for (int d = __lane_id() >> 5; d < dim; d += 2) {
+    float sum = 0.f;
+#pragma unroll 1
+    for (int j = first; j < last; ++j) {
+      const uint16_t x = value(j, d);
+      if (nonfinite<kBf>(x) != 0) sum += to_float<kBf>(x);
+    }
+    if (sum != 0.f) store(d, sum);
+  }
 }
 
 // A heads view as the kernels take it: strides in elements.

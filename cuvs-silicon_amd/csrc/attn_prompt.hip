@@ -19,6 +19,7 @@
 // read (ds_read_b64_tr_b16).  The permutation costs nothing: each lane of a
 // load picks the piece that belongs at its place.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_common.hpp"
 
@@ -125,6 +126,7 @@ __global__ __launch_bounds__(256, 2) void prompt_attn_kernel(const PromptArgs a)
 
   RowState<NB> st;
   st.init();
+  uint32_t bad = 0;
   const int tiles = (wg_max + kKeys - 1) / kKeys;
   if (tiles > 0) load_tile(0, 0);
   for (int t = 0; t < tiles; ++t) {
@@ -159,33 +161,32 @@ __global__ __launch_bounds__(256, 2) void prompt_attn_kernel(const PromptArgs a)
       const u32x2_t x = __builtin_bit_cast(u32x2_t, lo), y = __builtin_bit_cast(u32x2_t, hi);
       return u32x4{x[0], x[1], y[0], y[1]};
     };
-    uint32_t bad = 0;
+    auto add_values = [&](auto masked) CVS_INLINE {
 #pragma unroll
-    for (int k16 = 0; k16 < 4; ++k16) {
-      const u32x4 p = prob_operand<kBf>(s[k16 / 2], k16 % 2);
+      for (int k16 = 0; k16 < 4; ++k16) {
+        const u32x4 p = prob_operand<kBf>(s[k16 / 2], k16 % 2);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        u32x4 v = value_operand(b, k16);
-        if (mixed) v = clean<kBf>(v, bad);
-        st.o[b] = mfma<kBf>(v, p, st.o[b]);
+        for (int b = 0; b < NB; ++b) {
+          u32x4 v = value_operand(b, k16);
+          if constexpr (masked) v = clean<kBf>(v, bad);
+          st.o[b] = mfma<kBf>(v, p, st.o[b]);
+        }
       }
-    }
-    if (mixed && __ballot(bad != 0)) {
-#pragma unroll 1
-      for (int u = 0; u < 2; ++u)
-        add_nonfinite<kBf, NB>(st, u ? s[1] : s[0], key0 + 32 * u, limit, a.dim, [&](int j, int d) CVS_INLINE {
-          const int r = 32 * u + j, piece = d >> 3;
-          const int place = P == 16 ? piece ^ 4 * (r & 3) : piece ^ 4 * ((r >> 1) & 1);
-          return *reinterpret_cast<const uint16_t*>(s_v[buf] + r * kPitch + 16 * place + 2 * (d & 7));
-        });
-    }
+    };
+    if (mixed) add_values(std::true_type{});
+    else add_values(std::false_type{});
   }
   if (!busy) return;
   const float l = both_sum(st.l);
   // A row that sees no key gives zeros; one whose keys' weights are all 0 (or NaN) gives what the formula does.
   const float inv = limit > 0 ? 1.f / l : 0.f;
-  store_row<kBf, NB>(st, inv, reinterpret_cast<uint16_t*>(a.out.p) + (it.q0 + tok) * a.out.token + head * a.out.head,
-                     a.dim, there);
+  uint16_t* const out = reinterpret_cast<uint16_t*>(a.out.p) + (it.q0 + tok) * a.out.token + head * a.out.head;
+  store_row<kBf, NB>(st, inv, out, a.dim, there);
+  if (__ballot(bad != 0))
+    store_nonfinite<kBf>(
+        0, there && l == l ? limit : 0, a.dim,
+        [&](int j, int d) CVS_INLINE { return reinterpret_cast<const uint16_t*>(base_v)[j * a.v.token + d]; },
+        [&](int d, float x) CVS_INLINE { out[d] = uint16_t(pack2<kBf>(x, x)); });
   if (a.lse && there && half == 0)
     a.lse[int64_t(head) * a.q_tokens + it.q0 + tok] = limit > 0 ? (st.m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
 }
