@@ -109,9 +109,13 @@ __device__ CVS_INLINE float both_max(float x) { return fmaxf(x, xor_lanes_f(x, 3
 __device__ CVS_INLINE float both_sum(float x) { return x + xor_lanes_f(x, 32); }
 
 // Scores of NT 32-key tiles -> probabilities 2^(c s - m), with the state
-// rescaled to the new maximum.  Masked scores come in as -inf and leave as 0.
-// While a row has seen nothing its maximum is -inf; 0 stands in for it then,
-// so that -inf - (-inf) does not arise.
+// rescaled where a row's maximum has grown.  m trails the true maximum by up
+// to kSlack: the values then need rescaling in a row's first tiles only, and
+// probabilities stay below 2^kSlack, which costs no precision in either type.
+// Masked scores come in as -inf and leave as 0.  While a row has seen nothing
+// its maximum is -inf; 0 stands in for it then, so that -inf - (-inf) does
+// not arise.
+constexpr float kSlack = 6.f;
 template <int NB, int NT>
 __device__ CVS_INLINE void softmax_step(f32x16 (&s)[NT], RowState<NB>& st, float c) {
   float top = s[0][0];
@@ -119,10 +123,10 @@ __device__ CVS_INLINE void softmax_step(f32x16 (&s)[NT], RowState<NB>& st, float
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
-  const float m = fmaxf(st.m, both_max(top) * c);
-  const float base = m == -INFINITY ? 0.f : m;
-  if (__ballot(m != st.m)) {
-    const float alpha = __builtin_amdgcn_exp2f(st.m - base);
+  top = both_max(top) * c;
+  if (__ballot(top > st.m + kSlack)) {
+    const float m = fmaxf(st.m, top);
+    const float alpha = __builtin_amdgcn_exp2f(st.m - (m == -INFINITY ? 0.f : m));
     st.l *= alpha;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -130,6 +134,7 @@ __device__ CVS_INLINE void softmax_step(f32x16 (&s)[NT], RowState<NB>& st, float
       for (int r = 0; r < 16; ++r) st.o[b][r] *= alpha;
     st.m = m;
   }
+  const float base = st.m == -INFINITY ? 0.f : st.m;
   float sum = 0.f;
 #pragma unroll
   for (int t = 0; t < NT; ++t)

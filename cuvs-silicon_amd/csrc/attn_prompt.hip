@@ -82,79 +82,87 @@ __global__ __launch_bounds__(256, 2) void prompt_attn_kernel(const PromptArgs a)
       q[s] = 16 * s + 8 * half < a.dim ? *reinterpret_cast<const u32x4*>(src + 32 * s + 16 * half) : u32x4{};
   }
 
-  // Loads: LDS place n = 64 i + lane of a wave's share is row n / P, place n % P.
+  // Loads: LDS place n = 64 i + lane of a wave's share is row n / P, place n % P.  Out of range reads zeros: pieces
+  // past the head's end, and rows past the sequence's end in its last tile.
+  constexpr uint32_t kNowhere = 0x80000000u;
   uint32_t off_k[kLoads], off_v[kLoads];
-  int row_of[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
     const int n = (wave * kLoads + i) * 64 + lane, r = n / P, p = n % P;
     const int pk = P == 16 ? p ^ (r & 15) : p ^ ((r >> 1) & 7);
     const int pv = P == 16 ? p ^ 4 * (r & 3) : p ^ 4 * ((r >> 1) & 1);
-    row_of[i] = r;
-    // Out of range reads zeros: pieces past the head's end here, rows past the sequence's end below.
-    off_k[i] = 8 * pk < a.dim ? uint32_t(r * a.k.token * 2 + 16 * pk) : 0x80000000u;
-    off_v[i] = 8 * pv < a.dim ? uint32_t(r * a.v.token * 2 + 16 * pv) : 0x80000000u;
+    off_k[i] = 8 * pk < a.dim ? uint32_t(r * a.k.token * 2 + 16 * pk) : kNowhere;
+    off_v[i] = 8 * pv < a.dim ? uint32_t(r * a.v.token * 2 + 16 * pv) : kNowhere;
+    asm("" : "+v"(off_k[i]), "+v"(off_v[i]));  // kept, not computed again for every tile
   }
-  const char* base_k = a.k.p + 2 * (it.k0 * a.k.token + g * a.k.head);
-  const char* base_v = a.v.p + 2 * (it.k0 * a.v.token + g * a.v.head);
-  auto load_tile = [&](int t, int buf) CVS_INLINE {
-    const rsrc4 rk = make_rsrc(base_k + int64_t(t) * kKeys * a.k.token * 2, 0x7fffffff);
-    const rsrc4 rv = make_rsrc(base_v + int64_t(t) * kKeys * a.v.token * 2, 0x7fffffff);
-    const int left = it.k_len - t * kKeys;
-    const int m0 = wave * kLoads * 1024;
+  const char* const base_v = a.v.p + 2 * (it.k0 * a.v.token + g * a.v.head);
+  const char* next_k = a.k.p + 2 * (it.k0 * a.k.token + g * a.k.head);
+  const char* next_v = base_v;
+  const int64_t step_k = kKeys * a.k.token * 2, step_v = kKeys * a.v.token * 2;
+  const int lds_k = lds_addr(s_k[0]) + wave * kLoads * 1024, lds_v = lds_addr(s_v[0]) + wave * kLoads * 1024;
+  int left = it.k_len;
+  auto load_tile = [&](int buf) CVS_INLINE {
+    const rsrc4 rk = make_rsrc(next_k, 0x7fffffff);
+    const rsrc4 rv = make_rsrc(next_v, 0x7fffffff);
+    if (left >= kKeys) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-      lds_dma<16, false>(rk, lds_addr(s_k[buf]) + m0 + i * 1024, row_of[i] < left ? off_k[i] : 0x80000000u, 0);
+      for (int i = 0; i < kLoads; ++i) lds_dma<16, false>(rk, lds_k + buf * kBuf + i * 1024, off_k[i], 0);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-      lds_dma<16, false>(rv, lds_addr(s_v[buf]) + m0 + i * 1024, row_of[i] < left ? off_v[i] : 0x80000000u, 0);
+      for (int i = 0; i < kLoads; ++i) lds_dma<16, false>(rv, lds_v + buf * kBuf + i * 1024, off_v[i], 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const bool in = ((wave * kLoads + i) * 64 + lane) / P < left;
+        lds_dma<16, false>(rk, lds_k + buf * kBuf + i * 1024, in ? off_k[i] : kNowhere, 0);
+        lds_dma<16, false>(rv, lds_v + buf * kBuf + i * 1024, in ? off_v[i] : kNowhere, 0);
+      }
+    }
+    next_k += step_k;
+    next_v += step_v;
+    left -= kKeys;
   };
 
-  // Operand addresses within a buffer.
-  const int swz_k = P == 16 ? col & 15 : (col >> 1) & 7;
-  int addr_k[2 * NB];
-#pragma unroll
-  for (int s = 0; s < 2 * NB; ++s) addr_k[s] = col * kPitch + 16 * ((2 * s + half) ^ swz_k);
+  // Operand addresses within a buffer.  Column pair 2 s + half of a row is at its place in the row's order, a
+  // permutation by exclusive or: so is the step from one s (or one column block b) to another.
+  const int addr_k = col * kPitch + 16 * (half ^ (P == 16 ? col & 15 : (col >> 1) & 7));
   const int li = lane & 15, vkey = 4 * half + (li >> 2);
-  int addr_v[NB];
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    const int piece = 4 * b + 2 * ((lane >> 4) & 1) + ((li & 3) >> 1);
-    const int place = P == 16 ? piece ^ 4 * (vkey & 3) : piece ^ 4 * ((vkey >> 1) & 1);
-    addr_v[b] = vkey * kPitch + 16 * place + 8 * (li & 1);
-  }
+  const int v_piece = (2 * ((lane >> 4) & 1) + ((li & 3) >> 1)) ^ (P == 16 ? 4 * (vkey & 3) : 4 * ((vkey >> 1) & 1));
+  const int addr_v = vkey * kPitch + 16 * v_piece + 8 * (li & 1);
 
   RowState<NB> st;
   st.init();
   uint32_t bad = 0;
   const int tiles = (wg_max + kKeys - 1) / kKeys;
-  if (tiles > 0) load_tile(0, 0);
+  if (tiles > 0) load_tile(0);
   for (int t = 0; t < tiles; ++t) {
     const int buf = t & 1;
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part of tile t is in LDS
     __syncthreads();                     // everyone's is, and everyone is done with the other buffer
-    if (t + 1 < tiles) load_tile(t + 1, buf ^ 1);
+    if (t + 1 < tiles) load_tile(buf ^ 1);
     const int key0 = t * kKeys;
     if (key0 >= wave_max) continue;
-    f32x16 s[2] = {f32x16{}, f32x16{}};
+    f32x16 s[2];
+    const int at_k = addr_k + buf * kBuf, at_v = addr_v + buf * kBuf;
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i)
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        s[u] = mfma<kBf>(*reinterpret_cast<const u32x4*>(s_k[buf] + addr_k[i] + u * 32 * kPitch), q[i], s[u]);
+        s[u] = mfma<kBf>(*reinterpret_cast<const u32x4*>(s_k[0] + (at_k ^ 32 * i) + u * 32 * kPitch), q[i],
+                         i ? s[u] : f32x16{});
     const bool mixed = key0 + kKeys > wave_min;
     if (mixed) {
+      const int seen = limit - key0 - 4 * half;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (key0 + 32 * u + 8 * (r / 4) + 4 * half + r % 4 >= limit) s[u][r] = -INFINITY;
+          if (32 * u + 8 * (r / 4) + r % 4 >= seen) s[u][r] = -INFINITY;
     }
     softmax_step<NB, 2>(s, st, a.c);
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     auto value_operand = [&](int b, int k16) CVS_INLINE {
       typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-      char* p = s_v[buf] + addr_v[b] + k16 * 16 * kPitch;
+      char* p = s_v[0] + (at_v ^ 64 * b) + k16 * 16 * kPitch;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 8 * kPitch));
       typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
