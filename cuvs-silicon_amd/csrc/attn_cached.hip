@@ -104,9 +104,9 @@ __global__ __launch_bounds__(256, 2) void cached_attn_kernel(const CachedArgs a)
     load_keys(p);
     load_values(p);
     for (int i = wave; i < it.tiles; i += kWaves) {
-      f32x16 s[1] = {f32x16{}};
+      f32x16 s{};
 #pragma unroll
-      for (int k = 0; k < 2 * NB; ++k) s[0] = mfma<kBf>(kf[k], q[k], s[0]);
+      for (int k = 0; k < 2 * NB; ++k) s = mfma<kBf>(kf[k], q[k], s);
       p = tile_at(i + kWaves < it.tiles ? i + kWaves : i);
       load_keys(p);
       const int key0 = it.key0 + kTile * (it.tile0 + i);
@@ -114,9 +114,10 @@ __global__ __launch_bounds__(256, 2) void cached_attn_kernel(const CachedArgs a)
       if (mixed) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (key0 + 8 * (r / 4) + 4 * half + r % 4 >= limit) s[0][r] = -INFINITY;
+          if (key0 + 8 * (r / 4) + 4 * half + r % 4 >= limit) s[r] = -INFINITY;
       }
-      softmax_step<NB, 1>(s, st, a.c);
+      raise_max(s, st, a.c);
+      exponentials(s, st, a.c);
       if (mixed) {
         // Past the largest limit the page holds whatever was there: zeros instead.  Infinities and NaNs in keys that
         // some rows see go around the product.
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(256, 2) void cached_attn_kernel(const CachedArgs a)
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const u32x4 pr = prob_operand<kBf>(s[0], h);
+        const u32x4 pr = prob_operand<kBf>(s, h);
 #pragma unroll
         for (int b = 0; b < NB; ++b) st.o[b] = mfma<kBf>(vf[2 * b + h], pr, st.o[b]);
       }

@@ -108,24 +108,23 @@ struct RowState {
 __device__ CVS_INLINE float both_max(float x) { return fmaxf(x, xor_lanes_f(x, 32)); }
 __device__ CVS_INLINE float both_sum(float x) { return x + xor_lanes_f(x, 32); }
 
-// Scores of NT 32-key tiles -> probabilities 2^(c s - m), with the state
-// rescaled where a row's maximum has grown.  m trails the true maximum by up
-// to kSlack: the values then need rescaling in a row's first tiles only, and
+// A row's maximum m trails the largest score seen by up to kSlack (in log2
+// units): its values then need rescaling in its first tiles only, and
 // probabilities stay below 2^kSlack, which costs no precision in either type.
-// Masked scores come in as -inf and leave as 0.  While a row has seen nothing
-// its maximum is -inf; 0 stands in for it then, so that -inf - (-inf) does
-// not arise.
 constexpr float kSlack = 6.f;
-template <int NB, int NT>
-__device__ CVS_INLINE void softmax_step(f32x16 (&s)[NT], RowState<NB>& st, float c) {
-  float top = s[0][0];
+
+// Rescales the rows whose maximum a tile of scores passes by more than that.
+// A row that has seen nothing has maximum -inf; 0 stands in for it, so that
+// -inf - (-inf) does not arise.
+template <int NB>
+__device__ CVS_INLINE void raise_max(const f32x16& s, RowState<NB>& st, float c) {
+  float top = fmaxf(s[0], s[1]);
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
+  for (int r = 2; r < 16; ++r) top = fmaxf(top, s[r]);
   top = both_max(top) * c;
-  if (__ballot(top > st.m + kSlack)) {
-    const float m = fmaxf(st.m, top);
+  const bool passed = top > st.m + kSlack;
+  if (__ballot(passed)) {
+    const float m = passed ? top : st.m;  // the other rows as they are: a row's result does not depend on them
     const float alpha = __builtin_amdgcn_exp2f(st.m - (m == -INFINITY ? 0.f : m));
     st.l *= alpha;
 #pragma unroll
@@ -134,16 +133,20 @@ __device__ CVS_INLINE void softmax_step(f32x16 (&s)[NT], RowState<NB>& st, float
       for (int r = 0; r < 16; ++r) st.o[b][r] *= alpha;
     st.m = m;
   }
+}
+
+// Scores -> probabilities 2^(c s - m), summed up.  Masked scores come in as
+// -inf and leave as 0.
+template <int NB>
+__device__ CVS_INLINE void exponentials(f32x16& s, RowState<NB>& st, float c) {
   const float base = st.m == -INFINITY ? 0.f : st.m;
-  float sum = 0.f;
+  float sum[2] = {0.f, 0.f};
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], c, -base));
-      sum += s[t][r];
-    }
-  st.l += sum;
+  for (int r = 0; r < 16; ++r) {
+    s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -base));
+    sum[r & 1] += s[r];
+  }
+  st.l += sum[0] + sum[1];
 }
 
 // B operand of the 16 keys `step` (0 or 1) of a probability tile.  The

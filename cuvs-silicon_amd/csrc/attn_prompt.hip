@@ -70,9 +70,8 @@ __global__ __launch_bounds__(256, 2) void prompt_attn_kernel(const PromptArgs a)
   };
   const int limit = limit_of(tok);
   const bool busy = it.row0 + 32 * wave < rows;
-  const int wave_min = __builtin_amdgcn_readfirstlane(limit);
-  const int wave_max = busy ? __builtin_amdgcn_readlane(limit, 31) : 0;
-  const int wg_max = limit_of((min(it.row0 + kRows, rows) - 1) / a.group);
+  // Limits grow with the row, so the first and last row bound the workgroup's.
+  const int wg_min = limit_of(it.row0 / a.group), wg_max = limit_of((min(it.row0 + kRows, rows) - 1) / a.group);
 
   u32x4 q[2 * NB];
   {
@@ -95,31 +94,22 @@ __global__ __launch_bounds__(256, 2) void prompt_attn_kernel(const PromptArgs a)
     off_v[i] = 8 * pv < a.dim ? uint32_t(r * a.v.token * 2 + 16 * pv) : kNowhere;
     asm("" : "+v"(off_k[i]), "+v"(off_v[i]));  // kept, not computed again for every tile
   }
+  const char* const base_k = a.k.p + 2 * (it.k0 * a.k.token + g * a.k.head);
   const char* const base_v = a.v.p + 2 * (it.k0 * a.v.token + g * a.v.head);
-  const char* next_k = a.k.p + 2 * (it.k0 * a.k.token + g * a.k.head);
-  const char* next_v = base_v;
   const int64_t step_k = kKeys * a.k.token * 2, step_v = kKeys * a.v.token * 2;
   const int lds_k = lds_addr(s_k[0]) + wave * kLoads * 1024, lds_v = lds_addr(s_v[0]) + wave * kLoads * 1024;
-  int left = it.k_len;
-  auto load_tile = [&](int buf) CVS_INLINE {
-    const rsrc4 rk = make_rsrc(next_k, 0x7fffffff);
-    const rsrc4 rv = make_rsrc(next_v, 0x7fffffff);
+  auto load_tile = [&](const char* base, int64_t step, int lds, const uint32_t(&off)[kLoads], int t) CVS_INLINE {
+    const rsrc4 rs = make_rsrc(base + t * step, 0x7fffffff);
+    const int left = it.k_len - t * kKeys;
+    lds += (t & 1) * kBuf;
     if (left >= kKeys) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) lds_dma<16, false>(rk, lds_k + buf * kBuf + i * 1024, off_k[i], 0);
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) lds_dma<16, false>(rv, lds_v + buf * kBuf + i * 1024, off_v[i], 0);
+      for (int i = 0; i < kLoads; ++i) lds_dma<16, false>(rs, lds + i * 1024, off[i], 0);
     } else {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const bool in = ((wave * kLoads + i) * 64 + lane) / P < left;
-        lds_dma<16, false>(rk, lds_k + buf * kBuf + i * 1024, in ? off_k[i] : kNowhere, 0);
-        lds_dma<16, false>(rv, lds_v + buf * kBuf + i * 1024, in ? off_v[i] : kNowhere, 0);
-      }
+      for (int i = 0; i < kLoads; ++i)
+        lds_dma<16, false>(rs, lds + i * 1024, ((wave * kLoads + i) * 64 + lane) / P < left ? off[i] : kNowhere, 0);
     }
-    next_k += step_k;
-    next_v += step_v;
-    left -= kKeys;
   };
 
   // Operand addresses within a buffer.  Column pair 2 s + half of a row is at its place in the row's order, a
@@ -132,57 +122,76 @@ __global__ __launch_bounds__(256, 2) void prompt_attn_kernel(const PromptArgs a)
   RowState<NB> st;
   st.init();
   uint32_t bad = 0;
-  const int tiles = (wg_max + kKeys - 1) / kKeys;
-  if (tiles > 0) load_tile(0);
-  for (int t = 0; t < tiles; ++t) {
-    const int buf = t & 1;
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part of tile t is in LDS
-    __syncthreads();                     // everyone's is, and everyone is done with the other buffer
-    if (t + 1 < tiles) load_tile(buf ^ 1);
-    const int key0 = t * kKeys;
-    if (key0 >= wave_max) continue;
-    f32x16 s[2];
-    const int at_k = addr_k + buf * kBuf, at_v = addr_v + buf * kBuf;
+  f32x16 s[2];   // scores of a tile's two halves
+  u32x4 p[2][2];  // and their probabilities
+  auto scores = [&](int t, int h) CVS_INLINE {
+    const char* const at = s_k[0] + (t & 1) * kBuf + h * 32 * kPitch;
+    f32x16 x{};
 #pragma unroll
-    for (int i = 0; i < 2 * NB; ++i)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        s[u] = mfma<kBf>(*reinterpret_cast<const u32x4*>(s_k[0] + (at_k ^ 32 * i) + u * 32 * kPitch), q[i],
-                         i ? s[u] : f32x16{});
-    const bool mixed = key0 + kKeys > wave_min;
-    if (mixed) {
-      const int seen = limit - key0 - 4 * half;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (32 * u + 8 * (r / 4) + r % 4 >= seen) s[u][r] = -INFINITY;
-    }
-    softmax_step<NB, 2>(s, st, a.c);
+    for (int i = 0; i < 2 * NB; ++i) x = mfma<kBf>(*reinterpret_cast<const u32x4*>(at + (addr_k ^ 32 * i)), q[i], x);
+    return x;
+  };
+  auto add_values = [&](int t, int h, auto masked) CVS_INLINE {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
-    auto value_operand = [&](int b, int k16) CVS_INLINE {
-      typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-      char* p = s_v[0] + (at_v ^ 64 * b) + k16 * 16 * kPitch;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 8 * kPitch));
-      typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
-      const u32x2_t x = __builtin_bit_cast(u32x2_t, lo), y = __builtin_bit_cast(u32x2_t, hi);
-      return u32x4{x[0], x[1], y[0], y[1]};
-    };
-    auto add_values = [&](auto masked) CVS_INLINE {
+    typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+    char* const at = s_v[0] + (t & 1) * kBuf + h * 32 * kPitch;
 #pragma unroll
-      for (int k16 = 0; k16 < 4; ++k16) {
-        const u32x4 p = prob_operand<kBf>(s[k16 / 2], k16 % 2);
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          u32x4 v = value_operand(b, k16);
-          if constexpr (masked) v = clean<kBf>(v, bad);
-          st.o[b] = mfma<kBf>(v, p, st.o[b]);
-        }
+      for (int b = 0; b < NB; ++b) {
+        char* const from = at + (addr_v ^ 64 * b) + k * 16 * kPitch;
+        const auto x = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)from));
+        const auto y =
+            __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(from + 8 * kPitch)));
+        u32x4 v{x[0], x[1], y[0], y[1]};
+        if constexpr (masked) v = clean<kBf>(v, bad);
+        st.o[b] = mfma<kBf>(v, p[h][k], st.o[b]);
       }
-    };
-    if (mixed) add_values(std::true_type{});
-    else add_values(std::false_type{});
+  };
+  auto mask = [&](int t, int h) CVS_INLINE {
+    const int seen = limit - t * kKeys - 32 * h - 4 * half;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (8 * (r / 4) + r % 4 >= seen) s[h][r] = -INFINITY;
+  };
+  auto probabilities = [&](int h) CVS_INLINE {
+    exponentials(s[h], st, a.c);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) p[h][k] = prob_operand<kBf>(s[h], k);
+  };
+
+  // Half tiles in a pipeline of three: the products of one with the values and of the next with the keys run while
+  // the one between goes through its exponentials.  In the middle of tile t everyone is done with its keys and with
+  // the values before it; what was asked for one tile ago, the next keys and its values, has to be there.
+  const int tiles = (wg_max + kKeys - 1) / kKeys, open_tiles = wg_min / kKeys;  // no row is masked in the open ones
+  auto step = [&](int t, auto masked) CVS_INLINE {
+    if (t > 0) add_values(t - 1, 1, masked);
+    if constexpr (masked) mask(t, 0);
+    raise_max(s[0], st, a.c);
+    s[1] = scores(t, 1);
+    probabilities(0);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    __syncthreads();
+    if (t + 2 < tiles) load_tile(base_k, step_k, lds_k, off_k, t + 2);
+    if (t + 1 < tiles) load_tile(base_v, step_v, lds_v, off_v, t + 1);
+    add_values(t, 0, masked);
+    if constexpr (masked) mask(t, 1);
+    raise_max(s[1], st, a.c);
+    s[0] = scores(t + 1, 0);  // past the last tile: of whatever is there, and not used
+    probabilities(1);
+  };
+  if (tiles > 0) {
+    load_tile(base_k, step_k, lds_k, off_k, 0);
+    load_tile(base_v, step_v, lds_v, off_v, 0);
+    if (tiles > 1) load_tile(base_k, step_k, lds_k, off_k, 1);
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    __syncthreads();
+    s[0] = scores(0, 0);
+    int t = 0;
+    for (; t < open_tiles; ++t) step(t, std::false_type{});
+    for (; t < tiles; ++t) step(t, std::true_type{});
+    add_values(tiles - 1, 1, std::true_type{});
   }
   if (!busy) return;
   const float l = both_sum(st.l);
