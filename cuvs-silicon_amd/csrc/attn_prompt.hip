@@ -45,9 +45,22 @@ struct PromptArgs {
   float c;
 };
 
+// How the pieces of LDS row r are swapped (piece p stands at place p ^ swap)
+// so that the 64 4-byte banks are read evenly.  Rows of 192 bytes begin 48
+// banks apart, so 4 rows cover all banks and every 4th row is swapped within
+// groups of 4 pieces; rows of 128 and 256 bytes begin at the same banks.
+template <int P>
+__device__ CVS_INLINE int swap_k(int r) {  // a read takes one piece of 16 rows
+  return P == 12 ? (r >> 2) & 3 : P == 8 ? (r >> 1) & 7 : r & 15;
+}
+template <int P>
+__device__ CVS_INLINE int swap_v(int r) {  // a read takes 4 pieces of 4 rows
+  return P == 12 ? 0 : P == 8 ? 4 * ((r >> 1) & 1) : 4 * (r & 3);
+}
+
 template <bool kBf, int NB>
-__global__ __launch_bounds__(256, 2) void prompt_attn_kernel(const PromptArgs a) {
-  constexpr int P = NB <= 2 ? 8 : 16;       // 16-byte pieces of a row in LDS
+__global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 3 ? 3 : 4) void prompt_attn_kernel(const PromptArgs a) {
+  constexpr int P = 4 * NB;                 // 16-byte pieces of a row in LDS
   constexpr int kPitch = 16 * P;
   constexpr int kLoads = kKeys * P / 256;   // loads of a wave, keys or values
   constexpr int kBuf = kKeys * kPitch;
@@ -88,8 +101,7 @@ __global__ __launch_bounds__(256, 2) void prompt_attn_kernel(const PromptArgs a)
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
     const int n = (wave * kLoads + i) * 64 + lane, r = n / P, p = n % P;
-    const int pk = P == 16 ? p ^ (r & 15) : p ^ ((r >> 1) & 7);
-    const int pv = P == 16 ? p ^ 4 * (r & 3) : p ^ 4 * ((r >> 1) & 1);
+    const int pk = p ^ swap_k<P>(r), pv = p ^ swap_v<P>(r);
     off_k[i] = 8 * pk < a.dim ? uint32_t(r * a.k.token * 2 + 16 * pk) : kNowhere;
     off_v[i] = 8 * pv < a.dim ? uint32_t(r * a.v.token * 2 + 16 * pv) : kNowhere;
     asm("" : "+v"(off_k[i]), "+v"(off_v[i]));  // kept, not computed again for every tile
@@ -112,12 +124,14 @@ __global__ __launch_bounds__(256, 2) void prompt_attn_kernel(const PromptArgs a)
     }
   };
 
-  // Operand addresses within a buffer.  Column pair 2 s + half of a row is at its place in the row's order, a
-  // permutation by exclusive or: so is the step from one s (or one column block b) to another.
-  const int addr_k = col * kPitch + 16 * (half ^ (P == 16 ? col & 15 : (col >> 1) & 7));
-  const int li = lane & 15, vkey = 4 * half + (li >> 2);
-  const int v_piece = (2 * ((lane >> 4) & 1) + ((li & 3) >> 1)) ^ (P == 16 ? 4 * (vkey & 3) : 4 * ((vkey >> 1) & 1));
-  const int addr_v = vkey * kPitch + 16 * v_piece + 8 * (li & 1);
+  // Operand addresses within a buffer: of the keys' pieces 2 i + half (i even and odd: the piece order is swapped
+  // within groups of four, or by more where rows are 128 or 256 bytes), of 4 keys of a column group.
+  const int sw = swap_k<P>(col), li = lane & 15, vkey = 4 * half + (li >> 2);
+  const int k_even = col * kPitch + 16 * (half ^ sw), k_odd = col * kPitch + 16 * ((2 + half) ^ sw);
+  auto key_at = [&](int i) CVS_INLINE { return P == 12 ? (i & 1 ? k_odd : k_even) + 64 * (i / 2) : k_even ^ 32 * i; };
+  const int v_first = vkey * kPitch + 8 * (li & 1) +
+                      16 * ((2 * ((lane >> 4) & 1) + ((li & 3) >> 1)) ^ swap_v<P>(vkey));
+  auto value_at = [&](int b) CVS_INLINE { return P == 12 ? v_first + 64 * b : v_first ^ 64 * b; };
 
   RowState<NB> st;
   st.init();
@@ -128,7 +142,7 @@ __global__ __launch_bounds__(256, 2) void prompt_attn_kernel(const PromptArgs a)
     const char* const at = s_k[0] + (t & 1) * kBuf + h * 32 * kPitch;
     f32x16 x{};
 #pragma unroll
-    for (int i = 0; i < 2 * NB; ++i) x = mfma<kBf>(*reinterpret_cast<const u32x4*>(at + (addr_k ^ 32 * i)), q[i], x);
+    for (int i = 0; i < 2 * NB; ++i) x = mfma<kBf>(*reinterpret_cast<const u32x4*>(at + key_at(i)), q[i], x);
     return x;
   };
   auto add_values = [&](int t, int h, auto masked) CVS_INLINE {
@@ -140,7 +154,7 @@ __global__ __launch_bounds__(256, 2) void prompt_attn_kernel(const PromptArgs a)
     for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        char* const from = at + (addr_v ^ 64 * b) + k * 16 * kPitch;
+        char* const from = at + value_at(b) + k * 16 * kPitch;
         const auto x = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)from));
         const auto y =
             __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(from + 8 * kPitch)));
