@@ -3,13 +3,19 @@
 //
 // The plan lays the batch's page lists out as a tree: a run of pages and the
 // sequences that begin with it (kv_pages.hpp).  A run's rows are the (token,
-// head of the group) pairs of all its sequences; its keys are split into
-// chunks, and a workgroup takes 32 of the rows and one chunk.  Its 4 waves
-// take the chunk's 32-key tiles in turn, each with a running softmax of its
-// own, straight from memory into operand registers (the pool's tiles are the
-// operands), and join at the end through LDS.  A row's results from its runs
-// and chunks are (maximum, sum, values) in fp32, which a second kernel joins;
-// where every row has one part the first writes the output itself.
+// head of the group) pairs of all its sequences, taken in blocks; a block's
+// keys are cut into segments, so that every workgroup has about as many tiles
+// of 32 keys to go through.  Two shapes of block:
+//   up to 32 rows (the decoding of a sequence's own tokens, bound by the
+//   reading of the cache): the 4 waves take the segment's tiles in turn, each
+//   with a running softmax of its own, straight from memory into operand
+//   registers (the pool's tiles are the operands), and join through LDS;
+//   33 to 128 rows (many sequences on one prefix, or many new tokens, bound by
+//   the matrix cores as well): each wave has 32 of the rows, and the tiles go
+//   through LDS once for all of them (attend_tiles).
+// A row's results from its runs and segments are (maximum, sum, values) in
+// fp32, which a second kernel joins; where every row has one part the first
+// writes the output itself.
 #include <algorithm>
 #include <cstring>
 
@@ -19,30 +25,31 @@ namespace cvs {
 namespace attn {
 namespace {
 
-constexpr int kTile = 32;     // rows and keys of a tile
+constexpr int kTile = 32;       // keys of a tile, rows of a wave
 constexpr int kWaves = 4;
+constexpr int kBlock = kTile * kWaves;  // rows of a large block
+constexpr int kJoin = 8;        // parts of a row read at a time
 
-struct Item {
+struct Segment {
   int32_t page_first;     // first of the run's pages in the plan's page list
-  int32_t tile0, tiles;   // the chunk's tiles, counted from the run's first token
+  int32_t tile0, tiles;   // the segment's tiles, counted from the run's first token
   int32_t key0;           // position in the sequence of the run's first token
   int32_t row0, rows;     // (token * group + head) rows, tokens in the plan's order
   int32_t slot0;          // of row0's partial result
   int32_t min_limit, max_limit;  // keys the rows see: positions below their limit
 };
 
-// A run of pages as the join sees it.
-struct Run {
-  int32_t parent;         // the run before it in its sequences, -1 for none
-  int32_t slot0, chunks;  // chunk c of row row0 + i has slot slot0 + c * rows + i
-  int32_t row0, rows;
+// The parts that a run gives the rows of one of its sequences: part p of row r
+// has slot slot0 + p * rows + r.
+struct Parts {
+  int32_t slot0, rows, count;
 };
 
 struct CachedArgs {
   const char* pool;  // of the layer
   int64_t page_bytes, head_bytes;
   int page_shift;    // log2 of a page's tiles
-  const Item* items;
+  const Segment* segments;
   const int32_t* pages;
   const int32_t* limits;  // per token, in the plan's order
   const int32_t* q_rows;  // its row in q and out
@@ -56,82 +63,169 @@ struct CachedArgs {
   int64_t slots;  // 0: write the output
 };
 
+// Words of the plan: written before the kernel starts and never by it, which
+// the constant address space tells the compiler, so that a word at the same
+// place for all lanes is loaded to a scalar register.
+__device__ CVS_INLINE int32_t word(const int32_t* p, int64_t i) {
+  return reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p))[i];
+}
+template <typename T>
+__device__ CVS_INLINE T words(const T* p, int64_t i) {
+  constexpr int n = sizeof(T) / 4;
+  int32_t x[n];
+#pragma unroll
+  for (int k = 0; k < n; ++k) x[k] = word(reinterpret_cast<const int32_t*>(p + i), k);
+  T t;
+  __builtin_memcpy(&t, x, sizeof(T));
+  return t;
+}
+
+// A lane's query row.
+struct Row {
+  bool there;
+  int head, limit;
+  int64_t q_row;
+};
+
+// Everything of a segment that both shapes of block use.
 template <bool kBf, int NB>
-__global__ __launch_bounds__(256, 2) void cached_attn_kernel(const CachedArgs a) {
-  __shared__ float s_o[2][16 * NB][64];
-  __shared__ float s_m[kWaves][64], s_l[kWaves][64];
+struct Work {
+  const CachedArgs& a;
+  const Segment& it;
+  int g, lane, half;
 
-  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g = blockIdx.x % a.kv_heads;
-  const Item it = a.items[blockIdx.x / a.kv_heads];
-
-  const bool there = col < it.rows;
-  const int row = it.row0 + min(col, it.rows - 1);
-  const int tok = row / a.group, head = g * a.group + row % a.group;
-  const int limit = a.limits[tok];
-  const int64_t q_row = a.q_rows[tok];
-
-  const int page_mask = (1 << a.page_shift) - 1;
-  auto tile_at = [&](int i) CVS_INLINE {
+  __device__ CVS_INLINE const char* tile(int i) const {  // of the segment, this kv head's keys
     const int t = it.tile0 + i;
-    const int64_t page = a.pages[it.page_first + (t >> a.page_shift)];
-    return a.pool + page * a.page_bytes + g * a.head_bytes + (t & page_mask) * (2048 * NB) + lane * 16;
-  };
-  u32x4 kf[2 * NB], vf[2 * NB];
-  auto load_keys = [&](const char* p) CVS_INLINE {
-#pragma unroll
-    for (int s = 0; s < 2 * NB; ++s) kf[s] = *reinterpret_cast<const u32x4*>(p + s * 1024);
-  };
-  auto load_values = [&](const char* p) CVS_INLINE {
-#pragma unroll
-    for (int s = 0; s < 2 * NB; ++s) vf[s] = *reinterpret_cast<const u32x4*>(p + a.head_bytes / 2 + s * 1024);
-  };
-
-  u32x4 q[2 * NB];
-  {
-    const char* src = a.q.p + 2 * (q_row * a.q.token + head * a.q.head);
+    return at(word(a.pages, it.page_first + (t >> a.page_shift)), t);
+  }
+  __device__ CVS_INLINE const char* at(int64_t page, int t) const {
+    return a.pool + page * a.page_bytes + g * a.head_bytes + (t & ((1 << a.page_shift) - 1)) * (2048 * NB);
+  }
+  __device__ CVS_INLINE Row row(int i) const {  // past the last row, the last one's again (not stored)
+    const int r = it.row0 + min(i, it.rows - 1), tok = r / a.group;
+    return {i < it.rows, g * a.group + r % a.group, a.limits[tok], a.q_rows[tok]};
+  }
+  __device__ CVS_INLINE void load_q(const Row& r, u32x4 (&q)[2 * NB]) const {
+    const char* src = a.q.p + 2 * (r.q_row * a.q.token + r.head * a.q.head);
 #pragma unroll
     for (int s = 0; s < 2 * NB; ++s)
       q[s] = 16 * s + 8 * half < a.dim ? *reinterpret_cast<const u32x4*>(src + 32 * s + 16 * half) : u32x4{};
   }
+  // A tile's values that no row sees may be anything (the page's memory as it was): zeros instead.  key0: of the tile.
+  __device__ CVS_INLINE u32x4 hide(u32x4 v, int k16, int key0, int end) const {
+    const int left = end - key0 - 4 * half;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int t = 16 * k16 + 8 * (w / 2) + 2 * (w % 2);
+      v[w] &= (t < left ? 0xffffu : 0u) | (t + 1 < left ? 0xffff0000u : 0u);
+    }
+    return v;
+  }
+  // Stores row i of the segment: the output, or a part.  met: whether some row's values had infinities or NaNs in keys
+  // that others do not see.
+  __device__ CVS_INLINE void store(const RowState<NB>& st, float m, float l, const Row& r, int i, bool met) const {
+    auto value = [&](int key, int d) CVS_INLINE {
+      const int rel = key - it.key0 - kTile * it.tile0, j = rel & 31;
+      const char* const v = tile(rel / kTile) + a.head_bytes / 2;
+      const int at = (d & 31) + 32 * ((j >> 2) & 1), e = 4 * ((j >> 3) & 1) + (j & 3);
+      return *reinterpret_cast<const uint16_t*>(v + (2 * (d >> 5) + (j >> 4)) * 1024 + 16 * at + 2 * e);
+    };
+    const int first = it.key0 + kTile * it.tile0;
+    const int last = r.there && l == l ? min(first + kTile * it.tiles, r.limit) : 0;
+    if (a.slots == 0) {
+      uint16_t* const out = reinterpret_cast<uint16_t*>(a.out.p) + r.q_row * a.out.token + r.head * a.out.head;
+      store_row<kBf, NB>(st, 1.f / l, out, a.dim, r.there);
+      if (met)
+        store_nonfinite<kBf>(first, last, a.dim, value,
+                             [&](int d, float x) CVS_INLINE { out[d] = uint16_t(pack2<kBf>(x, x)); });
+      if (a.lse && r.there && half == 0)
+        a.lse[int64_t(r.head) * a.q_tokens + r.q_row] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+      return;
+    }
+    const int64_t slot = g * a.slots + it.slot0 + i;
+    float* const o = a.part_o + slot * (32 * NB);
+    if (r.there) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<float4*>(o + 32 * b + 8 * j + 4 * half) =
+              float4{st.o[b][4 * j], st.o[b][4 * j + 1], st.o[b][4 * j + 2], st.o[b][4 * j + 3]};
+      if (half == 0) a.part_ml[slot] = float2{m, l};
+    }
+    if (met) store_nonfinite<kBf>(first, last, a.dim, value, [&](int d, float x) CVS_INLINE { o[d] = x; });
+  }
+};
 
+// The segment's tiles in ascending order, page ids 64 at a time in a lane
+// each: in the loops a page is then a register away, where a load of its own
+// would be waited for at every tile.
+template <bool kBf, int NB>
+struct Tiles {
+  const Work<kBf, NB>& w;
+  int first, ids;  // of the pages held
+
+  __device__ CVS_INLINE explicit Tiles(const Work<kBf, NB>& w) : w(w) { hold(w.it.tile0 >> w.a.page_shift); }
+  __device__ CVS_INLINE void hold(int page) {
+    first = page;
+    // Lanes past the segment's last page hold that one again.
+    const int last = (w.it.tile0 + w.it.tiles - 1) >> w.a.page_shift;
+    ids = w.a.pages[w.it.page_first + min(page + w.lane, last)];
+  }
+  __device__ CVS_INLINE const char* operator()(int i) {
+    const int t = w.it.tile0 + i, page = t >> w.a.page_shift;
+    if (page >= first + 64) hold(page);
+    return w.at(__builtin_amdgcn_readlane(ids, page - first), t);
+  }
+};
+
+// Up to 32 rows: the waves share the tiles.
+template <bool kBf, int NB>
+__device__ CVS_INLINE void few_rows(const Work<kBf, NB>& w, int wave, char* lds) {
+  const CachedArgs& a = w.a;
+  const Segment& it = w.it;
+  const int lane = w.lane, half = w.half;
+  typedef float lanes_t[64];
+  lanes_t* const s_m = reinterpret_cast<lanes_t*>(lds);
+  lanes_t* const s_l = s_m + kWaves;
+  lanes_t* const s_o = s_l + kWaves;  // two states
+
+  const Row r = w.row(lane & 31);
+  u32x4 kf[2 * NB], vf[2 * NB], q[2 * NB];
+  auto load_keys = [&](const char* p) CVS_INLINE {
+#pragma unroll
+    for (int s = 0; s < 2 * NB; ++s) kf[s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + lane * 16 + s * 1024));
+  };
+  auto load_values = [&](const char* p) CVS_INLINE {
+#pragma unroll
+    for (int s = 0; s < 2 * NB; ++s)
+      vf[s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + a.head_bytes / 2 + lane * 16 + s * 1024));
+  };
   RowState<NB> st;
   st.init();
   uint32_t bad = 0;
   if (wave < it.tiles) {
-    const char* p = tile_at(wave);
+    Tiles<kBf, NB> tile(w);
+    const char* p = tile(wave);
     load_keys(p);
     load_values(p);
+    w.load_q(r, q);
     for (int i = wave; i < it.tiles; i += kWaves) {
       f32x16 s{};
 #pragma unroll
       for (int k = 0; k < 2 * NB; ++k) s = mfma<kBf>(kf[k], q[k], s);
-      p = tile_at(i + kWaves < it.tiles ? i + kWaves : i);
+      p = tile(i + kWaves < it.tiles ? i + kWaves : i);
       load_keys(p);
       const int key0 = it.key0 + kTile * (it.tile0 + i);
-      const bool mixed = key0 + kTile > it.min_limit;
-      if (mixed) {
+      if (key0 + kTile > it.min_limit) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (key0 + 8 * (r / 4) + 4 * half + r % 4 >= limit) s[r] = -INFINITY;
+        for (int k = 0; k < 16; ++k)
+          if (key0 + 8 * (k / 4) + 4 * half + k % 4 >= r.limit) s[k] = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 2 * NB; ++k) vf[k] = clean<kBf>(w.hide(vf[k], k & 1, key0, it.max_limit), bad);
       }
       raise_max(s, st, a.c);
       exponentials(s, st, a.c);
-      if (mixed) {
-        // Past the largest limit the page holds whatever was there: zeros instead.  Infinities and NaNs in keys that
-        // some rows see go around the product.
-        const int left = it.max_limit - key0 - 4 * half;
-#pragma unroll
-        for (int k = 0; k < 2 * NB; ++k) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int t = 16 * (k & 1) + 8 * (w / 2) + 2 * (w % 2);
-            vf[k][w] &= (t < left ? 0xffffu : 0u) | (t + 1 < left ? 0xffff0000u : 0u);
-          }
-          vf[k] = clean<kBf>(vf[k], bad);
-        }
-      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const u32x4 pr = prob_operand<kBf>(s, h);
@@ -144,122 +238,176 @@ __global__ __launch_bounds__(256, 2) void cached_attn_kernel(const CachedArgs a)
 
   // The waves' states joined, in the order 0 + 2, 1 + 3, then both.
   s_m[wave][lane] = st.m;
-  const bool met = __syncthreads_or(bad != 0);  // infinities or NaNs that some rows do not see
+  const bool met = __syncthreads_or(bad != 0);
   float m = s_m[0][lane];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_m[w][lane]);
+  for (int i = 1; i < kWaves; ++i) m = fmaxf(m, s_m[i][lane]);
   const float alpha = __builtin_amdgcn_exp2f(st.m - (m == -INFINITY ? 0.f : m));
   s_l[wave][lane] = st.l * alpha;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) st.o[b][r] *= alpha;
+    for (int k = 0; k < 16; ++k) st.o[b][k] *= alpha;
 #pragma unroll
   for (int step = 2; step >= 1; step >>= 1) {
     if (wave >= step && wave < 2 * step) {
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s_o[wave - step][16 * b + r][lane] = st.o[b][r];
+        for (int k = 0; k < 16; ++k) s_o[(wave - step) * 16 * NB + 16 * b + k][lane] = st.o[b][k];
     }
     __syncthreads();
     if (wave < step) {
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) st.o[b][r] += s_o[wave][16 * b + r][lane];
+        for (int k = 0; k < 16; ++k) st.o[b][k] += s_o[wave * 16 * NB + 16 * b + k][lane];
     }
-    __syncthreads();
+    if (step > 1) __syncthreads();
   }
-  if (wave != 0) return;
-  const float l = both_sum((s_l[0][lane] + s_l[2][lane]) + (s_l[1][lane] + s_l[3][lane]));
-  auto value = [&](int key, int d) CVS_INLINE {
-    const int rel = key - it.key0, j = rel & 31, t = rel / kTile;
-    const int64_t page = a.pages[it.page_first + (t >> a.page_shift)];
-    const char* const v = a.pool + page * a.page_bytes + g * a.head_bytes + a.head_bytes / 2 +
-                          (t & page_mask) * (2048 * NB);
-    const int at = (d & 31) + 32 * ((j >> 2) & 1), e = 4 * ((j >> 3) & 1) + (j & 3);
-    return *reinterpret_cast<const uint16_t*>(v + (2 * (d >> 5) + (j >> 4)) * 1024 + 16 * at + 2 * e);
-  };
-  const int first = it.key0 + kTile * it.tile0;
-  const int last = there && l == l ? min(first + kTile * it.tiles, limit) : 0;
-  if (a.slots == 0) {
-    uint16_t* const out = reinterpret_cast<uint16_t*>(a.out.p) + q_row * a.out.token + head * a.out.head;
-    store_row<kBf, NB>(st, 1.f / l, out, a.dim, there);
-    if (met)
-      store_nonfinite<kBf>(first, last, a.dim, value,
-                           [&](int d, float x) CVS_INLINE { out[d] = uint16_t(pack2<kBf>(x, x)); });
-    if (a.lse && there && half == 0)
-      a.lse[int64_t(head) * a.q_tokens + q_row] = (m + __builtin_amdgcn_logf(l)) * kLn2;
-    return;
+  if (wave == 0) {
+    const float l = both_sum((s_l[0][lane] + s_l[2][lane]) + (s_l[1][lane] + s_l[3][lane]));
+    w.store(st, m, l, r, lane & 31, met);
   }
-  const int64_t slot = g * a.slots + it.slot0 + col;
-  float* const o = a.part_o + slot * (32 * NB);
-  if (there) {
+}
+
+// The tiles of a segment through LDS, for attend_tiles: 64-key tile t is tiles 2 t and 2 t + 1.
+template <bool kBf, int NB>
+struct PageSource {
+  static constexpr int kHalf = 2048 * NB;  // a 32-key tile, keys or values
+  const Work<kBf, NB>& w;
+  Tiles<kBf, NB> tile;
+  const char* asked[2];  // where the keys of the last two tiles asked for are: their values are asked for later
+  char *lds_k, *lds_v;
+  int to_k, to_v, at_wave, wave, end;
+
+  __device__ CVS_INLINE PageSource(const Work<kBf, NB>& w, int wave, char* lds, int end)
+      : w(w), tile(w), lds_k(lds), lds_v(lds + 4 * kHalf), wave(wave), end(end) {
+    // A wave loads half of one of the two tiles.
+    at_wave = (wave & 1) * (kHalf / 2);
+    const int to = (wave >> 1) * kHalf + at_wave;
+    to_k = lds_addr(lds_k) + to;
+    to_v = lds_addr(lds_v) + to;
+  }
+  __device__ CVS_INLINE void load(const char* from, int to) {
+    const rsrc4 rs = make_rsrc(from + at_wave, kHalf / 2);
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<float4*>(o + 32 * b + 8 * j + 4 * half) =
-            float4{st.o[b][4 * j], st.o[b][4 * j + 1], st.o[b][4 * j + 2], st.o[b][4 * j + 3]};
-    if (half == 0) a.part_ml[slot] = float2{m, l};
+    for (int i = 0; i < NB; ++i) lds_dma<16, false>(rs, to + i * 1024, i * 1024 + w.lane * 16, 0);
   }
-  if (met) store_nonfinite<kBf>(first, last, a.dim, value, [&](int d, float x) CVS_INLINE { o[d] = x; });
+  __device__ CVS_INLINE void load_keys(int t) {
+    // The last tile again where the segment has an odd number; its keys are past the end.
+    const char* const from = tile(min(2 * t + (wave >> 1), w.it.tiles - 1));
+    asked[0] = asked[1];
+    asked[1] = from;
+    load(from, to_k + (t & 1) * 2 * kHalf);
+  }
+  // Called for each tile when the next one's keys have been asked for, or, for the last, its own.
+  __device__ CVS_INLINE void load_values(int t) {
+    load((2 * t + 2 < w.it.tiles ? asked[0] : asked[1]) + w.a.head_bytes / 2, to_v + (t & 1) * 2 * kHalf);
+  }
+  __device__ CVS_INLINE u32x4 keys(int t, int h, int i) {
+    return *reinterpret_cast<const u32x4*>(lds_k + (2 * (t & 1) + h) * kHalf + i * 1024 + w.lane * 16);
+  }
+  __device__ CVS_INLINE u32x4 values(int t, int h, int b, int k) {
+    return *reinterpret_cast<const u32x4*>(lds_v + (2 * (t & 1) + h) * kHalf + (2 * b + k) * 1024 + w.lane * 16);
+  }
+  __device__ CVS_INLINE u32x4 hide(u32x4 v, int t, int h, int k) { return w.hide(v, k, 64 * t + 32 * h, end); }
+};
+
+// Up to 128 rows: each wave has its own.
+template <bool kBf, int NB>
+__device__ CVS_INLINE void many_rows(const Work<kBf, NB>& w, int wave, char* lds) {
+  const Segment& it = w.it;
+  const int i = 32 * wave + (w.lane & 31);
+  const Row r = w.row(i);
+  u32x4 q[2 * NB];
+  w.load_q(r, q);
+  RowState<NB> st;
+  st.init();
+  uint32_t bad = 0;
+  // Positions from the segment's first key on.
+  const int key0 = it.key0 + kTile * it.tile0, keys = kTile * it.tiles;
+  PageSource<kBf, NB> src(w, wave, lds, min(it.max_limit - key0, keys));
+  attend_tiles<kBf, NB>(st, q, src, (it.tiles + 1) / 2, max(0, min(it.min_limit - key0, keys)) / 64,
+                        min(r.limit - key0, keys), w.a.c, bad);
+  const float l = both_sum(st.l);
+  const bool met = __ballot(bad != 0) != 0;
+  if (32 * wave < it.rows) w.store(st, st.m, l, r, i, met);
+}
+
+template <bool kBf, int NB>
+__global__ __launch_bounds__(256, 2) void cached_attn_kernel(const CachedArgs a) {
+  __shared__ __align__(16) char lds[16384 * NB];  // of many_rows; few_rows takes 8192 NB + 2048
+  static_assert(8192 * NB + 2048 <= 16384 * NB, "LDS of few_rows");
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = blockIdx.x % a.kv_heads, wg = blockIdx.x / a.kv_heads;
+  const Segment it = words(a.segments, wg);
+  const Work<kBf, NB> w{a, it, g, lane, lane >> 5};
+  if (it.rows > kTile) many_rows<kBf, NB>(w, wave, lds);
+  else few_rows<kBf, NB>(w, wave, lds);
 }
 
 struct JoinArgs {
-  const Run* runs;
-  const int32_t* leaves;  // per token, the last of its runs
+  const Parts* parts;      // of a sequence, run by run
+  const int32_t* paths;    // per token, first of its sequence's in `parts` and how many: first * 256 + runs
   const int32_t* q_rows;
   const float* part_o;
   const float2* part_ml;
-  int64_t slots, rows;    // rows: tokens * heads
+  int64_t slots, rows;     // rows: tokens * heads
   View out;
   float* lse;
   int64_t q_tokens;
   int heads, group, dim, nb;
 };
 
-// One wave a (token, head) row: lanes take 2 columns each.
+// One wave a (token, head) row, 2 columns a lane, in one pass over the row's
+// parts with a running maximum.
 template <bool kBf>
 __global__ __launch_bounds__(256) void join_parts_kernel(const JoinArgs a) {
   const int64_t i = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (i >= a.rows) return;
   const int lane = threadIdx.x & 63;
   const int tok = int(i / a.heads), head = int(i % a.heads);
-  const int64_t base = int64_t(head / a.group) * a.slots;
-  const int row = tok * a.group + head % a.group;
-  const int leaf = a.leaves[tok];
-  float m = -INFINITY;
-  for (int r = leaf; r >= 0;) {
-    const Run run = a.runs[r];
-    const int64_t s = base + run.slot0 + row - run.row0;
-    for (int c = lane; c < run.chunks; c += 64) m = fmaxf(m, a.part_ml[s + int64_t(c) * run.rows].x);
-    r = run.parent;
-  }
+  const int64_t base = int64_t(head / a.group) * a.slots + tok * a.group + head % a.group;
+  const int path = word(a.paths, tok);
+  const int64_t q_row = word(a.q_rows, tok);
+  const int d = 2 * lane, width = 32 * a.nb, dl = d < width ? d : 0;
+  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int r = path >> 8, end = r + (path & 255); r < end; ++r) {
+    const Parts run = words(a.parts, r);
+    const int64_t first = base + run.slot0;
+    for (int p = 0; p < run.count; p += kJoin) {
+      float2 ml[kJoin], o[kJoin];
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, xor_lanes_f(m, o));
-  const float from = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o0 = 0.f, o1 = 0.f;
-  const int d = 2 * lane, width = 32 * a.nb;
-  const int dl = d < width ? d : 0;
-  for (int r = leaf; r >= 0;) {
-    const Run run = a.runs[r];
-    const int64_t s = base + run.slot0 + row - run.row0;
-#pragma unroll 4
-    for (int c = 0; c < run.chunks; ++c) {
-      const int64_t at = s + int64_t(c) * run.rows;
-      const float2 ml = a.part_ml[at];
-      const float2 o = *reinterpret_cast<const float2*>(a.part_o + at * width + dl);
-      const float w = __builtin_amdgcn_exp2f(ml.x - from);
-      l += w * ml.y;
-      o0 += w * o.x;
-      o1 += w * o.y;
+      for (int k = 0; k < kJoin; ++k) {  // past the last part, that one again with no weight
+        const int64_t at = first + int64_t(min(p + k, run.count - 1)) * run.rows;
+        ml[k] = a.part_ml[at];
+        o[k] = *reinterpret_cast<const float2*>(a.part_o + at * width + dl);
+      }
+      float top = m;
+#pragma unroll
+      for (int k = 0; k < kJoin; ++k) {
+        if (p + k >= run.count) ml[k].x = -INFINITY;
+        top = fmaxf(top, ml[k].x);
+      }
+      const float from = top == -INFINITY ? 0.f : top;
+      const float keep = __builtin_amdgcn_exp2f(m - from);
+      l *= keep;
+      o0 *= keep;
+      o1 *= keep;
+#pragma unroll
+      for (int k = 0; k < kJoin; ++k) {
+        // A part of no weight has nothing the row sees, or what has underflowed beside the rest.
+        const float w = __builtin_amdgcn_exp2f(ml[k].x - from);
+        l += w * ml[k].y;
+        o0 += w * o[k].x;
+        o1 += w * o[k].y;
+      }
+      m = top;
     }
-    r = run.parent;
   }
   const float inv = 1.f / l;
-  const int64_t q_row = a.q_rows[tok];
   if (d < a.dim)
     *reinterpret_cast<uint32_t*>(a.out.p + 2 * (q_row * a.out.token + head * a.out.head + d)) =
         pack2<kBf>(o0 * inv, o1 * inv);
@@ -315,7 +463,7 @@ void plan_attention(cvs_kv_plan* plan, const int64_t* lengths, const int64_t* to
   const std::vector<kv::SharedRun> shared = kv::shared_runs(lists, counts, order);
 
   const size_t n = order.size();
-  std::vector<int32_t> limits, q_rows, leaves;
+  std::vector<int32_t> limits, q_rows;
   std::vector<int64_t> tok0(n + 1, 0);
   for (size_t p = 0; p < n; ++p) {
     const int64_t s = order[p], len = lengths[from[size_t(s)]], new_tokens = tokens[from[size_t(s)]];
@@ -326,65 +474,104 @@ void plan_attention(cvs_kv_plan* plan, const int64_t* lengths, const int64_t* to
     tok0[p + 1] = tok0[p] + new_tokens;
   }
 
-  // Work in (32 rows, 32 keys) tiles of one kv head, and the chunk that spreads it over the device: enough
-  // workgroups for four a compute unit, but at least two tiles a wave.
-  std::vector<int64_t> run_tiles(shared.size());
-  int64_t work = 0;
+  // Rows of a run go in blocks of up to 128, a block's tiles in equal segments, one a workgroup.  Splitting a block
+  // costs a second kernel and, for each segment, what a workgroup does before its first tile and after its last (about
+  // kOverhead tiles), so blocks are not split into segments of fewer tiles than these: one short sequence of 25 tiles
+  // takes 7.3 us whole and 8.8 in parts of 8, 32 questions of 5 tokens over 126 tiles 25.2 us in parts of 16, 31.6 in
+  // parts of 32 and 29.0 in parts of 8.
+  constexpr int64_t kFewTiles = 32, kManyTiles = 16, kOverhead = 4;
+  std::vector<int64_t> run_tiles(shared.size()), run_rows(shared.size());
+  int64_t longest = 1;
   for (size_t r = 0; r < shared.size(); ++r) {
     const kv::SharedRun& s = shared[r];
     int64_t most = 0;
     for (int64_t p = s.lo; p < s.hi; ++p) most = std::max(most, lengths[from[size_t(order[size_t(p)])]]);
     run_tiles[r] = (std::min((s.first + s.count) * pt, most) - s.first * pt + kTile - 1) / kTile;
-    const int64_t rows = (tok0[size_t(s.hi)] - tok0[size_t(s.lo)]) * group;
-    work += run_tiles[r] * ((rows + kTile - 1) / kTile);
+    run_rows[r] = (tok0[size_t(s.hi)] - tok0[size_t(s.lo)]) * group;
+    longest = std::max(longest, run_tiles[r]);
   }
-  const int64_t target = std::max<int64_t>(1, int64_t(4) * c->ctx->compute_units / c->kv_heads);
-  const int64_t chunk = std::max<int64_t>(2 * kWaves, (work + target - 1) / target);
+  // Segments of at most `share` tiles.
+  auto parts_of = [&](size_t r, int64_t share) {
+    const int64_t least = run_rows[r] > kTile ? kManyTiles : kFewTiles;
+    return (run_tiles[r] + std::max(share, least) - 1) / std::max(share, least);
+  };
+  auto segments_at = [&](int64_t share) {
+    int64_t sum = 0;
+    for (size_t r = 0; r < shared.size(); ++r) sum += parts_of(r, share) * ((run_rows[r] + kBlock - 1) / kBlock);
+    return sum;
+  };
+  // Two workgroups a compute unit run at a time: the smallest share that fits one such round, or two or three.
+  int64_t share = longest, cost = INT64_MAX;
+  for (int64_t rounds = 1; rounds <= 3; ++rounds) {
+    const int64_t fit = std::max<int64_t>(1, rounds * 2 * c->ctx->compute_units / c->kv_heads);
+    int64_t lo = 1, hi = longest;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) / 2;
+      if (segments_at(mid) <= fit) hi = mid;
+      else lo = mid + 1;
+    }
+    int64_t most = 0;  // tiles of the largest segment
+    for (size_t r = 0; r < shared.size(); ++r) {
+      const int64_t parts = parts_of(r, lo);
+      most = std::max(most, (run_tiles[r] + parts - 1) / parts);
+    }
+    if (rounds * (most + kOverhead) < cost) {
+      share = lo;
+      cost = rounds * (most + kOverhead);
+    }
+  }
 
-  std::vector<Item> items;
-  std::vector<Run> runs;
-  std::vector<int32_t> pages, cur(n, -1);
+  std::vector<Segment> segments;
+  std::vector<Parts> run_parts(shared.size()), parts;
+  std::vector<int32_t> pages, paths, cur(n, -1), parent(shared.size());
   int64_t slots = 0;
   bool one_part = true;
   for (size_t r = 0; r < shared.size(); ++r) {
     const kv::SharedRun& s = shared[r];
-    const int64_t t0 = tok0[size_t(s.lo)], t1 = tok0[size_t(s.hi)], rows = (t1 - t0) * group;
-    const int64_t chunks = (run_tiles[r] + chunk - 1) / chunk;
-    const int64_t each = (run_tiles[r] + chunks - 1) / chunks;
-    const int32_t parent = cur[size_t(s.lo)];
-    if (parent >= 0 || chunks > 1) one_part = false;
+    const int64_t t0 = tok0[size_t(s.lo)], count = parts_of(r, share), rows = run_rows[r];
+    parent[r] = cur[size_t(s.lo)];
     for (int64_t p = s.lo; p < s.hi; ++p) cur[size_t(p)] = int32_t(r);
-    if (slots + rows * chunks > (int64_t(1) << 31) - 1) fail(CVS_ERR_UNSUPPORTED, "too many partial results");
+    if (parent[r] >= 0 || count > 1) one_part = false;
+    if (slots + rows * count > kv::PageBook::kMaxTokens) fail(CVS_ERR_UNSUPPORTED, "too many partial results");
+    run_parts[r] = {int32_t(slots - t0 * group), int32_t(rows), int32_t(count)};
     const int32_t page_first = int32_t(pages.size());
     const int32_t* const list = lists[size_t(s.member)];
     pages.insert(pages.end(), list + s.first, list + s.first + s.count);
-    runs.push_back({parent, int32_t(slots), int32_t(chunks), int32_t(t0 * group), int32_t(rows)});
-    for (int64_t k = 0; k < chunks; ++k) {
-      const int64_t tile0 = k * each, tiles = std::min(each, run_tiles[r] - tile0);
-      for (int64_t row = 0; row < rows; row += kTile) {
-        const int64_t in = std::min<int64_t>(kTile, rows - row);
+    const int64_t each = (run_tiles[r] + count - 1) / count;
+    for (int64_t part = 0; part < count; ++part)
+      for (int64_t row = 0; row < rows; row += kBlock) {
+        const int64_t in = std::min<int64_t>(kBlock, rows - row), tile = part * each;
         int32_t lo = INT32_MAX, hi = 0;
         for (int64_t t = t0 + row / group; t <= t0 + (row + in - 1) / group; ++t) {
           lo = std::min(lo, limits[size_t(t)]);
           hi = std::max(hi, limits[size_t(t)]);
         }
-        items.push_back({page_first, int32_t(tile0), int32_t(tiles), int32_t(s.first * pt), int32_t(t0 * group + row),
-                         int32_t(in), int32_t(slots + k * rows + row), lo, hi});
+        segments.push_back({page_first, int32_t(tile), int32_t(std::min(each, run_tiles[r] - tile)),
+                            int32_t(s.first * pt), int32_t(t0 * group + row), int32_t(in),
+                            int32_t(slots + part * rows + row), lo, hi});
       }
-    }
-    slots += rows * chunks;
+    slots += rows * count;
   }
-  if (int64_t(items.size()) * c->kv_heads > (int64_t(1) << 31) - 1) fail(CVS_ERR_UNSUPPORTED, "too much work");
-  for (size_t p = 0; p < n; ++p)
-    for (int64_t t = tok0[p]; t < tok0[p + 1]; ++t) leaves.push_back(cur[p]);
-  plan->items = int(items.size());
+  // The longest first, so that the last workgroups to start are short ones.
+  std::stable_sort(segments.begin(), segments.end(),
+                   [](const Segment& x, const Segment& y) { return x.tiles > y.tiles; });
+  if (int64_t(segments.size()) * c->kv_heads > (int64_t(1) << 31) - 1) fail(CVS_ERR_UNSUPPORTED, "too much work");
+  for (size_t p = 0; p < n; ++p) {
+    const size_t at = parts.size();
+    for (int32_t r = cur[p]; r >= 0; r = parent[size_t(r)]) parts.push_back(run_parts[size_t(r)]);
+    const size_t runs = parts.size() - at;
+    if (runs > 255 || at >= (size_t(1) << 23)) fail(CVS_ERR_UNSUPPORTED, "prefixes shared in too many levels");
+    for (int64_t t = tok0[p]; t < tok0[p + 1]; ++t) paths.push_back(int32_t(at * 256 + runs));
+  }
+  plan->workgroups = int(segments.size());
   plan->slots = one_part ? 0 : slots;
-  plan->at_items = append(blob, items);
+  plan->at_segments = append(blob, segments);
   plan->at_pages = append(blob, pages);
   plan->at_limits = append(blob, limits);
   plan->at_rows = append(blob, q_rows);
-  plan->at_leaves = append(blob, leaves);
-  plan->at_runs = append(blob, runs);
+  if (one_part) return;
+  plan->at_paths = append(blob, paths);
+  plan->at_parts = append(blob, parts);
 }
 
 }  // namespace attn
@@ -416,7 +603,7 @@ extern "C" int cvs_kv_attention_async(cvs_kv_cache* cache, cvs_kv_plan* plan, in
         fail(CVS_ERR_INVALID_ARGUMENT, std::string(what) + " must have the cache's head_dim and type");
     }
     const float c = scale_log2(scale, cache->dim);
-    if (plan->items == 0) return;
+    if (plan->workgroups == 0) return;
     const char* const blob = plan->blob.as<char>();
     const int group = plan->heads / cache->kv_heads;
     float* part_o = nullptr;
@@ -430,18 +617,18 @@ extern "C" int cvs_kv_attention_async(cvs_kv_cache* cache, cvs_kv_plan* plan, in
     int shift = 0;
     while ((kTile << shift) < cache->book->page_tokens()) ++shift;
     const CachedArgs a{cache->pool + layer * cache->layer_bytes, cache->page_bytes, cache->head_bytes, shift,
-                       reinterpret_cast<const Item*>(blob + plan->at_items),
+                       reinterpret_cast<const Segment*>(blob + plan->at_segments),
                        reinterpret_cast<const int32_t*>(blob + plan->at_pages),
                        reinterpret_cast<const int32_t*>(blob + plan->at_limits),
                        reinterpret_cast<const int32_t*>(blob + plan->at_rows), view_of(q), view_of(out), lse,
                        plan->tokens, cache->kv_heads, group, cache->dim, c, part_o, part_ml, plan->slots};
-    const int64_t blocks = int64_t(plan->items) * cache->kv_heads;
+    const int64_t blocks = int64_t(plan->workgroups) * cache->kv_heads;
     const bool is_bf = cache->type == CVS_BF16;
     if (is_bf) launch<true>(ctx, a, cache->nb, blocks);
     else launch<false>(ctx, a, cache->nb, blocks);
     if (!slots) return;
-    const JoinArgs j{reinterpret_cast<const Run*>(blob + plan->at_runs),
-                     reinterpret_cast<const int32_t*>(blob + plan->at_leaves),
+    const JoinArgs j{reinterpret_cast<const Parts*>(blob + plan->at_parts),
+                     reinterpret_cast<const int32_t*>(blob + plan->at_paths),
                      reinterpret_cast<const int32_t*>(blob + plan->at_rows), part_o, part_ml, plan->slots,
                      plan->tokens * plan->heads, view_of(out), lse, plan->tokens, plan->heads, group, cache->dim,
                      cache->nb};

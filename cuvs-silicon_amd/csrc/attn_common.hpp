@@ -15,6 +15,7 @@
 #include <cmath>
 #include <cstdint>
 #include <memory>
+#include <type_traits>
 #include <vector>
 
 #include "bf_common.hpp"
@@ -161,6 +162,83 @@ __device__ CVS_INLINE u32x4 prob_operand(const f32x16& p, int step) {
   return r;
 }
 
+// Attention of a workgroup's 4 x 32 query rows over `tiles` 64-key tiles that
+// go through LDS, double-buffered.  A row sees the keys below `limit`, counted
+// from the first tile; in the first `open_tiles` tiles all rows see all keys.
+// The source moves the data: load_keys(t) and load_values(t) ask for a tile of
+// either (buffer t & 1; the workgroup's waves share the work; in ascending
+// order, a tile's values after the next one's keys), keys(t, h, i)
+// is the A operand of columns 16 i of half h's 32 keys, values(t, h, b, k) of
+// columns 32 b of its k-th 16 keys; hide(v, t, h, k) clears what a masked
+// tile's values must not show.
+//
+// Half tiles go through a pipeline of three: the products of one with the
+// values and of the next with the keys run while the one between goes through
+// its exponentials.  In the middle of tile t everyone is done with its keys
+// and with the values before it; what was asked for one tile ago, the next
+// keys and its values, has to be there.
+template <bool kBf, int NB, typename Source>
+__device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[2 * NB], Source& src, int tiles,
+                                        int open_tiles, int limit, float c, uint32_t& bad) {
+  const int half = __lane_id() >> 5;
+  f32x16 s[2];    // scores of a tile's two halves
+  u32x4 p[2][2];  // and their probabilities
+  auto scores = [&](int t, int h) CVS_INLINE {
+    f32x16 x{};
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) x = mfma<kBf>(src.keys(t, h, i), q[i], x);
+    return x;
+  };
+  auto add_values = [&](int t, int h, auto masked) CVS_INLINE {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        u32x4 v = src.values(t, h, b, k);
+        if constexpr (masked) v = clean<kBf>(src.hide(v, t, h, k), bad);
+        st.o[b] = mfma<kBf>(v, p[h][k], st.o[b]);
+      }
+  };
+  auto mask = [&](int t, int h) CVS_INLINE {
+    const int seen = limit - 64 * t - 32 * h - 4 * half;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (8 * (r / 4) + r % 4 >= seen) s[h][r] = -INFINITY;
+  };
+  auto probabilities = [&](int h) CVS_INLINE {
+    exponentials(s[h], st, c);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) p[h][k] = prob_operand<kBf>(s[h], k);
+  };
+  auto step = [&](int t, auto masked) CVS_INLINE {
+    if (t > 0) add_values(t - 1, 1, masked);
+    if constexpr (masked) mask(t, 0);
+    raise_max(s[0], st, c);
+    s[1] = scores(t, 1);
+    probabilities(0);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    __syncthreads();
+    if (t + 2 < tiles) src.load_keys(t + 2);
+    if (t + 1 < tiles) src.load_values(t + 1);
+    add_values(t, 0, masked);
+    if constexpr (masked) mask(t, 1);
+    raise_max(s[1], st, c);
+    s[0] = scores(t + 1, 0);  // past the last tile: of whatever is there, and not used
+    probabilities(1);
+  };
+  if (tiles <= 0) return;
+  src.load_keys(0);
+  if (tiles > 1) src.load_keys(1);
+  src.load_values(0);
+  __builtin_amdgcn_s_waitcnt(0x0F70);
+  __syncthreads();
+  s[0] = scores(0, 0);
+  int t = 0;
+  for (; t < open_tiles; ++t) step(t, std::false_type{});
+  for (; t < tiles; ++t) step(t, std::true_type{});
+  add_values(tiles - 1, 1, std::true_type{});
+}
+
 // Writes a lane's half of a row's 32 NB outputs, scaled.  Lanes l and l + 32
 // hold alternate groups of 4 elements; the pair exchanges them so that each
 // stores 16 bytes at a time.
@@ -254,9 +332,9 @@ struct cvs_kv_plan {
   // Offsets into the blob, in bytes.
   int spans = 0;       // of tokens, a page each (kv_cache.hip, Span)
   size_t at_spans = 0;
-  int items = 0;       // of attention work (attn_cached.hip, Item)
+  int workgroups = 0;  // of attention, a kv head (attn_cached.hip)
   int64_t slots = 0;   // rows of partial results a kv head; 0: every row has one part
-  size_t at_items = 0, at_pages = 0, at_limits = 0, at_rows = 0, at_leaves = 0, at_runs = 0;
+  size_t at_segments = 0, at_pages = 0, at_limits = 0, at_rows = 0, at_paths = 0, at_parts = 0;
 };
 
 namespace cvs {

@@ -19,7 +19,6 @@
 // read (ds_read_b64_tr_b16).  The permutation costs nothing: each lane of a
 // load picks the piece that belongs at its place.
 #include <algorithm>
-#include <type_traits>
 
 #include "attn_common.hpp"
 
@@ -58,14 +57,88 @@ __device__ CVS_INLINE int swap_v(int r) {  // a read takes 4 pieces of 4 rows
   return P == 12 ? 0 : P == 8 ? 4 * ((r >> 1) & 1) : 4 * (r & 3);
 }
 
+// A kv head of one sequence, for attend_tiles.
+template <int NB>
+struct PromptSource {
+  static constexpr int P = 4 * NB;  // 16-byte pieces of a row in LDS
+  static constexpr int kPitch = 16 * P;
+  static constexpr int kLoads = kKeys * P / 256;  // of a wave, keys or values
+  static constexpr int kBuf = kKeys * kPitch;
+  static constexpr uint32_t kNowhere = 0x80000000u;
+
+  char *lds_k, *lds_v;
+  int to_k, to_v;  // LDS addresses of the wave's share
+  const char *base_k, *base_v;
+  int64_t step_k, step_v;
+  int k_len, first;  // first: of the lane's places in a buffer
+  uint32_t off_k[kLoads], off_v[kLoads];
+  int k_even, k_odd, v_first;
+
+  __device__ CVS_INLINE PromptSource(const PromptArgs& a, const PromptItem& it, int g, int wave, char* sk, char* sv) {
+    const int lane = __lane_id(), col = lane & 31, half = lane >> 5;
+    lds_k = sk;
+    lds_v = sv;
+    to_k = lds_addr(sk) + wave * kLoads * 1024;
+    to_v = lds_addr(sv) + wave * kLoads * 1024;
+    base_k = a.k.p + 2 * (it.k0 * a.k.token + g * a.k.head);
+    base_v = a.v.p + 2 * (it.k0 * a.v.token + g * a.v.head);
+    step_k = kKeys * a.k.token * 2;
+    step_v = kKeys * a.v.token * 2;
+    k_len = it.k_len;
+    // LDS place n = 64 i + lane of a wave's share is row n / P, place n % P.  Out of range reads zeros: pieces past the
+    // head's end, and rows past the sequence's end in its last tile.
+    first = wave * kLoads * 64 + lane;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int n = first + i * 64, r = n / P, p = n % P;
+      const int pk = p ^ swap_k<P>(r), pv = p ^ swap_v<P>(r);
+      off_k[i] = 8 * pk < a.dim ? uint32_t(r * a.k.token * 2 + 16 * pk) : kNowhere;
+      off_v[i] = 8 * pv < a.dim ? uint32_t(r * a.v.token * 2 + 16 * pv) : kNowhere;
+      asm("" : "+v"(off_k[i]), "+v"(off_v[i]));  // kept, not computed again for every tile
+    }
+    // Operand addresses within a buffer: of the keys' pieces 2 i + half (i even and odd: the piece order is swapped
+    // within groups of four, or by more where rows are 128 or 256 bytes), of 4 keys of a column group.
+    const int sw = swap_k<P>(col), li = lane & 15, vkey = 4 * half + (li >> 2);
+    k_even = col * kPitch + 16 * (half ^ sw);
+    k_odd = col * kPitch + 16 * ((2 + half) ^ sw);
+    v_first = vkey * kPitch + 8 * (li & 1) + 16 * ((2 * ((lane >> 4) & 1) + ((li & 3) >> 1)) ^ swap_v<P>(vkey));
+  }
+  __device__ CVS_INLINE void load(const char* base, int64_t step, int to, const uint32_t (&off)[kLoads], int t) {
+    const rsrc4 rs = make_rsrc(base + t * step, 0x7fffffff);
+    const int left = k_len - t * kKeys;
+    to += (t & 1) * kBuf;
+    if (left >= kKeys) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) lds_dma<16, false>(rs, to + i * 1024, off[i], 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        lds_dma<16, false>(rs, to + i * 1024, (first + i * 64) / P < left ? off[i] : kNowhere, 0);
+    }
+  }
+  __device__ CVS_INLINE void load_keys(int t) { load(base_k, step_k, to_k, off_k, t); }
+  __device__ CVS_INLINE void load_values(int t) { load(base_v, step_v, to_v, off_v, t); }
+  __device__ CVS_INLINE u32x4 keys(int t, int h, int i) {
+    const int at = P == 12 ? (i & 1 ? k_odd : k_even) + 64 * (i / 2) : k_even ^ 32 * i;
+    return *reinterpret_cast<const u32x4*>(lds_k + (t & 1) * kBuf + h * 32 * kPitch + at);
+  }
+  __device__ CVS_INLINE u32x4 values(int t, int h, int b, int k) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+    char* const from = lds_v + (t & 1) * kBuf + (32 * h + 16 * k) * kPitch + (P == 12 ? v_first + 64 * b : v_first ^ 64 * b);
+    const auto x = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)from));
+    const auto y = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(from + 8 * kPitch)));
+    return u32x4{x[0], x[1], y[0], y[1]};
+  }
+  __device__ CVS_INLINE u32x4 hide(u32x4 v, int, int, int) { return v; }  // past the sequence's end are zeros
+};
+
 template <bool kBf, int NB>
 __global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 3 ? 3 : 4) void prompt_attn_kernel(const PromptArgs a) {
-  constexpr int P = 4 * NB;                 // 16-byte pieces of a row in LDS
-  constexpr int kPitch = 16 * P;
-  constexpr int kLoads = kKeys * P / 256;   // loads of a wave, keys or values
-  constexpr int kBuf = kKeys * kPitch;
-  __shared__ __align__(16) char s_k[2][kBuf];
-  __shared__ __align__(16) char s_v[2][kBuf];
+  typedef PromptSource<NB> Source;
+  __shared__ __align__(16) char s_k[2 * Source::kBuf];
+  __shared__ __align__(16) char s_v[2 * Source::kBuf];
 
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -82,7 +155,6 @@ __global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 3 ? 3 : 4) void prompt_att
     return a.causal ? max(0, min(it.k_len, t + 1 + it.k_len - it.q_len)) : it.k_len;
   };
   const int limit = limit_of(tok);
-  const bool busy = it.row0 + 32 * wave < rows;
   // Limits grow with the row, so the first and last row bound the workgroup's.
   const int wg_min = limit_of(it.row0 / a.group), wg_max = limit_of((min(it.row0 + kRows, rows) - 1) / a.group);
 
@@ -93,121 +165,13 @@ __global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 3 ? 3 : 4) void prompt_att
     for (int s = 0; s < 2 * NB; ++s)
       q[s] = 16 * s + 8 * half < a.dim ? *reinterpret_cast<const u32x4*>(src + 32 * s + 16 * half) : u32x4{};
   }
-
-  // Loads: LDS place n = 64 i + lane of a wave's share is row n / P, place n % P.  Out of range reads zeros: pieces
-  // past the head's end, and rows past the sequence's end in its last tile.
-  constexpr uint32_t kNowhere = 0x80000000u;
-  uint32_t off_k[kLoads], off_v[kLoads];
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int n = (wave * kLoads + i) * 64 + lane, r = n / P, p = n % P;
-    const int pk = p ^ swap_k<P>(r), pv = p ^ swap_v<P>(r);
-    off_k[i] = 8 * pk < a.dim ? uint32_t(r * a.k.token * 2 + 16 * pk) : kNowhere;
-    off_v[i] = 8 * pv < a.dim ? uint32_t(r * a.v.token * 2 + 16 * pv) : kNowhere;
-    asm("" : "+v"(off_k[i]), "+v"(off_v[i]));  // kept, not computed again for every tile
-  }
-  const char* const base_k = a.k.p + 2 * (it.k0 * a.k.token + g * a.k.head);
-  const char* const base_v = a.v.p + 2 * (it.k0 * a.v.token + g * a.v.head);
-  const int64_t step_k = kKeys * a.k.token * 2, step_v = kKeys * a.v.token * 2;
-  const int lds_k = lds_addr(s_k[0]) + wave * kLoads * 1024, lds_v = lds_addr(s_v[0]) + wave * kLoads * 1024;
-  auto load_tile = [&](const char* base, int64_t step, int lds, const uint32_t(&off)[kLoads], int t) CVS_INLINE {
-    const rsrc4 rs = make_rsrc(base + t * step, 0x7fffffff);
-    const int left = it.k_len - t * kKeys;
-    lds += (t & 1) * kBuf;
-    if (left >= kKeys) {
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) lds_dma<16, false>(rs, lds + i * 1024, off[i], 0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        lds_dma<16, false>(rs, lds + i * 1024, ((wave * kLoads + i) * 64 + lane) / P < left ? off[i] : kNowhere, 0);
-    }
-  };
-
-  // Operand addresses within a buffer: of the keys' pieces 2 i + half (i even and odd: the piece order is swapped
-  // within groups of four, or by more where rows are 128 or 256 bytes), of 4 keys of a column group.
-  const int sw = swap_k<P>(col), li = lane & 15, vkey = 4 * half + (li >> 2);
-  const int k_even = col * kPitch + 16 * (half ^ sw), k_odd = col * kPitch + 16 * ((2 + half) ^ sw);
-  auto key_at = [&](int i) CVS_INLINE { return P == 12 ? (i & 1 ? k_odd : k_even) + 64 * (i / 2) : k_even ^ 32 * i; };
-  const int v_first = vkey * kPitch + 8 * (li & 1) +
-                      16 * ((2 * ((lane >> 4) & 1) + ((li & 3) >> 1)) ^ swap_v<P>(vkey));
-  auto value_at = [&](int b) CVS_INLINE { return P == 12 ? v_first + 64 * b : v_first ^ 64 * b; };
-
+  Source src(a, it, g, wave, s_k, s_v);
+  const char* const base_v = src.base_v;
   RowState<NB> st;
   st.init();
   uint32_t bad = 0;
-  f32x16 s[2];   // scores of a tile's two halves
-  u32x4 p[2][2];  // and their probabilities
-  auto scores = [&](int t, int h) CVS_INLINE {
-    const char* const at = s_k[0] + (t & 1) * kBuf + h * 32 * kPitch;
-    f32x16 x{};
-#pragma unroll
-    for (int i = 0; i < 2 * NB; ++i) x = mfma<kBf>(*reinterpret_cast<const u32x4*>(at + key_at(i)), q[i], x);
-    return x;
-  };
-  auto add_values = [&](int t, int h, auto masked) CVS_INLINE {
-    typedef short s16x4 __attribute__((ext_vector_type(4)));
-    typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
-    typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-    char* const at = s_v[0] + (t & 1) * kBuf + h * 32 * kPitch;
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        char* const from = at + value_at(b) + k * 16 * kPitch;
-        const auto x = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)from));
-        const auto y =
-            __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(from + 8 * kPitch)));
-        u32x4 v{x[0], x[1], y[0], y[1]};
-        if constexpr (masked) v = clean<kBf>(v, bad);
-        st.o[b] = mfma<kBf>(v, p[h][k], st.o[b]);
-      }
-  };
-  auto mask = [&](int t, int h) CVS_INLINE {
-    const int seen = limit - t * kKeys - 32 * h - 4 * half;
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-      if (8 * (r / 4) + r % 4 >= seen) s[h][r] = -INFINITY;
-  };
-  auto probabilities = [&](int h) CVS_INLINE {
-    exponentials(s[h], st, a.c);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) p[h][k] = prob_operand<kBf>(s[h], k);
-  };
-
-  // Half tiles in a pipeline of three: the products of one with the values and of the next with the keys run while
-  // the one between goes through its exponentials.  In the middle of tile t everyone is done with its keys and with
-  // the values before it; what was asked for one tile ago, the next keys and its values, has to be there.
-  const int tiles = (wg_max + kKeys - 1) / kKeys, open_tiles = wg_min / kKeys;  // no row is masked in the open ones
-  auto step = [&](int t, auto masked) CVS_INLINE {
-    if (t > 0) add_values(t - 1, 1, masked);
-    if constexpr (masked) mask(t, 0);
-    raise_max(s[0], st, a.c);
-    s[1] = scores(t, 1);
-    probabilities(0);
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-    __syncthreads();
-    if (t + 2 < tiles) load_tile(base_k, step_k, lds_k, off_k, t + 2);
-    if (t + 1 < tiles) load_tile(base_v, step_v, lds_v, off_v, t + 1);
-    add_values(t, 0, masked);
-    if constexpr (masked) mask(t, 1);
-    raise_max(s[1], st, a.c);
-    s[0] = scores(t + 1, 0);  // past the last tile: of whatever is there, and not used
-    probabilities(1);
-  };
-  if (tiles > 0) {
-    load_tile(base_k, step_k, lds_k, off_k, 0);
-    load_tile(base_v, step_v, lds_v, off_v, 0);
-    if (tiles > 1) load_tile(base_k, step_k, lds_k, off_k, 1);
-    __builtin_amdgcn_s_waitcnt(0x0F70);
-    __syncthreads();
-    s[0] = scores(0, 0);
-    int t = 0;
-    for (; t < open_tiles; ++t) step(t, std::false_type{});
-    for (; t < tiles; ++t) step(t, std::true_type{});
-    add_values(tiles - 1, 1, std::true_type{});
-  }
-  if (!busy) return;
+  attend_tiles<kBf, NB>(st, q, src, (wg_max + kKeys - 1) / kKeys, wg_min / kKeys, limit, a.c, bad);
+  if (it.row0 + 32 * wave >= rows) return;
   const float l = both_sum(st.l);
   // A row that sees no key gives zeros; one whose keys' weights are all 0 (or NaN) gives what the formula does.
   const float inv = limit > 0 ? 1.f / l : 0.f;
