@@ -99,7 +99,7 @@ struct Work {
     return at(word(a.pages, it.page_first + (t >> a.page_shift)), t);
   }
   __device__ CVS_INLINE const char* at(int64_t page, int t) const {
-    return a.pool + page * a.page_bytes + g * a.head_bytes + (t & ((1 << a.page_shift) - 1)) * (2048 * NB);
+    return a.pool + page * a.page_bytes + g * a.head_bytes + (t & ((1 << a.page_shift) - 1)) * (4096 * NB);
   }
   __device__ CVS_INLINE Row row(int i) const {  // past the last row, the last one's again (not stored)
     const int r = it.row0 + min(i, it.rows - 1), tok = r / a.group;
@@ -126,7 +126,7 @@ struct Work {
   __device__ CVS_INLINE void store(const RowState<NB>& st, float m, float l, const Row& r, int i, bool met) const {
     auto value = [&](int key, int d) CVS_INLINE {
       const int rel = key - it.key0 - kTile * it.tile0, j = rel & 31;
-      const char* const v = tile(rel / kTile) + a.head_bytes / 2;
+      const char* const v = tile(rel / kTile) + 2048 * NB;
       const int at = (d & 31) + 32 * ((j >> 2) & 1), e = 4 * ((j >> 3) & 1) + (j & 3);
       return *reinterpret_cast<const uint16_t*>(v + (2 * (d >> 5) + (j >> 4)) * 1024 + 16 * at + 2 * e);
     };
@@ -199,7 +199,7 @@ __device__ CVS_INLINE void few_rows(const Work<kBf, NB>& w, int wave, char* lds)
   auto load_values = [&](const char* p) CVS_INLINE {
 #pragma unroll
     for (int s = 0; s < 2 * NB; ++s)
-      vf[s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + a.head_bytes / 2 + lane * 16 + s * 1024));
+      vf[s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + 2048 * NB + lane * 16 + s * 1024));
   };
   RowState<NB> st;
   st.init();
@@ -303,7 +303,7 @@ struct PageSource {
   }
   // Called for each tile when the next one's keys have been asked for, or, for the last, its own.
   __device__ CVS_INLINE void load_values(int t) {
-    load((2 * t + 2 < w.it.tiles ? asked[0] : asked[1]) + w.a.head_bytes / 2, to_v + (t & 1) * 2 * kHalf);
+    load((2 * t + 2 < w.it.tiles ? asked[0] : asked[1]) + 2048 * NB, to_v + (t & 1) * 2 * kHalf);
   }
   __device__ CVS_INLINE u32x4 keys(int t, int h, int i) {
     return *reinterpret_cast<const u32x4*>(lds_k + (2 * (t & 1) + h) * kHalf + i * 1024 + w.lane * 16);

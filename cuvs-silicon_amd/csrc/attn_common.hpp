@@ -304,6 +304,11 @@ float scale_log2(float scale, int dim);
 constexpr size_t kUploadBytes = 3840;
 void upload(cvs_context* ctx, void* dst, const void* src, size_t bytes);
 
+// Tokens [begin, end) of a page, rows row0 and on of the caller's arrays.
+struct Span {
+  int32_t page, begin, end, row0;
+};
+
 }  // namespace attn
 }  // namespace cvs
 
@@ -312,7 +317,7 @@ struct cvs_kv_cache {
   cvs_context* ctx = nullptr;
   int layers = 0, kv_heads = 0, dim = 0, type = 0;
   int nb = 0;                  // 32-element blocks of a padded row
-  int64_t head_bytes = 0;      // one head's keys (and, behind them, values) of a page: 2 * page_tokens * 64 nb
+  int64_t head_bytes = 0;      // one head's keys and values of a page: 2 * page_tokens * 64 nb
   int64_t page_bytes = 0;      // kv_heads * head_bytes
   int64_t layer_bytes = 0;     // pages * page_bytes
   char* pool = nullptr;
@@ -325,12 +330,11 @@ struct cvs_kv_plan {
   cvs_kv_cache* cache = nullptr;
   std::vector<int64_t> seqs;
   std::vector<uint64_t> versions;
-  std::vector<int32_t> written;  // the pages that the plan's tokens lie in
+  std::vector<cvs::attn::Span> spans;  // where the tokens lie, a page each
   int64_t tokens = 0;            // of all sequences
   int heads = 0;                 // query heads; 0: for reading and writing alone
   cvs::DeviceBuffer blob;
   // Offsets into the blob, in bytes.
-  int spans = 0;       // of tokens, a page each (kv_cache.hip, Span)
   size_t at_spans = 0;
   int workgroups = 0;  // of attention, a kv head (attn_cached.hip)
   int64_t slots = 0;   // rows of partial results a kv head; 0: every row has one part

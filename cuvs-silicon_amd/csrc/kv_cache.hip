@@ -2,9 +2,9 @@
 // that they may share, and the device work on pages - writing new tokens,
 // reading tokens back, copying pages.
 //
-// Layout of the pool: layer, page, kv head, then the head's keys and its
-// values, each in tiles of 32 tokens.  A tile is a run of 1 KiB blocks that
-// are operands of v_mfma_f32_32x32x16 as they stand, 16 bytes a lane, as the
+// Layout of the pool: layer, page, kv head, then the head's tokens in tiles of
+// 32, the keys of a tile followed by its values.  Either is a run of 1 KiB
+// blocks that are operands of v_mfma_f32_32x32x16 as they stand, 16 bytes a lane, as the
 // datasets' tiles are, so that attention streams whole blocks from memory
 // into operand registers:
 //   keys:   block s holds columns [16 s, 16 s + 16); lane l has token l % 32, columns 16 s + 8 (l / 32) + [0, 8);
@@ -64,92 +64,141 @@ void copy_pages(cvs_kv_cache* cache, const std::vector<kv::PageCopy>& copies) {
   }
 }
 
-// Tokens [begin, end) of a page, rows row0 and on of the caller's arrays.
-struct Span {
-  int32_t page, begin, end, row0;
+// Spans of a small plan go to the kernel as arguments, others are read from the plan's memory.
+constexpr int kInlineSpans = 192;
+struct Spans {
+  Span s[kInlineSpans];
 };
 
 struct MoveArgs {
   char* pool;  // of the first layer
   int64_t layer_bytes, page_bytes, head_bytes;
-  const Span* spans;
+  const Span* spans;  // null: inline
   View k, v;
   int64_t k_layer, v_layer;  // strides of the caller's arrays from layer to layer
-  int page_tokens, dim, kv_heads;
+  int page_tiles, dim, kv_heads;
+  int units;  // spans * page_tiles * kv_heads
 };
 
-// Between rows of the caller's arrays and tiles of the pool, one workgroup a
-// tile of 32 tokens, kv head and layer, through LDS: rows are read and
-// written 16 bytes at a time along the row, tiles along their blocks.  A
-// tile whose tokens the span does not cover keeps its other tokens; a span's
-// tiles belong to one sequence, so no other workgroup touches them.
+// Rows 2 w and 2 w + 1 of an 8 x 8 matrix of 16-bit elements are x[2 w], x[2 w + 1]; transposed in place.
+__device__ CVS_INLINE void transpose8(u32x4 (&x)[8]) {
+  u32x4 y[8];
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      y[c][k] = __builtin_amdgcn_perm(x[2 * k + 1][c / 2], x[2 * k][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+  for (int c = 0; c < 8; ++c) x[c] = y[c];
+}
+
+// Between rows of the caller's arrays and tiles of the pool, one wave a tile
+// of 32 tokens, kv head and layer; no wave waits for another.  Rows are read
+// and written along the row.  Keys change places 16 bytes at a time, through
+// LDS of the wave's own; values by transposing, in a lane's registers, 8
+// columns of the 8 tokens whose elements stand together.  A tile's tokens
+// before the span's keep what they hold, also where their values share 16
+// bytes with new ones; those after it are past the sequence's end.  A wave's
+// loads are all under way at once: of clamped rows, or all under one condition.
 template <int NB, bool kWrite>
-__global__ __launch_bounds__(256) void move_tokens_kernel(const MoveArgs a) {
-  constexpr int D = 32 * NB;
-  __shared__ __align__(16) uint16_t s[2][32][D];
-  const int tiles = a.page_tokens / 32;
-  const Span sp = a.spans[blockIdx.x / tiles];
-  const int tile = blockIdx.x % tiles;
+__global__ __launch_bounds__(256) void move_tokens_kernel(const MoveArgs a, const Spans inl) {
+  constexpr int P = 4 * NB;  // 16-byte pieces of a row
+  __shared__ __align__(16) u32x4 s[4][32 * P];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int unit = blockIdx.x * 4 + wave;
+  if (unit >= a.units) return;
+  const int g = unit % a.kv_heads, tile = unit / a.kv_heads % a.page_tiles, at = unit / a.kv_heads / a.page_tiles;
+  const Span sp = a.spans ? a.spans[at] : inl.s[at];
   const int lo = max(sp.begin - 32 * tile, 0), hi = min(sp.end - 32 * tile, 32);
   if (lo >= hi) return;
-  const int g = blockIdx.y;
-  char* const head = a.pool + blockIdx.z * a.layer_bytes + sp.page * a.page_bytes + g * a.head_bytes;
-  char* const kt = head + int64_t(tile) * 2048 * NB;
-  char* const vt = kt + a.head_bytes / 2;
+  char* const kt = a.pool + blockIdx.y * a.layer_bytes + sp.page * a.page_bytes + g * a.head_bytes +
+                   int64_t(tile) * 4096 * NB;
+  char* const vt = kt + 2048 * NB;
   const int64_t row = int64_t(sp.row0) + 32 * tile - sp.begin;  // of the tile's token 0
-  char* const ks = a.k.p + 2 * (blockIdx.z * a.k_layer + row * a.k.token + g * a.k.head);
-  char* const vs = a.v.p + 2 * (blockIdx.z * a.v_layer + row * a.v.token + g * a.v.head);
+  char* const ks = a.k.p + 2 * (blockIdx.y * a.k_layer + row * a.k.token + g * a.k.head);
+  char* const vs = a.v.p + 2 * (blockIdx.y * a.v_layer + row * a.v.token + g * a.v.head);
+  const int pieces = a.dim / 8;
+  auto held = [&](int t) CVS_INLINE { return min(max(t, lo), hi - 1); };
+
+  // Values: lane = (columns 8 c and on, tokens t0 + {0, 1, 2, 3, 8, 9, 10, 11}).
+  const int c = lane % P, t0 = 16 * (lane / P >> 1) + 4 * (lane / P & 1);
+  const bool mine = lane < 4 * P && t0 < hi && t0 + 11 >= lo;
+  u32x4* const slots = reinterpret_cast<u32x4*>(
+      vt + (2 * (c / 4) + (lane / P >> 1)) * 1024 + (32 * (lane / P & 1) + 8 * (c % 4)) * 16);
+  u32x4 x[8], y[P / 2];
+  auto token = [&](int j) CVS_INLINE { return t0 + 8 * (j / 4) + j % 4; };
   if constexpr (kWrite) {
-    for (int i = threadIdx.x; i < 2 * 32 * 4 * NB; i += 256) {
-      const int which = i / (32 * 4 * NB), t = i / (4 * NB) % 32, p = i % (4 * NB);
-      u32x4 x{};
-      if (t >= lo && t < hi && 8 * p < a.dim)
-        x = which ? *reinterpret_cast<const u32x4*>(vs + 2 * (t * a.v.token + 8 * p))
-                  : *reinterpret_cast<const u32x4*>(ks + 2 * (t * a.k.token + 8 * p));
-      *reinterpret_cast<u32x4*>(&s[which][t][8 * p]) = x;
-    }
-    __syncthreads();
-  }
-  // Keys.
-  for (int i = threadIdx.x; i < 2 * NB * 64; i += 256) {
-    const int t = i & 31, col = 16 * (i >> 6) + 8 * ((i >> 5) & 1);
-    if (t < lo || t >= hi) continue;
-    if constexpr (kWrite)
-      *reinterpret_cast<u32x4*>(kt + 16 * i) = *reinterpret_cast<const u32x4*>(&s[0][t][col]);
-    else
-      *reinterpret_cast<u32x4*>(&s[0][t][col]) = *reinterpret_cast<const u32x4*>(kt + 16 * i);
-  }
-  // Values: 8 tokens of a column.
-  for (int i = threadIdx.x; i < 2 * NB * 64; i += 256) {
-    const int l = i & 63, col = 32 * (i >> 7) + (l & 31), t0 = 16 * ((i >> 6) & 1) + 4 * (l >> 5);
-    if (t0 + 11 < lo || t0 >= hi) continue;
-    const bool whole = t0 >= lo && t0 + 11 < hi;
-    uint16_t x[8] = {};
-    if (!kWrite || !whole) {
-      const u32x4 old = *reinterpret_cast<const u32x4*>(vt + 16 * i);
-      __builtin_memcpy(x, &old, 16);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      x[j] = *reinterpret_cast<const u32x4*>(vs + 2 * (held(token(j)) * a.v.token + 8 * min(c, pieces - 1)));
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) {
+      const int n = 64 * i + lane;
+      y[i] = *reinterpret_cast<const u32x4*>(ks + 2 * (held(n / P) * a.k.token + 8 * min(n % P, pieces - 1)));
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int t = t0 + 8 * (j / 4) + j % 4;
-      if (t < lo || t >= hi) continue;
-      if constexpr (kWrite) x[j] = s[1][t][col];
-      else s[1][t][col] = x[j];
+    for (int j = 0; j < 8; ++j)
+      if (c >= pieces) x[j] = u32x4{};
+    transpose8(x);
+    if (mine && t0 < lo) {
+      uint32_t keep[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) keep[k] = (token(2 * k) < lo ? 0xffffu : 0u) | (token(2 * k + 1) < lo ? 0xffff0000u : 0u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const u32x4 old = slots[j];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[j][k] = (x[j][k] & ~keep[k]) | (old[k] & keep[k]);
+      }
     }
-    if constexpr (kWrite) {
-      u32x4 packed;
-      __builtin_memcpy(&packed, x, 16);
-      *reinterpret_cast<u32x4*>(vt + 16 * i) = packed;
+    if (mine) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) slots[j] = x[j];
     }
-  }
-  if constexpr (!kWrite) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < 2 * 32 * 4 * NB; i += 256) {
-      const int which = i / (32 * 4 * NB), t = i / (4 * NB) % 32, p = i % (4 * NB);
-      if (t < lo || t >= hi || 8 * p >= a.dim) continue;
-      const u32x4 x = *reinterpret_cast<const u32x4*>(&s[which][t][8 * p]);
-      if (which) *reinterpret_cast<u32x4*>(vs + 2 * (t * a.v.token + 8 * p)) = x;
-      else *reinterpret_cast<u32x4*>(ks + 2 * (t * a.k.token + 8 * p)) = x;
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) {
+      const int n = 64 * i + lane, t = n / P, p = n % P;
+      s[wave][t * P + (p ^ (t & 3))] = p < pieces ? y[i] : u32x4{};
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const int t = lane & 31;
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) y[i] = s[wave][t * P + ((2 * i + (lane >> 5)) ^ (t & 3))];
+    if (t >= lo && t < hi) {
+#pragma unroll
+      for (int i = 0; i < P / 2; ++i) *reinterpret_cast<u32x4*>(kt + 1024 * i + 16 * lane) = y[i];
+    }
+  } else {
+    const int t = lane & 31;
+    const bool key = t >= lo && t < hi;
+    if (key) {
+#pragma unroll
+      for (int i = 0; i < P / 2; ++i) y[i] = *reinterpret_cast<const u32x4*>(kt + 1024 * i + 16 * lane);
+    }
+    if (mine) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = slots[j];
+    }
+    if (key) {
+#pragma unroll
+      for (int i = 0; i < P / 2; ++i) s[wave][t * P + ((2 * i + (lane >> 5)) ^ (t & 3))] = y[i];
+    }
+    transpose8(x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (mine && token(j) >= lo && token(j) < hi && c < pieces)
+        *reinterpret_cast<u32x4*>(vs + 2 * (token(j) * a.v.token + 8 * c)) = x[j];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) {
+      const int n = 64 * i + lane, t = n / P, p = n % P;
+      if (t >= lo && t < hi && p < pieces)
+        *reinterpret_cast<u32x4*>(ks + 2 * (t * a.k.token + 8 * p)) = s[wave][t * P + (p ^ (t & 3))];
     }
   }
 }
@@ -172,17 +221,23 @@ void move_tokens(cvs_kv_plan* plan, int first_layer, int layers, const cvs_heads
   if (layers > 1 && (k_layer % 8 != 0 || v_layer % 8 != 0 || k_layer < 0 || v_layer < 0))
     fail(CVS_ERR_UNSUPPORTED, "layer strides must be non-negative multiples of 8 elements");
   if (write)
-    for (const int32_t pg : plan->written)
-      if (c->book->refs(pg) > 1)
+    for (const Span& sp : plan->spans)
+      if (c->book->refs(sp.page) > 1)
         fail(CVS_ERR_INVALID_ARGUMENT, "the plan's tokens lie in a page that sequences share: extend first");
-  if (plan->spans == 0) return;
+  if (plan->spans.empty()) return;
+  const int tiles = int(c->book->page_tokens() / 32);
+  const int64_t units = int64_t(plan->spans.size()) * tiles * c->kv_heads;
+  if (units > (int64_t(1) << 31) - 1) fail(CVS_ERR_UNSUPPORTED, "too many tokens");
+  Spans inl;
+  const bool small = plan->spans.size() <= size_t(kInlineSpans);
+  if (small) std::memcpy(inl.s, plan->spans.data(), plan->spans.size() * sizeof(Span));
   const MoveArgs a{c->pool + first_layer * c->layer_bytes, c->layer_bytes, c->page_bytes, c->head_bytes,
-                   reinterpret_cast<const Span*>(plan->blob.as<char>() + plan->at_spans), view_of(k), view_of(v),
-                   k_layer, v_layer, int(c->book->page_tokens()), c->dim, c->kv_heads};
-  const dim3 grid(unsigned(plan->spans * (c->book->page_tokens() / 32)), unsigned(c->kv_heads), unsigned(layers));
+                   small ? nullptr : reinterpret_cast<const Span*>(plan->blob.as<char>() + plan->at_spans),
+                   view_of(k), view_of(v), k_layer, v_layer, tiles, c->dim, c->kv_heads, int(units)};
+  const dim3 grid(unsigned((units + 3) / 4), unsigned(layers));
   const TimerSpan ts = timer_span(c->ctx, write ? "kv_write" : "kv_read");
   auto go = [&](auto kernel) {
-    hipExtLaunchKernelGGL(kernel, grid, dim3(256), 0, c->ctx->stream, ts.start, ts.stop, 0, a);
+    hipExtLaunchKernelGGL(kernel, grid, dim3(256), 0, c->ctx->stream, ts.start, ts.stop, 0, a, inl);
   };
   switch (c->nb) {
     case 1: write ? go(move_tokens_kernel<1, true>) : go(move_tokens_kernel<1, false>); break;
@@ -398,7 +453,7 @@ int cvs_kv_plan_create(cvs_kv_cache* cache, const int64_t* seqs, const int64_t* 
     plan->cache = cache;
     plan->heads = heads;
     std::vector<int64_t> lengths;
-    std::vector<Span> spans;
+    auto& spans = plan->spans;
     const int64_t pt = book.page_tokens();
     for (int64_t i = 0; i < n; ++i) {
       const kv::Sequence& s = book.at(seqs[i]);
@@ -413,15 +468,15 @@ int cvs_kv_plan_create(cvs_kv_cache* cache, const int64_t* seqs, const int64_t* 
         const int64_t in = t % pt, end = std::min(pt, in + s.length - t);
         const int32_t pg = s.pages[size_t(t / pt)];
         spans.push_back({pg, int32_t(in), int32_t(end), int32_t(plan->tokens)});
-        plan->written.push_back(pg);
         plan->tokens += end - in;
         t += end - in;
       }
     }
-    if (int64_t(spans.size()) * (pt / 32) > (int64_t(1) << 31) - 1) fail(CVS_ERR_UNSUPPORTED, "too many tokens");
-    plan->spans = int(spans.size());
-    std::vector<char> blob(spans.size() * sizeof(Span));
-    if (!spans.empty()) std::memcpy(blob.data(), spans.data(), blob.size());
+    std::vector<char> blob;
+    if (spans.size() > size_t(kInlineSpans)) {
+      blob.resize(spans.size() * sizeof(Span));
+      std::memcpy(blob.data(), spans.data(), blob.size());
+    }
     if (heads > 0) plan_attention(plan.get(), lengths.data(), tokens, blob);
     if (!blob.empty()) {
       plan->blob = take_blob(cache, blob.size());
