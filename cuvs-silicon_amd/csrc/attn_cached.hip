@@ -203,7 +203,7 @@ __device__ CVS_INLINE void few_rows(const Work<kBf, NB>& w, int wave, char* lds)
   };
   RowState<NB> st;
   st.init();
-  uint32_t bad = 0;
+  bool bad = false;
   if (wave < it.tiles) {
     Tiles<kBf, NB> tile(w);
     const char* p = tile(wave);
@@ -222,7 +222,8 @@ __device__ CVS_INLINE void few_rows(const Work<kBf, NB>& w, int wave, char* lds)
         for (int k = 0; k < 16; ++k)
           if (key0 + 8 * (k / 4) + 4 * half + k % 4 >= r.limit) s[k] = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < 2 * NB; ++k) vf[k] = clean<kBf>(w.hide(vf[k], k & 1, key0, it.max_limit), bad);
+        for (int k = 0; k < 2 * NB; ++k) vf[k] = w.hide(vf[k], k & 1, key0, it.max_limit);
+        if (it.min_limit < it.max_limit) bad |= clean<kBf>(vf);
       }
       raise_max(s, st, a.c);
       exponentials(s, st, a.c);
@@ -238,7 +239,7 @@ __device__ CVS_INLINE void few_rows(const Work<kBf, NB>& w, int wave, char* lds)
 
   // The waves' states joined, in the order 0 + 2, 1 + 3, then both.
   s_m[wave][lane] = st.m;
-  const bool met = __syncthreads_or(bad != 0);
+  const bool met = __syncthreads_or(bad);
   float m = s_m[0][lane];
 #pragma unroll
   for (int i = 1; i < kWaves; ++i) m = fmaxf(m, s_m[i][lane]);
@@ -324,15 +325,14 @@ __device__ CVS_INLINE void many_rows(const Work<kBf, NB>& w, int wave, char* lds
   w.load_q(r, q);
   RowState<NB> st;
   st.init();
-  uint32_t bad = 0;
+  bool bad = false;
   // Positions from the segment's first key on.
   const int key0 = it.key0 + kTile * it.tile0, keys = kTile * it.tiles;
   PageSource<kBf, NB> src(w, wave, lds, min(it.max_limit - key0, keys));
-  attend_tiles<kBf, NB>(st, q, src, (it.tiles + 1) / 2, max(0, min(it.min_limit - key0, keys)) / 64,
+  attend_tiles<kBf, NB>(st, q, src, (it.tiles + 1) / 2, max(0, min(it.min_limit - key0, keys)) / 64, it.min_limit < it.max_limit,
                         min(r.limit - key0, keys), w.a.c, bad);
   const float l = both_sum(st.l);
-  const bool met = __ballot(bad != 0) != 0;
-  if (32 * wave < it.rows) w.store(st, st.m, l, r, i, met);
+  if (32 * wave < it.rows) w.store(st, st.m, l, r, i, bad);
 }
 
 template <bool kBf, int NB>

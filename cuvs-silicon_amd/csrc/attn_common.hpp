@@ -72,22 +72,30 @@ __device__ CVS_INLINE float to_float(uint16_t x) {
 
 // Bits 15 and 31 set where the half-word is an infinity or NaN (all exponent
 // bits set: adding one unit of the exponent to the magnitude carries into
-// bit 15, and never past it).
+// bit 15, and never past it); the other bits are anything.
 template <bool kBf>
-__device__ CVS_INLINE uint32_t nonfinite(uint32_t x) {
-  return ((x & 0x7fff7fffu) + (kBf ? 0x00800080u : 0x04000400u)) & 0x80008000u;
+__device__ CVS_INLINE uint32_t carries(uint32_t x) {
+  return (x & 0x7fff7fffu) + (kBf ? 0x00800080u : 0x04000400u);
+}
+template <bool kBf>
+__device__ CVS_INLINE bool nonfinite(uint16_t x) {
+  return (carries<kBf>(x) & 0x8000u) != 0;
 }
 
-// Zeroes the infinities and NaNs of an operand; `bad` collects whether there were any.
-template <bool kBf>
-__device__ CVS_INLINE u32x4 clean(u32x4 v, uint32_t& bad) {
+// Zeroes the infinities and NaNs among a wave's operands; whether there were any.
+template <bool kBf, int N>
+__device__ CVS_INLINE bool clean(u32x4 (&v)[N]) {
+  uint32_t any = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t f = nonfinite<kBf>(v[i]);
-    bad |= f;
-    v[i] &= ~((f >> 15) * 0xffffu);
-  }
-  return v;
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any |= carries<kBf>(v[j][i]);
+  if (__ballot((any & 0x80008000u) != 0) == 0) return false;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[j][i] &= ~((((carries<kBf>(v[j][i]) & 0x80008000u)) >> 15) * 0xffffu);
+  return true;
 }
 
 // Running softmax of a lane's query row over the keys seen so far: m the
@@ -164,7 +172,8 @@ __device__ CVS_INLINE u32x4 prob_operand(const f32x16& p, int step) {
 
 // Attention of a workgroup's 4 x 32 query rows over `tiles` 64-key tiles that
 // go through LDS, double-buffered.  A row sees the keys below `limit`, counted
-// from the first tile; in the first `open_tiles` tiles all rows see all keys.
+// from the first tile; in the first `open_tiles` tiles all rows see all keys,
+// and `mixed` says that the rows' limits differ.
 // The source moves the data: load_keys(t) and load_values(t) ask for a tile of
 // either (buffer t & 1; the workgroup's waves share the work; in ascending
 // order, a tile's values after the next one's keys), keys(t, h, i)
@@ -179,7 +188,7 @@ __device__ CVS_INLINE u32x4 prob_operand(const f32x16& p, int step) {
 // keys and its values, has to be there.
 template <bool kBf, int NB, typename Source>
 __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[2 * NB], Source& src, int tiles,
-                                        int open_tiles, int limit, float c, uint32_t& bad) {
+                                        int open_tiles, bool mixed, int limit, float c, bool& bad) {
   const int half = __lane_id() >> 5;
   f32x16 s[2];    // scores of a tile's two halves
   u32x4 p[2][2];  // and their probabilities
@@ -190,14 +199,19 @@ __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[2 * N
     return x;
   };
   auto add_values = [&](int t, int h, auto masked) CVS_INLINE {
+    if constexpr (!masked) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        u32x4 v = src.values(t, h, b, k);
-        if constexpr (masked) v = clean<kBf>(src.hide(v, t, h, k), bad);
-        st.o[b] = mfma<kBf>(v, p[h][k], st.o[b]);
-      }
+        for (int b = 0; b < NB; ++b) st.o[b] = mfma<kBf>(src.values(t, h, b, k), p[h][k], st.o[b]);
+    } else {
+      u32x4 v[2 * NB];
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) v[i] = src.hide(src.values(t, h, i / 2, i % 2), t, h, i % 2);
+      if (mixed) bad |= clean<kBf>(v);
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) st.o[i / 2] = mfma<kBf>(v[i], p[h][i % 2], st.o[i / 2]);
+    }
   };
   auto mask = [&](int t, int h) CVS_INLINE {
     const int seen = limit - 64 * t - 32 * h - 4 * half;
@@ -279,7 +293,7 @@ __device__ CVS_INLINE void store_nonfinite(int first, int last, int dim, const V
 #pragma unroll 1
     for (int j = first; j < last; ++j) {
       const uint16_t x = value(j, d);
-      if (nonfinite<kBf>(x) != 0) sum += to_float<kBf>(x);
+      if (nonfinite<kBf>(x)) sum += to_float<kBf>(x);
     }
     if (sum != 0.f) store(d, sum);
   }

@@ -92,8 +92,8 @@ struct PromptSource {
     for (int i = 0; i < kLoads; ++i) {
       const int n = first + i * 64, r = n / P, p = n % P;
       const int pk = p ^ swap_k<P>(r), pv = p ^ swap_v<P>(r);
-      off_k[i] = 8 * pk < a.dim ? uint32_t(r * a.k.token * 2 + 16 * pk) : kNowhere;
-      off_v[i] = 8 * pv < a.dim ? uint32_t(r * a.v.token * 2 + 16 * pv) : kNowhere;
+      off_k[i] = 8 * pk < a.dim ? r * uint32_t(2 * a.k.token) + 16 * pk : kNowhere;
+      off_v[i] = 8 * pv < a.dim ? r * uint32_t(2 * a.v.token) + 16 * pv : kNowhere;
       asm("" : "+v"(off_k[i]), "+v"(off_v[i]));  // kept, not computed again for every tile
     }
     // Operand addresses within a buffer: of the keys' pieces 2 i + half (i even and odd: the piece order is swapped
@@ -169,15 +169,15 @@ __global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 3 ? 3 : 4) void prompt_att
   const char* const base_v = src.base_v;
   RowState<NB> st;
   st.init();
-  uint32_t bad = 0;
-  attend_tiles<kBf, NB>(st, q, src, (wg_max + kKeys - 1) / kKeys, wg_min / kKeys, limit, a.c, bad);
+  bool bad = false;
+  attend_tiles<kBf, NB>(st, q, src, (wg_max + kKeys - 1) / kKeys, wg_min / kKeys, wg_min < wg_max, limit, a.c, bad);
   if (it.row0 + 32 * wave >= rows) return;
   const float l = both_sum(st.l);
   // A row that sees no key gives zeros; one whose keys' weights are all 0 (or NaN) gives what the formula does.
   const float inv = limit > 0 ? 1.f / l : 0.f;
   uint16_t* const out = reinterpret_cast<uint16_t*>(a.out.p) + (it.q0 + tok) * a.out.token + head * a.out.head;
   store_row<kBf, NB>(st, inv, out, a.dim, there);
-  if (__ballot(bad != 0))
+  if (bad)
     store_nonfinite<kBf>(
         0, there && l == l ? limit : 0, a.dim,
         [&](int j, int d) CVS_INLINE { return reinterpret_cast<const uint16_t*>(base_v)[j * a.v.token + d]; },
