@@ -98,8 +98,8 @@ __device__ CVS_INLINE bool clean(u32x4 (&v)[N]) {
   return true;
 }
 
-// Running softmax of a lane's query row over the keys seen so far: m the
-// largest log2-scaled score, l this lane's share (its half of the keys) of
+// Running softmax of a lane's query row over the keys seen so far: m a
+// log2-scaled score to count from, l this lane's share (its half of the keys) of
 // the sum of 2^(score - m), o the weighted values.  All in fp32.
 template <int NB>
 struct RowState {
@@ -117,45 +117,60 @@ struct RowState {
 __device__ CVS_INLINE float both_max(float x) { return fmaxf(x, xor_lanes_f(x, 32)); }
 __device__ CVS_INLINE float both_sum(float x) { return x + xor_lanes_f(x, 32); }
 
-// A row's maximum m trails the largest score seen by up to kSlack (in log2
-// units): its values then need rescaling in its first tiles only, and
-// probabilities stay below 2^kSlack, which costs no precision in either type.
-constexpr float kSlack = 6.f;
-
-// Rescales the rows whose maximum a tile of scores passes by more than that.
-// A row that has seen nothing has maximum -inf; 0 stands in for it, so that
-// -inf - (-inf) does not arise.
-template <int NB>
-__device__ CVS_INLINE void raise_max(const f32x16& s, RowState<NB>& st, float c) {
+// A row's largest score among 32 keys, over its two lanes.
+__device__ CVS_INLINE float largest(const f32x16& s, float c) {
   float top = fmaxf(s[0], s[1]);
 #pragma unroll
   for (int r = 2; r < 16; ++r) top = fmaxf(top, s[r]);
-  top = both_max(top) * c;
-  const bool passed = top > st.m + kSlack;
-  if (__ballot(passed)) {
-    const float m = passed ? top : st.m;  // the other rows as they are: a row's result does not depend on them
-    const float alpha = __builtin_amdgcn_exp2f(st.m - (m == -INFINITY ? 0.f : m));
+  return both_max(top) * c;
+}
+
+// Scores of 32 keys -> probabilities 2^(c s - m), summed up.  Masked scores
+// come in as -inf and leave as 0.
+//
+// A row's m is the largest score of its first tile (the caller sets it so), or
+// of a later one, not always the largest of all: as long as the probabilities
+// of a tile sum to no more than kMost a lane, they fit either type and are as
+// precise as any (a larger one has the same number of bits), so m stays and
+// nothing needs rescaling.  The sum is needed anyway, so nearly all tiles take
+// no maximum at all, and the matrix products before are in one block with the
+// exponentials.  Where the sum is larger, or the row has not seen a score yet
+// (m is -inf, and 0 stands in for it, so that -inf - (-inf) does not arise),
+// the row takes the tile's largest score as its m and the tile's probabilities
+// are computed again.
+constexpr float kMost = 4096.f;
+template <int NB>
+__device__ CVS_INLINE void probabilities(f32x16& s, RowState<NB>& st, float c) {
+  f32x16 p;
+  auto exponentials = [&]() CVS_INLINE {
+    const float base = st.m == -INFINITY ? 0.f : st.m;
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -base));
+      sum[r & 1] += p[r];
+    }
+    return sum[0] + sum[1];
+  };
+  float sum = exponentials();
+  const bool over = !(sum <= kMost) || st.m == -INFINITY;
+  if (__ballot(over)) {
+    const float top = largest(s, c);
+    // Either of the row's two lanes (exchanged by all lanes, before any condition); the other rows stay as they are, so
+    // that a row's result depends on itself alone.
+    const uint32_t either = uint32_t(over) | xor_lanes(uint32_t(over), 32);
+    const bool raise = either != 0 && top > st.m;
+    const float alpha = raise ? __builtin_amdgcn_exp2f(st.m - top) : 1.f;
     st.l *= alpha;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) st.o[b][r] *= alpha;
-    st.m = m;
+    st.m = raise ? top : st.m;
+    sum = exponentials();
   }
-}
-
-// Scores -> probabilities 2^(c s - m), summed up.  Masked scores come in as
-// -inf and leave as 0.
-template <int NB>
-__device__ CVS_INLINE void exponentials(f32x16& s, RowState<NB>& st, float c) {
-  const float base = st.m == -INFINITY ? 0.f : st.m;
-  float sum[2] = {0.f, 0.f};
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -base));
-    sum[r & 1] += s[r];
-  }
-  st.l += sum[0] + sum[1];
+  st.l += sum;
+  s = p;
 }
 
 // B operand of the 16 keys `step` (0 or 1) of a probability tile.  The
@@ -219,26 +234,24 @@ __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[2 * N
     for (int r = 0; r < 16; ++r)
       if (8 * (r / 4) + r % 4 >= seen) s[h][r] = -INFINITY;
   };
-  auto probabilities = [&](int h) CVS_INLINE {
-    exponentials(s[h], st, c);
+  auto soften = [&](int h) CVS_INLINE {
+    probabilities(s[h], st, c);
 #pragma unroll
     for (int k = 0; k < 2; ++k) p[h][k] = prob_operand<kBf>(s[h], k);
   };
   auto step = [&](int t, auto masked) CVS_INLINE {
     if (t > 0) add_values(t - 1, 1, masked);
     if constexpr (masked) mask(t, 0);
-    raise_max(s[0], st, c);
     s[1] = scores(t, 1);
-    probabilities(0);
+    soften(0);
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     __syncthreads();
     if (t + 2 < tiles) src.load_keys(t + 2);
     if (t + 1 < tiles) src.load_values(t + 1);
     add_values(t, 0, masked);
     if constexpr (masked) mask(t, 1);
-    raise_max(s[1], st, c);
     s[0] = scores(t + 1, 0);  // past the last tile: of whatever is there, and not used
-    probabilities(1);
+    soften(1);
   };
   if (tiles <= 0) return;
   src.load_keys(0);
@@ -247,6 +260,8 @@ __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[2 * N
   __builtin_amdgcn_s_waitcnt(0x0F70);
   __syncthreads();
   s[0] = scores(0, 0);
+  mask(0, 0);
+  st.m = largest(s[0], c);
   int t = 0;
   for (; t < open_tiles; ++t) step(t, std::false_type{});
   for (; t < tiles; ++t) step(t, std::true_type{});
