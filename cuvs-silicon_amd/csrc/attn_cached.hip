@@ -106,10 +106,7 @@ struct Work {
     return {i < it.rows, g * a.group + r % a.group, a.limits[tok], a.q_rows[tok]};
   }
   __device__ CVS_INLINE void load_q(const Row& r, u32x4 (&q)[2 * NB]) const {
-    const char* src = a.q.p + 2 * (r.q_row * a.q.token + r.head * a.q.head);
-#pragma unroll
-    for (int s = 0; s < 2 * NB; ++s)
-      q[s] = 16 * s + 8 * half < a.dim ? *reinterpret_cast<const u32x4*>(src + 32 * s + 16 * half) : u32x4{};
+    load_row<NB>(a.q.p + 2 * (r.q_row * a.q.token + r.head * a.q.head), a.dim, q);
   }
   // A tile's values that no row sees may be anything (the page's memory as it was): zeros instead.  key0: of the tile.
   __device__ CVS_INLINE u32x4 hide(u32x4 v, int k16, int key0, int end) const {

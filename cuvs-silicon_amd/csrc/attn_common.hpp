@@ -268,6 +268,19 @@ __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[2 * N
   add_values(tiles - 1, 1, std::true_type{});
 }
 
+// A query row as the B operand of the scores' product, zeros past its end.
+// Every lane loads, from within the row: a load under a lane's condition
+// would be waited for before the next one.
+template <int NB>
+__device__ CVS_INLINE void load_row(const char* src, int dim, u32x4 (&q)[2 * NB]) {
+  const int half = __lane_id() >> 5;
+#pragma unroll
+  for (int s = 0; s < 2 * NB; ++s) q[s] = *reinterpret_cast<const u32x4*>(src + min(32 * s + 16 * half, 2 * dim - 16));
+#pragma unroll
+  for (int s = 0; s < 2 * NB; ++s)
+    if (16 * s + 8 * half >= dim) q[s] = u32x4{};
+}
+
 // Writes a lane's half of a row's 32 NB outputs, scaled.  Lanes l and l + 32
 // hold alternate groups of 4 elements; the pair exchanges them so that each
 // stores 16 bytes at a time.

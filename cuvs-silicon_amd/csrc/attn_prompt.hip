@@ -158,14 +158,9 @@ __global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 3 ? 3 : 4) void prompt_att
   // Limits grow with the row, so the first and last row bound the workgroup's.
   const int wg_min = limit_of(it.row0 / a.group), wg_max = limit_of((min(it.row0 + kRows, rows) - 1) / a.group);
 
-  u32x4 q[2 * NB];
-  {
-    const char* src = a.q.p + 2 * ((it.q0 + tok) * a.q.token + head * a.q.head);
-#pragma unroll
-    for (int s = 0; s < 2 * NB; ++s)
-      q[s] = 16 * s + 8 * half < a.dim ? *reinterpret_cast<const u32x4*>(src + 32 * s + 16 * half) : u32x4{};
-  }
   Source src(a, it, g, wave, s_k, s_v);
+  u32x4 q[2 * NB];
+  load_row<NB>(a.q.p + 2 * ((it.q0 + tok) * a.q.token + head * a.q.head), a.dim, q);
   const char* const base_v = src.base_v;
   RowState<NB> st;
   st.init();
