@@ -28,7 +28,7 @@ namespace {
 constexpr int kTile = 32;       // keys of a tile, rows of a wave
 constexpr int kWaves = 4;
 constexpr int kBlock = kTile * kWaves;  // rows of a large block
-constexpr int kJoin = 8;        // parts of a row read at a time
+constexpr int kJoin = 4;        // parts of a row that a lane reads at a time
 
 struct Segment {
   int32_t page_first;     // first of the run's pages in the plan's page list
@@ -355,60 +355,97 @@ struct JoinArgs {
   View out;
   float* lse;
   int64_t q_tokens;
-  int heads, group, dim, nb;
+  int heads, group, dim;
 };
 
-// One wave a (token, head) row, 2 columns a lane, in one pass over the row's
-// parts with a running maximum.
-template <bool kBf>
+// One wave a (token, head) row, in one pass over the row's parts with a
+// running maximum.  A lane takes 4 columns; 8 NB lanes have a part, and the
+// wave's groups of so many take the parts in turn and join at the end.
+template <bool kBf, int NB>
 __global__ __launch_bounds__(256) void join_parts_kernel(const JoinArgs a) {
+  constexpr int kLanes = 8 * NB, kGroups = 64 / kLanes;
   const int64_t i = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (i >= a.rows) return;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, in = lane % kLanes;
+  const int group = min(lane / kLanes, kGroups - 1);  // lanes past the last group repeat it and are not looked at
   const int tok = int(i / a.heads), head = int(i % a.heads);
   const int64_t base = int64_t(head / a.group) * a.slots + tok * a.group + head % a.group;
   const int path = word(a.paths, tok);
   const int64_t q_row = word(a.q_rows, tok);
-  const int d = 2 * lane, width = 32 * a.nb, dl = d < width ? d : 0;
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+  float m = -INFINITY, l = 0.f;
+  float4 o{0.f, 0.f, 0.f, 0.f};
   for (int r = path >> 8, end = r + (path & 255); r < end; ++r) {
     const Parts run = words(a.parts, r);
     const int64_t first = base + run.slot0;
-    for (int p = 0; p < run.count; p += kJoin) {
-      float2 ml[kJoin], o[kJoin];
+    for (int p = group; p < run.count; p += kGroups * kJoin) {
+      float2 ml[kJoin];
+      float4 x[kJoin];
 #pragma unroll
-      for (int k = 0; k < kJoin; ++k) {  // past the last part, that one again with no weight
-        const int64_t at = first + int64_t(min(p + k, run.count - 1)) * run.rows;
+      for (int k = 0; k < kJoin; ++k) {  // past the last part, that one again, and taken out below
+        const int64_t at = first + int64_t(min(p + k * kGroups, run.count - 1)) * run.rows;
         ml[k] = a.part_ml[at];
-        o[k] = *reinterpret_cast<const float2*>(a.part_o + at * width + dl);
+        x[k] = *reinterpret_cast<const float4*>(a.part_o + at * (32 * NB) + 4 * in);
       }
       float top = m;
 #pragma unroll
       for (int k = 0; k < kJoin; ++k) {
-        if (p + k >= run.count) ml[k].x = -INFINITY;
+        if (p + k * kGroups >= run.count) {
+          ml[k].x = -INFINITY;
+          x[k] = float4{0.f, 0.f, 0.f, 0.f};  // no weight times infinity would be no number
+        }
         top = fmaxf(top, ml[k].x);
       }
       const float from = top == -INFINITY ? 0.f : top;
       const float keep = __builtin_amdgcn_exp2f(m - from);
       l *= keep;
-      o0 *= keep;
-      o1 *= keep;
+      o.x *= keep;
+      o.y *= keep;
+      o.z *= keep;
+      o.w *= keep;
 #pragma unroll
       for (int k = 0; k < kJoin; ++k) {
         // A part of no weight has nothing the row sees, or what has underflowed beside the rest.
         const float w = __builtin_amdgcn_exp2f(ml[k].x - from);
         l += w * ml[k].y;
-        o0 += w * o[k].x;
-        o1 += w * o[k].y;
+        o.x += w * x[k].x;
+        o.y += w * x[k].y;
+        o.z += w * x[k].z;
+        o.w += w * x[k].w;
       }
       m = top;
     }
   }
-  const float inv = 1.f / l;
-  if (d < a.dim)
-    *reinterpret_cast<uint32_t*>(a.out.p + 2 * (q_row * a.out.token + head * a.out.head + d)) =
-        pack2<kBf>(o0 * inv, o1 * inv);
-  if (a.lse && lane == 0) a.lse[int64_t(head) * a.q_tokens + q_row] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+  float top = m;
+#pragma unroll
+  for (int k = 0; k < kGroups; ++k) top = fmaxf(top, __shfl(m, k * kLanes + in));
+  const float w = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
+  // In the order of the groups.
+  float sum[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+  const float mine[5] = {w * l, w * o.x, w * o.y, w * o.z, w * o.w};
+#pragma unroll
+  for (int k = 0; k < kGroups; ++k)
+#pragma unroll
+    for (int c = 0; c < 5; ++c) sum[c] += __shfl(mine[c], k * kLanes + in);
+  const float inv = 1.f / sum[0];
+  if (lane < kLanes && 4 * in < a.dim)
+    *reinterpret_cast<uint2*>(a.out.p + 2 * (q_row * a.out.token + head * a.out.head + 4 * in)) =
+        uint2{pack2<kBf>(sum[1] * inv, sum[2] * inv), pack2<kBf>(sum[3] * inv, sum[4] * inv)};
+  if (a.lse && lane == 0) a.lse[int64_t(head) * a.q_tokens + q_row] = (top + __builtin_amdgcn_logf(sum[0])) * kLn2;
+}
+
+template <bool kBf>
+void launch_join(cvs_context* ctx, const JoinArgs& a, int nb) {
+  const TimerSpan ts = timer_span(ctx, "kv_join");
+  auto go = [&](auto kernel) {
+    hipExtLaunchKernelGGL(kernel, dim3(unsigned((a.rows + 3) / 4)), dim3(256), 0, ctx->stream, ts.start, ts.stop, 0, a);
+  };
+  switch (nb) {
+    case 1: go(join_parts_kernel<kBf, 1>); break;
+    case 2: go(join_parts_kernel<kBf, 2>); break;
+    case 3: go(join_parts_kernel<kBf, 3>); break;
+    default: go(join_parts_kernel<kBf, 4>); break;
+  }
+  after_launch("join_parts_kernel");
 }
 
 template <typename T>
@@ -627,12 +664,8 @@ extern "C" int cvs_kv_attention_async(cvs_kv_cache* cache, cvs_kv_plan* plan, in
     const JoinArgs j{reinterpret_cast<const Parts*>(blob + plan->at_parts),
                      reinterpret_cast<const int32_t*>(blob + plan->at_paths),
                      reinterpret_cast<const int32_t*>(blob + plan->at_rows), part_o, part_ml, plan->slots,
-                     plan->tokens * plan->heads, view_of(out), lse, plan->tokens, plan->heads, group, cache->dim,
-                     cache->nb};
-    const TimerSpan ts = timer_span(ctx, "kv_join");
-    const dim3 grid(unsigned((j.rows + 3) / 4));
-    if (is_bf) hipExtLaunchKernelGGL(join_parts_kernel<true>, grid, dim3(256), 0, ctx->stream, ts.start, ts.stop, 0, j);
-    else hipExtLaunchKernelGGL(join_parts_kernel<false>, grid, dim3(256), 0, ctx->stream, ts.start, ts.stop, 0, j);
-    after_launch("join_parts_kernel");
+                     plan->tokens * plan->heads, view_of(out), lse, plan->tokens, plan->heads, group, cache->dim};
+    if (is_bf) launch_join<true>(ctx, j, cache->nb);
+    else launch_join<false>(ctx, j, cache->nb);
   });
 }

@@ -352,6 +352,30 @@ def test_values_in_keys_not_seen(tctx, dtype, value):
     f.cache.close()
 
 
+@pytest.mark.parametrize("at", [0, 4000, 9000, 9003])
+def test_an_infinite_value_in_one_of_many_parts(tctx, at):
+    """Infinite in one column of one key that all rows see: infinite in that column of every row, finite elsewhere, in
+    whichever of a long row's parts it stands (the last key of the shared run and one of a row's own among them)."""
+    def make(seed, *shape):
+        t = rand(seed, *shape, dtype="fp16")
+        if seed % 2 == 0 and shape[1] == 9001 and at <= 9000:  # values: Filled.append makes them with the even seed
+            t[:, at, :, 3] = float("inf")
+        if seed % 2 == 0 and shape[1] != 9001 and at > 9000:
+            t[:, :, :, 3] = float("inf")
+        return t
+
+    f = Filled(tctx, 1, 400, 64, 4, 64, "fp16", 43)
+    (root,) = f.new()
+    f.append([root], [9001], make=make)
+    seqs = f.fork(root, 3)
+    f.append(seqs, [1, 700, 65], make=make)
+    q, out = rand(3, 3, 8, 64, dtype="fp16", spread=0.1), torch.zeros(3, 8, 64, dtype=torch.float16, device="cuda")
+    f.cache.attention_async(f.cache.plan(seqs, [1, 1, 1], heads=8), q, out)
+    assert (out[..., 3] == float("inf")).all()
+    assert torch.isfinite(out[..., :3].float()).all() and torch.isfinite(out[..., 4:].float()).all()
+    f.cache.close()
+
+
 def test_layers_past_4_gib(tctx):
     """Pages whose offsets pass 32 bits, in every kernel: written, copied, read and attended to."""
     page, kv, dim = 4096, 8, 128
