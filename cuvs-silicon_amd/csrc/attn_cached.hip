@@ -106,7 +106,7 @@ struct Work {
     return {i < it.rows, g * a.group + r % a.group, a.limits[tok], a.q_rows[tok]};
   }
   __device__ CVS_INLINE void load_q(const Row& r, u32x4 (&q)[2 * NB]) const {
-    load_row<NB>(a.q.p + 2 * (r.q_row * a.q.token + r.head * a.q.head), a.dim, q);
+    load_row<2 * NB>(a.q.p + 2 * (r.q_row * a.q.token + r.head * a.q.head), a.dim, q);
   }
   // A tile's values that no row sees may be anything (the page's memory as it was): zeros instead.  key0: of the tile.
   __device__ CVS_INLINE u32x4 hide(u32x4 v, int k16, int key0, int end) const {
@@ -326,7 +326,7 @@ __device__ CVS_INLINE void many_rows(const Work<kBf, NB>& w, int wave, char* lds
   // Positions from the segment's first key on.
   const int key0 = it.key0 + kTile * it.tile0, keys = kTile * it.tiles;
   PageSource<kBf, NB> src(w, wave, lds, min(it.max_limit - key0, keys));
-  attend_tiles<kBf, NB>(st, q, src, (it.tiles + 1) / 2, max(0, min(it.min_limit - key0, keys)) / 64, it.min_limit < it.max_limit,
+  attend_tiles<kBf, NB, 2 * NB>(st, q, src, (it.tiles + 1) / 2, max(0, min(it.min_limit - key0, keys)) / 64, it.min_limit < it.max_limit,
                         min(r.limit - key0, keys), w.a.c, bad);
   const float l = both_sum(st.l);
   if (32 * wave < it.rows) w.store(st, st.m, l, r, i, bad);

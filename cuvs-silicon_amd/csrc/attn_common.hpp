@@ -185,7 +185,8 @@ __device__ CVS_INLINE u32x4 prob_operand(const f32x16& p, int step) {
   return r;
 }
 
-// Attention of a workgroup's 4 x 32 query rows over `tiles` 64-key tiles that
+// Attention of a workgroup's 4 x 32 query rows, of KS 16-column steps and NB
+// 32-column blocks, over `tiles` 64-key tiles that
 // go through LDS, double-buffered.  A row sees the keys below `limit`, counted
 // from the first tile; in the first `open_tiles` tiles all rows see all keys,
 // and `mixed` says that the rows' limits differ.
@@ -201,8 +202,8 @@ __device__ CVS_INLINE u32x4 prob_operand(const f32x16& p, int step) {
 // its exponentials.  In the middle of tile t everyone is done with its keys
 // and with the values before it; what was asked for one tile ago, the next
 // keys and its values, has to be there.
-template <bool kBf, int NB, typename Source>
-__device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[2 * NB], Source& src, int tiles,
+template <bool kBf, int NB, int KS, typename Source>
+__device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[KS], Source& src, int tiles,
                                         int open_tiles, bool mixed, int limit, float c, bool& bad) {
   const int half = __lane_id() >> 5;
   f32x16 s[2];    // scores of a tile's two halves
@@ -210,7 +211,7 @@ __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[2 * N
   auto scores = [&](int t, int h) CVS_INLINE {
     f32x16 x{};
 #pragma unroll
-    for (int i = 0; i < 2 * NB; ++i) x = mfma<kBf>(src.keys(t, h, i), q[i], x);
+    for (int i = 0; i < KS; ++i) x = mfma<kBf>(src.keys(t, h, i), q[i], x);
     return x;
   };
   auto add_values = [&](int t, int h, auto masked) CVS_INLINE {
@@ -271,13 +272,13 @@ __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[2 * N
 // A query row as the B operand of the scores' product, zeros past its end.
 // Every lane loads, from within the row: a load under a lane's condition
 // would be waited for before the next one.
-template <int NB>
-__device__ CVS_INLINE void load_row(const char* src, int dim, u32x4 (&q)[2 * NB]) {
+template <int KS>
+__device__ CVS_INLINE void load_row(const char* src, int dim, u32x4 (&q)[KS]) {
   const int half = __lane_id() >> 5;
 #pragma unroll
-  for (int s = 0; s < 2 * NB; ++s) q[s] = *reinterpret_cast<const u32x4*>(src + min(32 * s + 16 * half, 2 * dim - 16));
+  for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const u32x4*>(src + min(32 * s + 16 * half, 2 * dim - 16));
 #pragma unroll
-  for (int s = 0; s < 2 * NB; ++s)
+  for (int s = 0; s < KS; ++s)
     if (16 * s + 8 * half >= dim) q[s] = u32x4{};
 }
 

@@ -134,7 +134,7 @@ struct PromptSource {
   __device__ CVS_INLINE u32x4 hide(u32x4 v, int, int, int) { return v; }  // past the sequence's end are zeros
 };
 
-template <bool kBf, int NB>
+template <bool kBf, int NB, int KS>
 __global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 3 ? 3 : 4) void prompt_attn_kernel(const PromptArgs a) {
   typedef PromptSource<NB> Source;
   __shared__ __align__(16) char s_k[2 * Source::kBuf];
@@ -159,13 +159,13 @@ __global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 3 ? 3 : 4) void prompt_att
   const int wg_min = limit_of(it.row0 / a.group), wg_max = limit_of((min(it.row0 + kRows, rows) - 1) / a.group);
 
   Source src(a, it, g, wave, s_k, s_v);
-  u32x4 q[2 * NB];
-  load_row<NB>(a.q.p + 2 * ((it.q0 + tok) * a.q.token + head * a.q.head), a.dim, q);
+  u32x4 q[KS];
+  load_row<KS>(a.q.p + 2 * ((it.q0 + tok) * a.q.token + head * a.q.head), a.dim, q);
   const char* const base_v = src.base_v;
   RowState<NB> st;
   st.init();
   bool bad = false;
-  attend_tiles<kBf, NB>(st, q, src, (wg_max + kKeys - 1) / kKeys, wg_min / kKeys, wg_min < wg_max, limit, a.c, bad);
+  attend_tiles<kBf, NB, KS>(st, q, src, (wg_max + kKeys - 1) / kKeys, wg_min / kKeys, wg_min < wg_max, limit, a.c, bad);
   if (it.row0 + 32 * wave >= rows) return;
   const float l = both_sum(st.l);
   // A row that sees no key gives zeros; one whose keys' weights are all 0 (or NaN) gives what the formula does.
@@ -187,9 +187,13 @@ void launch(cvs_context* ctx, const PromptArgs& a, int64_t blocks) {
   auto go = [&](auto kernel) {
     hipExtLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(256), 0, ctx->stream, ts.start, ts.stop, 0, a);
   };
-  if (a.dim <= 64) go(prompt_attn_kernel<kBf, 2>);
-  else if (a.dim <= 96) go(prompt_attn_kernel<kBf, 3>);
-  else go(prompt_attn_kernel<kBf, 4>);
+  // Blocks of 32 columns for the values, steps of 16 for the scores: heads of 72 and 80, 104 and 112 go without a step
+  // that would multiply zeros.
+  if (a.dim <= 64) go(prompt_attn_kernel<kBf, 2, 4>);
+  else if (a.dim <= 80) go(prompt_attn_kernel<kBf, 3, 5>);
+  else if (a.dim <= 96) go(prompt_attn_kernel<kBf, 3, 6>);
+  else if (a.dim <= 112) go(prompt_attn_kernel<kBf, 4, 7>);
+  else go(prompt_attn_kernel<kBf, 4, 8>);
   after_launch("prompt_attn_kernel");
 }
 

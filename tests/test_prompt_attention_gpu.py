@@ -58,6 +58,13 @@ def test_ragged(tctx, dtype, causal, heads, kv, dim):
     check(tctx, q, k, v, lengths, None, dtype, causal)
 
 
+@pytest.mark.parametrize("dim", list(range(8, 129, 8)))
+def test_every_head_size(tctx, dim):
+    lengths, dtype = [70, 129, 1], "fp16" if dim % 16 else "bf16"
+    q, k, v = (rand(dim + i, 200, h, dim, dtype=dtype) for i, h in enumerate((6, 2, 2)))
+    check(tctx, q, k, v, lengths, None, dtype, True)
+
+
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 @pytest.mark.parametrize("causal", [True, False])
 def test_key_lengths_of_their_own(tctx, dtype, causal):
