@@ -376,6 +376,54 @@ def test_an_infinite_value_in_one_of_many_parts(tctx, at):
     f.cache.close()
 
 
+@pytest.mark.parametrize("dim,heads", [(64, 8), (128, 4)])
+def test_a_whole_prompt_over_the_cache(tctx, dim, heads):
+    """Many new tokens at once: rows in blocks whose keys end at different places, alone and behind a shared prefix,
+    in one part and in several."""
+    f = Filled(tctx, 1, 120, 32, 2, dim, "bf16", 47)
+    (a,) = f.new()
+    f.append([a], [333])
+    attend(f, [a], [333], heads)
+    kids = f.fork(a, 2, 301)
+    f.append(kids, [150, 7])
+    attend(f, kids + [a], [150, 7, 200], heads)
+    f.append([a], [1500])
+    attend(f, kids + [a], [151, 40, 3], heads)
+    f.cache.close()
+
+
+def test_rows_that_see_nothing_of_a_run(tctx):
+    """New tokens that begin inside the shared run: in the runs behind it the first of them have no key."""
+    f = Filled(tctx, 1, 60, 32, 2, 64, "fp16", 53)
+    (a,) = f.new()
+    f.append([a], [64])
+    kids = f.fork(a, 3)
+    f.append(kids, [100, 33, 500])
+    attend(f, kids, [160, 95, 560], 16)
+    f.cache.close()
+
+
+def test_after_memory_runs_out(tctx):
+    """A cache that does not fit is refused, and the next calls are not told of it again."""
+    with pytest.raises(RuntimeError, match="memory"):
+        tctx.kv_cache(1, 40_000, 4096, 8, 128)
+    f = Filled(tctx, 1, 8, 32, 2, 64, "fp16", 59)
+    (s,) = f.new()
+    f.append([s], [50])
+    attend(f, [s], [1], 4)
+    f.check()
+    f.cache.close()
+
+
+def test_whole_numbers_of_any_kind(tctx):
+    f = Filled(tctx, 1, 8, 32, 2, 64, "fp16", 61)
+    seqs = np.array(f.new(2))
+    f.cache.extend(seqs, torch.tensor([3, 4]))
+    assert f.cache.lengths(seqs) == [3, 4]
+    f.cache.free(seqs)
+    f.cache.close()
+
+
 def test_layers_past_4_gib(tctx):
     """Pages whose offsets pass 32 bits, in every kernel: written, copied, read and attended to."""
     page, kv, dim = 4096, 8, 128

@@ -169,6 +169,15 @@ def test_rows_outside_the_sequences(tctx):
     assert (big[:16] == 3).all() and (big[48:] == 3).all()
 
 
+def test_strides_that_are_not_used(tctx):
+    """A single token or head may have any stride."""
+    q, k, v = (rand(70 + i, 40, h, 64, dtype="fp16") for i, h in enumerate((4, 2, 2)))
+    one = torch.as_strided(q, (1, 4, 64), ((1 << 40) + 3, 64, 1))
+    check(tctx, one, k, v, [1], [40], "fp16", True, out=torch.zeros(1, 4, 64, dtype=torch.float16, device="cuda"))
+    head = torch.as_strided(k, (40, 1, 64), (128, 7, 1))
+    check(tctx, q, head, head, [40], None, "fp16", True)
+
+
 def test_same_bits_again(tctx):
     q, k, v = (rand(40 + i, 700, h, 128, dtype="bf16") for i, h in enumerate((8, 2, 2)))
     plan = tctx.prompt_plan([300, 400], 8, 2)
