@@ -353,7 +353,10 @@ def _i64(a, n=None):
     """A list of whole numbers as a C array."""
     if n is not None and len(a) != n:
         raise ValueError(f"{n} values are needed, {len(a)} given")
-    return (c_int64 * len(a))(*a)
+    try:
+        return (c_int64 * len(a))(*a)
+    except TypeError:  # numpy's or torch's whole numbers
+        return (c_int64 * len(a))(*map(int, a))
 
 
 class Context:

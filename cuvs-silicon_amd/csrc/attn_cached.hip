@@ -166,7 +166,7 @@ struct Tiles {
   __device__ CVS_INLINE void hold(int page) {
     first = page;
     // Lanes past the segment's last page hold that one again.
-    const int last = (w.it.tile0 + w.it.tiles - 1) >> w.a.page_shift;
+    const int last = max(page, (w.it.tile0 + w.it.tiles - 1) >> w.a.page_shift);
     ids = w.a.pages[w.it.page_first + min(page + w.lane, last)];
   }
   __device__ CVS_INLINE const char* operator()(int i) {
@@ -580,7 +580,9 @@ void plan_attention(cvs_kv_plan* plan, const int64_t* lengths, const int64_t* to
           lo = std::min(lo, limits[size_t(t)]);
           hi = std::max(hi, limits[size_t(t)]);
         }
-        segments.push_back({page_first, int32_t(tile), int32_t(std::min(each, run_tiles[r] - tile)),
+        // Not the tiles that none of the block's rows sees; a segment that has no others still writes its (empty) part.
+        const int64_t seen = std::min(run_tiles[r], (hi - s.first * pt + kTile - 1) / kTile);
+        segments.push_back({page_first, int32_t(tile), int32_t(std::clamp<int64_t>(seen - tile, 0, each)),
                             int32_t(s.first * pt), int32_t(t0 * group + row), int32_t(in),
                             int32_t(slots + part * rows + row), lo, hi});
       }
@@ -589,7 +591,8 @@ void plan_attention(cvs_kv_plan* plan, const int64_t* lengths, const int64_t* to
   // The longest first, so that the last workgroups to start are short ones.
   std::stable_sort(segments.begin(), segments.end(),
                    [](const Segment& x, const Segment& y) { return x.tiles > y.tiles; });
-  if (int64_t(segments.size()) * c->kv_heads > (int64_t(1) << 31) - 1) fail(CVS_ERR_UNSUPPORTED, "too much work");
+  if (int64_t(segments.size()) * c->kv_heads > kMaxBlocks || (!one_part && plan->tokens * plan->heads > kMaxBlocks * 4))
+    fail(CVS_ERR_UNSUPPORTED, "too many query rows");
   for (size_t p = 0; p < n; ++p) {
     const size_t at = parts.size();
     for (int32_t r = cur[p]; r >= 0; r = parent[size_t(r)]) parts.push_back(run_parts[size_t(r)]);

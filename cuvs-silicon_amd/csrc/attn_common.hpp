@@ -336,7 +336,13 @@ struct View {
 
 // Checks a view's geometry; `what` names it in messages.
 void check_view(const cvs_heads* x, const char* what);
-inline View view_of(const cvs_heads* x) { return {static_cast<char*>(x->data), x->token_stride, x->head_stride}; }
+inline View view_of(const cvs_heads* x) {
+  // The stride of a single token or head is not looked at.
+  return {static_cast<char*>(x->data), x->tokens > 1 ? x->token_stride : 0, x->heads > 1 ? x->head_stride : 0};
+}
+
+// Workgroups of 256 threads that a launch's x dimension holds.
+constexpr int64_t kMaxBlocks = (int64_t(1) << 24) - 1;
 
 // The softmax scale in log2 units: 0 stands for 1 / sqrt(dim).
 float scale_log2(float scale, int dim);

@@ -209,7 +209,7 @@ void check_view(const cvs_heads* x, const char* what) {
   if (x->tokens > 0 && !x->data) fail(CVS_ERR_INVALID_ARGUMENT, "null data of " + w);
   // The kernels read and write 16 bytes at a time and count rows within 31 bits of bytes.
   const int64_t most = int64_t(1) << 23;
-  if (x->token_stride < 0 || x->head_stride < 0 || x->token_stride > most)
+  if (x->token_stride < 0 || x->head_stride < 0 || (x->tokens > 1 && x->token_stride > most))
     fail(CVS_ERR_UNSUPPORTED, w + ": strides must be non-negative, the tokens' at most 2^23 elements");
   if (reinterpret_cast<uintptr_t>(x->data) % 16 != 0 || (x->tokens > 1 && x->token_stride % 8 != 0) ||
       (x->heads > 1 && x->head_stride % 8 != 0))
@@ -264,7 +264,7 @@ int cvs_prompt_plan_create(cvs_context* ctx, const int64_t* q_lengths, const int
       tq += ql;
       tk += kl;
     }
-    if (int64_t(items.size()) * kv_heads > (int64_t(1) << 31) - 1) fail(CVS_ERR_UNSUPPORTED, "too many rows");
+    if (int64_t(items.size()) * kv_heads > kMaxBlocks) fail(CVS_ERR_UNSUPPORTED, "too many rows");
     // Longest first, so that the last workgroups to start are short ones.
     std::vector<int64_t> order(items.size());
     for (size_t i = 0; i < order.size(); ++i) order[i] = int64_t(i);

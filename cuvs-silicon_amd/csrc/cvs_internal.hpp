@@ -27,6 +27,7 @@ struct Error : std::runtime_error {
 
 inline void check_hip(hipError_t e, const char* what) {
   if (e == hipSuccess) return;
+  (void)hipGetLastError();  // reported here: the next launch's check must not find it again
   const int code = (e == hipErrorOutOfMemory || e == hipErrorMemoryAllocation)
                        ? CVS_ERR_OUT_OF_MEMORY
                        : CVS_ERR_RUNTIME;

@@ -227,7 +227,7 @@ void move_tokens(cvs_kv_plan* plan, int first_layer, int layers, const cvs_heads
   if (plan->spans.empty()) return;
   const int tiles = int(c->book->page_tokens() / 32);
   const int64_t units = int64_t(plan->spans.size()) * tiles * c->kv_heads;
-  if (units > (int64_t(1) << 31) - 1) fail(CVS_ERR_UNSUPPORTED, "too many tokens");
+  if (units > kMaxBlocks * 4) fail(CVS_ERR_UNSUPPORTED, "too many tokens");
   Spans inl;
   const bool small = plan->spans.size() <= size_t(kInlineSpans);
   if (small) std::memcpy(inl.s, plan->spans.data(), plan->spans.size() * sizeof(Span));
