@@ -10,6 +10,7 @@ everything else -> RuntimeError.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import os
 import weakref
@@ -349,14 +350,16 @@ def _lse(ctx: "Context", lse, heads: int, tokens: int):
     return lse.data_ptr()
 
 
-def _i64(a, n=None):
-    """A list of whole numbers as a C array."""
+def _i64(a, n=None) -> array.array:
+    """A list of whole numbers as 64-bit ones."""
     if n is not None and len(a) != n:
         raise ValueError(f"{n} values are needed, {len(a)} given")
-    try:
-        return (c_int64 * len(a))(*a)
-    except TypeError:  # numpy's or torch's whole numbers
-        return (c_int64 * len(a))(*map(int, a))
+    return array.array("q", a)
+
+
+def _at(a: array.array):
+    """The address of its numbers."""
+    return a.buffer_info()[0]
 
 
 class Context:
@@ -800,8 +803,8 @@ class PromptPlan:
         self.handle = None
         n = len(q_lengths)
         h = c_void_p()
-        _check(load().cvs_prompt_plan_create(ctx.handle, _i64(q_lengths),
-                                             None if k_lengths is None else _i64(k_lengths, n), n, int(heads),
+        ql, kl = _i64(q_lengths), None if k_lengths is None else _i64(k_lengths, n)
+        _check(load().cvs_prompt_plan_create(ctx.handle, _at(ql), None if kl is None else _at(kl), n, int(heads),
                                              int(kv_heads), 1 if causal else 0, byref(h)))
         self.handle = h
         ctx._adopt(self)
@@ -858,9 +861,9 @@ class KvCache:
 
     def sequences(self, n: int) -> list:
         """n new sequences without tokens."""
-        ids = (c_int64 * n)()
-        _check(load().cvs_kv_sequence_create(self.handle, n, ids))
-        return list(ids)
+        ids = array.array("q", bytes(8 * n))
+        _check(load().cvs_kv_sequence_create(self.handle, n, _at(ids)))
+        return ids.tolist()
 
     def sequence(self) -> int:
         return self.sequences(1)[0]
@@ -868,33 +871,35 @@ class KvCache:
     def fork(self, parent: int, n: int, length: int = -1) -> list:
         """n new sequences of the parent's first `length` tokens (-1: all), on
         its pages."""
-        ids = (c_int64 * n)()
-        _check(load().cvs_kv_sequence_fork(self.handle, int(parent), int(length), n, ids))
-        return list(ids)
+        ids = array.array("q", bytes(8 * n))
+        _check(load().cvs_kv_sequence_fork(self.handle, int(parent), int(length), n, _at(ids)))
+        return ids.tolist()
 
     def extend(self, seqs, tokens) -> None:
         """Room for tokens[i] more tokens in seqs[i]; RuntimeError and no change
         when the free pages do not suffice."""
         n = len(seqs)
-        _check(load().cvs_kv_sequence_extend(self.handle, _i64(seqs), _i64(tokens, n), n))
+        ids, more = _i64(seqs), _i64(tokens, n)
+        _check(load().cvs_kv_sequence_extend(self.handle, _at(ids), _at(more), n))
 
     def truncate(self, seq: int, length: int) -> None:
         _check(load().cvs_kv_sequence_truncate(self.handle, int(seq), int(length)))
 
     def free(self, seqs) -> None:
-        _check(load().cvs_kv_sequence_free(self.handle, _i64(seqs), len(seqs)))
+        ids = _i64(seqs)
+        _check(load().cvs_kv_sequence_free(self.handle, _at(ids), len(ids)))
 
     def lengths(self, seqs) -> list:
-        out = (c_int64 * len(seqs))()
-        _check(load().cvs_kv_sequence_pages(self.handle, _i64(seqs), len(seqs), out, None, 0, None))
-        return list(out)
+        ids, out = _i64(seqs), array.array("q", bytes(8 * len(seqs)))
+        _check(load().cvs_kv_sequence_pages(self.handle, _at(ids), len(ids), _at(out), None, 0, None))
+        return out.tolist()
 
     def pages(self, seqs) -> np.ndarray:
         """The sequences' page ids, one list behind another."""
-        ids, n, count = _i64(seqs), len(seqs), c_int64(0)
-        _check(load().cvs_kv_sequence_pages(self.handle, ids, n, None, None, 0, byref(count)))
+        ids, count = _i64(seqs), c_int64(0)
+        _check(load().cvs_kv_sequence_pages(self.handle, _at(ids), len(ids), None, None, 0, byref(count)))
         out = np.empty(count.value, np.uint32)
-        _check(load().cvs_kv_sequence_pages(self.handle, ids, n, None, out.ctypes.data, count.value, None))
+        _check(load().cvs_kv_sequence_pages(self.handle, _at(ids), len(ids), None, out.ctypes.data, count.value, None))
         return out
 
     def compact(self) -> int:
@@ -941,7 +946,8 @@ class KvPlan:
         self.handle = None
         n = len(seqs)
         h = c_void_p()
-        _check(load().cvs_kv_plan_create(cache.handle, _i64(seqs), _i64(tokens, n), n, int(heads), byref(h)))
+        ids, newest = _i64(seqs), _i64(tokens, n)
+        _check(load().cvs_kv_plan_create(cache.handle, _at(ids), _at(newest), n, int(heads), byref(h)))
         self.handle = h
         cache._plans.add(self)
 

@@ -76,8 +76,8 @@ struct MoveArgs {
   const Span* spans;  // null: inline
   View k, v;
   int64_t k_layer, v_layer;  // strides of the caller's arrays from layer to layer
-  int page_tiles, dim, kv_heads;
-  int units;  // spans * page_tiles * kv_heads
+  int n_spans, page_tiles, by_tile, dim, kv_heads;
+  int units;  // spans * tiles of a page * kv_heads
 };
 
 // Rows 2 w and 2 w + 1 of an 8 x 8 matrix of 16-bit elements are x[2 w], x[2 w + 1]; transposed in place.
@@ -108,7 +108,11 @@ __global__ __launch_bounds__(256) void move_tokens_kernel(const MoveArgs a, cons
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int unit = blockIdx.x * 4 + wave;
   if (unit >= a.units) return;
-  const int g = unit % a.kv_heads, tile = unit / a.kv_heads % a.page_tiles, at = unit / a.kv_heads / a.page_tiles;
+  // Span by span, or, where spans fill few of a page's tiles, all spans' first tiles, then all second ones, so that
+  // whole ranges of workgroups are without work and not every other one, which would be every other XCD: 64 spans of 9
+  // tokens in pages of 64 are written in 22 us by tiles and 38 by spans, 12 times 700 tokens in 217 and 211.
+  const int g = unit % a.kv_heads, n = unit / a.kv_heads;
+  const int at = a.by_tile ? n % a.n_spans : n / a.page_tiles, tile = a.by_tile ? n / a.n_spans : n % a.page_tiles;
   const Span sp = a.spans ? a.spans[at] : inl.s[at];
   const int lo = max(sp.begin - 32 * tile, 0), hi = min(sp.end - 32 * tile, 32);
   if (lo >= hi) return;
@@ -233,7 +237,8 @@ void move_tokens(cvs_kv_plan* plan, int first_layer, int layers, const cvs_heads
   if (small) std::memcpy(inl.s, plan->spans.data(), plan->spans.size() * sizeof(Span));
   const MoveArgs a{c->pool + first_layer * c->layer_bytes, c->layer_bytes, c->page_bytes, c->head_bytes,
                    small ? nullptr : reinterpret_cast<const Span*>(plan->blob.as<char>() + plan->at_spans),
-                   view_of(k), view_of(v), k_layer, v_layer, tiles, c->dim, c->kv_heads, int(units)};
+                   view_of(k), view_of(v), k_layer, v_layer, int(plan->spans.size()), tiles,
+                   2 * plan->tokens < int64_t(plan->spans.size()) * c->book->page_tokens(), c->dim, c->kv_heads, int(units)};
   const dim3 grid(unsigned((units + 3) / 4), unsigned(layers));
   const TimerSpan ts = timer_span(c->ctx, write ? "kv_write" : "kv_read");
   auto go = [&](auto kernel) {
@@ -448,7 +453,7 @@ int cvs_kv_plan_create(cvs_kv_cache* cache, const int64_t* seqs, const int64_t* 
       fail(CVS_ERR_INVALID_ARGUMENT, "heads must be a multiple of the cache's kv heads (0: no attention)");
     bind(cache->ctx);
     kv::PageBook& book = *cache->book;
-    book.check_ids(seqs, n);
+    const std::vector<kv::Sequence*> found = book.find(seqs, n);
     auto plan = std::make_unique<cvs_kv_plan>();
     plan->cache = cache;
     plan->heads = heads;
@@ -456,7 +461,7 @@ int cvs_kv_plan_create(cvs_kv_cache* cache, const int64_t* seqs, const int64_t* 
     auto& spans = plan->spans;
     const int64_t pt = book.page_tokens();
     for (int64_t i = 0; i < n; ++i) {
-      const kv::Sequence& s = book.at(seqs[i]);
+      const kv::Sequence& s = *found[size_t(i)];
       if (tokens[i] < 0 || tokens[i] > s.length)
         fail(CVS_ERR_INVALID_ARGUMENT, "sequence " + std::to_string(seqs[i]) + " has " + std::to_string(s.length) +
                                            " tokens, the plan asks for " + std::to_string(tokens[i]));

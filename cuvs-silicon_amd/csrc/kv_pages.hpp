@@ -57,14 +57,17 @@ class PageBook {
     return it->second;
   }
 
-  // Each of `n` ids names a sequence, none twice.
-  void check_ids(const int64_t* ids, int64_t n) {
+  // The sequences that `n` ids name, none twice.
+  std::vector<Sequence*> find(const int64_t* ids, int64_t n) {
+    std::vector<Sequence*> found(static_cast<size_t>(n));
     ++mark_;
     for (int64_t i = 0; i < n; ++i) {
       Sequence& s = at(ids[i]);
       if (s.mark == mark_) throw PageError{"sequence " + std::to_string(ids[i]) + " is given twice", false};
       s.mark = mark_;
+      found[size_t(i)] = &s;
     }
+    return found;
   }
 
   int64_t create() {
@@ -94,12 +97,12 @@ class PageBook {
   // Makes room for tokens[i] more tokens in sequence ids[i], in this order; all of it or, when the pages do not
   // suffice, nothing.  Returns the copies that have to be made before the new tokens are written.
   std::vector<PageCopy> extend(const int64_t* ids, const int64_t* tokens, int64_t n) {
-    check_ids(ids, n);
+    const std::vector<Sequence*> seqs = find(ids, n);
     // What it takes: `dropped` counts the holders that a shared page loses to copies earlier in this call.
     int64_t need = 0;
     std::unordered_map<int32_t, int32_t> dropped;
     for (int64_t i = 0; i < n; ++i) {
-      const Sequence& s = at(ids[i]);
+      const Sequence& s = *seqs[size_t(i)];
       if (tokens[i] < 0 || tokens[i] > kMaxTokens - s.length)
         throw PageError{"a sequence of " + std::to_string(s.length) + " tokens cannot grow by " +
                             std::to_string(tokens[i]),
@@ -122,7 +125,7 @@ class PageBook {
     copies.reserve(size_t(n));
     for (int64_t i = 0; i < n; ++i) {
       if (tokens[i] == 0) continue;
-      Sequence& s = at(ids[i]);
+      Sequence& s = *seqs[size_t(i)];
       s.pages.reserve(size_t(pages_for(s.length + tokens[i])));
       if (s.length % page_tokens_ != 0 && refs_[size_t(s.pages.back())] > 1) {
         const int32_t own = take();
@@ -152,9 +155,9 @@ class PageBook {
   }
 
   void release(const int64_t* ids, int64_t n) {
-    check_ids(ids, n);
+    const std::vector<Sequence*> seqs = find(ids, n);
     for (int64_t i = 0; i < n; ++i) {
-      for (const int32_t pg : at(ids[i]).pages) drop(pg);
+      for (const int32_t pg : seqs[size_t(i)]->pages) drop(pg);
       seqs_.erase(ids[i]);
     }
   }
