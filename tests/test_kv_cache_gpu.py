@@ -264,6 +264,28 @@ def test_shared_prefixes(tctx, dtype, new):
     f.cache.close()
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("new,heads", [(1, 8), (3, 2), (40, 4)])
+def test_a_tree_of_long_prefixes(tctx, dtype, new, heads):
+    """The same tree with more tokens than a small batch has: shared runs three deep, joined with what is behind them."""
+    f = Filled(tctx, 1, 300, 32, 2, 64, dtype, 15)
+    (root,) = f.new()
+    f.append([root], [1203])
+    first = f.fork(root, 4) + f.fork(root, 2, 1100) + f.fork(root, 2, 1088) + f.fork(root, 1, 1)
+    f.append(first, [new, new + 3, 70, new, new, 45, new, 90, new])
+    second = f.fork(first[2], 3) + f.fork(first[7], 2, 1100)
+    f.append(second, [new, new + 1, 33 + new, new, new + 64])
+    alone = f.new(2)
+    f.append(alone, [new, 400])
+    seqs = [second[1], alone[0], first[3], first[0], second[4], first[8], alone[1], first[5], second[0], first[1],
+            second[3], first[6], first[4], second[2]]
+    attend(f, seqs, [new] * len(seqs), heads)
+    attend(f, seqs, [1 + i % new for i in range(len(seqs))], heads)
+    same = f.fork(root, 3) + f.fork(root, 1, 1056) + f.fork(root, 2, 1050)
+    attend(f, [root] + same, [new] * 7, heads)
+    f.cache.close()
+
+
 @pytest.mark.parametrize("dtype,heads", [("fp16", 8), ("bf16", 64)])
 def test_long_prefix_split_over_workgroups(tctx, dtype, heads):
     """Thousands of keys for few rows: parts of a row joined, some of them empty for the rows of earlier tokens."""
