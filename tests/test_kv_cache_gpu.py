@@ -469,6 +469,28 @@ def test_layers_past_4_gib(tctx):
     f.cache.close()
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("length", [3, 33, 64, 1500, 9000])
+def test_few_rows_and_a_key_that_only_the_last_sees(tctx, dtype, value, length):
+    """Three new tokens of a sequence, in one part and in several: what the last one holds does not reach the others."""
+    got = []
+    for fill in (0.0, value):
+        def make(seed, *shape):
+            t = rand(seed, *shape, dtype=dtype)
+            t[:, -1] = fill
+            return t
+        f = Filled(tctx, 1, 300, 32, 2, 80, dtype, 67)
+        (s,) = f.new()
+        f.append([s], [length], make=make)
+        out = torch.zeros(3, 4, 80, dtype=TORCH[dtype], device="cuda")
+        f.cache.attention_async(f.cache.plan([s], [3], heads=4), rand(3, 3, 4, 80, dtype=dtype), out)
+        got.append(out.clone())
+        f.cache.close()
+    assert torch.equal(bits(got[0][:2]), bits(got[1][:2]))
+    assert torch.isfinite(got[1][:2].float()).all() and not torch.isfinite(got[1][2].float()).any()
+
+
 def test_same_bits_again(tctx):
     f = Filled(tctx, 1, 200, 64, 2, 128, "bf16", 37)
     (root,) = f.new()
