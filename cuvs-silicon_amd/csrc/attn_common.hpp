@@ -347,6 +347,12 @@ constexpr int64_t kMaxBlocks = (int64_t(1) << 24) - 1;
 // The softmax scale in log2 units: 0 stands for 1 / sqrt(dim).
 float scale_log2(float scale, int dim);
 
+// Memory for a plan: of those that destroyed plans left in `pool`, the
+// smallest that fits, or new.  Plans are made and destroyed at every step of a
+// program; all that reads or writes their memory is on one stream, in order,
+// so it passes from one plan to the next without a wait.
+DeviceBuffer take_blob(std::vector<DeviceBuffer>& pool, int live_plans, size_t bytes);
+
 // Copies host bytes to device memory as arguments of kernels, kUploadBytes a
 // launch: the host buffer is free on return and nothing is pinned, staged or
 // waited for.

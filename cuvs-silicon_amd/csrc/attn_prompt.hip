@@ -233,7 +233,7 @@ struct cvs_prompt_plan {
   int64_t q_tokens = 0, k_tokens = 0;
   int heads = 0, kv_heads = 0, causal = 0;
   int64_t items = 0;
-  void* dev = nullptr;
+  DeviceBuffer blob;
 };
 
 extern "C" {
@@ -281,14 +281,15 @@ int cvs_prompt_plan_create(cvs_context* ctx, const int64_t* q_lengths, const int
     plan->items = int64_t(items.size());
     if (!sorted.empty()) {
       const size_t bytes = sorted.size() * sizeof(PromptItem);
-      CVS_HIP(hipMalloc(&plan->dev, bytes));
+      plan->blob = take_blob(ctx->plan_blobs, ctx->live_prompt_plans, bytes);
       try {
-        upload(ctx, plan->dev, sorted.data(), bytes);
+        upload(ctx, plan->blob.ptr, sorted.data(), bytes);
       } catch (...) {
-        (void)hipFree(plan->dev);
+        ctx->plan_blobs.push_back(plan->blob);
         throw;
       }
     }
+    ++ctx->live_prompt_plans;
     ++ctx->live_children;
     *out_plan = plan.release();
   });
@@ -297,9 +298,9 @@ int cvs_prompt_plan_create(cvs_context* ctx, const int64_t* q_lengths, const int
 int cvs_prompt_plan_destroy(cvs_prompt_plan* plan) {
   return guarded([&] {
     if (!plan) return;
-    bind(plan->ctx);
-    (void)hipStreamSynchronize(plan->ctx->stream);
-    if (plan->dev) (void)hipFree(plan->dev);
+    // Later plans use the memory on the same stream, after whatever still reads it.
+    if (plan->blob.ptr) plan->ctx->plan_blobs.push_back(plan->blob);
+    --plan->ctx->live_prompt_plans;
     --plan->ctx->live_children;
     delete plan;
   });
@@ -329,7 +330,7 @@ int cvs_prompt_attention_async(cvs_context* ctx, const cvs_prompt_plan* plan, co
     const float c = scale_log2(scale, q->head_dim);
     if (plan->items == 0) return;
     const PromptArgs a{view_of(q), view_of(k), view_of(v), view_of(out), lse,
-                       static_cast<const PromptItem*>(plan->dev), plan->q_tokens, plan->kv_heads,
+                       plan->blob.as<PromptItem>(), plan->q_tokens, plan->kv_heads,
                        plan->heads / plan->kv_heads, q->head_dim, plan->causal, c};
     if (q->type == CVS_BF16) launch<true>(ctx, a, plan->items * plan->kv_heads);
     else launch<false>(ctx, a, plan->items * plan->kv_heads);

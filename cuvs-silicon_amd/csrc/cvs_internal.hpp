@@ -94,6 +94,8 @@ struct cvs_context {
   cvs::DeviceBuffer ws_io;        // staging of host queries / results
   cvs::DeviceBuffer ws_teams;     // per-team lists of multi-team graph search
   cvs::DeviceBuffer ws_attn;      // attention over a cache: partial results of split rows
+  std::vector<cvs::DeviceBuffer> plan_blobs;  // memory of destroyed prompt plans, for the next ones
+  int live_prompt_plans = 0;
   // Pinned host memory of kPinnedIoBytes for small blocking calls (host_call);
   // made by the first one.
   char* pinned_io = nullptr;

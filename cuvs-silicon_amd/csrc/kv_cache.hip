@@ -275,9 +275,9 @@ void need_list(const void* p, int64_t n, const char* what) {
   if (n > 0) need(p, what);
 }
 
-// The blob of a destroyed plan that fits, or a new one.
-DeviceBuffer take_blob(cvs_kv_cache* cache, size_t bytes) {
-  auto& pool = cache->blobs;
+}  // namespace
+
+DeviceBuffer take_blob(std::vector<DeviceBuffer>& pool, int live_plans, size_t bytes) {
   size_t best = pool.size();
   for (size_t i = 0; i < pool.size(); ++i)
     if (pool[i].bytes >= bytes && (best == pool.size() || pool[i].bytes < pool[best].bytes)) best = i;
@@ -287,12 +287,10 @@ DeviceBuffer take_blob(cvs_kv_cache* cache, size_t bytes) {
     pool.erase(pool.begin() + int64_t(best));
     return b;
   }
-  cache->blobs.reserve(cache->blobs.size() + size_t(cache->live_plans) + 1);  // destroying a plan does not allocate
+  pool.reserve(pool.size() + size_t(live_plans) + 1);  // destroying a plan does not allocate
   b.reserve(std::max(bytes, size_t(65536)));
   return b;
 }
-
-}  // namespace
 
 void upload(cvs_context* ctx, void* dst, const void* src, size_t bytes) {
   for (size_t at = 0; at < bytes; at += kUploadBytes) {
@@ -484,7 +482,7 @@ int cvs_kv_plan_create(cvs_kv_cache* cache, const int64_t* seqs, const int64_t* 
     }
     if (heads > 0) plan_attention(plan.get(), lengths.data(), tokens, blob);
     if (!blob.empty()) {
-      plan->blob = take_blob(cache, blob.size());
+      plan->blob = take_blob(cache->blobs, cache->live_plans, blob.size());
       try {
         upload(cache->ctx, plan->blob.ptr, blob.data(), blob.size());
       } catch (...) {

@@ -226,6 +226,24 @@ def test_context_of_its_own_stream_and_device_arrays(cvs, ctx):
     assert_within(got, want, tol, "bfloat16 device arrays")
 
 
+def test_plans_made_and_dropped(tctx):
+    """A plan dropped while its call may still run, and the next ones in its memory: nothing waits, nothing mixes."""
+    q, k, v = (rand(80 + i, 900, h, 64, dtype="fp16") for i, h in enumerate((8, 2, 2)))
+    batches = [[900], [450, 450], [1] * 900, [300, 0, 600], [899, 1]]
+    outs = []
+    for lengths in batches * 4:
+        outs.append(torch.zeros_like(q))
+        tctx.prompt_attention_async(tctx.prompt_plan(lengths, 8, 2), q, k, v, outs[-1])
+    for lengths, out in zip(batches, outs[-len(batches):]):
+        kept = tctx.prompt_plan(lengths, 8, 2)
+        again = torch.zeros_like(q)
+        tctx.prompt_attention_async(kept, q, k, v, again)
+        torch.cuda.synchronize()
+        assert torch.equal(out.view(torch.int16), again.view(torch.int16)), lengths
+    for i, out in enumerate(outs):
+        assert torch.equal(out.view(torch.int16), outs[i % len(batches)].view(torch.int16))
+
+
 def test_refusals(cvs, tctx):
     t = 16
     q, k, v = (rand(60 + i, t, h, 64, dtype="fp16") for i, h in enumerate((4, 2, 2)))
