@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 3 ? 3 : 4) void prompt_att
   const int rc = there ? row : rows - 1;
   const int tok = rc / a.group, head = g * a.group + rc % a.group;
   auto limit_of = [&](int t) CVS_INLINE {
-    return a.causal ? max(0, min(it.k_len, t + 1 + it.k_len - it.q_len)) : it.k_len;
+    return a.causal ? max(0, min(it.k_len, it.k_len + (t + 1 - it.q_len))) : it.k_len;
   };
   const int limit = limit_of(tok);
   // Limits grow with the row, so the first and last row bound the workgroup's.
@@ -267,7 +267,8 @@ int cvs_prompt_plan_create(cvs_context* ctx, const int64_t* q_lengths, const int
     for (int64_t i = 0; i < n; ++i) {
       const int64_t ql = q_lengths[i], kl = k_lengths ? k_lengths[i] : ql;
       if (ql < 0 || kl < 0) fail(CVS_ERR_INVALID_ARGUMENT, "negative length");
-      if (tq + ql > kv::PageBook::kMaxTokens || tk + kl > kv::PageBook::kMaxTokens || ql * group > kv::PageBook::kMaxTokens)
+      constexpr int64_t most = kv::PageBook::kMaxTokens;
+      if (ql > most - tq || kl > most - tk || ql > most / group)
         fail(CVS_ERR_UNSUPPORTED, "token and row counts must fit 31 bits");
       for (int64_t row = 0; row < ql * group; row += kRows) {
         items.push_back({int32_t(tq), int32_t(ql), int32_t(tk), int32_t(kl), int32_t(row)});

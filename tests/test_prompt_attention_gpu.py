@@ -297,3 +297,10 @@ def test_plans_end_with_their_context(cvs):
         assert b"plan(s)" in lib.cvs_last_error()
     assert plan.handle is None
     plan.close()
+
+
+def test_lengths_beyond_any_sum(cvs, tctx):
+    top = 2**63 - 1
+    for q, k, heads in (([1, top], None, 2), ([1, 1], [1, top], 2), ([1, 1], [top, top], 1), ([2**62], None, 4)):
+        with pytest.raises(ValueError, match="31 bits"):
+            tctx.prompt_plan(q, heads, 1, k)
