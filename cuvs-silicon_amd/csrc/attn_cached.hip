@@ -45,10 +45,10 @@ struct Segment {
   int32_t min_limit, max_limit;  // keys the rows see: positions below their limit
 };
 
-// The parts that a run gives the rows of one of its sequences: part p of row r
-// has slot slot0 + p * rows + r.
+// The parts that a run gives the rows of its sequences: part p of row r has
+// slot slot0 + p * rows + r.  parent: the run that its pages follow, or -1.
 struct Parts {
-  int32_t slot0, rows, count;
+  int32_t slot0, rows, count, parent;
 };
 
 struct CachedArgs {
@@ -352,8 +352,8 @@ __global__ __launch_bounds__(256, 2) void cached_attn_kernel(const CachedArgs a)
 }
 
 struct JoinArgs {
-  const Parts* parts;      // of a sequence, run by run
-  const int32_t* paths;    // per token, first of its sequence's in `parts` and how many: first * 256 + runs
+  const Parts* parts;      // run by run
+  const int32_t* runs;     // per token, the last of its sequence's
   const int32_t* q_rows;
   const float* part_o;
   const float2* part_ml;
@@ -378,12 +378,13 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const JoinArgs a) {
   const int group = min(lane / kLanes, kGroups - 1);  // lanes past the last group repeat it and are not looked at
   const int tok = int(i / a.heads), head = int(i % a.heads);
   const int64_t base = int64_t(head / a.group) * a.slots + tok * a.group + head % a.group;
-  const int path = word(a.paths, tok);
+  int r = word(a.runs, tok);
   const int64_t q_row = word(a.q_rows, tok);
   float m = -INFINITY, l = 0.f;
   float4 o{0.f, 0.f, 0.f, 0.f};
-  for (int r = path >> 8, end = r + (path & 255); r < end; ++r) {
+  while (r >= 0) {
     const Parts run = words(a.parts, r);
+    r = run.parent;
     const int64_t first = base + run.slot0;
     for (int p = group; p < run.count; p += kGroups * kJoin) {
       float2 ml[kJoin];
@@ -589,18 +590,18 @@ void plan_attention(cvs_kv_plan* plan, const int64_t* lengths, const int64_t* to
   }
 
   std::vector<Segment> segments;
-  std::vector<Parts> run_parts(shared.size()), parts;
-  std::vector<int32_t> pages, paths, cur(n, -1), parent(shared.size());
+  std::vector<Parts> parts(shared.size());
+  std::vector<int32_t> pages, last_runs, cur(n, -1);
   int64_t slots = 0;
   bool one_part = true;
   for (size_t r = 0; r < shared.size(); ++r) {
     const kv::SharedRun& s = shared[r];
     const int64_t t0 = tok0[size_t(s.lo)], count = parts_of(r, share), rows = run_rows[r];
-    parent[r] = cur[size_t(s.lo)];
+    const int32_t parent = cur[size_t(s.lo)];
     for (int64_t p = s.lo; p < s.hi; ++p) cur[size_t(p)] = int32_t(r);
-    if (parent[r] >= 0 || count > 1) one_part = false;
+    if (parent >= 0 || count > 1) one_part = false;
     if (slots + rows * count > kv::PageBook::kMaxTokens) fail(CVS_ERR_UNSUPPORTED, "too many partial results");
-    run_parts[r] = {int32_t(slots - t0 * group), int32_t(rows), int32_t(count)};
+    parts[r] = {int32_t(slots - t0 * group), int32_t(rows), int32_t(count), parent};
     const int32_t page_first = int32_t(pages.size());
     const int32_t* const list = lists[size_t(s.member)];
     pages.insert(pages.end(), list + s.first, list + s.first + s.count);
@@ -626,13 +627,7 @@ void plan_attention(cvs_kv_plan* plan, const int64_t* lengths, const int64_t* to
                    [](const Segment& x, const Segment& y) { return x.tiles > y.tiles; });
   if (int64_t(segments.size()) * c->kv_heads > kMaxBlocks || (!one_part && plan->tokens * plan->heads > kMaxBlocks * 4))
     fail(CVS_ERR_UNSUPPORTED, "too many query rows");
-  for (size_t p = 0; p < n; ++p) {
-    const size_t at = parts.size();
-    for (int32_t r = cur[p]; r >= 0; r = parent[size_t(r)]) parts.push_back(run_parts[size_t(r)]);
-    const size_t runs = parts.size() - at;
-    if (runs > 255 || at >= (size_t(1) << 23)) fail(CVS_ERR_UNSUPPORTED, "prefixes shared in too many levels");
-    for (int64_t t = tok0[p]; t < tok0[p + 1]; ++t) paths.push_back(int32_t(at * 256 + runs));
-  }
+  for (size_t p = 0; p < n; ++p) last_runs.insert(last_runs.end(), size_t(tok0[p + 1] - tok0[p]), cur[p]);
   plan->workgroups = int(segments.size());
   plan->slots = one_part ? 0 : slots;
   plan->at_segments = append(blob, segments);
@@ -640,7 +635,7 @@ void plan_attention(cvs_kv_plan* plan, const int64_t* lengths, const int64_t* to
   plan->at_limits = append(blob, limits);
   plan->at_rows = append(blob, q_rows);
   if (one_part) return;
-  plan->at_paths = append(blob, paths);
+  plan->at_runs = append(blob, last_runs);
   plan->at_parts = append(blob, parts);
 }
 
@@ -698,7 +693,7 @@ extern "C" int cvs_kv_attention_async(cvs_kv_cache* cache, cvs_kv_plan* plan, in
     else launch<false>(ctx, a, cache->nb, blocks);
     if (!slots) return;
     const JoinArgs j{reinterpret_cast<const Parts*>(blob + plan->at_parts),
-                     reinterpret_cast<const int32_t*>(blob + plan->at_paths),
+                     reinterpret_cast<const int32_t*>(blob + plan->at_runs),
                      reinterpret_cast<const int32_t*>(blob + plan->at_rows), part_o, part_ml, plan->slots,
                      plan->tokens * plan->heads, view_of(out), lse, plan->tokens, plan->heads, group, cache->dim};
     if (is_bf) launch_join<true>(ctx, j, cache->nb);

@@ -393,7 +393,7 @@ struct cvs_kv_plan {
   size_t at_spans = 0;
   int workgroups = 0;  // of attention, a kv head (attn_cached.hip)
   int64_t slots = 0;   // rows of partial results a kv head; 0: every row has one part
-  size_t at_segments = 0, at_pages = 0, at_limits = 0, at_rows = 0, at_paths = 0, at_parts = 0;
+  size_t at_segments = 0, at_pages = 0, at_limits = 0, at_rows = 0, at_runs = 0, at_parts = 0;
 };
 
 namespace cvs {

@@ -571,3 +571,15 @@ def test_refusals(tctx, cvs):
     other.close()
     c.close()
     assert plan.handle is None and c.handle is None
+
+
+def test_many_levels_of_shared_prefixes(tctx):
+    f = Filled(tctx, 1, 601, 32, 1, 32, "bf16")
+    (main,) = f.new()
+    forks = []
+    for _ in range(300):
+        f.append([main], [32])
+        forks += f.fork(main, 1)
+    f.append(forks, [1] * 300)
+    attend(f, forks, [1] * 300, 2)
+    f.cache.close()
