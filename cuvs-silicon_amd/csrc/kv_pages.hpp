@@ -121,12 +121,17 @@ class PageBook {
       throw PageError{"the cache has " + std::to_string(free_pages()) + " free pages, " + std::to_string(need) +
                           " are needed",
                       true};
+    // All memory first, so that nothing throws once something has changed.
     std::vector<PageCopy> copies;
     copies.reserve(size_t(n));
     for (int64_t i = 0; i < n; ++i) {
+      std::vector<int32_t>& held = seqs[size_t(i)]->pages;
+      const size_t room = size_t(pages_for(seqs[size_t(i)]->length + tokens[i]));
+      if (room > held.capacity()) held.reserve(std::max(room, 2 * held.capacity()));
+    }
+    for (int64_t i = 0; i < n; ++i) {
       if (tokens[i] == 0) continue;
       Sequence& s = *seqs[size_t(i)];
-      s.pages.reserve(size_t(pages_for(s.length + tokens[i])));
       if (s.length % page_tokens_ != 0 && refs_[size_t(s.pages.back())] > 1) {
         const int32_t own = take();
         copies.push_back({s.pages.back(), own});
