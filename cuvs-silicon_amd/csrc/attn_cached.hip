@@ -667,6 +667,7 @@ extern "C" int cvs_kv_attention_async(cvs_kv_cache* cache, cvs_kv_plan* plan, in
       if (x->head_dim != cache->dim || x->type != cache->type)
         fail(CVS_ERR_INVALID_ARGUMENT, std::string(what) + " must have the cache's head_dim and type");
     }
+    check_rows_apart(out, "out");
     const float c = scale_log2(scale, cache->dim);
     if (plan->workgroups == 0) return;
     const char* const blob = plan->blob.as<char>();

@@ -336,6 +336,8 @@ struct View {
 
 // Checks a view's geometry; `what` names it in messages.
 void check_view(const cvs_heads* x, const char* what);
+// Checks that no two rows of an output lie over each other; layers of them, layer_stride apart.
+void check_rows_apart(const cvs_heads* x, const char* what, int64_t layers = 1, int64_t layer_stride = 0);
 inline View view_of(const cvs_heads* x) {
   // The stride of a single token or head is not looked at.
   return {static_cast<char*>(x->data), x->tokens > 1 ? x->token_stride : 0, x->heads > 1 ? x->head_stride : 0};

@@ -229,6 +229,19 @@ void check_view(const cvs_heads* x, const char* what) {
     fail(CVS_ERR_UNSUPPORTED, w + ": data must be 16-byte aligned, strides multiples of 8 elements");
 }
 
+void check_rows_apart(const cvs_heads* x, const char* what, int64_t layers, int64_t layer_stride) {
+  if (x->tokens == 0) return;
+  // From the axis of the smallest stride on, each has to step over all that the ones before it span.
+  std::pair<int64_t, int64_t> axes[3] = {{x->token_stride, x->tokens}, {x->head_stride, x->heads}, {layer_stride, layers}};
+  std::sort(axes, axes + 3);
+  __int128 span = x->head_dim;
+  for (const auto& [stride, count] : axes) {
+    if (count == 1) continue;
+    if (stride < span) fail(CVS_ERR_INVALID_ARGUMENT, std::string(what) + ": rows of an output must not overlap");
+    span += __int128(stride) * (count - 1);
+  }
+}
+
 float scale_log2(float scale, int dim) {
   if (!(scale >= 0.f) || std::isinf(scale))
     fail(CVS_ERR_INVALID_ARGUMENT, "scale must be finite and positive, or 0 for 1 / sqrt(head_dim)");
@@ -341,6 +354,7 @@ int cvs_prompt_attention_async(cvs_context* ctx, const cvs_prompt_plan* plan, co
       fail(CVS_ERR_INVALID_ARGUMENT, "q, k, v and out must have one head_dim");
     if (q->type != k->type || q->type != v->type || q->type != out->type)
       fail(CVS_ERR_INVALID_ARGUMENT, "q, k, v and out must have one type");
+    check_rows_apart(out, "out");
     const float c = scale_log2(scale, q->head_dim);
     if (plan->items == 0) return;
     const PromptArgs a{view_of(q), view_of(k), view_of(v), view_of(out), lse,

@@ -231,10 +231,13 @@ void move_tokens(cvs_kv_plan* plan, int first_layer, int layers, const cvs_heads
   }
   if (layers > 1 && (k_layer % 8 != 0 || v_layer % 8 != 0 || k_layer < 0 || v_layer < 0))
     fail(CVS_ERR_UNSUPPORTED, "layer strides must be non-negative multiples of 8 elements");
-  if (write)
-    for (const Span& sp : plan->spans)
-      if (c->book->refs(sp.page) > 1)
-        fail(CVS_ERR_INVALID_ARGUMENT, "the plan's tokens lie in a page that sequences share: extend first");
+  if (!write) {
+    check_rows_apart(k, "k", layers, k_layer);
+    check_rows_apart(v, "v", layers, v_layer);
+  }
+  for (const Span& sp : plan->spans)
+    if (write && c->book->refs(sp.page) > 1)
+      fail(CVS_ERR_INVALID_ARGUMENT, "the plan's tokens lie in a page that sequences share: extend first");
   if (plan->spans.empty()) return;
   const int tiles = int(c->book->page_tokens() / 32);
   const int64_t units = int64_t(plan->spans.size()) * tiles * c->kv_heads;

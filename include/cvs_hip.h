@@ -513,7 +513,8 @@ int cvs_cagra_build_reference_ex(cvs_context* ctx, const float* rows, int64_t n,
  * so q, k and v may be views of one projection, and a batch's sequences lie
  * one behind another.  data 16-byte aligned, strides multiples of 8
  * (CVS_ERR_UNSUPPORTED otherwise), token_stride at most 2^23, head_dim a
- * multiple of 8 from 8 to CVS_ATTN_MAX_DIM.  Outputs must not overlap. */
+ * multiple of 8 from 8 to CVS_ATTN_MAX_DIM.  Outputs must not overlap (one
+ * whose own rows do is refused). */
 #define CVS_ATTN_MAX_DIM 128
 typedef struct cvs_heads {
   void* data;

@@ -583,3 +583,30 @@ def test_many_levels_of_shared_prefixes(tctx):
     f.append(forks, [1] * 300)
     attend(f, forks, [1] * 300, 2)
     f.cache.close()
+
+
+def test_rows_of_an_output_that_overlap(tctx):
+    f = Filled(tctx, 3, 4, 32, 2, 16, "fp16")
+    (s,) = f.new()
+    f.append([s], [40])
+    plan = f.cache.plan([s], [40], heads=2)
+    room, other = (torch.zeros(3 * 40 * 64, dtype=torch.float16, device="cuda") for _ in "kv")
+    good = other.as_strided((3, 40, 2, 16), (1280, 32, 16, 1))
+    for strides in ((0, 32, 16), (1272, 32, 16), (16, 32, 16), (1280, 0, 16), (32, 80, 16)):
+        bad = room.as_strided((3, 40, 2, 16), (*strides, 1))
+        for k, v in ((bad, good), (good, bad)):
+            with pytest.raises(ValueError, match="must not overlap"):
+                f.cache.read_async(plan, k, v)
+    for strides in ((1280, 32, 16), (32, 96, 16), (16, 96, 48), (40, 120, 16)):  # layers outermost, between, innermost
+        k = room.zero_().as_strided((3, 40, 2, 16), (*strides, 1))
+        f.cache.read_async(plan, k, good)
+        assert torch.equal(k, f.held[s][0]) and torch.equal(good, f.held[s][1]), strides
+    q = rand(3, 40, 2, 16, dtype="fp16")
+    with pytest.raises(ValueError, match="must not overlap"):
+        f.cache.attention_async(plan, q, room.as_strided((40, 2, 16), (16, 16, 1)), 0)
+    # Inputs may: one row for all tokens and layers.
+    row = rand(4, 1, 1, 1, 16, dtype="fp16").expand(3, 40, 2, 16)
+    f.cache.write_async(plan, row, row)
+    f.cache.read_async(plan, good, room.as_strided((3, 40, 2, 16), (1280, 32, 16, 1)))
+    assert torch.equal(good, row)
+    f.cache.close()

@@ -304,3 +304,18 @@ def test_lengths_beyond_any_sum(cvs, tctx):
     for q, k, heads in (([1, top], None, 2), ([1, 1], [1, top], 2), ([1, 1], [top, top], 1), ([2**62], None, 4)):
         with pytest.raises(ValueError, match="31 bits"):
             tctx.prompt_plan(q, heads, 1, k)
+
+
+def test_rows_of_an_output_that_overlap(tctx):
+    plan = tctx.prompt_plan([5, 4], 2, 1)
+    q, k, v = (rand(i, 9, h, 16, dtype="fp16") for i, h in enumerate((2, 1, 1)))
+    room = torch.zeros(9 * 64, dtype=torch.float16, device="cuda")
+    for strides in ((0, 16), (32, 0), (16, 16), (8, 144), (32, 8), (16, 136)):
+        with pytest.raises(ValueError, match="must not overlap"):
+            tctx.prompt_attention_async(plan, q, k, v, room.as_strided((9, 2, 16), (*strides, 1)))
+    want = torch.empty_like(q)
+    tctx.prompt_attention_async(plan, q, k, v, want)
+    for strides in ((32, 16), (48, 24), (16, 144), (64, 16), (24, 216)):  # token by token, head by head, with gaps
+        out = room.zero_().as_strided((9, 2, 16), (*strides, 1))
+        tctx.prompt_attention_async(plan, q, k, v, out)
+        assert torch.equal(out, want), strides
