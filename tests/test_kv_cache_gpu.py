@@ -610,3 +610,48 @@ def test_rows_of_an_output_that_overlap(tctx):
     f.cache.read_async(plan, good, room.as_strided((3, 40, 2, 16), (1280, 32, 16, 1)))
     assert torch.equal(good, row)
     f.cache.close()
+
+
+def test_captured_and_replayed(cvs):
+    """A step's calls in a graph, replayed over changed inputs, against the same calls outside it, bit for bit."""
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        ctx = cvs.Context(0, stream=stream.cuda_stream)
+        f = Filled(ctx, 2, 96, 32, 2, 64, "bf16")
+        (root,) = f.new()
+        f.append([root], [2000])
+        seqs = f.fork(root, 3)
+        f.append(seqs, [1, 40, 7])
+        f.cache.extend(seqs, [1, 1, 1])
+        step, prompt = f.cache.plan(seqs, [1, 1, 1], heads=8), ctx.prompt_plan([1, 0, 2], 8, 2)
+        q, k, v = (torch.empty(3, h, 64, dtype=torch.bfloat16, device="cuda") for h in (8, 2, 2))
+        outs = [torch.empty_like(q), torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)]
+
+        def calls():
+            f.cache.write_async(step, k, v, layer=1)
+            f.cache.attention_async(step, q, outs[0], layer=1)
+            ctx.prompt_attention_async(prompt, q, k, v, outs[1])
+            f.cache.read_async(step, outs[2], outs[3], layer=1)
+
+        def fill(seed):
+            for i, x in enumerate((q, k, v)):
+                x.copy_(rand(seed + i, *x.shape, dtype="bf16"))
+
+        fill(1)
+        calls()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            calls()
+        for seed in (10, 20, 30, 40):
+            fill(seed)
+            calls()
+            want = [x.clone() for x in outs]
+            for x in outs:
+                x.fill_(9.0)
+            graph.replay()
+            stream.synchronize()
+            for x, y in zip(outs, want):
+                assert torch.equal(bits(x), bits(y)), seed
+        f.cache.close()
+        ctx.close()
