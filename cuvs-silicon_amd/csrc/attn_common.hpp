@@ -189,7 +189,8 @@ __device__ CVS_INLINE u32x4 prob_operand(const f32x16& p, int step) {
 // 32-column blocks, over `tiles` 64-key tiles that go through LDS,
 // double-buffered.  A row sees the keys below `limit`, counted from the first
 // tile; in the first `open_tiles` tiles all rows see all keys, and `mixed` says
-// that the rows' limits differ.
+// that the tiles behind them may hold values that `hide` leaves and that some
+// row does not see.
 // The source moves the data: load_keys(t) and load_values(t) ask for a tile of
 // either (buffer t & 1; the workgroup's waves share the work; in ascending
 // order, a tile's values after the next one's keys), keys(t, h, i)

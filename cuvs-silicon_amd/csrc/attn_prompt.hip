@@ -178,7 +178,9 @@ __global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 3 ? 3 : 4) void prompt_att
   RowState<NB> st;
   st.init();
   bool bad = false;
-  attend_tiles<kBf, NB, KS>(st, q, src, (wg_max + kKeys - 1) / kKeys, wg_min / kKeys, wg_min < wg_max, limit, a.c, bad);
+  // Keys between the first row's limit and the sequence's end: not only where limits differ, as the rows of a block may
+  // all be one token's (128 and more heads on a kv head).
+  attend_tiles<kBf, NB, KS>(st, q, src, (wg_max + kKeys - 1) / kKeys, wg_min / kKeys, wg_min < it.k_len, limit, a.c, bad);
   if (it.row0 + 32 * wave >= rows) return;
   const float l = both_sum(st.l);
   // A row that sees no key gives zeros; one whose keys' weights are all 0 (or NaN) gives what the formula does.
