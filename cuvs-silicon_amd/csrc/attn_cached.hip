@@ -228,8 +228,8 @@ __device__ CVS_INLINE void few_rows(const Work<kBf, NB>& w, int wave, char* lds)
         for (int k = 0; k < 2 * NB; ++k) vf[k] = w.hide(vf[k], k & 1, key0, it.max_limit);
         if (it.min_limit < it.max_limit) bad |= clean<kBf>(vf);
       }
-      if (i == wave) st.m = largest(s, a.c);
-      probabilities(s, st, a.c);
+      if (i == wave) st.m = largest(s, a.c) - kLift<kBf>;
+      probabilities<kBf>(s, st, a.c);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const u32x4 pr = prob_operand<kBf>(s, h);

@@ -99,7 +99,7 @@ __device__ CVS_INLINE bool clean(u32x4 (&v)[N]) {
 }
 
 // Running softmax of a lane's query row over the keys seen so far: m a
-// log2-scaled score to count from, l this lane's share (its half of the keys) of
+// log2-scaled score, or a little less (kLift), to count from, l this lane's share (its half of the keys) of
 // the sum of 2^(score - m), o the weighted values.  All in fp32.
 template <int NB>
 struct RowState {
@@ -128,18 +128,31 @@ __device__ CVS_INLINE float largest(const f32x16& s, float c) {
 // Scores of 32 keys -> probabilities 2^(c s - m), summed up.  Masked scores
 // come in as -inf and leave as 0.
 //
-// A row's m is the largest score of its first tile (the caller sets it so), or
-// of a later one, not always the largest of all: as long as the probabilities
-// of a tile sum to no more than kMost a lane, they fit either type and are as
-// precise as any (a larger one has the same number of bits), so m stays and
-// nothing needs rescaling.  The sum is needed anyway, so nearly all tiles take
-// no maximum at all, and the matrix products before are in one block with the
-// exponentials.  Where the sum is larger, or the row has not seen a score yet
-// (m is -inf, and 0 stands in for it, so that -inf - (-inf) does not arise),
-// the row takes the tile's largest score as its m and the tile's probabilities
-// are computed again.
-constexpr float kMost = 4096.f;
-template <int NB>
+// A row's m is a score's: of its first tile's largest (the caller sets it so),
+// or of a later tile's, not always of the largest of all: as long as the
+// probabilities of a tile sum to no more than kMost a lane, they fit the type
+// that they are rounded to and are as precise as any (a larger one has the same
+// number of bits), so m stays and nothing needs rescaling.  The sum is needed
+// anyway, so nearly all tiles take no maximum at all, and the matrix products
+// before are in one block with the exponentials.  Where the sum is larger, or
+// the row has not seen a score yet (m is -inf, and 0 stands in for it, so that
+// -inf - (-inf) does not arise), the row takes its m from the tile's largest
+// score and the tile's probabilities are computed again.
+//
+// bf16 has the range of fp32, and m is the score itself.  fp16 ends at 2^-24, so
+// m stands kLift below the score, whose probability is then 2^kLift: those of
+// 2^-22 of it keep all bits, and smaller ones are off by 2^-33 of it at most
+// (counted from 1, 100,000 keys of 2^-26 each beside one heavy key were all
+// rounded to 0).  What kLift takes from the room above it costs rows that meet
+// much larger scores late: 8,000 causal tokens, 16/4 heads of 64, take 161 us at
+// a lift of 0, 8 or 10 where scores are spread by 1, and 162, 170 or 176 us where
+// they are spread by 2.6 (natural units).  A tile that sums to more than kMost
+// has a probability above kMost / 16 > 2^(kLift + 1), so its row does rise.
+template <bool kBf>
+constexpr float kLift = kBf ? 0.f : 8.f;
+template <bool kBf>
+constexpr float kMost = kBf ? 4096.f : 65504.f;
+template <bool kBf, int NB>
 __device__ CVS_INLINE void probabilities(f32x16& s, RowState<NB>& st, float c) {
   f32x16 p;
   auto exponentials = [&]() CVS_INLINE {
@@ -153,9 +166,9 @@ __device__ CVS_INLINE void probabilities(f32x16& s, RowState<NB>& st, float c) {
     return sum[0] + sum[1];
   };
   float sum = exponentials();
-  const bool over = !(sum <= kMost) || st.m == -INFINITY;
+  const bool over = !(sum <= kMost<kBf>) || st.m == -INFINITY;
   if (__ballot(over)) {
-    const float top = largest(s, c);
+    const float top = largest(s, c) - kLift<kBf>;
     // Either of the row's two lanes (exchanged by all lanes, before any condition); the other rows stay as they are, so
     // that a row's result depends on itself alone.
     const uint32_t either = uint32_t(over) | xor_lanes(uint32_t(over), 32);
@@ -175,8 +188,9 @@ __device__ CVS_INLINE void probabilities(f32x16& s, RowState<NB>& st, float c) {
 
 // B operand of the 16 keys `step` (0 or 1) of a probability tile.  The
 // probabilities are rounded to the values' type here, the product's operand
-// type: each is off by at most half a unit of its own last place, which the
-// sum over keys averages; the sum l keeps them unrounded.
+// type: each is off by at most half a unit of its own last place (in fp16, of
+// 2^-24 for those below 2^-14), which the sum over keys averages; the sum l
+// keeps them unrounded.
 template <bool kBf>
 __device__ CVS_INLINE u32x4 prob_operand(const f32x16& p, int step) {
   u32x4 r;
@@ -237,7 +251,7 @@ __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[KS], 
       if (8 * (r / 4) + r % 4 >= seen) s[h][r] = -INFINITY;
   };
   auto soften = [&](int h) CVS_INLINE {
-    probabilities(s[h], st, c);
+    probabilities<kBf>(s[h], st, c);
 #pragma unroll
     for (int k = 0; k < 2; ++k) p[h][k] = prob_operand<kBf>(s[h], k);
   };
@@ -263,7 +277,7 @@ __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[KS], 
   __syncthreads();
   s[0] = scores(0, 0);
   mask(0, 0);
-  st.m = largest(s[0], c);
+  st.m = largest(s[0], c) - kLift<kBf>;
   int t = 0;
   for (; t < open_tiles; ++t) step(t, std::false_type{});
   for (; t < tiles; ++t) step(t, std::true_type{});

@@ -502,8 +502,11 @@ int cvs_cagra_build_reference_ex(cvs_context* ctx, const float* rows, int64_t n,
  * a query that sees no key gets zeros and lse = -inf.  Products take fp16 or
  * bf16 operands and accumulate in fp32, the softmax's maxima and sums are
  * fp32, probabilities are rounded to the operands' type for the second
- * product and the output once.  Keys and values a query does not see do not
- * reach its result, infinities and NaNs included. */
+ * product and the output once; in fp16 the weights below 2^-22 of a row's
+ * largest are off by up to 2^-33 of it.  Keys and values a query does not see
+ * do not reach its result, infinities and NaNs included; an infinite value
+ * that it sees is its element's result, or NaN where its weight underflows
+ * (below 2^-33 of the largest in fp16, 2^-126 in bf16). */
 
 #define CVS_FP16 0 /* IEEE half */
 #define CVS_BF16 1 /* bfloat16 */
