@@ -133,14 +133,17 @@ struct Work {
       const int at = (d & 31) + 32 * ((j >> 2) & 1), e = 4 * ((j >> 3) & 1) + (j & 3);
       return *reinterpret_cast<const uint16_t*>(v + (2 * (d >> 5) + (j >> 4)) * 1024 + 16 * at + 2 * e);
     };
-    const int first = it.key0 + kTile * it.tile0;
-    const int last = r.there && l == l ? min(first + kTile * it.tiles, r.limit) : 0;
+    const int key0 = it.key0 + kTile * it.tile0, keys = kTile * it.tiles;
+    const int first = key0 + first_cleaned(it.min_limit - key0, keys);
+    const int last = r.there && l == l ? min(key0 + keys, r.limit) : 0;
     if (a.slots == 0) {
       uint16_t* const out = reinterpret_cast<uint16_t*>(a.out.p) + r.q_row * a.out.token + r.head * a.out.head;
       store_row<kBf, NB>(st, 1.f / l, out, a.dim, r.there);
       if (met)
-        store_nonfinite<kBf>(first, last, a.dim, value,
-                             [&](int d, float x) CVS_INLINE { out[d] = uint16_t(pack2<kBf>(x, x)); });
+        add_nonfinite<kBf>(first, last, a.dim, value, [&](int d, float x) CVS_INLINE {
+          x += to_float<kBf>(out[d]);
+          out[d] = uint16_t(pack2<kBf>(x, x));
+        });
       if (a.lse && r.there && half == 0)
         a.lse[int64_t(r.head) * a.q_tokens + r.q_row] = (m + __builtin_amdgcn_logf(l)) * kLn2;
       return;
@@ -156,7 +159,7 @@ struct Work {
               float4{st.o[b][4 * j], st.o[b][4 * j + 1], st.o[b][4 * j + 2], st.o[b][4 * j + 3]};
       if (half == 0) a.part_ml[slot] = float2{m, l};
     }
-    if (met) store_nonfinite<kBf>(first, last, a.dim, value, [&](int d, float x) CVS_INLINE { o[d] = x; });
+    if (met) add_nonfinite<kBf>(first, last, a.dim, value, [&](int d, float x) CVS_INLINE { o[d] += x; });
   }
 };
 

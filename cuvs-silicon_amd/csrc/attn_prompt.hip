@@ -188,10 +188,13 @@ __global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 3 ? 3 : 4) void prompt_att
   uint16_t* const out = reinterpret_cast<uint16_t*>(a.out.p) + (it.q0 + tok) * a.out.token + head * a.out.head;
   store_row<kBf, NB>(st, inv, out, a.dim, there);
   if (bad)
-    store_nonfinite<kBf>(
-        0, there && l == l ? limit : 0, a.dim,
+    add_nonfinite<kBf>(
+        first_cleaned(wg_min, wg_max), there && l == l ? limit : 0, a.dim,
         [&](int j, int d) CVS_INLINE { return reinterpret_cast<const uint16_t*>(base_v)[j * a.v.token + d]; },
-        [&](int d, float x) CVS_INLINE { out[d] = uint16_t(pack2<kBf>(x, x)); });
+        [&](int d, float x) CVS_INLINE {
+          x += to_float<kBf>(out[d]);
+          out[d] = uint16_t(pack2<kBf>(x, x));
+        });
   if (a.lse && there && half == 0)
     a.lse[int64_t(head) * a.q_tokens + it.q0 + tok] = limit > 0 ? (st.m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
 }
