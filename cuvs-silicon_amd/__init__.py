@@ -13,6 +13,7 @@ from __future__ import annotations
 import array
 import ctypes
 import os
+import sys
 import weakref
 from ctypes import POINTER, byref, c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
 
@@ -151,6 +152,7 @@ ATTN_MAX_DIM = 128
 
 _HEADS = POINTER(Heads)
 _SIGNATURES["cvs_context_create_on_stream"] = (c_int, [c_int, c_void_p, POINTER(c_void_p)])
+_SIGNATURES["cvs_context_stream"] = (c_int, [c_void_p, POINTER(c_void_p)])
 _SIGNATURES["cvs_prompt_plan_create"] = (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int,
                                                  POINTER(c_void_p)])
 _SIGNATURES["cvs_prompt_plan_destroy"] = (c_int, [c_void_p])
@@ -306,9 +308,12 @@ _HEAD_TYPES = {"float16": FP16, "torch.float16": FP16, "fp16": FP16, "half": FP1
 
 
 def _head_type(dtype) -> int:
-    t = _HEAD_TYPES.get(str(dtype))
+    t = _HEAD_TYPES.get(dtype)
     if t is None:
-        raise ValueError(f"type {dtype}: attention takes float16 or bfloat16")
+        t = _HEAD_TYPES.get(str(dtype))
+        if t is None:
+            raise ValueError(f"type {dtype}: attention takes float16 or bfloat16")
+        _HEAD_TYPES[dtype] = t  # a torch dtype's name takes longer to make than all else here
     return t
 
 
@@ -325,7 +330,7 @@ def _heads(ctx: "Context", x, what: str, layered: bool = False):
         ptr, stride = x.ptr.value, (shape[-2] * shape[-1], shape[-1])
         layer = shape[-3] * stride[0] if nd == 4 else 0
     elif hasattr(x, "data_ptr"):
-        if not x.is_cuda or x.device.index != ctx.device:
+        if not x.is_cuda or x.get_device() != ctx.device:
             raise ValueError(f"{what} must be on the context's device")
         st = x.stride()
         if st[-1] != 1 and shape[-1] > 1:
@@ -350,6 +355,14 @@ def _lse(ctx: "Context", lse, heads: int, tokens: int):
     return lse.data_ptr()
 
 
+def _raw_stream(torch, device: int) -> int:
+    """The address of torch's current stream."""
+    try:
+        return torch._C._cuda_getCurrentRawStream(device)  # a twentieth of the time of making the stream's object
+    except AttributeError:
+        return torch.cuda.current_stream(device).cuda_stream
+
+
 def _i64(a, n=None) -> array.array:
     """A list of whole numbers as 64-bit ones."""
     if n is not None and len(a) != n:
@@ -366,7 +379,12 @@ class Context:
     """One device + one HIP stream (C: cvs_context).  stream: None for a
     stream of its own, or the address of a HIP stream of the caller's (a torch
     stream's cuda_stream) that the context works on, in order with the
-    caller's own work there."""
+    caller's own work there.
+
+    Calls on torch tensors are in order with torch's current stream of the
+    device: where that is not the context's, the context's waits for what is
+    on it before the call, and it waits for the call.  DeviceArrays are in
+    order on the context's stream alone."""
 
     def __init__(self, device: int = 0, stream: int = None):
         h = c_void_p()
@@ -376,10 +394,34 @@ class Context:
             _check(load().cvs_context_create_on_stream(int(device), c_void_p(int(stream)), byref(h)))
         self.handle = h
         self.device = int(device)
+        p = c_void_p()
+        _check(load().cvs_context_stream(h, byref(p)))
+        self.stream = p.value or 0
         # What was made on this context (datasets, graph indexes, caches,
         # prompt plans): the C library refuses to destroy a context that still
         # owns any, so close() closes the live ones first.
         self._children = weakref.WeakSet()
+
+    def _behind_torch(self, *arrays):
+        """Before a call on these arrays: if some are torch tensors and torch's
+        current stream is not the context's, the context's stream waits for it.
+        Returns what the call has to be followed by: None or a function that
+        makes torch's stream wait for the call."""
+        for x in arrays:
+            if x is not None and not isinstance(x, DeviceArray):
+                break
+        else:
+            return None
+        if self.handle is None:
+            return None  # closed: the call refuses
+        torch = sys.modules["torch"]
+        if _raw_stream(torch, self.device) == self.stream:
+            return None
+        theirs = torch.cuda.current_stream(self.device)
+        ours = (torch.cuda.ExternalStream(self.stream, device=self.device) if self.stream
+                else torch.cuda.default_stream(self.device))
+        ours.wait_stream(theirs)
+        return lambda: theirs.wait_stream(ours)
 
     def _adopt(self, child) -> None:
         self._children.add(child)
@@ -471,8 +513,11 @@ class Context:
         head_dim); lse, when given, (heads, query tokens) float32; scale 0:
         1 / sqrt(head_dim)."""
         hq, hk, hv, ho = (_heads(self, x, w)[0] for x, w in ((q, "q"), (k, "k"), (v, "v"), (out, "out")))
-        _check(load().cvs_prompt_attention_async(self.handle, plan.handle, hq, hk, hv, ho,
-                                                 _lse(self, lse, hq.heads, hq.tokens), scale))
+        hl = _lse(self, lse, hq.heads, hq.tokens)
+        after = self._behind_torch(q, k, v, out, lse)
+        _check(load().cvs_prompt_attention_async(self.handle, plan.handle, hq, hk, hv, ho, hl, scale))
+        if after:
+            after()
 
     def kv_cache(self, layers: int, pages: int, page_tokens: int, kv_heads: int, head_dim: int,
                  dtype="bf16") -> "KvCache":
@@ -918,7 +963,10 @@ class KvCache:
         if nk != nv:
             raise ValueError("k and v must have the same layers")
         if nk:
+            after = self.ctx._behind_torch(k, v)
             _check(call(self.handle, plan.handle, layer, nk, hk, lk, hv, lv))
+            if after:
+                after()
 
     def write_async(self, plan: "KvPlan", k, v, layer: int = 0) -> None:
         """Writes the plan's tokens: k, v (tokens, kv_heads, head_dim) of one
@@ -934,8 +982,11 @@ class KvCache:
         cvs_kv_attention_async): q, out (tokens, heads, head_dim); lse, when
         given, (heads, tokens) float32; scale 0: 1 / sqrt(head_dim)."""
         hq, ho = _heads(self.ctx, q, "q")[0], _heads(self.ctx, out, "out")[0]
-        _check(load().cvs_kv_attention_async(self.handle, plan.handle, layer, hq, ho,
-                                             _lse(self.ctx, lse, hq.heads, hq.tokens), scale))
+        hl = _lse(self.ctx, lse, hq.heads, hq.tokens)
+        after = self.ctx._behind_torch(q, out, lse)
+        _check(load().cvs_kv_attention_async(self.handle, plan.handle, layer, hq, ho, hl, scale))
+        if after:
+            after()
 
 
 class KvPlan:

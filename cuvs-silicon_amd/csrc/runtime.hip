@@ -537,6 +537,14 @@ int cvs_context_create_on_stream(int device, void* stream, cvs_context** out_ctx
   return guarded([&] { create_context(device, false, static_cast<hipStream_t>(stream), out_ctx); });
 }
 
+int cvs_context_stream(cvs_context* ctx, void** out_stream) {
+  return guarded([&] {
+    if (!ctx) fail(CVS_ERR_INVALID_ARGUMENT, "null context");
+    if (!out_stream) fail(CVS_ERR_INVALID_ARGUMENT, "null out_stream");
+    *out_stream = ctx->stream;
+  });
+}
+
 int cvs_context_destroy(cvs_context* ctx) {
   return guarded([&] {
     if (!ctx) return;

@@ -81,10 +81,15 @@ int cvs_device_count(int* out_count);
  * metal_context.hpp:15, and is_available(), metal_context.hpp:19). */
 int cvs_context_create(int device, cvs_context** out_ctx);
 /* The same on a stream of the caller's (a hipStream_t; null: the default
- * stream), which the context does not destroy: its calls then run in order
- * with the caller's own work on that stream, and arrays that work makes or
- * reads need no synchronization in between. */
+ * stream), which has to outlive the context and which the context does not
+ * destroy: its calls then run in order with the caller's own work on that
+ * stream, and arrays that work makes or reads need no synchronization in
+ * between. */
 int cvs_context_create_on_stream(int device, void* stream, cvs_context** out_ctx);
+/* The context's stream (a hipStream_t; null: the default stream).  Work of
+ * other streams that makes, reads or frees the arrays of an _async call has to
+ * be ordered with it by the caller, with events or by waiting. */
+int cvs_context_stream(cvs_context* ctx, void** out_stream);
 int cvs_context_destroy(cvs_context* ctx);
 int cvs_context_synchronize(cvs_context* ctx);
 
