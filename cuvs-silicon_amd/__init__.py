@@ -317,6 +317,13 @@ def _head_type(dtype) -> int:
     return t
 
 
+def _no_gradient(what: str) -> None:
+    """The calls compute no gradients: a torch tensor that requires grad would
+    lose it without a word, and is refused while gradients are recorded."""
+    if sys.modules["torch"].is_grad_enabled():
+        raise ValueError(f"{what} requires grad, and attention has no backward pass: detach it, or call under no_grad")
+
+
 def _heads(ctx: "Context", x, what: str, layered: bool = False):
     """The cvs_heads view of a (tokens, heads, head_dim) device array, a
     DeviceArray or a torch tensor on the context's device, whose last axis is
@@ -332,6 +339,8 @@ def _heads(ctx: "Context", x, what: str, layered: bool = False):
     elif hasattr(x, "data_ptr"):
         if not x.is_cuda or x.get_device() != ctx.device:
             raise ValueError(f"{what} must be on the context's device")
+        if x.requires_grad:
+            _no_gradient(what)
         st = x.stride()
         if st[-1] != 1 and shape[-1] > 1:
             raise ValueError(f"{what}: the last axis must be contiguous")
@@ -352,6 +361,8 @@ def _lse(ctx: "Context", lse, heads: int, tokens: int):
         return lse.ptr
     if not lse.is_cuda or lse.device.index != ctx.device or not lse.is_contiguous():
         raise ValueError("lse must be contiguous and on the context's device")
+    if lse.requires_grad:
+        _no_gradient("lse")
     return lse.data_ptr()
 
 

@@ -1,11 +1,11 @@
 """Attention and the cache on torch tensors whose stream is not the context's: in order with torch's current stream all
-the same."""
+the same, and tensors that require grad refused."""
 import ctypes
 
 import pytest
 import torch
 
-from test_kv_cache_gpu import rand
+from test_kv_cache_gpu import bits, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +69,33 @@ def test_the_streams_address(cvs):
     assert lib.cvs_context_stream(None, ctypes.byref(p)) == cvs.CVS_ERR_INVALID_ARGUMENT
     with pytest.raises(ValueError, match="null"):
         own.prompt_attention_async(own.prompt_plan([1], 1, 1), *[rand(0, 1, 1, 64, dtype="fp16")] * 4)
+
+
+def test_tensors_that_require_grad(cvs):
+    with cvs.Context(0, stream=torch.cuda.current_stream().cuda_stream) as c:
+        q, k, v = (rand(i, 9, h, 64, dtype="fp16") for i, h in enumerate((4, 2, 2)))
+        plan, out, lse = c.prompt_plan([9], 4, 2), torch.empty_like(q), torch.empty(4, 9, device="cuda")
+        cache = c.kv_cache(1, 4, 32, 2, 64, "fp16")
+        s = cache.sequence()
+        cache.extend([s], [9])
+        rows = cache.plan([s], [9], heads=4)
+        for x in (q, k, v, lse):
+            x.requires_grad_()
+            with pytest.raises(ValueError, match="requires grad"):
+                c.prompt_attention_async(plan, q, k, v, out, lse)
+            x.requires_grad_(False)
+        k.requires_grad_()
+        with pytest.raises(ValueError, match="requires grad"):
+            cache.write_async(rows, k, v)
+        cache.write_async(rows, k.detach(), v)
+        with torch.no_grad():
+            c.prompt_attention_async(plan, q, k, v, out, lse)
+            cache.write_async(rows, k, v)
+        q.requires_grad_()
+        other = torch.empty_like(out)
+        with pytest.raises(ValueError, match="requires grad"):
+            cache.attention_async(rows, q, other)
+        with torch.inference_mode():
+            cache.attention_async(rows, q, other)
+        assert torch.equal(bits(out), bits(other))
+        cache.close()
