@@ -678,8 +678,18 @@ extern "C" int cvs_kv_attention_async(cvs_kv_cache* cache, cvs_kv_plan* plan, in
     float* part_o = nullptr;
     float2* part_ml = nullptr;
     const size_t slots = size_t(plan->slots) * size_t(cache->kv_heads), width = size_t(32 * cache->nb);
+    const bool captured = captured_call(plan);
     if (slots) {
-      ctx->ws_attn.reserve(slots * (width * sizeof(float) + sizeof(float2)));
+      const size_t bytes = slots * (width * sizeof(float) + sizeof(float2));
+      if (bytes > ctx->ws_attn.bytes) {
+        if (ctx->ws_attn_captured) {
+          ctx->kept.push_back(ctx->ws_attn);
+          ctx->ws_attn = DeviceBuffer();
+          ctx->ws_attn_captured = false;
+        }
+      }
+      ctx->ws_attn.reserve(bytes);
+      ctx->ws_attn_captured |= captured;
       part_o = ctx->ws_attn.as<float>();
       part_ml = reinterpret_cast<float2*>(part_o + slots * width);
     }

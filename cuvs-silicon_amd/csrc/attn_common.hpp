@@ -385,6 +385,13 @@ float scale_log2(float scale, int dim);
 // so it passes from one plan to the next without a wait.
 DeviceBuffer take_blob(std::vector<DeviceBuffer>& pool, int live_plans, size_t bytes);
 
+// Whether the context's stream is being captured into a HIP graph.  What a
+// captured call has been given is read again at every replay, which no one
+// tells the library of: the memory of its plan and of its parts goes to a
+// `kept` list and is neither used for anything else nor freed before the
+// context's or cache's end.
+bool capturing(const cvs_context* ctx);
+
 // Copies host bytes to device memory as arguments of kernels, kUploadBytes a
 // launch: the host buffer is free on return and nothing is pinned, staged or
 // waited for.
@@ -411,6 +418,7 @@ struct cvs_kv_cache {
   std::unique_ptr<cvs::kv::PageBook> book;
   int live_plans = 0;
   std::vector<cvs::DeviceBuffer> blobs;  // device memory of destroyed plans, for the next ones
+  std::vector<cvs::DeviceBuffer> kept;   // of plans of captured calls, until the cache's end
 };
 
 struct cvs_kv_plan {
@@ -421,6 +429,7 @@ struct cvs_kv_plan {
   int64_t tokens = 0;            // of all sequences
   int heads = 0;                 // query heads; 0: for reading and writing alone
   cvs::DeviceBuffer blob;
+  bool captured = false;  // the blob is the cache's to keep
   // Offsets into the blob, in bytes.
   size_t at_spans = 0;
   int workgroups = 0;  // of attention, a kv head (attn_cached.hip)
@@ -434,5 +443,7 @@ namespace attn {
 void plan_attention(cvs_kv_plan* plan, const int64_t* lengths, const int64_t* tokens, std::vector<char>& blob);
 // The plan is the cache's and its sequences are as they were when it was made.
 void check_plan(const cvs_kv_plan* plan);
+// Before a call with the plan is launched: whether it is being captured; the plan's memory is then kept.
+bool captured_call(cvs_kv_plan* plan);
 }  // namespace attn
 }  // namespace cvs

@@ -265,6 +265,7 @@ struct cvs_prompt_plan {
   int heads = 0, kv_heads = 0, causal = 0;
   int64_t items = 0;
   DeviceBuffer blob;
+  mutable bool captured = false;  // the blob is the context's to keep
 };
 
 extern "C" {
@@ -331,7 +332,7 @@ int cvs_prompt_plan_destroy(cvs_prompt_plan* plan) {
   return guarded([&] {
     if (!plan) return;
     // Later plans use the memory on the same stream, after whatever still reads it.
-    if (plan->blob.ptr) plan->ctx->plan_blobs.push_back(plan->blob);
+    if (plan->blob.ptr && !plan->captured) plan->ctx->plan_blobs.push_back(plan->blob);
     --plan->ctx->live_prompt_plans;
     --plan->ctx->live_children;
     delete plan;
@@ -362,6 +363,10 @@ int cvs_prompt_attention_async(cvs_context* ctx, const cvs_prompt_plan* plan, co
     check_rows_apart(out, "out");
     const float c = scale_log2(scale, q->head_dim);
     if (plan->items == 0) return;
+    if (!plan->captured && capturing(ctx)) {
+      ctx->kept.push_back(plan->blob);
+      plan->captured = true;
+    }
     const PromptArgs a{view_of(q), view_of(k), view_of(v), view_of(out), lse,
                        plan->blob.as<PromptItem>(), plan->q_tokens, plan->kv_heads,
                        plan->heads / plan->kv_heads, q->head_dim, plan->causal, c};

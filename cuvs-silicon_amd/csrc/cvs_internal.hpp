@@ -94,7 +94,9 @@ struct cvs_context {
   cvs::DeviceBuffer ws_io;        // staging of host queries / results
   cvs::DeviceBuffer ws_teams;     // per-team lists of multi-team graph search
   cvs::DeviceBuffer ws_attn;      // attention over a cache: partial results of split rows
+  bool ws_attn_captured = false;  // calls captured into a HIP graph use ws_attn
   std::vector<cvs::DeviceBuffer> plan_blobs;  // memory of destroyed prompt plans, for the next ones
+  std::vector<cvs::DeviceBuffer> kept;  // what captured calls use, until the context's end
   int live_prompt_plans = 0;
   // Pinned host memory of kPinnedIoBytes for small blocking calls (host_call);
   // made by the first one.

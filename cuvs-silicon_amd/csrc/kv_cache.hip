@@ -239,6 +239,7 @@ void move_tokens(cvs_kv_plan* plan, int first_layer, int layers, const cvs_heads
     if (write && c->book->refs(sp.page) > 1)
       fail(CVS_ERR_INVALID_ARGUMENT, "the plan's tokens lie in a page that sequences share: extend first");
   if (plan->spans.empty()) return;
+  captured_call(plan);
   const int tiles = int(c->book->page_tokens() / 32);
   const int64_t units = int64_t(plan->spans.size()) * tiles * c->kv_heads;
   if (units > kMaxBlocks * 4) fail(CVS_ERR_UNSUPPORTED, "too many tokens");
@@ -313,6 +314,22 @@ void upload(cvs_context* ctx, void* dst, const void* src, size_t bytes) {
   }
 }
 
+bool capturing(const cvs_context* ctx) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  // An error (the default stream while another one is captured) is the launch's to report.
+  if (hipStreamIsCapturing(ctx->stream, &status) != hipSuccess) (void)hipGetLastError();
+  return status != hipStreamCaptureStatusNone;
+}
+
+bool captured_call(cvs_kv_plan* plan) {
+  if (!capturing(plan->cache->ctx)) return false;
+  if (!plan->captured && plan->blob.ptr) {
+    plan->cache->kept.push_back(plan->blob);
+    plan->captured = true;
+  }
+  return true;
+}
+
 void check_plan(const cvs_kv_plan* plan) {
   if (!plan) fail(CVS_ERR_INVALID_ARGUMENT, "null plan");
   try {
@@ -376,6 +393,7 @@ int cvs_kv_cache_destroy(cvs_kv_cache* cache) {
     bind(cache->ctx);
     (void)hipStreamSynchronize(cache->ctx->stream);
     for (auto& b : cache->blobs) b.release();
+    for (auto& b : cache->kept) b.release();
     (void)hipFree(cache->pool);
     --cache->ctx->live_children;
     delete cache;
@@ -509,7 +527,7 @@ int cvs_kv_plan_destroy(cvs_kv_plan* plan) {
   return guarded([&] {
     if (!plan) return;
     // Later plans use the memory on the same stream, after whatever still reads it.
-    if (plan->blob.ptr) plan->cache->blobs.push_back(plan->blob);
+    if (plan->blob.ptr && !plan->captured) plan->cache->blobs.push_back(plan->blob);
     --plan->cache->live_plans;
     delete plan;
   });

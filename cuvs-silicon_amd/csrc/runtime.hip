@@ -565,6 +565,7 @@ int cvs_context_destroy(cvs_context* ctx) {
     ctx->ws_teams.release();
     ctx->ws_attn.release();
     for (auto& b : ctx->plan_blobs) b.release();
+    for (auto& b : ctx->kept) b.release();
     if (ctx->pinned_io) (void)hipHostFree(ctx->pinned_io);
     if (ctx->bf_counters) (void)hipFree(ctx->bf_counters);
     if (ctx->owns_stream) (void)hipStreamDestroy(ctx->stream);

@@ -603,7 +603,16 @@ int cvs_kv_cache_compact(cvs_kv_cache* cache, int64_t* out_live);
  * heads: query heads, a multiple of the cache's kv heads, or 0 for a plan
  * that only reads and writes.  Made once for a step and used for every
  * layer; calls with it fail once one of its sequences has changed
- * (extended, truncated, freed, or moved by compaction). */
+ * (extended, truncated, freed, or moved by compaction).
+ *
+ * HIP graphs: calls of cvs_prompt_attention_async, cvs_kv_write_async,
+ * cvs_kv_read_async and cvs_kv_attention_async can be captured, the last once
+ * the same call has been made before (its workspace is there then).  The memory
+ * of their plans and workspace stays as it is until the context or cache is
+ * destroyed, also when the plans are destroyed or larger calls follow.  Replays
+ * belong in order with the context's stream, and end when one of the plans'
+ * sequences changes: a replay does not see that, and goes on with the pages the
+ * sequence had. */
 int cvs_kv_plan_create(cvs_kv_cache* cache, const int64_t* seqs, const int64_t* tokens, int64_t n, int heads,
                        cvs_kv_plan** out_plan);
 int cvs_kv_plan_destroy(cvs_kv_plan* plan);

@@ -1,0 +1,91 @@
+"""Calls of attention and the cache in HIP graphs that outlive what they were captured with: plans that are dropped, a
+workspace that larger calls outgrow."""
+import pytest
+import torch
+
+from test_kv_cache_gpu import Filled, bits, rand
+
+pytestmark = pytest.mark.gpu
+
+
+class Case:
+    """Calls whose plans are all in device memory: 200 sequences' tokens, prompts, rows in several parts."""
+
+    def __init__(self, cvs, stream):
+        self.ctx = cvs.Context(0, stream=stream.cuda_stream)
+        self.f = Filled(self.ctx, 1, 900, 32, 2, 64, "bf16")
+        (root,) = self.f.new()
+        self.f.append([root], [9000])
+        self.seqs = self.f.fork(root, 200)
+        self.f.append(self.seqs, [1 + i % 5 for i in range(200)])
+        self.q, self.k, self.v = (rand(i, 200, h, 64, dtype="bf16") for i, h in enumerate((8, 2, 2)))
+        self.outs = [torch.empty_like(x) for x in (self.q, self.q, self.k, self.v)]
+
+    def plans(self, shift=0):
+        """Other plans of the same sizes for another shift."""
+        seqs = self.seqs[shift:] + self.seqs[:shift]
+        return self.f.cache.plan(seqs, [1] * 200, heads=8), self.ctx.prompt_plan([3 + shift, 100 - shift, 97], 8, 2)
+
+    def calls(self, step, prompt):
+        self.f.cache.attention_async(step, self.q, self.outs[0])
+        self.ctx.prompt_attention_async(prompt, self.q, self.k, self.v, self.outs[1])
+        self.f.cache.read_async(step, self.outs[2], self.outs[3])
+
+    def capture(self, stream, plans):
+        self.calls(*plans)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            self.calls(*plans)
+        return graph
+
+    def check(self, stream, graph, want):
+        for seed in range(3):
+            for x in self.outs:
+                x.fill_(9.0)
+            graph.replay()
+            stream.synchronize()
+            for x, y in zip(self.outs, want):
+                assert torch.equal(bits(x), bits(y)), seed
+            torch.randn(1000, 1000, device="cuda").sum().item()
+
+
+def test_plans_dropped_before_a_replay(cvs):
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        c = Case(cvs, stream)
+        plans = c.plans()
+        graph = c.capture(stream, plans)
+        c.calls(*plans)
+        want = [x.clone() for x in c.outs]
+        del plans
+        others = [c.plans(shift) for shift in (1, 7, 50)]  # not in the captured plans' memory
+        for p in others:
+            c.calls(*p)
+        c.check(stream, graph, want)
+        del others
+        c.calls(*c.plans())
+        for x, y in zip(c.outs, want):
+            assert torch.equal(bits(x), bits(y))
+        c.f.cache.close()
+        c.ctx.close()
+
+
+def test_a_workspace_outgrown_before_a_replay(cvs):
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        c = Case(cvs, stream)
+        plans = c.plans()
+        graph = c.capture(stream, plans)
+        c.calls(*plans)
+        want = [x.clone() for x in c.outs]
+        q = rand(9, 200, 64, 64, dtype="bf16")
+        big, out = c.f.cache.plan(c.seqs, [1] * 200, heads=64), torch.empty_like(q)
+        c.f.cache.attention_async(big, q, out)  # 8 times the parts
+        filler = torch.full((1 << 26,), float("nan"), device="cuda")  # where freed memory would be
+        c.check(stream, graph, want)
+        c.f.cache.attention_async(big, q, out.zero_())
+        assert torch.isfinite(out.float()).all()
+        del filler
+        c.f.cache.close()
+        c.ctx.close()
