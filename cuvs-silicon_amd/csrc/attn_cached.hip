@@ -682,6 +682,9 @@ extern "C" int cvs_kv_attention_async(cvs_kv_cache* cache, cvs_kv_plan* plan, in
     if (slots) {
       const size_t bytes = slots * (width * sizeof(float) + sizeof(float2));
       if (bytes > ctx->ws_attn.bytes) {
+        if (captured)
+          fail(CVS_ERR_INVALID_ARGUMENT, "a call's memory cannot be made while the context's stream is being captured "
+                                         "into a graph: make the call once before");
         if (ctx->ws_attn_captured) {
           ctx->kept.push_back(ctx->ws_attn);
           ctx->ws_attn = DeviceBuffer();

@@ -391,6 +391,8 @@ DeviceBuffer take_blob(std::vector<DeviceBuffer>& pool, int live_plans, size_t b
 // `kept` list and is neither used for anything else nor freed before the
 // context's or cache's end.
 bool capturing(const cvs_context* ctx);
+// Refuses what would be done at every replay, and not now.
+void need_no_capture(const cvs_context* ctx, const char* what);
 
 // Copies host bytes to device memory as arguments of kernels, kUploadBytes a
 // launch: the host buffer is free on return and nothing is pinned, staged or

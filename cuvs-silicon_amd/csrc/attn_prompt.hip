@@ -313,6 +313,7 @@ int cvs_prompt_plan_create(cvs_context* ctx, const int64_t* q_lengths, const int
     plan->causal = causal != 0;
     plan->items = int64_t(items.size());
     if (!sorted.empty()) {
+      need_no_capture(ctx, "plans cannot be made");
       const size_t bytes = sorted.size() * sizeof(PromptItem);
       plan->blob = take_blob(ctx->plan_blobs, ctx->live_prompt_plans, bytes);
       try {

@@ -321,6 +321,11 @@ bool capturing(const cvs_context* ctx) {
   return status != hipStreamCaptureStatusNone;
 }
 
+void need_no_capture(const cvs_context* ctx, const char* what) {
+  if (capturing(ctx))
+    fail(CVS_ERR_INVALID_ARGUMENT, std::string(what) + " while the context's stream is being captured into a graph");
+}
+
 bool captured_call(cvs_kv_plan* plan) {
   if (!capturing(plan->cache->ctx)) return false;
   if (!plan->captured && plan->blob.ptr) {
@@ -427,6 +432,7 @@ int cvs_kv_sequence_extend(cvs_kv_cache* cache, const int64_t* seqs, const int64
     need_list(seqs, n, "sequences");
     need_list(tokens, n, "tokens");
     bind(cache->ctx);
+    need_no_capture(cache->ctx, "sequences cannot be extended");
     copy_pages(cache, cache->book->extend(seqs, tokens, n));
   });
 }
@@ -463,6 +469,7 @@ int cvs_kv_sequence_pages(cvs_kv_cache* cache, const int64_t* seqs, int64_t n, i
 int cvs_kv_cache_compact(cvs_kv_cache* cache, int64_t* out_live) {
   return on_book(cache, [&] {
     bind(cache->ctx);
+    need_no_capture(cache->ctx, "a cache cannot be compacted");
     copy_pages(cache, cache->book->compact());
     if (out_live) *out_live = cache->book->pages() - cache->book->free_pages();
   });
@@ -510,6 +517,7 @@ int cvs_kv_plan_create(cvs_kv_cache* cache, const int64_t* seqs, const int64_t* 
     }
     if (heads > 0) plan_attention(plan.get(), lengths.data(), tokens, blob);
     if (!blob.empty()) {
+      need_no_capture(cache->ctx, "plans cannot be made");
       plan->blob = take_blob(cache->blobs, cache->live_plans, blob.size());
       try {
         upload(cache->ctx, plan->blob.ptr, blob.data(), blob.size());

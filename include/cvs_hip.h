@@ -612,7 +612,9 @@ int cvs_kv_cache_compact(cvs_kv_cache* cache, int64_t* out_live);
  * destroyed, also when the plans are destroyed or larger calls follow.  Replays
  * belong in order with the context's stream, and end when one of the plans'
  * sequences changes: a replay does not see that, and goes on with the pages the
- * sequence had. */
+ * sequence had.  Making plans, cvs_kv_sequence_extend and cvs_kv_cache_compact
+ * are refused during a capture: they would be done at each replay, and not in
+ * between. */
 int cvs_kv_plan_create(cvs_kv_cache* cache, const int64_t* seqs, const int64_t* tokens, int64_t n, int heads,
                        cvs_kv_plan** out_plan);
 int cvs_kv_plan_destroy(cvs_kv_plan* plan);

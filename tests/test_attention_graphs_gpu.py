@@ -1,5 +1,5 @@
 """Calls of attention and the cache in HIP graphs that outlive what they were captured with: plans that are dropped, a
-workspace that larger calls outgrow."""
+workspace that larger calls outgrow; and what cannot be captured."""
 import pytest
 import torch
 
@@ -88,4 +88,37 @@ def test_a_workspace_outgrown_before_a_replay(cvs):
         assert torch.isfinite(out.float()).all()
         del filler
         c.f.cache.close()
+        c.ctx.close()
+
+
+def test_what_cannot_be_captured(cvs):
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        c = Case(cvs, stream)
+        cache, plans = c.f.cache, c.plans()
+        (kid,) = c.f.fork(c.seqs[0], 1)
+        before = cache.pages([kid, *c.seqs]).tolist()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        refused = []
+        with torch.cuda.graph(graph, stream=stream):
+            for call in (lambda: cache.plan(c.seqs, [1] * 200, heads=8), lambda: c.ctx.prompt_plan([5], 8, 2),
+                         lambda: cache.extend([kid], [1]), lambda: cache.compact(),
+                         lambda: cache.attention_async(plans[0], c.q, c.outs[0])):
+                try:
+                    call()
+                except ValueError as e:
+                    refused.append(str(e))
+            c.ctx.prompt_attention_async(plans[1], c.q, c.k, c.v, c.outs[1])
+        assert len(refused) == 5 and all("captured" in m for m in refused), refused
+        assert "make the call once before" in refused[-1]
+        assert cache.pages([kid, *c.seqs]).tolist() == before
+        c.outs[1].zero_()
+        graph.replay()
+        got = c.outs[1].clone()
+        c.ctx.prompt_attention_async(plans[1], c.q, c.k, c.v, c.outs[1])
+        assert torch.equal(bits(got), bits(c.outs[1]))
+        cache.extend([kid], [1])
+        cache.compact()
+        cache.close()
         c.ctx.close()
