@@ -316,8 +316,11 @@ void upload(cvs_context* ctx, void* dst, const void* src, size_t bytes) {
 
 bool capturing(const cvs_context* ctx) {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  // An error (the default stream while another one is captured) is the launch's to report.
-  if (hipStreamIsCapturing(ctx->stream, &status) != hipSuccess) (void)hipGetLastError();
+  if (hipStreamIsCapturing(ctx->stream, &status) != hipSuccess) {
+    // The default stream while another one is captured: a launch on it says so itself, and the status is anything.
+    (void)hipGetLastError();
+    return false;
+  }
   return status != hipStreamCaptureStatusNone;
 }
 
