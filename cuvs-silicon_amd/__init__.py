@@ -334,6 +334,8 @@ def _heads(ctx: "Context", x, what: str, layered: bool = False):
     if nd != 3 and not (layered and nd == 4):
         raise ValueError(f"{what} must be (tokens, heads, head_dim)" + (" or (layers, ...)" if layered else ""))
     if isinstance(x, DeviceArray):
+        if x.ctx.device != ctx.device:
+            raise ValueError(f"{what} must be on the context's device")
         ptr, stride = x.ptr.value, (shape[-2] * shape[-1], shape[-1])
         layer = shape[-3] * stride[0] if nd == 4 else 0
     elif hasattr(x, "data_ptr"):
@@ -358,6 +360,8 @@ def _lse(ctx: "Context", lse, heads: int, tokens: int):
     if tuple(lse.shape) != (heads, tokens) or str(lse.dtype) not in ("float32", "torch.float32"):
         raise ValueError(f"lse must be a float32 device array of shape {(heads, tokens)}")
     if isinstance(lse, DeviceArray):
+        if lse.ctx.device != ctx.device:
+            raise ValueError("lse must be on the context's device")
         return lse.ptr
     if not lse.is_cuda or lse.device.index != ctx.device or not lse.is_contiguous():
         raise ValueError("lse must be contiguous and on the context's device")

@@ -431,6 +431,13 @@ void create_context(int device, bool own_stream, hipStream_t stream, cvs_context
     fail(CVS_ERR_NO_DEVICE, "no HIP device available");
   if (device < 0 || device >= count)
     fail(CVS_ERR_INVALID_ARGUMENT, "device index out of range");
+  if (stream) {
+    hipDevice_t on = device;
+    CVS_HIP(hipStreamGetDevice(stream, &on));
+    if (on != device)
+      fail(CVS_ERR_INVALID_ARGUMENT, "the stream is device " + std::to_string(on) + "'s, the context is for device " +
+                                         std::to_string(device));
+  }
   hipDeviceProp_t prop;
   CVS_HIP(hipGetDeviceProperties(&prop, device));
   if (std::strncmp(prop.gcnArchName, "gfx950", 6) != 0)

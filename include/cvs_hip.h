@@ -80,8 +80,8 @@ int cvs_device_count(int* out_count);
 /* Create a context on `device` (replaces MetalContext::instance(),
  * metal_context.hpp:15, and is_available(), metal_context.hpp:19). */
 int cvs_context_create(int device, cvs_context** out_ctx);
-/* The same on a stream of the caller's (a hipStream_t; null: the default
- * stream), which has to outlive the context and which the context does not
+/* The same on a stream of the caller's (a hipStream_t of that device; null:
+ * the default stream), which has to outlive the context and which the context does not
  * destroy: its calls then run in order with the caller's own work on that
  * stream, and arrays that work makes or reads need no synchronization in
  * between. */

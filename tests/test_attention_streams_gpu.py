@@ -99,3 +99,9 @@ def test_tensors_that_require_grad(cvs):
             cache.attention_async(rows, q, other)
         assert torch.equal(bits(out), bits(other))
         cache.close()
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs a second GPU")
+def test_a_stream_of_another_device(cvs):
+    with pytest.raises(ValueError, match="the stream is device 1's"):
+        cvs.Context(0, stream=torch.cuda.Stream(device=1).cuda_stream)
