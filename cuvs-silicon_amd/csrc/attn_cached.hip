@@ -18,9 +18,9 @@
 // writes the output itself.
 //
 // Bounds: long sequences the memory (48 of 100 to 6,000 tokens, 8 kv heads of
-// 128, bf16, a token each: 104 us = 6.2 TB/s of distinct cache bytes; 8 over
-// 100,003 shared tokens: 67 us = 6.1 TB/s of the shared ones alone), short ones
-// latency: one sequence of 777 tokens, 16/4 heads of 64, takes 7.0 us, in which
+// 128, bf16, a token each: 103 us = 6.3 TB/s of distinct cache bytes; 8 over
+// 100,003 shared tokens: 69 us = 5.9 TB/s of the shared ones alone), short ones
+// latency: one sequence of 777 tokens, 16/4 heads of 64, takes 7.1 us, in which
 // the plan, a page's id and its tiles are loaded one after another.
 #include <algorithm>
 #include <cstring>
@@ -370,8 +370,8 @@ struct JoinArgs {
 // One wave a (token, head) row, in one pass over the row's parts with a
 // running maximum.  A lane takes 4 columns; 8 NB lanes have a part, and the
 // wave's groups of so many take the parts in turn and join at the end.  Bound
-// by latency: 5.0 us for 8 sequences' 256 rows over 100,003 shared tokens, 4.8
-// to 5.7 in other batches.
+// by latency: 5.0 us for 8 sequences' 256 rows over 100,003 shared tokens, 4.7
+// to 6.0 in other batches.
 template <bool kBf, int NB>
 __global__ __launch_bounds__(256) void join_parts_kernel(const JoinArgs a) {
   constexpr int kLanes = 8 * NB, kGroups = 64 / kLanes;

@@ -25,12 +25,15 @@
 // tiles in flight leave two waves a SIMD their 256 registers.  Heads of 64 and
 // 96 run four and three workgroups.
 //
-// Bounds: long prompts with heads of 128 the matrix cores (busy 62% of the
-// cycles: 12,000 causal tokens, 32/8 heads, bf16, in 1.06 ms = 1.11 PFLOP/s,
-// 0.92 of the vendor's plain product); heads of 64 the vector unit, whose 32
-// exponentials a step of 512 product cycles take 512 themselves (64 passages
-// of 40 to 512 tokens, 12 heads, in 45 us); short prompts each workgroup's
-// first loads.
+// Bounds: long prompts with heads of 128 the matrix cores (busy 61% of the
+// cycles, the vector unit 52%: 12,000 causal tokens, 32/8 heads, bf16, in
+// 1.03 ms = 1.14 PFLOP/s, 0.80 of the vendor's plain product).  Prompts with
+// smaller heads no one unit: 64 passages of 40 to 512 tokens, 12 heads of 64,
+// take 45 us with the vector unit busy 51% of the cycles (193 instructions a
+// 64-key step, 32 exponentials among them), the matrix cores 27%, the waves 27%
+// of their time waiting, and 146 MB fetched for 88 MB of inputs: row blocks
+// that share keys run on different XCDs, each with an L2 of its own.  Short
+// prompts each workgroup's first loads.
 #include <algorithm>
 
 #include "attn_common.hpp"

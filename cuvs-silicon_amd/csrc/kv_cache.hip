@@ -38,7 +38,7 @@ struct Copies {
 };
 
 // Bound by the memory: 24 pages of 256 KiB in 16 layers, 201 MB read and
-// written in 38 us, 5.3 TB/s.
+// written in 37 us, 5.4 TB/s.
 constexpr int kCopyBytes = 16384;  // of a workgroup: 4 loads of 16 bytes a thread in flight
 
 __global__ __launch_bounds__(256) void copy_pages_kernel(char* __restrict__ pool, int64_t layer_bytes,
@@ -106,7 +106,7 @@ __device__ CVS_INLINE void transpose8(u32x4 (&x)[8]) {
 // bytes with new ones; those after it are past the sequence's end.  A wave's
 // loads are all under way at once: of clamped rows, or all under one condition.
 // Bound by the memory: 12 sequences of 700 tokens, 16 layers of 8 heads of
-// 128, 1.1 GB read and written in 209 us (write) and 205 us (read), 5.3 TB/s.
+// 128, 1.1 GB read and written in 206 us (write) and 207 us (read), 5.3 TB/s.
 template <int NB, bool kWrite>
 __global__ __launch_bounds__(256) void move_tokens_kernel(const MoveArgs a, const Spans inl) {
   constexpr int P = 4 * NB;  // 16-byte pieces of a row
