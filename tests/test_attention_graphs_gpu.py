@@ -122,3 +122,25 @@ def test_what_cannot_be_captured(cvs):
         cache.compact()
         cache.close()
         c.ctx.close()
+
+
+def test_captured_on_torchs_stream_with_a_context_of_its_own(cvs):
+    """The context's stream joins the capture by the events that order it with torch's."""
+    q, k, v = (rand(i, 90, h, 64, dtype="fp16") for i, h in enumerate((4, 2, 2)))
+    out, want = torch.empty_like(q), torch.empty_like(q)
+    with cvs.Context(0) as ctx:
+        plan = ctx.prompt_plan([40, 50], 4, 2)
+        ctx.prompt_attention_async(plan, q, k, v, want)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ctx.prompt_attention_async(plan, q * 1, k * 1, v * 1, out)
+            doubled = out * 2
+        for seed in (0, 20, 40):
+            for i, x in enumerate((q, k, v)):
+                x.copy_(rand(seed + i, *x.shape, dtype="fp16"))
+            ctx.prompt_attention_async(plan, q, k, v, want)
+            out.fill_(9.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(bits(out), bits(want)) and torch.equal(bits(doubled), bits(want * 2)), seed
