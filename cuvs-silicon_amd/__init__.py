@@ -176,6 +176,31 @@ _SIGNATURES["cvs_kv_write_async"] = (c_int, [c_void_p, c_void_p, c_int, c_int, _
 _SIGNATURES["cvs_kv_read_async"] = (c_int, [c_void_p, c_void_p, c_int, c_int, _HEADS, c_int64, _HEADS, c_int64])
 _SIGNATURES["cvs_kv_attention_async"] = (c_int, [c_void_p, c_void_p, c_int, _HEADS, _HEADS, c_void_p, c_float])
 
+
+
+class RotaryScaling(ctypes.Structure):
+    """cvs_rotary_scaling (include/cvs_hip.h)."""
+    _fields_ = [("kind", c_int), ("factor", c_double), ("original_length", c_double), ("low", c_double),
+                ("high", c_double)]
+
+
+class HeadNorm(ctypes.Structure):
+    """cvs_head_norm (include/cvs_hip.h)."""
+    _fields_ = [("weight", c_void_p), ("type", c_int), ("eps", c_float)]
+
+
+FP32 = 2
+ROTARY_HALVES, ROTARY_NEIGHBOURS = 0, 1
+SCALINGS = {None: 0, "linear": 1, "base": 2, "turns": 3}
+
+_NORM = POINTER(HeadNorm)
+_SIGNATURES["cvs_rotary_frequencies"] = (c_int, [c_int, c_double, POINTER(RotaryScaling), c_void_p])
+_SIGNATURES["cvs_rotary_create"] = (c_int, [c_void_p, c_int, c_int, c_void_p, c_float, POINTER(c_void_p)])
+_SIGNATURES["cvs_rotary_destroy"] = (c_int, [c_void_p])
+_SIGNATURES["cvs_rotate_async"] = (c_int, [c_void_p, c_void_p, c_void_p, _HEADS, _HEADS])
+_SIGNATURES["cvs_norm_rotate_async"] = (c_int, [c_void_p, c_void_p, c_void_p, _HEADS, _HEADS, _NORM, _HEADS, _HEADS,
+                                                _NORM])
+
 # The bucketing permutation seed of the reference (src/metal_context.mm:803).
 DEFAULT_BUILD_SEED = 0xFEDCBA9876543210
 
@@ -370,6 +395,44 @@ def _lse(ctx: "Context", lse, heads: int, tokens: int):
     return lse.data_ptr()
 
 
+_KINDS = {}  # dtypes' names: making a torch dtype's takes longer than all else in a call
+
+
+def _vector(ctx: "Context", x, what: str, length: int, dtypes):
+    """Device address of an array of `length` elements of one of `dtypes`,
+    contiguous, and its type's place among them."""
+    kind = _KINDS.get(x.dtype)
+    if kind is None:
+        kind = _KINDS[x.dtype] = str(x.dtype).replace("torch.", "")
+    if len(x.shape) != 1 or x.shape[0] != length or kind not in dtypes:
+        raise ValueError(f"{what} must be {length} elements of {' or '.join(dtypes)}, in one dimension")
+    if isinstance(x, DeviceArray):
+        if x.ctx.device != ctx.device:
+            raise ValueError(f"{what} must be on the context's device")
+        return x.ptr.value, dtypes.index(kind)
+    if not hasattr(x, "data_ptr"):
+        raise ValueError(f"{what} must be a DeviceArray or a torch tensor")
+    if not x.is_cuda or x.get_device() != ctx.device:
+        raise ValueError(f"{what} must be on the context's device")
+    if length > 1 and x.stride(0) != 1:
+        raise ValueError(f"{what} must be contiguous")
+    if x.requires_grad:
+        _no_gradient(what)
+    return x.data_ptr(), dtypes.index(kind)
+
+
+# A norm's weight: fp32 or the type of the heads.
+_WEIGHT_TYPES = {FP16: ("float32", "float16"), BF16: ("float32", "bfloat16", "uint16")}
+
+
+def _norm(ctx: "Context", weight, heads, eps: float, what: str):
+    """The cvs_head_norm of heads, None without a weight."""
+    if weight is None:
+        return None
+    ptr, kind = _vector(ctx, weight, what, heads.head_dim, _WEIGHT_TYPES[heads.type])
+    return HeadNorm(ptr, heads.type if kind else FP32, eps)
+
+
 def _raw_stream(torch, device: int) -> int:
     """The address of torch's current stream."""
     try:
@@ -533,6 +596,54 @@ class Context:
         _check(load().cvs_prompt_attention_async(self.handle, plan.handle, hq, hk, hv, ho, hl, scale))
         if after:
             after()
+
+    def rotary(self, dims: int, base: float = 10000.0, interleaved: bool = False, scaling: str = None,
+               factor: float = 1.0, original_length: float = 0.0, low: float = 1.0, high: float = 32.0,
+               magnitude: float = 1.0, frequencies=None) -> "Rotary":
+        """Rotary positions of the first `dims` channels of heads: frequencies
+        of a base, scaled if need be (rotary_frequencies), or the given ones."""
+        if frequencies is None:
+            frequencies = rotary_frequencies(dims, base, scaling, factor, original_length, low, high)
+        return Rotary(self, dims, frequencies, interleaved, magnitude)
+
+    def rotate_async(self, rotary: "Rotary", positions, x, out) -> None:
+        """x (tokens, heads, head_dim) rotated to out, which may be x itself;
+        positions (tokens,) int64 (C: cvs_rotate_async)."""
+        hx, ho = _heads(self, x, "x")[0], _heads(self, out, "out")[0]
+        at = _vector(self, positions, "positions", hx.tokens, ("int64",))[0]
+        after = self._behind_torch(positions, x, out)
+        _check(load().cvs_rotate_async(self.handle, rotary.handle, at, hx, ho))
+        if after:
+            after()
+
+    def norm_rotate_async(self, rotary, positions, q, q_out, k=None, k_out=None, q_weight=None, k_weight=None,
+                          eps: float = 1e-6) -> None:
+        """Queries and keys (tokens, heads, head_dim), normed where they have
+        a weight (head_dim,) and rotated where there is a rotary, to their
+        outputs in one pass (C: cvs_norm_rotate_async)."""
+        hq, hqo, nq = self._ready(q, q_out, q_weight, eps, "q")
+        hk, hko, nk = self._ready(k, k_out, k_weight, eps, "k")
+        if hq is None and hk is None:
+            raise ValueError("neither q nor k")
+        at = None
+        if rotary is not None:
+            at = _vector(self, positions, "positions", (hq or hk).tokens, ("int64",))[0]
+        after = self._behind_torch(q, q_out, k, k_out, q_weight, k_weight, positions)
+        _check(load().cvs_norm_rotate_async(self.handle, None if rotary is None else rotary.handle, at, hq, hqo, nq,
+                                            hk, hko, nk))
+        if after:
+            after()
+
+    def _ready(self, x, out, weight, eps: float, what: str):
+        """Heads, their output and norm as C takes them; None, all three, without heads."""
+        if x is None:
+            if out is not None or weight is not None:
+                raise ValueError(f"an output or a weight of {what} without {what}")
+            return None, None, None
+        if out is None:
+            raise ValueError(f"{what} needs {what}_out")
+        h = _heads(self, x, what)[0]
+        return h, _heads(self, out, what + "_out")[0], _norm(self, weight, h, eps, what + "_weight")
 
     def kv_cache(self, layers: int, pages: int, page_tokens: int, kv_heads: int, head_dim: int,
                  dtype="bf16") -> "KvCache":
@@ -873,6 +984,47 @@ class PromptPlan:
         # A plan dies with its context (Context.close closes it first).
         if self.handle is not None and self.ctx.handle is not None:
             _check(load().cvs_prompt_plan_destroy(self.handle))
+        self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def rotary_frequencies(dims: int, base: float = 10000.0, scaling: str = None, factor: float = 1.0,
+                       original_length: float = 0.0, low: float = 1.0, high: float = 32.0) -> np.ndarray:
+    """Radians a position of each pair of channels (C: cvs_rotary_frequencies):
+    base^(-2i/dims), for contexts longer than the trained one scaled "linear",
+    by "base", or by the "turns" of a pair over original_length positions."""
+    if scaling not in SCALINGS:
+        raise ValueError(f"scaling must be one of {list(SCALINGS)}")
+    out = np.empty(max(int(dims), 0) // 2, np.float64)
+    _check(load().cvs_rotary_frequencies(int(dims), base, RotaryScaling(SCALINGS[scaling], factor, original_length, low,
+                                                                        high), out.ctypes.data))
+    return out
+
+
+class Rotary:
+    """Rotary positions of a model's heads (C: cvs_rotary)."""
+
+    def __init__(self, ctx: Context, dims: int, frequencies, interleaved: bool = False, magnitude: float = 1.0):
+        self.ctx = ctx
+        self.handle = None
+        f = np.ascontiguousarray(frequencies, np.float64)
+        if f.shape != (max(int(dims), 0) // 2,):
+            raise ValueError(f"{dims} channels have {int(dims) // 2} frequencies, {f.shape} given")
+        h = c_void_p()
+        _check(load().cvs_rotary_create(ctx.handle, int(dims), ROTARY_NEIGHBOURS if interleaved else ROTARY_HALVES,
+                                        f.ctypes.data, magnitude, byref(h)))
+        self.handle = h
+        ctx._adopt(self)
+
+    def close(self) -> None:
+        # A rotary dies with its context (Context.close closes it first).
+        if self.handle is not None and self.ctx.handle is not None:
+            _check(load().cvs_rotary_destroy(self.handle))
         self.handle = None
 
     def __del__(self):

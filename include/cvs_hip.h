@@ -640,6 +640,75 @@ int cvs_kv_read_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int first_layer, i
 int cvs_kv_attention_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int layer, const cvs_heads* q,
                            const cvs_heads* out, float* lse, float scale);
 
+/* ---- positions and norms of heads ----------------------------------------- */
+
+/* What lies between a projection and its attention: the norm of each head and
+ * the rotation of its channels by position.  Forward only, like the rest.
+ *
+ *   n = w x / sqrt(mean x^2 + eps)           a head's norm, if it has one
+ *   y_a = m (n_a cos t - n_b sin t)          for each pair (a, b) of its first
+ *   y_b = m (n_b cos t + n_a sin t)          `dims` channels; y = n elsewhere
+ *
+ * with t = position * frequency of the pair and m the magnitude.  Everything
+ * is in fp32 and rounded once; t is exact modulo whole turns (2^-63 turns a
+ * position), so far positions are as precise as near ones.  Positions are 64
+ * bit, may be negative (the inverse rotation) and may repeat.  Squares that
+ * pass the range of fp32 make their head's norm infinite, and the head 0. */
+
+#define CVS_ROTARY_HALVES 0     /* pair i: channels i and i + dims / 2 */
+#define CVS_ROTARY_NEIGHBOURS 1 /* pair i: channels 2 i and 2 i + 1 */
+
+/* Frequencies of a model run on contexts longer than it was trained on, from
+ * the trained f_i = base^(-2 i / dims):
+ *   LINEAR  f_i / factor;
+ *   BASE    the base times factor^(dims / (dims - 2)): the first pair stays, the last is divided by factor;
+ *   TURNS   a pair that makes n = original_length f_i / 2 pi turns over the trained length keeps the share
+ *           w = (n - low) / (high - low), within 0 to 1, of its frequency: f_i (w + (1 - w) / factor). */
+#define CVS_SCALING_NONE 0
+#define CVS_SCALING_LINEAR 1
+#define CVS_SCALING_BASE 2
+#define CVS_SCALING_TURNS 3
+typedef struct cvs_rotary_scaling {
+  int kind;
+  double factor;          /* LINEAR, BASE, TURNS */
+  double original_length; /* TURNS */
+  double low, high;       /* TURNS: 0 <= low < high */
+} cvs_rotary_scaling;
+
+/* The dims / 2 frequencies, in radians a position, to host memory; scaling
+ * may be null.  Needs no GPU. */
+int cvs_rotary_frequencies(int dims, double base, const cvs_rotary_scaling* scaling, double* out_radians);
+
+/* Rotary positions of a model: dims (even, up to CVS_ATTN_MAX_DIM) channels of
+ * each head, dims / 2 host frequencies (of cvs_rotary_frequencies or any
+ * others from -1024 to 1024), and the factor of all that is rotated.  Made once
+ * for all layers and calls of its context. */
+typedef struct cvs_rotary cvs_rotary;
+int cvs_rotary_create(cvs_context* ctx, int dims, int layout, const double* radians, float magnitude,
+                      cvs_rotary** out_rotary);
+int cvs_rotary_destroy(cvs_rotary* rotary);
+
+/* The norm of heads: a device array of head_dim weights, fp32 or of the heads' type. */
+#define CVS_FP32 2
+typedef struct cvs_head_norm {
+  const void* weight;
+  int type;  /* CVS_FP32, or the heads' */
+  float eps; /* finite, not negative */
+} cvs_head_norm;
+
+/* x (tokens x heads) rotated to out, token t at positions[t] (device memory).
+ * out may be x itself, and must not share memory with it otherwise.  Device
+ * memory; enqueued on the context stream. */
+int cvs_rotate_async(cvs_context* ctx, const cvs_rotary* rotary, const int64_t* positions, const cvs_heads* x,
+                     const cvs_heads* out);
+
+/* Queries and keys of the same tokens, normed and rotated in one pass.  q or k
+ * (with its output and norm), either norm, and rotary (with positions) may be
+ * null.  Outputs as in cvs_rotate_async. */
+int cvs_norm_rotate_async(cvs_context* ctx, const cvs_rotary* rotary, const int64_t* positions, const cvs_heads* q,
+                          const cvs_heads* q_out, const cvs_head_norm* q_norm, const cvs_heads* k,
+                          const cvs_heads* k_out, const cvs_head_norm* k_norm);
+
 #ifdef __cplusplus
 }
 #endif
