@@ -200,6 +200,8 @@ _SIGNATURES["cvs_rotary_destroy"] = (c_int, [c_void_p])
 _SIGNATURES["cvs_rotate_async"] = (c_int, [c_void_p, c_void_p, c_void_p, _HEADS, _HEADS])
 _SIGNATURES["cvs_norm_rotate_async"] = (c_int, [c_void_p, c_void_p, c_void_p, _HEADS, _HEADS, _NORM, _HEADS, _HEADS,
                                                 _NORM])
+_SIGNATURES["cvs_kv_append_async"] = (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, _HEADS, _NORM, _HEADS,
+                                              _HEADS, _HEADS, _NORM])
 
 # The bucketing permutation seed of the reference (src/metal_context.mm:803).
 DEFAULT_BUILD_SEED = 0xFEDCBA9876543210
@@ -433,6 +435,18 @@ def _norm(ctx: "Context", weight, heads, eps: float, what: str):
     return HeadNorm(ptr, heads.type if kind else FP32, eps)
 
 
+def _ready(ctx: "Context", x, out, weight, eps: float, what: str):
+    """Heads, their output and norm as C takes them; None, all three, without heads."""
+    if x is None:
+        if out is not None or weight is not None:
+            raise ValueError(f"an output or a weight of {what} without {what}")
+        return None, None, None
+    if out is None:
+        raise ValueError(f"{what} needs {what}_out")
+    h = _heads(ctx, x, what)[0]
+    return h, _heads(ctx, out, what + "_out")[0], _norm(ctx, weight, h, eps, what + "_weight")
+
+
 def _raw_stream(torch, device: int) -> int:
     """The address of torch's current stream."""
     try:
@@ -621,8 +635,8 @@ class Context:
         """Queries and keys (tokens, heads, head_dim), normed where they have
         a weight (head_dim,) and rotated where there is a rotary, to their
         outputs in one pass (C: cvs_norm_rotate_async)."""
-        hq, hqo, nq = self._ready(q, q_out, q_weight, eps, "q")
-        hk, hko, nk = self._ready(k, k_out, k_weight, eps, "k")
+        hq, hqo, nq = _ready(self, q, q_out, q_weight, eps, "q")
+        hk, hko, nk = _ready(self, k, k_out, k_weight, eps, "k")
         if hq is None and hk is None:
             raise ValueError("neither q nor k")
         at = None
@@ -633,17 +647,6 @@ class Context:
                                             hk, hko, nk))
         if after:
             after()
-
-    def _ready(self, x, out, weight, eps: float, what: str):
-        """Heads, their output and norm as C takes them; None, all three, without heads."""
-        if x is None:
-            if out is not None or weight is not None:
-                raise ValueError(f"an output or a weight of {what} without {what}")
-            return None, None, None
-        if out is None:
-            raise ValueError(f"{what} needs {what}_out")
-        h = _heads(self, x, what)[0]
-        return h, _heads(self, out, what + "_out")[0], _norm(self, weight, h, eps, what + "_weight")
 
     def kv_cache(self, layers: int, pages: int, page_tokens: int, kv_heads: int, head_dim: int,
                  dtype="bf16") -> "KvCache":
@@ -1143,6 +1146,23 @@ class KvCache:
     def read_async(self, plan: "KvPlan", k, v, layer: int = 0) -> None:
         """Reads the plan's tokens into k, v (shapes as write_async)."""
         self._move(load().cvs_kv_read_async, plan, k, v, layer)
+
+    def append_async(self, plan: "KvPlan", k, v, layer: int = 0, rotary: "Rotary" = None, positions=None,
+                     k_weight=None, q=None, q_out=None, q_weight=None, eps: float = 1e-6) -> None:
+        """Writes the plan's tokens (tokens, kv_heads, head_dim) into a layer,
+        keys normed where they have a weight and rotated where there is a
+        rotary, at positions (tokens,) int64 or their places in their
+        sequences; queries q (tokens, heads, head_dim), made ready in the same
+        way, go to q_out (C: cvs_kv_append_async)."""
+        hk, hv = _heads(self.ctx, k, "k")[0], _heads(self.ctx, v, "v")[0]
+        nk = _norm(self.ctx, k_weight, hk, eps, "k_weight")
+        hq, hqo, nq = _ready(self.ctx, q, q_out, q_weight, eps, "q")
+        at = None if positions is None else _vector(self.ctx, positions, "positions", hk.tokens, ("int64",))[0]
+        after = self.ctx._behind_torch(k, v, q, q_out, k_weight, q_weight, positions)
+        _check(load().cvs_kv_append_async(self.handle, plan.handle, layer, None if rotary is None else rotary.handle, at,
+                                          hk, nk, hv, hq, hqo, nq))
+        if after:
+            after()
 
     def attention_async(self, plan: "KvPlan", q, out, layer: int = 0, lse=None, scale: float = 0.0) -> None:
         """Attention of the plan's tokens over a layer (C:

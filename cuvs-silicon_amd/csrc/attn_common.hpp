@@ -400,9 +400,21 @@ void need_no_capture(const cvs_context* ctx, const char* what);
 constexpr size_t kUploadBytes = 3840;
 void upload(cvs_context* ctx, void* dst, const void* src, size_t bytes);
 
-// Tokens [begin, end) of a page, rows row0 and on of the caller's arrays.
+// Tokens [begin, end) of a page, rows row0 and on of the caller's arrays; the
+// page is its sequence's index-th.
 struct Span {
-  int32_t page, begin, end, row0;
+  int32_t page, range, row0, index;
+  static Span of(int32_t page, int64_t begin, int64_t end, int64_t row0, int64_t index) {
+    return {page, int32_t(begin | end << 16), int32_t(row0), int32_t(index)};  // both are at most 4096
+  }
+  __host__ __device__ int begin() const { return range & 0xffff; }
+  __host__ __device__ int end() const { return range >> 16; }
+};
+
+// Spans of a small plan go to the kernels as arguments, others are read from the plan's memory.
+constexpr int kInlineSpans = 192;
+struct Spans {
+  Span s[kInlineSpans];
 };
 
 }  // namespace attn

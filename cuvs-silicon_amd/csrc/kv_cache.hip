@@ -15,6 +15,7 @@
 #include <cstring>
 
 #include "attn_common.hpp"
+#include "kv_tiles.hpp"
 
 namespace cvs {
 namespace attn {
@@ -69,12 +70,6 @@ void copy_pages(cvs_kv_cache* cache, const std::vector<kv::PageCopy>& copies) {
   }
 }
 
-// Spans of a small plan go to the kernel as arguments, others are read from the plan's memory.
-constexpr int kInlineSpans = 192;
-struct Spans {
-  Span s[kInlineSpans];
-};
-
 struct MoveArgs {
   char* pool;  // of the first layer
   int64_t layer_bytes, page_bytes, head_bytes;
@@ -84,18 +79,6 @@ struct MoveArgs {
   int n_spans, page_tiles, by_tile, dim, kv_heads;
   int units;  // spans * tiles of a page * kv_heads
 };
-
-// Rows 2 w and 2 w + 1 of an 8 x 8 matrix of 16-bit elements are x[2 w], x[2 w + 1]; transposed in place.
-__device__ CVS_INLINE void transpose8(u32x4 (&x)[8]) {
-  u32x4 y[8];
-#pragma unroll
-  for (int c = 0; c < 8; ++c)
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      y[c][k] = __builtin_amdgcn_perm(x[2 * k + 1][c / 2], x[2 * k][c / 2], c & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-  for (int c = 0; c < 8; ++c) x[c] = y[c];
-}
 
 // Between rows of the caller's arrays and tiles of the pool, one wave a tile
 // of 32 tokens, kv head and layer; no wave waits for another.  Rows are read
@@ -121,67 +104,32 @@ __global__ __launch_bounds__(256) void move_tokens_kernel(const MoveArgs a, cons
   const int g = unit % a.kv_heads, n = unit / a.kv_heads;
   const int at = a.by_tile ? n % a.n_spans : n / a.page_tiles, tile = a.by_tile ? n / a.n_spans : n % a.page_tiles;
   const Span sp = a.spans ? a.spans[at] : inl.s[at];
-  const int lo = max(sp.begin - 32 * tile, 0), hi = min(sp.end - 32 * tile, 32);
+  const int lo = max(sp.begin() - 32 * tile, 0), hi = min(sp.end() - 32 * tile, 32);
   if (lo >= hi) return;
   char* const kt = a.pool + blockIdx.y * a.layer_bytes + sp.page * a.page_bytes + g * a.head_bytes +
                    int64_t(tile) * 4096 * NB;
   char* const vt = kt + 2048 * NB;
-  const int64_t row = int64_t(sp.row0) + 32 * tile - sp.begin;  // of the tile's token 0
+  const int64_t row = int64_t(sp.row0) + 32 * tile - sp.begin();  // of the tile's token 0
   char* const ks = a.k.p + 2 * (blockIdx.y * a.k_layer + row * a.k.token + g * a.k.head);
   char* const vs = a.v.p + 2 * (blockIdx.y * a.v_layer + row * a.v.token + g * a.v.head);
   const int pieces = a.dim / 8;
-  auto held = [&](int t) CVS_INLINE { return min(max(t, lo), hi - 1); };
-
-  // Values: lane = (columns 8 c and on, tokens t0 + {0, 1, 2, 3, 8, 9, 10, 11}).
-  const int c = lane % P, t0 = 16 * (lane / P >> 1) + 4 * (lane / P & 1);
-  const bool mine = lane < 4 * P && t0 < hi && t0 + 11 >= lo;
-  u32x4* const slots = reinterpret_cast<u32x4*>(
-      vt + (2 * (c / 4) + (lane / P >> 1)) * 1024 + (32 * (lane / P & 1) + 8 * (c % 4)) * 16);
-  u32x4 x[8], y[P / 2];
-  auto token = [&](int j) CVS_INLINE { return t0 + 8 * (j / 4) + j % 4; };
+  TileValues<NB> values(vt, lo, hi);
+  u32x4 y[P / 2];
   if constexpr (kWrite) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      x[j] = *reinterpret_cast<const u32x4*>(vs + 2 * (held(token(j)) * a.v.token + 8 * min(c, pieces - 1)));
+    values.load(vs, a.v.token, pieces);
 #pragma unroll
     for (int i = 0; i < P / 2; ++i) {
       const int n = 64 * i + lane;
-      y[i] = *reinterpret_cast<const u32x4*>(ks + 2 * (held(n / P) * a.k.token + 8 * min(n % P, pieces - 1)));
+      y[i] = *reinterpret_cast<const u32x4*>(ks + 2 * (values.held(n / P) * a.k.token + 8 * min(n % P, pieces - 1)));
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c >= pieces) x[j] = u32x4{};
-    transpose8(x);
-    if (mine && t0 < lo) {
-      uint32_t keep[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) keep[k] = (token(2 * k) < lo ? 0xffffu : 0u) | (token(2 * k + 1) < lo ? 0xffff0000u : 0u);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const u32x4 old = slots[j];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[j][k] = (x[j][k] & ~keep[k]) | (old[k] & keep[k]);
-      }
-    }
-    if (mine) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) slots[j] = x[j];
-    }
+    values.store(pieces);
 #pragma unroll
     for (int i = 0; i < P / 2; ++i) {
       const int n = 64 * i + lane, t = n / P, p = n % P;
-      s[wave][t * P + (p ^ (t & 3))] = p < pieces ? y[i] : u32x4{};
+      s[wave][staged<NB>(t, p)] = p < pieces ? y[i] : u32x4{};
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    const int t = lane & 31;
-#pragma unroll
-    for (int i = 0; i < P / 2; ++i) y[i] = s[wave][t * P + ((2 * i + (lane >> 5)) ^ (t & 3))];
-    if (t >= lo && t < hi) {
-#pragma unroll
-      for (int i = 0; i < P / 2; ++i) *reinterpret_cast<u32x4*>(kt + 1024 * i + 16 * lane) = y[i];
-    }
+    wave_lds_ready();
+    store_keys<NB>(s[wave], kt, lo, hi);
   } else {
     const int t = lane & 31;
     const bool key = t >= lo && t < hi;
@@ -189,55 +137,43 @@ __global__ __launch_bounds__(256) void move_tokens_kernel(const MoveArgs a, cons
 #pragma unroll
       for (int i = 0; i < P / 2; ++i) y[i] = *reinterpret_cast<const u32x4*>(kt + 1024 * i + 16 * lane);
     }
-    if (mine) {
+    u32x4 (&x)[8] = values.x;
+    if (values.mine) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = slots[j];
+      for (int j = 0; j < 8; ++j) x[j] = values.slots[j];
     }
     if (key) {
 #pragma unroll
-      for (int i = 0; i < P / 2; ++i) s[wave][t * P + ((2 * i + (lane >> 5)) ^ (t & 3))] = y[i];
+      for (int i = 0; i < P / 2; ++i) s[wave][staged<NB>(t, 2 * i + (lane >> 5))] = y[i];
     }
     transpose8(x);
+    const int c = values.c;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (mine && token(j) >= lo && token(j) < hi && c < pieces)
-        *reinterpret_cast<u32x4*>(vs + 2 * (token(j) * a.v.token + 8 * c)) = x[j];
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    for (int j = 0; j < 8; ++j) {
+      const int at = values.token(j);
+      if (values.mine && at >= lo && at < hi && c < pieces)
+        *reinterpret_cast<u32x4*>(vs + 2 * (at * a.v.token + 8 * c)) = x[j];
+    }
+    wave_lds_ready();
 #pragma unroll
     for (int i = 0; i < P / 2; ++i) {
       const int n = 64 * i + lane, t = n / P, p = n % P;
       if (t >= lo && t < hi && p < pieces)
-        *reinterpret_cast<u32x4*>(ks + 2 * (t * a.k.token + 8 * p)) = s[wave][t * P + (p ^ (t & 3))];
+        *reinterpret_cast<u32x4*>(ks + 2 * (t * a.k.token + 8 * p)) = s[wave][staged<NB>(t, p)];
     }
   }
 }
 
 void move_tokens(cvs_kv_plan* plan, int first_layer, int layers, const cvs_heads* k, int64_t k_layer,
                  const cvs_heads* v, int64_t v_layer, bool write) {
-  check_plan(plan);
+  check_move(plan, first_layer, layers, k, v, write);
   cvs_kv_cache* const c = plan->cache;
-  if (first_layer < 0 || layers < 1 || first_layer > c->layers - layers)
-    fail(CVS_ERR_INVALID_ARGUMENT, "layers outside the cache's " + std::to_string(c->layers));
-  for (const cvs_heads* x : {k, v}) {
-    const char* const what = x == k ? "k" : "v";
-    check_view(x, what);
-    if (x->tokens != plan->tokens)
-      fail(CVS_ERR_INVALID_ARGUMENT, std::string(what) + " must have the plan's " + std::to_string(plan->tokens) +
-                                         " tokens");
-    if (x->heads != c->kv_heads || x->head_dim != c->dim || x->type != c->type)
-      fail(CVS_ERR_INVALID_ARGUMENT, std::string(what) + " must have the cache's heads, head_dim and type");
-  }
   if (layers > 1 && (k_layer % 8 != 0 || v_layer % 8 != 0 || k_layer < 0 || v_layer < 0))
     fail(CVS_ERR_UNSUPPORTED, "layer strides must be non-negative multiples of 8 elements");
   if (!write) {
     check_rows_apart(k, "k", layers, k_layer);
     check_rows_apart(v, "v", layers, v_layer);
   }
-  for (const Span& sp : plan->spans)
-    if (write && c->book->refs(sp.page) > 1)
-      fail(CVS_ERR_INVALID_ARGUMENT, "the plan's tokens lie in a page that sequences share: extend first");
   if (plan->spans.empty()) return;
   captured_call(plan);
   const int tiles = int(c->book->page_tokens() / 32);
@@ -249,7 +185,7 @@ void move_tokens(cvs_kv_plan* plan, int first_layer, int layers, const cvs_heads
   const MoveArgs a{c->pool + first_layer * c->layer_bytes, c->layer_bytes, c->page_bytes, c->head_bytes,
                    small ? nullptr : reinterpret_cast<const Span*>(plan->blob.as<char>() + plan->at_spans),
                    view_of(k), view_of(v), k_layer, v_layer, int(plan->spans.size()), tiles,
-                   2 * plan->tokens < int64_t(plan->spans.size()) * c->book->page_tokens(), c->dim, c->kv_heads, int(units)};
+                   spans_by_tile(plan), c->dim, c->kv_heads, int(units)};
   const dim3 grid(unsigned((units + 3) / 4), unsigned(layers));
   const TimerSpan ts = timer_span(c->ctx, write ? "kv_write" : "kv_read");
   auto go = [&](auto kernel) {
@@ -336,6 +272,25 @@ bool captured_call(cvs_kv_plan* plan) {
     plan->captured = true;
   }
   return true;
+}
+
+void check_move(cvs_kv_plan* plan, int first_layer, int layers, const cvs_heads* k, const cvs_heads* v, bool write) {
+  check_plan(plan);
+  cvs_kv_cache* const c = plan->cache;
+  if (first_layer < 0 || layers < 1 || first_layer > c->layers - layers)
+    fail(CVS_ERR_INVALID_ARGUMENT, "layers outside the cache's " + std::to_string(c->layers));
+  for (const cvs_heads* x : {k, v}) {
+    const char* const what = x == k ? "k" : "v";
+    check_view(x, what);
+    if (x->tokens != plan->tokens)
+      fail(CVS_ERR_INVALID_ARGUMENT, std::string(what) + " must have the plan's " + std::to_string(plan->tokens) +
+                                         " tokens");
+    if (x->heads != c->kv_heads || x->head_dim != c->dim || x->type != c->type)
+      fail(CVS_ERR_INVALID_ARGUMENT, std::string(what) + " must have the cache's heads, head_dim and type");
+  }
+  for (const Span& sp : plan->spans)
+    if (write && c->book->refs(sp.page) > 1)
+      fail(CVS_ERR_INVALID_ARGUMENT, "the plan's tokens lie in a page that sequences share: extend first");
 }
 
 void check_plan(const cvs_kv_plan* plan) {
@@ -508,7 +463,7 @@ int cvs_kv_plan_create(cvs_kv_cache* cache, const int64_t* seqs, const int64_t* 
       for (int64_t t = s.length - tokens[i]; t < s.length;) {
         const int64_t in = t % pt, end = std::min(pt, in + s.length - t);
         const int32_t pg = s.pages[size_t(t / pt)];
-        spans.push_back({pg, int32_t(in), int32_t(end), int32_t(plan->tokens)});
+        spans.push_back(Span::of(pg, in, end, plan->tokens, t / pt));
         plan->tokens += end - in;
         t += end - in;
       }

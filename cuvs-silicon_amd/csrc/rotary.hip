@@ -20,7 +20,6 @@ namespace attn {
 namespace {
 
 constexpr int kTokens = 16;  // of a workgroup at most
-constexpr int kAhead = 4;    // rows of a lane under way
 constexpr int kMaxPairs = kMaxDim / 2;
 
 struct RotateArgs {
@@ -38,145 +37,36 @@ struct RotateArgs {
 
 template <bool kBf, int kLanes, Pairs kPairs, bool kNorm>
 __global__ __launch_bounds__(256) void rotate_kernel(const RotateArgs a) {
-  constexpr int kGroups = 256 / kLanes;
   __shared__ __align__(16) float s_cos[kTokens * kMaxPairs], s_sin[kTokens * kMaxPairs];
   __shared__ __align__(16) float s_w[kNorm ? 2 * kMaxDim : 1];
   __shared__ __align__(16) u32x4 s_rows[kPairs == kChannels ? 256 : 1];
   const int64_t t0 = int64_t(blockIdx.x) * a.per_block;
   const int nt = int(min(int64_t(a.per_block), a.tokens - t0));
   const int h0 = blockIdx.y * a.chunk, nh = min(a.chunk, a.heads[0] + a.heads[1] - h0);
-  const int rows = nt * nh, group = threadIdx.x / kLanes, in = threadIdx.x % kLanes;
-  const int half = a.dims / 2, pieces = a.dim / 8, piece = min(in, pieces - 1);
-
-  struct Row {
-    int token, head;  // of the workgroup's, and of all
+  const HeadLane<kLanes> l(a.dim, a.dims);
+  auto place = [&](int r) CVS_INLINE {
+    const int t = r / nh, h = h0 + r % nh, k = h >= a.heads[0], head = k ? h - a.heads[0] : h;
+    const View& in = k ? a.in[1] : a.in[0];
+    const View& out = k ? a.out[1] : a.out[0];
+    const Norm& n = k ? a.norm[1] : a.norm[0];
+    return HeadRow{in.p + 2 * ((t0 + t) * in.token + head * in.head),
+                   out.p + 2 * ((t0 + t) * out.token + head * out.head), s_cos + t * kMaxPairs, s_sin + t * kMaxPairs,
+                   kNorm && n.weight ? s_w + k * kMaxDim : nullptr, n.eps};
   };
-  auto row_of = [&](int r) CVS_INLINE {
-    const int n = min(r, rows - 1);  // past the last row, that one again (not stored)
-    return Row{n / nh, h0 + n % nh};
-  };
-  auto at = [&](const View (&v)[2], const Row& r) CVS_INLINE {
-    const bool k = r.head >= a.heads[0];
-    const View& x = k ? v[1] : v[0];
-    return reinterpret_cast<u32x4*>(x.p + 2 * ((t0 + r.token) * x.token + (k ? r.head - a.heads[0] : r.head) * x.head) +
-                                    16 * piece);
-  };
-  u32x4 x[kAhead];
-  auto load = [&](int first) CVS_INLINE {
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) x[i] = *at(a.in, row_of(first + i * kGroups));
-  };
-  load(group);
-  for (int i = threadIdx.x; i < nt * half; i += 256) {
-    const int t = i / half, p = i % half;
-    const float2 cs = cos_sin(a.turns[p] * uint64_t(a.positions[t0 + t]));
-    s_cos[t * kMaxPairs + p] = a.magnitude * cs.x;
-    s_sin[t * kMaxPairs + p] = a.magnitude * cs.y;
-  }
-  if constexpr (kNorm) {
-    for (int i = threadIdx.x; i < 2 * kMaxDim; i += 256) {
-      const Norm n = a.norm[i / kMaxDim];
-      const int c = i % kMaxDim;
-      if (n.weight && c < a.dim)
-        s_w[i] = n.fp32 ? static_cast<const float*>(n.weight)[c] : to_float<kBf>(static_cast<const uint16_t*>(n.weight)[c]);
+  auto before = [&]() CVS_INLINE {
+    for (int i = threadIdx.x; i < nt * l.half; i += 256) {
+      const int t = i / l.half, p = i % l.half;
+      const float2 cs = cos_sin(a.turns[p] * uint64_t(a.positions[t0 + t]));
+      s_cos[t * kMaxPairs + p] = a.magnitude * cs.x;
+      s_sin[t * kMaxPairs + p] = a.magnitude * cs.y;
     }
-  }
-  __syncthreads();
-
-  for (int first = group; first < rows; first += kAhead * kGroups) {
-    u32x4 y[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const Row r = row_of(first + i * kGroups);
-      float f[8], o[8], w[8];
-      unpack8<kBf>(x[i], f);
-      float inv = 1.f;
-      bool normed = false;
-      const int which = r.head >= a.heads[0] ? 1 : 0;
-      if constexpr (kNorm) {
-        const Norm& n = a.norm[which];
-        normed = n.weight != nullptr;
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(f[e], f[e], sum);
-        if (in >= pieces) sum = 0.f;
-#pragma unroll
-        for (int m = 1; m < kLanes; m <<= 1) sum += xor_lanes_f(sum, m);
-        if (normed) inv = 1.f / __builtin_sqrtf(sum / float(a.dim) + n.eps);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          w[e] = normed ? s_w[which * kMaxDim + 8 * piece + e] : 1.f;
-          f[e] *= w[e];
-        }
-      }
-      const float* const cs = s_cos + r.token * kMaxPairs;
-      const float* const sn = s_sin + r.token * kMaxPairs;
-      if constexpr (kPairs == kNeighbours) {
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const int p = 4 * piece + e / 2;
-          const bool turned = p < half;
-          const float c = cs[turned ? p : 0], s = sn[turned ? p : 0];
-          o[e] = turned ? f[e] * c - f[e + 1] * s : f[e];
-          o[e + 1] = turned ? f[e + 1] * c + f[e] * s : f[e + 1];
-        }
-      } else if constexpr (kPairs == kPieces) {
-        // A piece of the first half, of the second, or behind both.
-        const bool turned = 8 * piece < a.dims, low = 8 * piece < half;
-        const int lane = __lane_id();
-        const int from = !turned ? lane : low ? lane + half / 8 : lane - half / 8;
-        u32x4 px;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) px[k] = uint32_t(__builtin_amdgcn_ds_bpermute(4 * from, int(x[i][k])));
-        float g[8];
-        unpack8<kBf>(px, g);
-        const int other = !turned ? piece : low ? piece + half / 8 : piece - half / 8;
-        const int p = !turned ? 0 : low ? 8 * piece : 8 * piece - half;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if constexpr (kNorm) {
-            if (normed) g[e] *= s_w[which * kMaxDim + 8 * other + e];
-          }
-          const float s = low ? -sn[p + e] : sn[p + e];
-          o[e] = turned ? f[e] * cs[p + e] + g[e] * s : f[e];
-        }
-      } else {
-        // The row's pieces side by side in LDS of the wave's own.
-        s_rows[threadIdx.x] = x[i];
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        const uint16_t* const row = reinterpret_cast<const uint16_t*>(s_rows + (threadIdx.x - in));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int c = 8 * piece + e;
-          const bool turned = c < a.dims, low = c < half;
-          const int other = !turned ? c : low ? c + half : c - half, p = !turned ? 0 : low ? c : c - half;
-          float g = to_float<kBf>(row[other]);
-          if constexpr (kNorm) {
-            if (normed) g *= s_w[which * kMaxDim + other];
-          }
-          const float s = low ? -sn[p] : sn[p];
-          o[e] = turned ? f[e] * cs[p] + g * s : f[e];
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-      }
-      if constexpr (kNorm) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] *= inv;
-      }
-      y[i] = pack8<kBf>(o);
+    if constexpr (kNorm) {
+      load_weight<kBf>(s_w, a.norm[0], a.dim);
+      load_weight<kBf>(s_w + kMaxDim, a.norm[1], a.dim);
     }
-    // The next rows before these are stored: no two rows of an output share memory, and a row's input may be its own
-    // output alone.
-    load(first + kAhead * kGroups);
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int r = first + i * kGroups;
-      if (r < rows && in < pieces) *at(a.out, row_of(r)) = y[i];
-    }
-  }
+    __syncthreads();
+  };
+  ready_rows<kBf, kLanes, kPairs, kNorm>(l, nt * nh, s_rows + (kPairs == kChannels ? threadIdx.x : 0), place, before);
 }
 
 template <bool kBf, int kLanes>

@@ -12,7 +12,7 @@
 // off by 0.004 radians at position 100,000.
 #pragma once
 
-#include "attn_common.hpp"
+#include "kv_tiles.hpp"
 
 // Rotary positions of a model, rotary.hip.
 struct cvs_rotary {
@@ -73,6 +73,143 @@ struct Norm {
   int fp32;  // the weight's type: fp32, or the heads'
   float eps;
 };
+
+// A head is a row of 16-byte pieces, one a lane; the power of two of lanes that
+// holds the largest head of a kernel has a row.
+template <int kLanes>
+struct HeadLane {
+  int in, piece, pieces;  // lanes past the row's end repeat its last piece
+  int dim, half;          // half: pairs that turn
+  float inv_dim;
+  __device__ CVS_INLINE HeadLane(int dim, int dims)
+      : in(threadIdx.x % kLanes), piece(min(in, dim / 8 - 1)), pieces(dim / 8), dim(dim), half(dims / 2),
+        inv_dim(1.f / float(dim)) {}
+};
+
+// A norm's weights to LDS in fp32.
+template <bool kBf>
+__device__ CVS_INLINE void load_weight(float* s, const Norm& n, int dim) {
+  if (!n.weight) return;
+  for (int i = threadIdx.x; i < dim; i += blockDim.x)
+    s[i] = n.fp32 ? static_cast<const float*>(n.weight)[i] : to_float<kBf>(static_cast<const uint16_t*>(n.weight)[i]);
+}
+
+// The lane's piece x of a head, normed and rotated.  cs, sn: the head's cosines
+// and sines, times the magnitude; w: its norm's weights, null for none; scratch:
+// a place in LDS for each lane of the wave, this one's (kChannels alone).
+template <bool kBf, int kLanes, Pairs kPairs, bool kNorm>
+__device__ CVS_INLINE u32x4 ready(u32x4 x, const HeadLane<kLanes>& l, const float* cs, const float* sn, const float* w,
+                                  float eps, u32x4* scratch) {
+  const int half = l.half, piece = l.piece;
+  float f[8], o[8];
+  unpack8<kBf>(x, f);
+  float inv = 1.f;
+  if constexpr (kNorm) {
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = __builtin_fmaf(f[e], f[e], sum);
+    if (l.in >= l.pieces) sum = 0.f;
+#pragma unroll
+    for (int m = 1; m < kLanes; m <<= 1) sum += xor_lanes_f(sum, m);
+    if (w) {
+      inv = 1.f / __builtin_sqrtf(__builtin_fmaf(sum, l.inv_dim, eps));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] *= w[8 * piece + e];
+    }
+  }
+  if constexpr (kPairs == kNeighbours) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const int p = 4 * piece + e / 2;
+      const bool turned = p < half;
+      const float c = cs[turned ? p : 0], s = sn[turned ? p : 0];
+      o[e] = turned ? f[e] * c - f[e + 1] * s : f[e];
+      o[e + 1] = turned ? f[e + 1] * c + f[e] * s : f[e + 1];
+    }
+  } else if constexpr (kPairs == kPieces) {
+    // A piece of the first half, of the second, or behind both.
+    const bool turned = 8 * piece < 2 * half, low = 8 * piece < half;
+    const int to = !turned ? 0 : low ? half / 8 : -half / 8;  // where its partner is
+    u32x4 px;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      px[k] = uint32_t(__builtin_amdgcn_ds_bpermute(4 * (int(__lane_id()) + to), int(x[k])));
+    float g[8];
+    unpack8<kBf>(px, g);
+    const int p = !turned ? 0 : low ? 8 * piece : 8 * piece - half;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (kNorm) {
+        if (w) g[e] *= w[8 * (piece + to) + e];
+      }
+      const float s = low ? -sn[p + e] : sn[p + e];
+      o[e] = turned ? f[e] * cs[p + e] + g[e] * s : f[e];
+    }
+  } else {
+    // The row's pieces side by side.
+    *scratch = x;
+    wave_lds_ready();
+    const uint16_t* const row = reinterpret_cast<const uint16_t*>(scratch - l.in);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = 8 * piece + e;
+      const bool turned = c < 2 * half, low = c < half;
+      const int other = !turned ? c : low ? c + half : c - half, p = !turned ? 0 : low ? c : c - half;
+      float g = to_float<kBf>(row[other]);
+      if constexpr (kNorm) {
+        if (w) g *= w[other];
+      }
+      const float s = low ? -sn[p] : sn[p];
+      o[e] = turned ? f[e] * cs[p] + g * s : f[e];
+    }
+    wave_lds_ready();  // read before the next row's pieces are written
+  }
+  if constexpr (kNorm) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= inv;
+  }
+  return pack8<kBf>(o);
+}
+
+// A head on its way.
+struct HeadRow {
+  const char* in;
+  char* out;
+  const float *cs, *sn, *w;
+  float eps;
+};
+
+// Rows [0, rows) by a workgroup, kAhead of each group of lanes under way at
+// once; place(r) is row r, before() is run behind the first loads.  A row's
+// input may be its own output and no other row's.
+constexpr int kAhead = 4;
+template <bool kBf, int kLanes, Pairs kPairs, bool kNorm, typename Place, typename Before>
+__device__ CVS_INLINE void ready_rows(const HeadLane<kLanes>& l, int rows, u32x4* scratch, const Place& place,
+                                      const Before& before) {
+  const int groups = blockDim.x / kLanes, group = threadIdx.x / kLanes;
+  u32x4 x[kAhead];
+  auto load = [&](int first) CVS_INLINE {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)  // past the last row, that one again (not stored)
+      x[i] = *reinterpret_cast<const u32x4*>(place(min(first + i * groups, rows - 1)).in + 16 * l.piece);
+  };
+  load(group);
+  before();
+  for (int first = group; first - group < rows; first += kAhead * groups) {
+    u32x4 y[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const HeadRow r = place(min(first + i * groups, rows - 1));
+      y[i] = ready<kBf, kLanes, kPairs, kNorm>(x[i], l, r.cs, r.sn, r.w, r.eps, scratch);
+    }
+    load(first + kAhead * groups);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int r = first + i * groups;
+      if (r < rows && l.in < l.pieces) *reinterpret_cast<u32x4*>(place(r).out + 16 * l.piece) = y[i];
+    }
+  }
+}
 
 // Checks a norm of heads of `type`; null: none.
 Norm norm_of(const cvs_head_norm* norm, int type, const char* what);

@@ -709,6 +709,19 @@ int cvs_norm_rotate_async(cvs_context* ctx, const cvs_rotary* rotary, const int6
                           const cvs_heads* q_out, const cvs_head_norm* q_norm, const cvs_heads* k,
                           const cvs_heads* k_out, const cvs_head_norm* k_norm);
 
+/* A step's new tokens on their way into layer `layer` of a cache, in one pass:
+ * the plan's keys k, normed and rotated, and values v, as
+ * cvs_kv_write_async would write them, and its queries q, normed and rotated,
+ * to q_out.  Token t is at positions[t] (device memory, in the plan's order),
+ * or, where positions is null, at its place in its sequence.  rotary, either
+ * norm, and q (with its output and norm) may be null; q_out may be q itself.
+ * q has any number of heads, a plan's with query heads its number.  Device
+ * memory; enqueued on the context stream; can be captured like
+ * cvs_kv_write_async. */
+int cvs_kv_append_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int layer, const cvs_rotary* rotary,
+                        const int64_t* positions, const cvs_heads* k, const cvs_head_norm* k_norm, const cvs_heads* v,
+                        const cvs_heads* q, const cvs_heads* q_out, const cvs_head_norm* q_norm);
+
 #ifdef __cplusplus
 }
 #endif
