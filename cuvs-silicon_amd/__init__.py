@@ -203,6 +203,20 @@ _SIGNATURES["cvs_norm_rotate_async"] = (c_int, [c_void_p, c_void_p, c_void_p, _H
 _SIGNATURES["cvs_kv_append_async"] = (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, _HEADS, _NORM, _HEADS,
                                               _HEADS, _HEADS, _NORM])
 
+
+class ScoreOptions(ctypes.Structure):
+    """cvs_scores (include/cvs_hip.h)."""
+    _fields_ = [("cap", c_float), ("slopes", c_void_p)]
+
+
+_SCORES = POINTER(ScoreOptions)
+_SIGNATURES["cvs_prompt_plan_create_prefix"] = (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int,
+                                                        POINTER(c_void_p)])
+_SIGNATURES["cvs_prompt_attention_scored_async"] = (c_int, [c_void_p, c_void_p, _HEADS, _HEADS, _HEADS, _HEADS,
+                                                            c_void_p, c_float, _SCORES])
+_SIGNATURES["cvs_kv_attention_scored_async"] = (c_int, [c_void_p, c_void_p, c_int, _HEADS, _HEADS, c_void_p, c_float,
+                                                        _SCORES])
+
 # The bucketing permutation seed of the reference (src/metal_context.mm:803).
 DEFAULT_BUILD_SEED = 0xFEDCBA9876543210
 
@@ -435,6 +449,13 @@ def _norm(ctx: "Context", weight, heads, eps: float, what: str):
     return HeadNorm(ptr, heads.type if kind else FP32, eps)
 
 
+def _scores(ctx: "Context", cap: float, slopes, heads: int):
+    """The cvs_scores of a call, None where scores stay as they are."""
+    if slopes is None:
+        return ScoreOptions(cap, None) if cap else None
+    return ScoreOptions(cap, _vector(ctx, slopes, "slopes", heads, ("float32",))[0])
+
+
 def _ready(ctx: "Context", x, out, weight, eps: float, what: str):
     """Heads, their output and norm as C takes them; None, all three, without heads."""
     if x is None:
@@ -596,18 +617,22 @@ class Context:
     def dataset(self, rows) -> "Dataset":
         return Dataset(self, rows)
 
-    def prompt_plan(self, q_lengths, heads: int, kv_heads: int, k_lengths=None, causal: bool = True) -> "PromptPlan":
-        return PromptPlan(self, q_lengths, heads, kv_heads, k_lengths, causal)
+    def prompt_plan(self, q_lengths, heads: int, kv_heads: int, k_lengths=None, causal: bool = True,
+                    prefixes=None) -> "PromptPlan":
+        return PromptPlan(self, q_lengths, heads, kv_heads, k_lengths, causal, prefixes)
 
-    def prompt_attention_async(self, plan: "PromptPlan", q, k, v, out, lse=None, scale: float = 0.0) -> None:
+    def prompt_attention_async(self, plan: "PromptPlan", q, k, v, out, lse=None, scale: float = 0.0, cap: float = 0.0,
+                               slopes=None) -> None:
         """Attention over packed sequences (C: cvs_prompt_attention_async):
         q, out (query tokens, heads, head_dim), k, v (key tokens, kv_heads,
         head_dim); lse, when given, (heads, query tokens) float32; scale 0:
-        1 / sqrt(head_dim)."""
+        1 / sqrt(head_dim).  Scores are capped to cap * tanh(score / cap) where
+        it is not 0, and lose slopes[head] (float32) times their distance."""
         hq, hk, hv, ho = (_heads(self, x, w)[0] for x, w in ((q, "q"), (k, "k"), (v, "v"), (out, "out")))
         hl = _lse(self, lse, hq.heads, hq.tokens)
-        after = self._behind_torch(q, k, v, out, lse)
-        _check(load().cvs_prompt_attention_async(self.handle, plan.handle, hq, hk, hv, ho, hl, scale))
+        sc = _scores(self, cap, slopes, hq.heads)
+        after = self._behind_torch(q, k, v, out, lse, slopes)
+        _check(load().cvs_prompt_attention_scored_async(self.handle, plan.handle, hq, hk, hv, ho, hl, scale, sc))
         if after:
             after()
 
@@ -972,14 +997,23 @@ class PromptPlan:
     """How a batch of packed sequences is worked on, for every layer of a
     model (C: cvs_prompt_plan)."""
 
-    def __init__(self, ctx: Context, q_lengths, heads: int, kv_heads: int, k_lengths=None, causal: bool = True):
+    def __init__(self, ctx: Context, q_lengths, heads: int, kv_heads: int, k_lengths=None, causal: bool = True,
+                 prefixes=None):
         self.ctx = ctx
         self.handle = None
         n = len(q_lengths)
         h = c_void_p()
         ql, kl = _i64(q_lengths), None if k_lengths is None else _i64(k_lengths, n)
-        _check(load().cvs_prompt_plan_create(ctx.handle, _at(ql), None if kl is None else _at(kl), n, int(heads),
-                                             int(kv_heads), 1 if causal else 0, byref(h)))
+        kl_at = None if kl is None else _at(kl)
+        if prefixes is None:
+            _check(load().cvs_prompt_plan_create(ctx.handle, _at(ql), kl_at, n, int(heads), int(kv_heads),
+                                                 1 if causal else 0, byref(h)))
+        else:
+            if not causal:
+                raise ValueError("prefixes belong to a causal plan")
+            seen = _i64(prefixes, n)
+            _check(load().cvs_prompt_plan_create_prefix(ctx.handle, _at(ql), kl_at, _at(seen), n, int(heads),
+                                                        int(kv_heads), byref(h)))
         self.handle = h
         ctx._adopt(self)
 
@@ -1164,14 +1198,17 @@ class KvCache:
         if after:
             after()
 
-    def attention_async(self, plan: "KvPlan", q, out, layer: int = 0, lse=None, scale: float = 0.0) -> None:
+    def attention_async(self, plan: "KvPlan", q, out, layer: int = 0, lse=None, scale: float = 0.0, cap: float = 0.0,
+                        slopes=None) -> None:
         """Attention of the plan's tokens over a layer (C:
         cvs_kv_attention_async): q, out (tokens, heads, head_dim); lse, when
-        given, (heads, tokens) float32; scale 0: 1 / sqrt(head_dim)."""
+        given, (heads, tokens) float32; scale 0: 1 / sqrt(head_dim); cap and
+        slopes as in prompt_attention_async."""
         hq, ho = _heads(self.ctx, q, "q")[0], _heads(self.ctx, out, "out")[0]
         hl = _lse(self.ctx, lse, hq.heads, hq.tokens)
-        after = self.ctx._behind_torch(q, out, lse)
-        _check(load().cvs_kv_attention_async(self.handle, plan.handle, layer, hq, ho, hl, scale))
+        sc = _scores(self.ctx, cap, slopes, hq.heads)
+        after = self.ctx._behind_torch(q, out, lse, slopes)
+        _check(load().cvs_kv_attention_scored_async(self.handle, plan.handle, layer, hq, ho, hl, scale, sc))
         if after:
             after()
 

@@ -125,6 +125,95 @@ __device__ CVS_INLINE float largest(const f32x16& s, float c) {
   return both_max(top) * c;
 }
 
+// What becomes of a product s = q.k on its way to a score.  Plain: the score
+// is c s in log2 units, c = scale log2(e).  Otherwise `finish` makes the scores
+// of a lane's 16 keys of it, already in log2 units, and c is 1 from there on:
+//
+//   cap: log2(e) C tanh(scale s / C).  With u = scale s / C, y = s^2: up to |u| =
+//   0.75 that is c s P(y), P of degree 4 fitted to tanh(u) / u (least squares
+//   weighted to an even relative error: 6e-7), its coefficients with c and the
+//   powers of scale / C in them; above, C (1 - 2 / (1 + e^2u)), whose error is
+//   that of its last places, 2^-22 C.  A tile with no large |u|, all of them in
+//   models whose scores stay within half of the cap, takes six instructions a
+//   score and no exponential;
+//
+//   bias: minus log2(e) slope |place - key|, by the row's place and slope.
+struct ScoreArgs {
+  float c;             // of plain scores and of caps' small ones
+  float cap;           // log2(e) C
+  float twice;         // log2(e) 2 scale / C
+  float largest_y;     // of small scores; -1: none is small
+  float a[4];          // P's coefficients behind c
+  const float* slopes;  // of the heads, natural units; null: none
+};
+struct PlainScores {
+  static constexpr bool kPlain = true, kDown = false;
+  float c;
+};
+template <bool kCap, bool kBias>
+struct Scores {
+  static constexpr bool kPlain = false;
+  // Scores fall with the distance: the nearest keys first, or every tile would have a larger maximum than the one before.
+  static constexpr bool kDown = kBias;
+  static constexpr float c = 1.f;
+  const ScoreArgs& a;
+  float slope;  // log2(e) times the row's
+  int place;    // the row's, counted like the keys
+
+  // Keys key + 8 (r / 4) + r % 4.
+  __device__ CVS_INLINE void finish(f32x16& s, int key) const {
+    if constexpr (kCap) {
+      f32x16 x;
+      float top = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float y = s[r] * s[r];
+        top = fmaxf(top, y);
+        float p = __builtin_fmaf(y, a.a[3], a.a[2]);
+        p = __builtin_fmaf(y, p, a.a[1]);
+        p = __builtin_fmaf(y, p, a.a[0]);
+        x[r] = s[r] * __builtin_fmaf(y, p, a.c);
+      }
+      if (__ballot(!(top <= a.largest_y))) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float e = 1.f + __builtin_amdgcn_exp2f(s[r] * a.twice);
+          const float large = __builtin_fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(e), a.cap);
+          x[r] = s[r] * s[r] <= a.largest_y ? x[r] : large;
+        }
+      }
+      s = x;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] *= a.c;
+    }
+    if constexpr (kBias) {
+      const float far = float(place - key);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        s[r] = __builtin_fmaf(-slope, __builtin_fabsf(far - float(8 * (r / 4) + r % 4)), s[r]);
+    }
+  }
+};
+// A call's scores, checked; cap 0 for none.
+ScoreArgs score_args(const cvs_scores* scores, float scale, int dim);
+// Calls go with the type of a call's capped or biased scores (a std::common_type of it).
+template <typename Go>
+void pick_scores(const ScoreArgs& a, const Go& go) {
+  if (a.cap > 0.f && a.slopes) go(std::common_type<Scores<true, true>>{});
+  else if (a.slopes) go(std::common_type<Scores<false, true>>{});
+  else go(std::common_type<Scores<true, false>>{});
+}
+
+// The order in which a row's tiles are taken: ascending, or from tile `top` - 1 down to 0 and then up from `top`.
+struct Ascending {
+  __device__ CVS_INLINE int operator()(int step) const { return step; }
+};
+struct FromTheMiddle {
+  int top;
+  __device__ CVS_INLINE int operator()(int step) const { return step < top ? top - 1 - step : step; }
+};
+
 // Scores of 32 keys -> probabilities 2^(c s - m), summed up.  Masked scores
 // come in as -inf and leave as 0.
 //
@@ -205,82 +294,106 @@ __device__ CVS_INLINE u32x4 prob_operand(const f32x16& p, int step) {
 // tile; in the first `open_tiles` tiles all rows see all keys, and `mixed` says
 // that the tiles behind them may hold values that `hide` leaves and that some
 // row does not see.
-// The source moves the data: load_keys(t) and load_values(t) ask for a tile of
-// either (buffer t & 1; the workgroup's waves share the work; in ascending
-// order, a tile's values after the next one's keys), keys(t, h, i)
-// is the A operand of columns 16 i of half h's 32 keys, values(t, h, b, k) of
-// columns 32 b of its k-th 16 keys; hide(v, t, h, k) clears what a masked
-// tile's values must not show.
+// Tiles are taken in `order`, an open one behind a masked one only where scores
+// fall with the distance.
+// The source moves the data: load_keys(n, t) and load_values(n, t) ask for the
+// n-th tile, which is tile t, of either (buffer n & 1; the workgroup's waves
+// share the work; in this order, a tile's values after the next one's keys),
+// keys(n, h, i) is the A operand of columns 16 i of half h's 32 keys, values(n,
+// h, b, k) of columns 32 b of its k-th 16 keys; hide(v, t, h, k) clears what a
+// masked tile's values must not show.
 //
 // Half tiles go through a pipeline of three: the products of one with the
 // values and of the next with the keys run while the one between goes through
 // its exponentials.  In the middle of tile t everyone is done with its keys
 // and with the values before it; what was asked for one tile ago, the next
 // keys and its values, has to be there.
-template <bool kBf, int NB, int KS, typename Source>
+template <bool kBf, int NB, int KS, typename Source, typename Scoring, typename Order>
 __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[KS], Source& src, int tiles,
-                                        int open_tiles, bool mixed, int limit, float c, bool& bad) {
+                                        int open_tiles, bool mixed, int limit, const Scoring& scoring,
+                                        const Order& order, bool& bad) {
   const int half = __lane_id() >> 5;
   f32x16 s[2];    // scores of a tile's two halves
   u32x4 p[2][2];  // and their probabilities
-  auto scores = [&](int t, int h) CVS_INLINE {
+  auto scores = [&](int n, int h) CVS_INLINE {
     f32x16 x{};
 #pragma unroll
-    for (int i = 0; i < KS; ++i) x = mfma<kBf>(src.keys(t, h, i), q[i], x);
+    for (int i = 0; i < KS; ++i) x = mfma<kBf>(src.keys(n, h, i), q[i], x);
     return x;
   };
-  auto add_values = [&](int t, int h, auto masked) CVS_INLINE {
+  auto add_values = [&](int n, int h, auto masked) CVS_INLINE {
     if constexpr (!masked) {
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int b = 0; b < NB; ++b) st.o[b] = mfma<kBf>(src.values(t, h, b, k), p[h][k], st.o[b]);
+        for (int b = 0; b < NB; ++b) st.o[b] = mfma<kBf>(src.values(n, h, b, k), p[h][k], st.o[b]);
     } else {
+      const int t = order(n);
       u32x4 v[2 * NB];
 #pragma unroll
-      for (int i = 0; i < 2 * NB; ++i) v[i] = src.hide(src.values(t, h, i / 2, i % 2), t, h, i % 2);
-      if (mixed) bad |= clean<kBf>(v);
+      for (int i = 0; i < 2 * NB; ++i) v[i] = src.hide(src.values(n, h, i / 2, i % 2), t, h, i % 2);
+      if (mixed && (!Scoring::kDown || t >= open_tiles)) bad |= clean<kBf>(v);
 #pragma unroll
       for (int i = 0; i < 2 * NB; ++i) st.o[i / 2] = mfma<kBf>(v[i], p[h][i % 2], st.o[i / 2]);
     }
   };
-  auto mask = [&](int t, int h) CVS_INLINE {
-    const int seen = limit - 64 * t - 32 * h - 4 * half;
+  auto finish = [&](int n, int h) CVS_INLINE {
+    if constexpr (!Scoring::kPlain) scoring.finish(s[h], 64 * order(n) + 32 * h + 4 * half);
+  };
+  auto mask = [&](int n, int h) CVS_INLINE {
+    const int seen = limit - 64 * order(n) - 32 * h - 4 * half;
 #pragma unroll
     for (int r = 0; r < 16; ++r)
       if (8 * (r / 4) + r % 4 >= seen) s[h][r] = -INFINITY;
   };
   auto soften = [&](int h) CVS_INLINE {
-    probabilities<kBf>(s[h], st, c);
+    probabilities<kBf>(s[h], st, scoring.c);
 #pragma unroll
     for (int k = 0; k < 2; ++k) p[h][k] = prob_operand<kBf>(s[h], k);
   };
-  auto step = [&](int t, auto masked) CVS_INLINE {
-    if (t > 0) add_values(t - 1, 1, masked);
-    if constexpr (masked) mask(t, 0);
-    s[1] = scores(t, 1);
+  auto step = [&](int n, auto masked) CVS_INLINE {
+    if (n > 0) add_values(n - 1, 1, masked);
+    finish(n, 0);
+    if constexpr (masked) mask(n, 0);
+    s[1] = scores(n, 1);
     soften(0);
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     __syncthreads();
-    if (t + 2 < tiles) src.load_keys(t + 2);
-    if (t + 1 < tiles) src.load_values(t + 1);
-    add_values(t, 0, masked);
-    if constexpr (masked) mask(t, 1);
-    s[0] = scores(t + 1, 0);  // past the last tile: of whatever is there, and not used
+    if (n + 2 < tiles) src.load_keys(n + 2, order(n + 2));
+    if (n + 1 < tiles) src.load_values(n + 1, order(n + 1));
+    add_values(n, 0, masked);
+    finish(n, 1);
+    if constexpr (masked) mask(n, 1);
+    s[0] = scores(n + 1, 0);  // past the last tile: of whatever is there, and not used
     soften(1);
   };
   if (tiles <= 0) return;
-  src.load_keys(0);
-  if (tiles > 1) src.load_keys(1);
-  src.load_values(0);
+  src.load_keys(0, order(0));
+  if (tiles > 1) src.load_keys(1, order(1));
+  src.load_values(0, order(0));
   __builtin_amdgcn_s_waitcnt(0x0F70);
   __syncthreads();
   s[0] = scores(0, 0);
-  mask(0, 0);
-  st.m = largest(s[0], c) - kLift<kBf>;
-  int t = 0;
-  for (; t < open_tiles; ++t) step(t, std::false_type{});
-  for (; t < tiles; ++t) step(t, std::true_type{});
+  if constexpr (Scoring::kPlain) {
+    mask(0, 0);
+    st.m = largest(s[0], scoring.c) - kLift<kBf>;
+  } else {
+    const f32x16 products = s[0];
+    finish(0, 0);
+    mask(0, 0);
+    st.m = largest(s[0], scoring.c) - kLift<kBf>;
+    s[0] = products;
+  }
+  if constexpr (!Scoring::kDown) {
+    int n = 0;
+    for (; n < open_tiles; ++n) step(n, std::false_type{});
+    for (; n < tiles; ++n) step(n, std::true_type{});
+  } else {
+    for (int n = 0; n < tiles; ++n) {
+      if (order(n) >= open_tiles || (n > 0 && order(n - 1) >= open_tiles)) step(n, std::true_type{});
+      else step(n, std::false_type{});
+    }
+  }
   add_values(tiles - 1, 1, std::true_type{});
 }
 

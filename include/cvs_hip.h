@@ -553,6 +553,29 @@ int cvs_prompt_plan_destroy(cvs_prompt_plan* plan);
 int cvs_prompt_attention_async(cvs_context* ctx, const cvs_prompt_plan* plan, const cvs_heads* q, const cvs_heads* k,
                                const cvs_heads* v, const cvs_heads* out, float* lse, float scale);
 
+/* A causal plan whose queries all see the first prefixes[i] keys of their
+ * sequence besides (0 up to its key length): query i sees its keys up to the
+ * larger of i + k_length - q_length and prefixes[i] - 1. */
+int cvs_prompt_plan_create_prefix(cvs_context* ctx, const int64_t* q_lengths, const int64_t* k_lengths,
+                                  const int64_t* prefixes, int64_t n, int heads, int kv_heads,
+                                  cvs_prompt_plan** out_plan);
+
+/* What becomes of a score x = scale * q . k: cap * tanh(x / cap) where cap is
+ * not 0 (finite, 1e-30 to 2e38), then less slopes[h] times the distance |p - j|
+ * of the key's place j from the query's, p = i + k_length - q_length in a
+ * prompt and the token's place in its sequence in a cache.  slopes: device
+ * memory, a finite float for each query head, or null.  Both are in fp32; a
+ * capped score is off by at most 2^-20 of itself and 2^-22 of the cap. */
+typedef struct cvs_scores {
+  float cap;
+  const float* slopes;
+} cvs_scores;
+
+/* cvs_prompt_attention_async with such scores (null: as they are). */
+int cvs_prompt_attention_scored_async(cvs_context* ctx, const cvs_prompt_plan* plan, const cvs_heads* q,
+                                      const cvs_heads* k, const cvs_heads* v, const cvs_heads* out, float* lse,
+                                      float scale, const cvs_scores* scores);
+
 /* A cache of keys and values: `layers` layers of `pages` pages of
  * page_tokens tokens (a power of two from 32 to 4096), each token kv_heads x
  * head_dim elements of keys and of values.  Allocated once, in the layout
@@ -639,6 +662,10 @@ int cvs_kv_read_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int first_layer, i
  * through a workspace that the context keeps. */
 int cvs_kv_attention_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int layer, const cvs_heads* q,
                            const cvs_heads* out, float* lse, float scale);
+
+/* cvs_kv_attention_async with such scores (null: as they are). */
+int cvs_kv_attention_scored_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int layer, const cvs_heads* q,
+                                  const cvs_heads* out, float* lse, float scale, const cvs_scores* scores);
 
 /* ---- positions and norms of heads ----------------------------------------- */
 
