@@ -207,6 +207,7 @@ void pick_scores(const ScoreArgs& a, const Go& go) {
 
 // The order in which a row's tiles are taken: ascending, or from tile `top` - 1 down to 0 and then up from `top`.
 struct Ascending {
+  static constexpr int top = 0;
   __device__ CVS_INLINE int operator()(int step) const { return step; }
 };
 struct FromTheMiddle {
@@ -384,14 +385,17 @@ __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[KS], 
     st.m = largest(s[0], scoring.c) - kLift<kBf>;
     s[0] = products;
   }
+  int n = 0;
   if constexpr (!Scoring::kDown) {
-    int n = 0;
     for (; n < open_tiles; ++n) step(n, std::false_type{});
     for (; n < tiles; ++n) step(n, std::true_type{});
   } else {
-    for (int n = 0; n < tiles; ++n) {
-      if (order(n) >= open_tiles || (n > 0 && order(n - 1) >= open_tiles)) step(n, std::true_type{});
-      else step(n, std::false_type{});
+    // Masked tiles come first, down to the open ones, and last; a step behind a masked one still adds its values.
+    const int first = order.top > open_tiles ? order.top - open_tiles + 1 : 0, last = max(order.top, open_tiles);
+    for (int masked = min(first, tiles), open = min(last, tiles);; masked = open = tiles) {
+      for (; n < masked; ++n) step(n, std::true_type{});
+      for (; n < open; ++n) step(n, std::false_type{});
+      if (n >= tiles) break;
     }
   }
   add_values(tiles - 1, 1, std::true_type{});
