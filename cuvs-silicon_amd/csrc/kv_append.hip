@@ -3,12 +3,12 @@
 // normed and rotated, in one launch.
 //
 // A workgroup takes one tile of up to 32 tokens: a wave for each of up to 4 kv
-// heads, or some query heads by all of them.  Its threads first make the
-// cosines and sines of the tile's tokens, one each, for all heads.  A wave's
-// keys are normed and rotated as rows of pieces (rotary.hpp) on their way to
-// LDS, where they change places; values go straight from their rows to the
-// pool (kv_tiles.hpp).  All of a wave's loads are under way before the cosines
-// are made.
+// heads, or some query heads by all of them.  Its threads first make the factors
+// of the tile's tokens, a pair of channels each, for all heads (rotary.hpp).  A
+// wave's keys are normed and rotated as rows of pieces on their way to LDS,
+// where they change places, in the factors' room; values go straight from their
+// rows to the pool (kv_tiles.hpp).  All of a wave's loads are under way before
+// the factors are made.
 #include <algorithm>
 #include <cstring>
 
@@ -25,12 +25,13 @@ struct AppendArgs {
   View k, v, q, q_out;
   Norm k_norm, q_norm;
   const int64_t* positions;  // null: the tokens' places in their sequences
-  const uint64_t* turns;
-  float magnitude;
-  int n_spans, page_tiles, by_tile, dim, dims;
-  int kv_heads, kv_groups;             // workgroups of a tile's kv heads
-  int q_heads, q_chunk, q_chunks;      // and of its query heads
+  Turning turning;
+  int n_spans, page_tiles, by_tile;
+  int kv_heads, kv_groups;         // workgroups of a tile's kv heads
+  int q_heads, q_chunk, q_chunks;  // and of its query heads
+  uint32_t q_magic, q_last_magic;  // of a chunk's heads, and of the last one's
   int kv_blocks;
+  int at_rows;  // in LDS, of kChannels' rows
 };
 
 template <bool kBf, int NB, Pairs kPairs, bool kNorm>
@@ -39,7 +40,7 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a, const S
   constexpr int kRows = 64 / kLanes, kSteps = 32 / kRows;  // tokens of a wave's step
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool queries = int(blockIdx.x) >= a.kv_blocks;
   const int block = queries ? blockIdx.x - a.kv_blocks : blockIdx.x, each = queries ? a.q_chunks : a.kv_groups;
   const int part = block % each, n = block / each;
@@ -49,35 +50,28 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a, const S
   if (lo >= hi) return;
   const int64_t row = int64_t(sp.row0) + 32 * tile - sp.begin();  // of the tile's token 0
 
-  const HeadLane<kLanes> l(a.dim, a.dims);
-  const int pitch = (l.half + 3) & ~3;
-  u32x4* const s_keys = reinterpret_cast<u32x4*>(lds) + wave * 32 * P;  // the wave's
-  float* const s_w = reinterpret_cast<float*>(lds + waves * 512 * P);
-  float* const s_cos = s_w + (kNorm ? kMaxDim : 0);
-  float* const s_sin = s_cos + 32 * pitch;
+  const HeadLane<kLanes> l(a.turning.dim, a.turning.half);
+  // The factors, and, when all waves are through with them, the keys that change places: each wave its own.
+  float* const s_own = reinterpret_cast<float*>(lds) - lo * l.dim;
+  float* const s_other = s_own + 32 * l.dim;
+  u32x4* const s_keys = reinterpret_cast<u32x4*>(lds) + wave * 32 * P;
+  u32x4* const s_rows = reinterpret_cast<u32x4*>(lds + a.at_rows) + threadIdx.x;
   auto before = [&]() CVS_INLINE {
     const int64_t first = int64_t(sp.index) * (32 * a.page_tiles) + 32 * tile;
-    for (int i = threadIdx.x; i < (hi - lo) * l.half; i += blockDim.x) {
-      const int t = lo + i / l.half, p = i % l.half;
-      const int64_t position = a.positions ? a.positions[row + t] : first + t;
-      const float2 cs = cos_sin(a.turns[p] * uint64_t(position));
-      s_cos[t * pitch + p] = a.magnitude * cs.x;
-      s_sin[t * pitch + p] = a.magnitude * cs.y;
-    }
-    if constexpr (kNorm) load_weight<kBf>(s_w, queries ? a.q_norm : a.k_norm, a.dim);
+    make_turning<kBf, kPairs>(a.turning, queries ? a.q_norm : a.k_norm, lo, hi, s_own, s_other, [&](int t) CVS_INLINE {
+      return a.positions ? a.positions[row + t] : first + t;
+    });
     __syncthreads();
   };
 
   if (queries) {
     const int h0 = part * a.q_chunk, nh = min(a.q_chunk, a.q_heads - h0);
-    const bool normed = kNorm && a.q_norm.weight;
-    auto place = [&](int r) CVS_INLINE {
-      const int t = lo + r / nh, h = h0 + r % nh;
-      return HeadRow{a.q.p + 2 * ((row + t) * a.q.token + h * a.q.head),
-                     a.q_out.p + 2 * ((row + t) * a.q_out.token + h * a.q_out.head), s_cos + t * pitch,
-                     s_sin + t * pitch, normed ? s_w : nullptr, a.q_norm.eps};
+    auto first = [&](const View& v) CVS_INLINE {
+      return RowView{v.p + 2 * ((row + lo) * v.token + h0 * v.head), uint32_t(2 * v.token), uint32_t(2 * v.head)};
     };
-    ready_rows<kBf, kLanes, kPairs, kNorm>(l, (hi - lo) * nh, s_keys + lane, place, before);
+    const Rows rows{(hi - lo) * nh, nh, nh == a.q_chunk ? a.q_magic : a.q_last_magic, first(a.q), first(a.q_out),
+                    s_own + lo * l.dim, s_other + lo * l.dim, a.q_norm.weight != nullptr, a.q_norm.eps};
+    ready_rows<kBf, kLanes, kPairs, kNorm>(l, rows, s_rows, before);
     return;
   }
 
@@ -95,16 +89,17 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a, const S
     x[i] = *reinterpret_cast<const u32x4*>(ks + 2 * (values.held(kRows * i + lane / kLanes) * a.k.token + 8 * l.piece));
   values.load(vs, a.v.token, l.pieces);
   before();
-  if (spare) return;
-  values.store(l.pieces);
+  if (!spare) values.store(l.pieces);
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
     if (kRows * i + kRows <= lo || kRows * i >= hi) continue;  // none of the step's tokens is the call's
-    const int t = kRows * i + lane / kLanes, tc = values.held(t);
-    x[i] = ready<kBf, kLanes, kPairs, kNorm>(x[i], l, s_cos + tc * pitch, s_sin + tc * pitch,
-                                             kNorm && a.k_norm.weight ? s_w : nullptr, a.k_norm.eps, s_keys + lane);
+    const int t = values.held(kRows * i + lane / kLanes);
+    x[i] = ready<kBf, kLanes, kPairs, kNorm>(x[i], l, s_own + t * l.dim, s_other + t * l.dim, a.k_norm.weight != nullptr,
+                                             a.k_norm.eps, s_rows);
+    row_done(x[i]);
   }
-  // Staged behind all of them, whose raw rows may have passed through the same places.
+  __syncthreads();  // everyone has read the factors
+  if (spare) return;
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
     const int t = kRows * i + lane / kLanes;
@@ -115,9 +110,11 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a, const S
 }
 
 template <bool kBf, int NB>
-void launch(cvs_context* ctx, const AppendArgs& a, const Spans& inl, Pairs pairs, bool norm, unsigned blocks, int waves) {
-  const size_t pitch = size_t((a.dims / 2 + 3) / 4 * 4);
-  const size_t lds = size_t(waves) * 512 * 4 * NB + (norm ? kMaxDim * 4 : 0) + 2 * 32 * pitch * 4;
+void launch(cvs_context* ctx, const AppendArgs& args, const Spans& inl, Pairs pairs, bool norm, unsigned blocks,
+            int waves) {
+  AppendArgs a = args;
+  a.at_rows = std::max(waves * 512 * 4 * NB, 2 * 32 * 4 * a.turning.dim);
+  const size_t lds = size_t(a.at_rows) + (pairs == kChannels ? size_t(waves) * 1024 : 0);
   const TimerSpan ts = timer_span(ctx, "kv_append");
   auto go = [&](auto kernel) {
     hipExtLaunchKernelGGL(kernel, dim3(blocks), dim3(unsigned(64 * waves)), lds, ctx->stream, ts.start, ts.stop, 0, a, inl);
@@ -132,7 +129,7 @@ void launch(cvs_context* ctx, const AppendArgs& a, const Spans& inl, Pairs pairs
 
 template <bool kBf>
 void launch(cvs_context* ctx, const AppendArgs& a, const Spans& inl, Pairs pairs, bool norm, unsigned blocks, int waves) {
-  switch ((a.dim + 31) / 32) {
+  switch ((a.turning.dim + 31) / 32) {
     case 1: launch<kBf, 1>(ctx, a, inl, pairs, norm, blocks, waves); break;
     case 2: launch<kBf, 2>(ctx, a, inl, pairs, norm, blocks, waves); break;
     case 3: launch<kBf, 3>(ctx, a, inl, pairs, norm, blocks, waves); break;
@@ -174,7 +171,7 @@ extern "C" int cvs_kv_append_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int l
         if (x->heads != q->heads) fail(CVS_ERR_INVALID_ARGUMENT, "q_out must have the heads of q");
         if (plan->heads > 0 && x->heads != plan->heads)
           fail(CVS_ERR_INVALID_ARGUMENT, std::string(what) + " must have the plan's heads");
-        if (x->heads > 65536) fail(CVS_ERR_UNSUPPORTED, "too many heads");
+        if (x->heads > 65535) fail(CVS_ERR_UNSUPPORTED, "too many heads");
       }
       check_rows_apart(q_out, "q_out");
       a.q_norm = norm_of(q_norm, cache->type, "q");
@@ -191,14 +188,14 @@ extern "C" int cvs_kv_append_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int l
     if (rotary) {
       captured_rotary(rotary);
       a.positions = positions;
-      a.turns = rotary->turns.as<uint64_t>();
-      a.magnitude = rotary->magnitude;
-      a.dims = rotary->dims;
+      a.turning.turns = rotary->turns.as<uint64_t>();
+      a.turning.magnitude = rotary->magnitude;
+      a.turning.half = rotary->dims / 2;
     }
     a.n_spans = int(plan->spans.size());
     a.page_tiles = int(cache->book->page_tokens() / 32);
     a.by_tile = spans_by_tile(plan);
-    a.dim = cache->dim;
+    a.turning.dim = cache->dim;
     a.kv_heads = cache->kv_heads;
     a.kv_groups = (cache->kv_heads + 3) / 4;
     const int waves = (cache->kv_heads + a.kv_groups - 1) / a.kv_groups;
@@ -209,10 +206,15 @@ extern "C" int cvs_kv_append_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int l
       a.q = view_of(q);
       a.q_out = view_of(q_out);
       a.q_heads = q->heads;
-      // About 128 rows a workgroup.
-      const int64_t fill = std::max<int64_t>(1, plan->tokens / tiles);
-      a.q_chunk = int(std::min<int64_t>(q->heads, std::max<int64_t>(1, 128 / fill)));
+      // All heads by one workgroup, which makes a tile's factors once, or, where that leaves compute units without one,
+      // down to 16 rows each.
+      const int64_t fill = std::max<int64_t>(1, plan->tokens / tiles), filled = (plan->tokens + fill - 1) / fill;
+      const int64_t fit = std::clamp<int64_t>(2 * ctx->compute_units / filled, 1, (q->heads * fill + 15) / 16);
+      a.q_chunk = int(std::min<int64_t>((q->heads + fit - 1) / fit, 1024));
+      if (!rows_near(a.q, a.q_chunk) || !rows_near(a.q_out, a.q_chunk)) a.q_chunk = 1;
       a.q_chunks = (q->heads + a.q_chunk - 1) / a.q_chunk;
+      a.q_magic = magic_of(a.q_chunk);
+      a.q_last_magic = magic_of(q->heads - (a.q_chunks - 1) * a.q_chunk);
       blocks += tiles * a.q_chunks;
     }
     if (blocks > kMaxBlocks) fail(CVS_ERR_UNSUPPORTED, "too many tokens");

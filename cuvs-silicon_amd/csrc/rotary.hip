@@ -1,14 +1,14 @@
 // Rotary positions of heads, with or without the norm of each head before
 // them, from array to array: queries and keys in one launch.
 //
-// A workgroup takes a few tokens, all of their heads or a part of them.  Its
-// threads first make the cosines and sines of those tokens, one each, for all
-// heads; then a head is a row of 16-byte pieces, one a lane, and 1 to 16 lanes
-// (the power of two that holds the head) have a row.  The sum of squares goes
-// over those lanes, a channel's partner comes from its own piece, from the
-// lane that has it, or, where the halves are no whole pieces apart, through
-// LDS.  Rows are read kAhead at a time, the first of them before the cosines
-// are made.  Bound by the memory.
+// A workgroup takes a few tokens, all of their query or key heads or a part of
+// them.  Its threads first make the factors of those tokens' channels, a pair
+// each, for all heads (rotary.hpp); then a head is a row of 16-byte pieces, one
+// a lane, and 4 to 16 lanes (the power of two that holds the head) have a row.
+// The sum of squares goes over those lanes, a channel's partner comes from its
+// own piece, from the lane that has it, or, where the halves are no whole pieces
+// apart, through LDS.  Rows are read kAhead at a time, the first of them before
+// the factors are made.  Bound by the memory.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -20,53 +20,44 @@ namespace attn {
 namespace {
 
 constexpr int kTokens = 16;  // of a workgroup at most
-constexpr int kMaxPairs = kMaxDim / 2;
+
+// Queries or keys.
+struct Part {
+  View in, out;
+  Norm norm;
+  int heads, per_block, chunk, chunks;  // tokens and heads of a workgroup, workgroups of the heads
+  uint32_t magic, last_magic;           // of a chunk's heads, and of the last one's
+  int blocks;
+};
 
 struct RotateArgs {
-  View in[2], out[2];  // queries, keys
-  Norm norm[2];
-  int heads[2];
+  Part part[2];
   const int64_t* positions;
-  const uint64_t* turns;
+  Turning turning;
   int64_t tokens;
-  int dim, dims;
-  float magnitude;
-  int per_block;  // tokens of a workgroup
-  int chunk;      // heads of a workgroup
 };
 
 template <bool kBf, int kLanes, Pairs kPairs, bool kNorm>
 __global__ __launch_bounds__(256) void rotate_kernel(const RotateArgs a) {
-  __shared__ __align__(16) float s_cos[kTokens * kMaxPairs], s_sin[kTokens * kMaxPairs];
-  __shared__ __align__(16) float s_w[kNorm ? 2 * kMaxDim : 1];
+  __shared__ __align__(16) float s_own[kTokens * kMaxDim], s_other[kTokens * kMaxDim];
   __shared__ __align__(16) u32x4 s_rows[kPairs == kChannels ? 256 : 1];
-  const int64_t t0 = int64_t(blockIdx.x) * a.per_block;
-  const int nt = int(min(int64_t(a.per_block), a.tokens - t0));
-  const int h0 = blockIdx.y * a.chunk, nh = min(a.chunk, a.heads[0] + a.heads[1] - h0);
-  const HeadLane<kLanes> l(a.dim, a.dims);
-  auto place = [&](int r) CVS_INLINE {
-    const int t = r / nh, h = h0 + r % nh, k = h >= a.heads[0], head = k ? h - a.heads[0] : h;
-    const View& in = k ? a.in[1] : a.in[0];
-    const View& out = k ? a.out[1] : a.out[0];
-    const Norm& n = k ? a.norm[1] : a.norm[0];
-    return HeadRow{in.p + 2 * ((t0 + t) * in.token + head * in.head),
-                   out.p + 2 * ((t0 + t) * out.token + head * out.head), s_cos + t * kMaxPairs, s_sin + t * kMaxPairs,
-                   kNorm && n.weight ? s_w + k * kMaxDim : nullptr, n.eps};
+  const bool second = int(blockIdx.x) >= a.part[0].blocks;
+  const Part& p = a.part[second];
+  const int block = blockIdx.x - (second ? a.part[0].blocks : 0);
+  const int64_t t0 = int64_t(block / p.chunks) * p.per_block;
+  const int nt = int(min(int64_t(p.per_block), a.tokens - t0));
+  const int h0 = block % p.chunks * p.chunk, nh = min(p.chunk, p.heads - h0);
+  const HeadLane<kLanes> l(a.turning.dim, a.turning.half);
+  auto first = [&](const View& v) CVS_INLINE {
+    return RowView{v.p + 2 * (t0 * v.token + h0 * v.head), uint32_t(2 * v.token), uint32_t(2 * v.head)};
   };
-  auto before = [&]() CVS_INLINE {
-    for (int i = threadIdx.x; i < nt * l.half; i += 256) {
-      const int t = i / l.half, p = i % l.half;
-      const float2 cs = cos_sin(a.turns[p] * uint64_t(a.positions[t0 + t]));
-      s_cos[t * kMaxPairs + p] = a.magnitude * cs.x;
-      s_sin[t * kMaxPairs + p] = a.magnitude * cs.y;
-    }
-    if constexpr (kNorm) {
-      load_weight<kBf>(s_w, a.norm[0], a.dim);
-      load_weight<kBf>(s_w + kMaxDim, a.norm[1], a.dim);
-    }
+  const Rows rows{nt * nh, nh, nh == p.chunk ? p.magic : p.last_magic, first(p.in), first(p.out), s_own, s_other,
+                  p.norm.weight != nullptr, p.norm.eps};
+  ready_rows<kBf, kLanes, kPairs, kNorm>(l, rows, s_rows + (kPairs == kChannels ? threadIdx.x : 0), [&]() CVS_INLINE {
+    make_turning<kBf, kPairs>(a.turning, p.norm, 0, nt, s_own, s_other,
+                              [&](int t) CVS_INLINE { return a.positions[t0 + t]; });
     __syncthreads();
-  };
-  ready_rows<kBf, kLanes, kPairs, kNorm>(l, nt * nh, s_rows + (kPairs == kChannels ? threadIdx.x : 0), place, before);
+  });
 }
 
 template <bool kBf, int kLanes>
@@ -85,8 +76,8 @@ void launch(cvs_context* ctx, const RotateArgs& a, Pairs pairs, bool norm, dim3 
 
 template <bool kBf>
 void launch(cvs_context* ctx, const RotateArgs& a, Pairs pairs, bool norm, dim3 grid) {
-  if (a.dim > 64) launch<kBf, 16>(ctx, a, pairs, norm, grid);
-  else if (a.dim > 32) launch<kBf, 8>(ctx, a, pairs, norm, grid);
+  if (a.turning.dim > 64) launch<kBf, 16>(ctx, a, pairs, norm, grid);
+  else if (a.turning.dim > 32) launch<kBf, 8>(ctx, a, pairs, norm, grid);
   else launch<kBf, 4>(ctx, a, pairs, norm, grid);
 }
 
@@ -110,35 +101,46 @@ void rotate(cvs_context* ctx, const cvs_rotary* rotary, const int64_t* positions
     if (in[i]->tokens != first->tokens || in[i]->head_dim != first->head_dim || in[i]->type != first->type)
       fail(CVS_ERR_INVALID_ARGUMENT, "q and k must have the same tokens, head_dim and type");
     check_rows_apart(out[i], (w + "_out").c_str());
-    a.in[i] = view_of(in[i]);
-    a.out[i] = view_of(out[i]);
-    a.norm[i] = norm_of(norm[i], in[i]->type, names[i]);
-    a.heads[i] = in[i]->heads;
+    if (in[i]->heads > 65535) fail(CVS_ERR_UNSUPPORTED, "too many heads");
+    a.part[i].in = view_of(in[i]);
+    a.part[i].out = view_of(out[i]);
+    a.part[i].norm = norm_of(norm[i], in[i]->type, names[i]);
+    a.part[i].heads = in[i]->heads;
   }
   if (!first) fail(CVS_ERR_INVALID_ARGUMENT, "neither q nor k");
   if (rotary) check_rotary(rotary, ctx, first->head_dim);
   if (first->tokens == 0) return;
   if (rotary && !positions) fail(CVS_ERR_INVALID_ARGUMENT, "null positions");
-  const int64_t heads = int64_t(a.heads[0]) + a.heads[1];
-  if (heads > 65536) fail(CVS_ERR_UNSUPPORTED, "too many heads");
   a.positions = positions;
   a.tokens = first->tokens;
-  a.dim = first->head_dim;
+  a.turning.dim = first->head_dim;
   if (rotary) {
     captured_rotary(rotary);
-    a.dims = rotary->dims;
-    a.turns = rotary->turns.as<uint64_t>();
-    a.magnitude = rotary->magnitude;
+    a.turning.half = rotary->dims / 2;
+    a.turning.turns = rotary->turns.as<uint64_t>();
+    a.turning.magnitude = rotary->magnitude;
   }
-  // A workgroup makes its tokens' cosines once for all rows, about 128 of them; few tokens' heads are spread over more
-  // workgroups, down to 16 rows each.
-  a.per_block = int(std::clamp<int64_t>(128 / heads, 1, kTokens));
-  const int64_t blocks = (a.tokens + a.per_block - 1) / a.per_block;
+  // A workgroup makes its tokens' cosines once for all of its rows, about 128.  Where tokens are few it takes one, and
+  // their heads are spread over more workgroups, down to 16 rows each.
+  int64_t blocks = 0;
+  for (Part& p : a.part) {
+    if (!p.heads) continue;
+    const int64_t least = 2 * ctx->compute_units;
+    p.per_block = int(std::clamp<int64_t>(std::min<int64_t>(128 / p.heads, a.tokens / least), 1, kTokens));
+    const int64_t groups = (a.tokens + p.per_block - 1) / p.per_block;
+    const int64_t fit = std::clamp<int64_t>(least / groups, 1, (p.heads + 15) / 16);
+    p.chunk = int(std::min<int64_t>((p.heads + fit - 1) / fit, 1024));
+    if (!rows_near(p.in, p.chunk) || !rows_near(p.out, p.chunk)) p.chunk = 1;
+    p.chunks = (p.heads + p.chunk - 1) / p.chunk;
+    p.magic = magic_of(p.chunk);
+    p.last_magic = magic_of(p.heads - (p.chunks - 1) * p.chunk);
+    if (groups * p.chunks > kMaxBlocks) fail(CVS_ERR_UNSUPPORTED, "too many tokens");
+    p.blocks = int(groups * p.chunks);
+    blocks += p.blocks;
+  }
   if (blocks > kMaxBlocks) fail(CVS_ERR_UNSUPPORTED, "too many tokens");
-  const int64_t fit = std::max<int64_t>(1, 2 * ctx->compute_units / blocks);
-  a.chunk = int(std::max<int64_t>(std::min<int64_t>(heads, 16), (heads + fit - 1) / fit));
-  const dim3 grid(unsigned(blocks), unsigned((heads + a.chunk - 1) / a.chunk));
-  const bool is_norm = a.norm[0].weight || a.norm[1].weight;
+  const dim3 grid{unsigned(blocks)};
+  const bool is_norm = a.part[0].norm.weight || a.part[1].norm.weight;
   if (first->type == CVS_BF16) launch<true>(ctx, a, pairs_of(rotary), is_norm, grid);
   else launch<false>(ctx, a, pairs_of(rotary), is_norm, grid);
 }

@@ -74,34 +74,78 @@ struct Norm {
   float eps;
 };
 
+// A weight of a norm, 1 without one.
+template <bool kBf>
+__device__ CVS_INLINE float weight_of(const Norm& n, int c) {
+  if (!n.weight) return 1.f;
+  return n.fp32 ? static_cast<const float*>(n.weight)[c] : to_float<kBf>(static_cast<const uint16_t*>(n.weight)[c]);
+}
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// What turns a token's heads: y_c = x_c own[c] + x_partner other[c], with the
+// norm's weights, the magnitude and the sign of the sine in both.  A channel
+// that does not turn has own = w and other = -0 for a partner of 0, which
+// leaves x w as it is, its sign included.  In LDS, `dim` floats each.
+struct Turning {
+  const uint64_t* turns;
+  float magnitude;
+  int dim, half;  // half: pairs that turn
+};
+// Tokens [lo, hi) by a workgroup: a thread has one of the dim / 2 pairs (turned
+// ones, then the rest by twos) of every so many tokens; position(t) is a token's.
+template <bool kBf, Pairs kPairs, typename Position>
+__device__ CVS_INLINE void make_turning(const Turning& a, const Norm& n, int lo, int hi, float* own, float* other,
+                                        const Position& position) {
+  const int slots = a.dim / 2, step = blockDim.x / slots, first = threadIdx.x / slots, p = threadIdx.x % slots;
+  if (first >= step) return;
+  const bool turned = p < a.half;
+  const int c0 = kPairs == kNeighbours || !turned ? 2 * p : p;
+  const int c1 = kPairs == kNeighbours || !turned ? 2 * p + 1 : p + a.half;
+  const float w0 = weight_of<kBf>(n, c0), w1 = weight_of<kBf>(n, c1);
+  const uint64_t each = turned ? a.turns[p] : 0;
+  for (int t = lo + first; t < hi; t += step) {
+    const float2 cs = turned ? cos_sin(each * uint64_t(position(t))) : float2{1.f, 0.f};
+    const float m = turned ? a.magnitude : 1.f, c = m * cs.x, s = m * cs.y;
+    float* const o = own + t * a.dim;
+    float* const r = other + t * a.dim;
+    o[c0] = c * w0;
+    o[c1] = c * w1;
+    r[c0] = turned ? -s * w1 : -0.f;
+    r[c1] = turned ? s * w0 : -0.f;
+  }
+}
+
 // A head is a row of 16-byte pieces, one a lane; the power of two of lanes that
 // holds the largest head of a kernel has a row.
 template <int kLanes>
 struct HeadLane {
   int in, piece, pieces;  // lanes past the row's end repeat its last piece
-  int dim, half;          // half: pairs that turn
+  int dim, half;
   float inv_dim;
-  __device__ CVS_INLINE HeadLane(int dim, int dims)
-      : in(threadIdx.x % kLanes), piece(min(in, dim / 8 - 1)), pieces(dim / 8), dim(dim), half(dims / 2),
-        inv_dim(1.f / float(dim)) {}
+  bool turned, low;  // kPieces: a piece of either half, of the first
+  int from;          // 4 times the lane that has its partners
+  __device__ CVS_INLINE HeadLane(int dim, int half)
+      : in(threadIdx.x % kLanes), piece(min(in, dim / 8 - 1)), pieces(dim / 8), dim(dim), half(half),
+        inv_dim(1.f / float(dim)), turned(piece < half / 4), low(piece < half / 8) {
+    const int to = !turned ? 0 : low ? half / 8 : -half / 8;
+    from = 4 * (int(__lane_id()) + piece - in + to);
+  }
 };
 
-// A norm's weights to LDS in fp32.
-template <bool kBf>
-__device__ CVS_INLINE void load_weight(float* s, const Norm& n, int dim) {
-  if (!n.weight) return;
-  for (int i = threadIdx.x; i < dim; i += blockDim.x)
-    s[i] = n.fp32 ? static_cast<const float*>(n.weight)[i] : to_float<kBf>(static_cast<const uint16_t*>(n.weight)[i]);
+// 1 / sqrt(x) for a row's lanes; the instruction takes subnormal numbers for 0.
+__device__ CVS_INLINE float inverse_root(float x) {
+  const bool tiny = x < 1e-35f;
+  const float r = __builtin_amdgcn_rsqf(tiny ? x * 1.2676506002282294e30f : x);  // 2^100
+  return tiny ? r * 1.125899906842624e15f : r;                                    // 2^50
 }
 
-// The lane's piece x of a head, normed and rotated.  cs, sn: the head's cosines
-// and sines, times the magnitude; w: its norm's weights, null for none; scratch:
-// a place in LDS for each lane of the wave, this one's (kChannels alone).
+// The lane's piece x of a head, normed (if kNorm and `normed`) and turned.
+// scratch: the wave's lanes' places in LDS, this one's (kChannels alone).
 template <bool kBf, int kLanes, Pairs kPairs, bool kNorm>
-__device__ CVS_INLINE u32x4 ready(u32x4 x, const HeadLane<kLanes>& l, const float* cs, const float* sn, const float* w,
+__device__ CVS_INLINE u32x4 ready(u32x4 x, const HeadLane<kLanes>& l, const float* own, const float* other, bool normed,
                                   float eps, u32x4* scratch) {
-  const int half = l.half, piece = l.piece;
-  float f[8], o[8];
+  float f[8], g[8], o[8];
   unpack8<kBf>(x, f);
   float inv = 1.f;
   if constexpr (kNorm) {
@@ -111,40 +155,21 @@ __device__ CVS_INLINE u32x4 ready(u32x4 x, const HeadLane<kLanes>& l, const floa
     if (l.in >= l.pieces) sum = 0.f;
 #pragma unroll
     for (int m = 1; m < kLanes; m <<= 1) sum += xor_lanes_f(sum, m);
-    if (w) {
-      inv = 1.f / __builtin_sqrtf(__builtin_fmaf(sum, l.inv_dim, eps));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] *= w[8 * piece + e];
-    }
+    const float root = inverse_root(__builtin_fmaf(sum, l.inv_dim, eps));
+    inv = normed ? root : 1.f;
   }
   if constexpr (kPairs == kNeighbours) {
+    // Whole pairs are in or out.
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const int p = 4 * piece + e / 2;
-      const bool turned = p < half;
-      const float c = cs[turned ? p : 0], s = sn[turned ? p : 0];
-      o[e] = turned ? f[e] * c - f[e + 1] * s : f[e];
-      o[e + 1] = turned ? f[e + 1] * c + f[e] * s : f[e + 1];
-    }
+    for (int e = 0; e < 8; ++e) g[e] = 4 * l.piece + e / 2 < l.half ? f[e ^ 1] : 0.f;
   } else if constexpr (kPairs == kPieces) {
-    // A piece of the first half, of the second, or behind both.
-    const bool turned = 8 * piece < 2 * half, low = 8 * piece < half;
-    const int to = !turned ? 0 : low ? half / 8 : -half / 8;  // where its partner is
     u32x4 px;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      px[k] = uint32_t(__builtin_amdgcn_ds_bpermute(4 * (int(__lane_id()) + to), int(x[k])));
-    float g[8];
-    unpack8<kBf>(px, g);
-    const int p = !turned ? 0 : low ? 8 * piece : 8 * piece - half;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if constexpr (kNorm) {
-        if (w) g[e] *= w[8 * (piece + to) + e];
-      }
-      const float s = low ? -sn[p + e] : sn[p + e];
-      o[e] = turned ? f[e] * cs[p + e] + g[e] * s : f[e];
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t w = uint32_t(__builtin_amdgcn_ds_bpermute(l.from, int(x[k])));
+      px[k] = l.turned ? w : 0;
     }
+    unpack8<kBf>(px, g);
   } else {
     // The row's pieces side by side.
     *scratch = x;
@@ -152,61 +177,88 @@ __device__ CVS_INLINE u32x4 ready(u32x4 x, const HeadLane<kLanes>& l, const floa
     const uint16_t* const row = reinterpret_cast<const uint16_t*>(scratch - l.in);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int c = 8 * piece + e;
-      const bool turned = c < 2 * half, low = c < half;
-      const int other = !turned ? c : low ? c + half : c - half, p = !turned ? 0 : low ? c : c - half;
-      float g = to_float<kBf>(row[other]);
-      if constexpr (kNorm) {
-        if (w) g *= w[other];
-      }
-      const float s = low ? -sn[p] : sn[p];
-      o[e] = turned ? f[e] * cs[p] + g * s : f[e];
+      const int c = 8 * l.piece + e;
+      const float v = to_float<kBf>(row[c < l.half ? c + l.half : c < 2 * l.half ? c - l.half : c]);
+      g[e] = c < 2 * l.half ? v : 0.f;
     }
     wave_lds_ready();  // read before the next row's pieces are written
   }
-  if constexpr (kNorm) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] *= inv;
+  for (int i = 0; i < 2; ++i) {
+    const f32x4 a = reinterpret_cast<const f32x4*>(own)[2 * l.piece + i];
+    const f32x4 b = reinterpret_cast<const f32x4*>(other)[2 * l.piece + i];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int e = 4 * i + k;
+      o[e] = __builtin_fmaf(f[e], a[k], g[e] * b[k]);
+      if constexpr (kNorm) o[e] *= inv;
+    }
   }
   return pack8<kBf>(o);
 }
 
-// A head on its way.
-struct HeadRow {
-  const char* in;
-  char* out;
-  const float *cs, *sn, *w;
-  float eps;
-};
+// A row's result here and not where it is stored: left to the compiler, the
+// factors of all rows under way are read first and kept, in registers that
+// leave a SIMD two or three waves.
+__device__ CVS_INLINE void row_done(u32x4& y) {
+  asm volatile("" : "+v"(y));
+  __builtin_amdgcn_sched_barrier(0);
+}
 
-// Rows [0, rows) by a workgroup, kAhead of each group of lanes under way at
-// once; place(r) is row r, before() is run behind the first loads.  A row's
+// Rows of an array by a workgroup: offsets in bytes from its first token and
+// head, within 31 bits.
+struct RowView {
+  char* p;
+  uint32_t token, head;
+};
+// Whether `heads` heads of up to 32 tokens lie within 31 bits of bytes.
+inline bool rows_near(const View& v, int64_t heads) {
+  return 2 * (31 * v.token + kMaxDim) + 2 * __int128(heads - 1) * v.head < (int64_t(1) << 31);
+}
+
+// Rows [0, rows) of tokens x heads by a workgroup, kAhead of each group of
+// lanes under way at once.  before() is run behind the first loads.  A row's
 // input may be its own output and no other row's.
 constexpr int kAhead = 4;
-template <bool kBf, int kLanes, Pairs kPairs, bool kNorm, typename Place, typename Before>
-__device__ CVS_INLINE void ready_rows(const HeadLane<kLanes>& l, int rows, u32x4* scratch, const Place& place,
-                                      const Before& before) {
+struct Rows {
+  int rows, heads;
+  uint32_t magic;  // magic_of(heads)
+  RowView in, out;
+  const float *own, *other;  // of the first token
+  bool normed;
+  float eps;
+};
+// r / heads is 2 r magic / 2^32 for r below 2^16.
+inline uint32_t magic_of(int heads) { return ((uint32_t(1) << 31) + uint32_t(heads) - 1) / uint32_t(heads); }
+template <bool kBf, int kLanes, Pairs kPairs, bool kNorm, typename Before>
+__device__ CVS_INLINE void ready_rows(const HeadLane<kLanes>& l, const Rows& a, u32x4* scratch, const Before& before) {
   const int groups = blockDim.x / kLanes, group = threadIdx.x / kLanes;
+  auto token_of = [&](int r) CVS_INLINE { return __umulhi(2u * uint32_t(r), a.magic); };
+  auto place = [&](const RowView& v, int r) CVS_INLINE {
+    const uint32_t t = token_of(r), h = uint32_t(r) - t * uint32_t(a.heads);
+    return v.p + (t * v.token + h * v.head + 16u * uint32_t(l.piece));
+  };
   u32x4 x[kAhead];
   auto load = [&](int first) CVS_INLINE {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)  // past the last row, that one again (not stored)
-      x[i] = *reinterpret_cast<const u32x4*>(place(min(first + i * groups, rows - 1)).in + 16 * l.piece);
+      x[i] = *reinterpret_cast<const u32x4*>(place(a.in, min(first + i * groups, a.rows - 1)));
   };
   load(group);
   before();
-  for (int first = group; first - group < rows; first += kAhead * groups) {
+  for (int first = group; first - group < a.rows; first += kAhead * groups) {
     u32x4 y[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const HeadRow r = place(min(first + i * groups, rows - 1));
-      y[i] = ready<kBf, kLanes, kPairs, kNorm>(x[i], l, r.cs, r.sn, r.w, r.eps, scratch);
+      const int at = int(token_of(min(first + i * groups, a.rows - 1))) * l.dim;
+      y[i] = ready<kBf, kLanes, kPairs, kNorm>(x[i], l, a.own + at, a.other + at, a.normed, a.eps, scratch);
+      row_done(y[i]);
     }
-    load(first + kAhead * groups);
+    if (first - group + kAhead * groups < a.rows) load(first + kAhead * groups);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int r = first + i * groups;
-      if (r < rows && l.in < l.pieces) *reinterpret_cast<u32x4*>(place(r).out + 16 * l.piece) = y[i];
+      if (r < a.rows && l.in < l.pieces) *reinterpret_cast<u32x4*>(place(a.out, r)) = y[i];
     }
   }
 }
