@@ -371,27 +371,35 @@ def _heads(ctx: "Context", x, what: str, layered: bool = False):
     contiguous; with layered, of (layers, tokens, heads, head_dim) as well.
     Returns (view, layers, layer stride)."""
     shape = x.shape
-    nd = len(shape)
-    if nd != 3 and not (layered and nd == 4):
+    if len(shape) == 3:
+        tokens, heads, dim = shape
+        layers, layer = 1, 0
+    elif layered and len(shape) == 4:
+        layers, tokens, heads, dim = shape
+        layer = None
+    else:
         raise ValueError(f"{what} must be (tokens, heads, head_dim)" + (" or (layers, ...)" if layered else ""))
     if isinstance(x, DeviceArray):
         if x.ctx.device != ctx.device:
             raise ValueError(f"{what} must be on the context's device")
-        ptr, stride = x.ptr.value, (shape[-2] * shape[-1], shape[-1])
-        layer = shape[-3] * stride[0] if nd == 4 else 0
+        ptr, by_token, by_head = x.ptr.value, heads * dim, dim
+        if layer is None:
+            layer = tokens * by_token
     elif hasattr(x, "data_ptr"):
-        if not x.is_cuda or x.get_device() != ctx.device:
+        if x.get_device() != ctx.device:  # -1 for a tensor that is on no GPU
             raise ValueError(f"{what} must be on the context's device")
         if x.requires_grad:
             _no_gradient(what)
-        st = x.stride()
-        if st[-1] != 1 and shape[-1] > 1:
+        *first, by_token, by_head, step = x.stride()
+        if step != 1 and dim > 1:
             raise ValueError(f"{what}: the last axis must be contiguous")
-        ptr, stride, layer = x.data_ptr(), st[-3:-1], st[0] if nd == 4 else 0
+        ptr = x.data_ptr()
+        if layer is None:
+            layer = first[0]
     else:
         raise ValueError(f"{what} must be a DeviceArray or a torch tensor")
-    view = Heads(ptr, shape[-3], stride[0], stride[1], shape[-2], shape[-1], _head_type(x.dtype))
-    return view, (shape[0] if nd == 4 else 1), layer
+    kind = _HEAD_TYPES.get(x.dtype)
+    return Heads(ptr, tokens, by_token, by_head, heads, dim, _head_type(x.dtype) if kind is None else kind), layers, layer
 
 
 def _lse(ctx: "Context", lse, heads: int, tokens: int):
@@ -416,25 +424,26 @@ _KINDS = {}  # dtypes' names: making a torch dtype's takes longer than all else 
 
 def _vector(ctx: "Context", x, what: str, length: int, dtypes):
     """Device address of an array of `length` elements of one of `dtypes`,
-    contiguous, and its type's place among them."""
+    contiguous, and which of them."""
     kind = _KINDS.get(x.dtype)
     if kind is None:
         kind = _KINDS[x.dtype] = str(x.dtype).replace("torch.", "")
-    if len(x.shape) != 1 or x.shape[0] != length or kind not in dtypes:
+    shape = x.shape
+    if len(shape) != 1 or shape[0] != length or kind not in dtypes:
         raise ValueError(f"{what} must be {length} elements of {' or '.join(dtypes)}, in one dimension")
     if isinstance(x, DeviceArray):
         if x.ctx.device != ctx.device:
             raise ValueError(f"{what} must be on the context's device")
-        return x.ptr.value, dtypes.index(kind)
+        return x.ptr.value, kind
     if not hasattr(x, "data_ptr"):
         raise ValueError(f"{what} must be a DeviceArray or a torch tensor")
-    if not x.is_cuda or x.get_device() != ctx.device:
+    if x.get_device() != ctx.device:
         raise ValueError(f"{what} must be on the context's device")
     if length > 1 and x.stride(0) != 1:
         raise ValueError(f"{what} must be contiguous")
     if x.requires_grad:
         _no_gradient(what)
-    return x.data_ptr(), dtypes.index(kind)
+    return x.data_ptr(), kind
 
 
 # A norm's weight: fp32 or the type of the heads.
@@ -446,7 +455,7 @@ def _norm(ctx: "Context", weight, heads, eps: float, what: str):
     if weight is None:
         return None
     ptr, kind = _vector(ctx, weight, what, heads.head_dim, _WEIGHT_TYPES[heads.type])
-    return HeadNorm(ptr, heads.type if kind else FP32, eps)
+    return HeadNorm(ptr, FP32 if kind == "float32" else heads.type, eps)
 
 
 def _scores(ctx: "Context", cap: float, slopes, heads: int):

@@ -56,7 +56,7 @@ def test_null_arguments_are_refused(cvs):
 def test_arrays_the_binding_refuses(cvs):
     ctx = types.SimpleNamespace(device=0)
     at = lambda device, shape, dtype: array_on(cvs, device, shape, dtype)
-    assert cvs._vector(ctx, at(0, (5,), np.int64), "positions", 5, ("int64",)) == (4096, 0)
+    assert cvs._vector(ctx, at(0, (5,), np.int64), "positions", 5, ("int64",)) == (4096, "int64")
     for x in (at(0, (4,), np.int64), at(0, (5, 1), np.int64), at(0, (5,), np.int32), at(0, (5,), np.float64)):
         with pytest.raises(ValueError, match="positions must be 5 elements of int64"):
             cvs._vector(ctx, x, "positions", 5, ("int64",))
