@@ -302,7 +302,7 @@ struct PageSource {
   __device__ CVS_INLINE void load(const char* from, int to) {
     const rsrc4 rs = make_rsrc(from + at_wave, kHalf / 2);
 #pragma unroll
-    for (int i = 0; i < NB; ++i) lds_dma<16, false>(rs, to + i * 1024, i * 1024 + w.lane * 16, 0);
+    for (int i = 0; i < NB; ++i) dma16(rs, to + i * 1024, i * 1024 + w.lane * 16);
   }
   __device__ CVS_INLINE void load_keys(int n, int t) {
     // The last tile again where the segment has an odd number; its keys are past the end.

@@ -28,7 +28,6 @@ namespace attn {
 
 using bf::f32x16;
 using bf::lds_addr;
-using bf::lds_dma;
 using bf::make_rsrc;
 using bf::rsrc4;
 using bf::u32x4;
@@ -36,6 +35,17 @@ using bf::u32x4;
 constexpr int kMaxDim = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+
+// 16 bytes a lane from a buffer straight to LDS address to + 16 lane, as
+// bf::lds_dma, but five wait states before it: a descriptor that the compiler
+// has spilled comes back through vector instructions just before the load,
+// which it does not look into, and a scalar register that a vector instruction
+// has written is there for a load after five.  (With one, a kernel of capped and
+// biased scores read through descriptors of before, and gave other results from
+// run to run.)
+__device__ CVS_INLINE void dma16(rsrc4 rs, int to, uint32_t off) {
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rs), "{m0}"(to) : "memory");
+}
 
 // One 16-byte MFMA operand: 8 elements of fp16 or bf16.
 template <bool kBf>
@@ -125,74 +135,86 @@ __device__ CVS_INLINE float largest(const f32x16& s, float c) {
   return both_max(top) * c;
 }
 
-// What becomes of a product s = q.k on its way to a score.  Plain: the score
-// is c s in log2 units, c = scale log2(e).  Otherwise `finish` makes the scores
-// of a lane's 16 keys of it, already in log2 units, and c is 1 from there on:
+// What becomes of a product s = q.k on its way to a score, in log2 units.
+// Plain: c s, c = scale log2(e).  Otherwise (scored_probabilities):
 //
 //   cap: log2(e) C tanh(scale s / C).  With u = scale s / C, y = s^2: up to |u| =
-//   0.75 that is c s P(y), P of degree 4 fitted to tanh(u) / u (least squares
-//   weighted to an even relative error: 6e-7), its coefficients with c and the
-//   powers of scale / C in them; above, C (1 - 2 / (1 + e^2u)), whose error is
-//   that of its last places, 2^-22 C.  A tile with no large |u|, all of them in
-//   models whose scores stay within half of the cap, takes six instructions a
-//   score and no exponential;
+//   1/2 that is s P(y), P of degree 3 fitted to c tanh(u) / u (least squares
+//   weighted to an even relative error: 6e-7), with the powers of scale / C in
+//   its coefficients; above, C (1 - 2 / (1 + e^2u)), off by its last places, 2^-22
+//   C, which is as much beside the score.  A tile with no |u| above 1/2, all of
+//   them in models whose scores stay within half of the cap, takes five
+//   instructions a score more than a plain one and no exponential;
 //
 //   bias: minus log2(e) slope |place - key|, by the row's place and slope.
 struct ScoreArgs {
-  float c;             // of plain scores and of caps' small ones
-  float cap;           // log2(e) C
-  float twice;         // log2(e) 2 scale / C
-  float largest_y;     // of small scores; -1: none is small
-  float a[4];          // P's coefficients behind c
+  float c;
+  float cap;            // log2(e) C
+  float twice;          // log2(e) 2 scale / C
+  float largest_y;      // of P's range; -1: P is not used
+  float a[3];           // P's coefficients behind c
   const float* slopes;  // of the heads, natural units; null: none
 };
 struct PlainScores {
   static constexpr bool kPlain = true, kDown = false;
   float c;
 };
-template <bool kCap, bool kBias>
+template <bool kCap_, bool kBias_>
 struct Scores {
-  static constexpr bool kPlain = false;
+  static constexpr bool kPlain = false, kCap = kCap_, kBias = kBias_;
   // Scores fall with the distance: the nearest keys first, or every tile would have a larger maximum than the one before.
   static constexpr bool kDown = kBias;
-  static constexpr float c = 1.f;
+  static constexpr float c = 1.f;  // of finished scores
   const ScoreArgs& a;
   float slope;  // log2(e) times the row's
   int place;    // the row's, counted like the keys
 
-  // Keys key + 8 (r / 4) + r % 4.
-  __device__ CVS_INLINE void finish(f32x16& s, int key) const {
+  // P(s^2), or c.
+  __device__ CVS_INLINE float factor(float y) const {
+    if constexpr (!kCap) return a.c;
+    else return __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, a.a[2], a.a[1]), a.a[0]), a.c);
+  }
+  // Score r of a lane's 16 less `base`, up to the cap's small scores; far: the place less that of r = 0.
+  __device__ CVS_INLINE float less(float s, float base, float far, int r) const {
+    const float x = __builtin_fmaf(s, factor(s * s), -base);
+    return biased(x, far, r);
+  }
+  // The same, of any score.  one: 1, which the compiler does not know: it would keep what this has in common with
+  // `less`, 16 registers of it, for a pass that hardly ever comes.
+  __device__ CVS_INLINE float any_less(float s, float base, float far, int r, float one) const {
+    const float t = s * one, y = s * t;
+    float x = __builtin_fmaf(t, factor(y), -base);
     if constexpr (kCap) {
-      f32x16 x;
-      float top = 0.f;
+      x = y <= a.largest_y ? x : large(t) - base;
+    }
+    return biased(x, far * one, r);
+  }
+  // Products of keys key + 8 (r / 4) + r % 4 to scores, in place: for `probabilities` with a c of 1.
+  __device__ CVS_INLINE void finish(f32x16& s, int key) const {
+    const float far = kBias ? float(place - key) : 0.f;
+    f32x16 x;
+    float top = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float y = s[r] * s[r];
-        top = fmaxf(top, y);
-        float p = __builtin_fmaf(y, a.a[3], a.a[2]);
-        p = __builtin_fmaf(y, p, a.a[1]);
-        p = __builtin_fmaf(y, p, a.a[0]);
-        x[r] = s[r] * __builtin_fmaf(y, p, a.c);
-      }
+    for (int r = 0; r < 16; ++r) {
+      if constexpr (kCap) top = fmaxf(top, s[r] * s[r]);
+      x[r] = s[r] * factor(s[r] * s[r]);
+    }
+    if constexpr (kCap) {
       if (__ballot(!(top <= a.largest_y))) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float e = 1.f + __builtin_amdgcn_exp2f(s[r] * a.twice);
-          const float large = __builtin_fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(e), a.cap);
-          x[r] = s[r] * s[r] <= a.largest_y ? x[r] : large;
-        }
+        for (int r = 0; r < 16; ++r) x[r] = s[r] * s[r] <= a.largest_y ? x[r] : large(s[r]);
       }
-      s = x;
-    } else {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] *= a.c;
     }
-    if constexpr (kBias) {
-      const float far = float(place - key);
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        s[r] = __builtin_fmaf(-slope, __builtin_fabsf(far - float(8 * (r / 4) + r % 4)), s[r]);
-    }
+    for (int r = 0; r < 16; ++r) s[r] = biased(x[r], far, r);
+  }
+  __device__ CVS_INLINE float large(float s) const {
+    const float e = 1.f + __builtin_amdgcn_exp2f(s * a.twice);
+    return __builtin_fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(e), a.cap);
+  }
+  __device__ CVS_INLINE float biased(float x, float far, int r) const {
+    if constexpr (kBias) return __builtin_fmaf(-slope, __builtin_fabsf(far - float(8 * (r / 4) + r % 4)), x);
+    else return x;
   }
 };
 // A call's scores, checked; cap 0 for none.
@@ -276,6 +298,68 @@ __device__ CVS_INLINE void probabilities(f32x16& s, RowState<NB>& st, float c) {
   s = p;
 }
 
+// `probabilities` of products s of capped or biased scores of keys key + 8 (r /
+// 4) + r % 4.  Where all are P's, and nothing has to rise, one pass does, in one
+// block with the matrix products before it; else the scores are taken once more,
+// larger ones by their exponential.  Which of the two is used changes no bit of
+// a row whose own scores are small.
+template <bool kBf, int NB, typename Scoring>
+__device__ CVS_INLINE void scored_probabilities(f32x16& s, RowState<NB>& st, const Scoring& sc, int key) {
+  const float far = Scoring::kBias ? float(sc.place - key) : 0.f;
+  f32x16 p;
+  float sum;
+  {
+    const float base = st.m == -INFINITY ? 0.f : st.m;
+    float part[2] = {0.f, 0.f}, top = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      if constexpr (Scoring::kCap) top = fmaxf(top, s[r] * s[r]);
+      p[r] = __builtin_amdgcn_exp2f(sc.less(s[r], base, far, r));
+      part[r & 1] += p[r];
+    }
+    sum = part[0] + part[1];
+    const bool over = !(sum <= kMost<kBf>) | (st.m == -INFINITY), large = Scoring::kCap & !(top <= sc.a.largest_y);
+    if (__ballot(over | large) == 0) {
+      st.l += sum;
+      s = p;
+      return;
+    }
+  }
+  float most;
+  auto pass = [&]() CVS_INLINE {
+    const float base = st.m == -INFINITY ? 0.f : st.m;
+    float one = 1.f, part[2] = {0.f, 0.f};
+    asm volatile("" : "+s"(one));
+    most = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float x = sc.any_less(s[r], base, far, r, one);
+      most = fmaxf(most, x);
+      p[r] = __builtin_amdgcn_exp2f(x);
+      part[r & 1] += p[r];
+    }
+    sum = part[0] + part[1];
+    return base;
+  };
+  const float base = pass();
+  const bool over = !(sum <= kMost<kBf>) || st.m == -INFINITY;
+  if (__ballot(over)) {
+    const float rise = both_max(most) + base - kLift<kBf>;
+    const uint32_t either = uint32_t(over) | xor_lanes(uint32_t(over), 32);
+    const bool raise = either != 0 && rise > st.m;
+    const float alpha = raise ? __builtin_amdgcn_exp2f(st.m - rise) : 1.f;
+    st.l *= alpha;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st.o[b][r] *= alpha;
+    st.m = raise ? rise : st.m;
+    pass();  // from the scores again: less the m of before they have its last place
+  }
+  st.l += sum;
+  s = p;
+}
+
 // B operand of the 16 keys `step` (0 or 1) of a probability tile.  The
 // probabilities are rounded to the values' type here, the product's operand
 // type: each is off by at most half a unit of its own last place (in fp16, of
@@ -333,40 +417,41 @@ __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[KS], 
       u32x4 v[2 * NB];
 #pragma unroll
       for (int i = 0; i < 2 * NB; ++i) v[i] = src.hide(src.values(n, h, i / 2, i % 2), t, h, i % 2);
-      if (mixed && (!Scoring::kDown || t >= open_tiles)) bad |= clean<kBf>(v);
+      if (mixed && (Scoring::kPlain || t >= open_tiles)) bad |= clean<kBf>(v);
 #pragma unroll
       for (int i = 0; i < 2 * NB; ++i) st.o[i / 2] = mfma<kBf>(v[i], p[h][i % 2], st.o[i / 2]);
     }
   };
-  auto finish = [&](int n, int h) CVS_INLINE {
-    if constexpr (!Scoring::kPlain) scoring.finish(s[h], 64 * order(n) + 32 * h + 4 * half);
-  };
   auto mask = [&](int n, int h) CVS_INLINE {
+    if constexpr (!Scoring::kPlain) scoring.finish(s[h], 64 * order(n) + 32 * h + 4 * half);
     const int seen = limit - 64 * order(n) - 32 * h - 4 * half;
 #pragma unroll
     for (int r = 0; r < 16; ++r)
       if (8 * (r / 4) + r % 4 >= seen) s[h][r] = -INFINITY;
   };
-  auto soften = [&](int h) CVS_INLINE {
-    probabilities<kBf>(s[h], st, scoring.c);
+  auto soften = [&](int n, int h, auto masked) CVS_INLINE {
+    if constexpr (Scoring::kPlain || masked) probabilities<kBf>(s[h], st, scoring.c);
+    else scored_probabilities<kBf>(s[h], st, scoring, 64 * order(n) + 32 * h + 4 * half);
 #pragma unroll
     for (int k = 0; k < 2; ++k) p[h][k] = prob_operand<kBf>(s[h], k);
   };
-  auto step = [&](int n, auto masked) CVS_INLINE {
-    if (n > 0) add_values(n - 1, 1, masked);
-    finish(n, 0);
+  auto step = [&](int n, auto masked, auto first) CVS_INLINE {
+    if constexpr (!Scoring::kPlain) {
+      if constexpr (!first) add_values(n - 1, 1, masked);
+    } else if (n > 0) {
+      add_values(n - 1, 1, masked);
+    }
     if constexpr (masked) mask(n, 0);
     s[1] = scores(n, 1);
-    soften(0);
+    soften(n, 0, masked);
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     __syncthreads();
     if (n + 2 < tiles) src.load_keys(n + 2, order(n + 2));
     if (n + 1 < tiles) src.load_values(n + 1, order(n + 1));
     add_values(n, 0, masked);
-    finish(n, 1);
     if constexpr (masked) mask(n, 1);
     s[0] = scores(n + 1, 0);  // past the last tile: of whatever is there, and not used
-    soften(1);
+    soften(n, 1, masked);
   };
   if (tiles <= 0) return;
   src.load_keys(0, order(0));
@@ -375,26 +460,26 @@ __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[KS], 
   __builtin_amdgcn_s_waitcnt(0x0F70);
   __syncthreads();
   s[0] = scores(0, 0);
-  if constexpr (Scoring::kPlain) {
+  if constexpr (Scoring::kPlain) {  // others find the first tile's maximum as any later one's
     mask(0, 0);
     st.m = largest(s[0], scoring.c) - kLift<kBf>;
-  } else {
-    const f32x16 products = s[0];
-    finish(0, 0);
-    mask(0, 0);
-    st.m = largest(s[0], scoring.c) - kLift<kBf>;
-    s[0] = products;
   }
   int n = 0;
+  auto steps = [&](int end, auto masked) CVS_INLINE {
+    for (; n < end; ++n) step(n, masked, std::false_type{});
+  };
+  // The first step has no values to add.  The compiler takes it out of loops of plain scores, and not out of others, where
+  // a branch would split the blocks that overlap products and exponentials; it is there a masked one, of any tile.
+  if constexpr (!Scoring::kPlain) step(n++, std::true_type{}, std::true_type{});
   if constexpr (!Scoring::kDown) {
-    for (; n < open_tiles; ++n) step(n, std::false_type{});
-    for (; n < tiles; ++n) step(n, std::true_type{});
+    steps(open_tiles, std::false_type{});
+    steps(tiles, std::true_type{});
   } else {
     // Masked tiles come first, down to the open ones, and last; a step behind a masked one still adds its values.
     const int first = order.top > open_tiles ? order.top - open_tiles + 1 : 0, last = max(order.top, open_tiles);
     for (int masked = min(first, tiles), open = min(last, tiles);; masked = open = tiles) {
-      for (; n < masked; ++n) step(n, std::true_type{});
-      for (; n < open; ++n) step(n, std::false_type{});
+      steps(masked, std::true_type{});
+      steps(open, std::false_type{});
       if (n >= tiles) break;
     }
   }

@@ -62,10 +62,10 @@ ScoreArgs score_args(const cvs_scores* scores, float scale, int dim) {
     a.largest_y = -1.f;
     return a;
   }
-  a.largest_y = float(std::min(0.5625 / y, 1e37));
-  const double fit[4] = {-3.332984262e-01, 1.327011141e-01, -5.033518577e-02, 1.315864465e-02};
+  a.largest_y = float(std::min(0.25 / y, 1e37));
+  const double fit[3] = {-3.332826464e-01, 1.320671470e-01, -4.478946771e-02};
   double power = double(a.c);
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 3; ++i) {
     power *= y;
     a.a[i] = float(fit[i] * power);
   }

@@ -124,11 +124,11 @@ struct PromptSource {
     to += (n & 1) * kBuf;
     if (left >= kKeys) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) lds_dma<16, false>(rs, to + i * 1024, off[i], 0);
+      for (int i = 0; i < kLoads; ++i) dma16(rs, to + i * 1024, off[i]);
     } else {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
-        lds_dma<16, false>(rs, to + i * 1024, (first + i * 64) / P < left ? off[i] : kNowhere, 0);
+        dma16(rs, to + i * 1024, (first + i * 64) / P < left ? off[i] : kNowhere);
     }
   }
   __device__ CVS_INLINE void load_keys(int n, int t) { load(base_k, step_k, to_k, off_k, n, t); }
@@ -150,7 +150,7 @@ struct PromptSource {
 };
 
 template <bool kBf, int NB, int KS, typename Scoring>
-__global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 3 ? 3 : 4) void prompt_attn_kernel(const PromptArgs a) {
+__global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 3 ? (Scoring::kPlain ? 3 : 2) : (Scoring::kPlain ? 4 : 3)) void prompt_attn_kernel(const PromptArgs a) {
   typedef PromptSource<NB> Source;
   __shared__ __align__(16) char s_k[2 * Source::kBuf];
   __shared__ __align__(16) char s_v[2 * Source::kBuf];
