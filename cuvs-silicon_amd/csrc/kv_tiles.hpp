@@ -47,26 +47,25 @@ struct TileValues {
     for (int j = 0; j < 8; ++j)
       x[j] = *reinterpret_cast<const u32x4*>(vs + 2 * (held(token(j)) * stride + 8 * min(c, pieces - 1)));
   }
-  // To the pool.  Tokens before the call's keep what they hold, also where they share 16 bytes with new ones.
+  // To the pool.  Tokens before the call's keep what they hold: where they share 16 bytes with new ones, those are written
+  // one by one, as there are few of them and reading the old ones first would be one more wait.
   __device__ CVS_INLINE void store(int pieces) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (c >= pieces) x[j] = u32x4{};
     transpose8(x);
-    if (mine && t0 < lo) {
-      uint32_t keep[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) keep[k] = (token(2 * k) < lo ? 0xffffu : 0u) | (token(2 * k + 1) < lo ? 0xffff0000u : 0u);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const u32x4 old = slots[j];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[j][k] = (x[j][k] & ~keep[k]) | (old[k] & keep[k]);
-      }
-    }
-    if (mine) {
+    if (!mine) return;
+    if (t0 >= lo) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) slots[j] = x[j];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (token(k) < lo || token(k) >= hi) continue;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          reinterpret_cast<uint16_t*>(slots + j)[k] = uint16_t(x[j][k / 2] >> (16 * (k % 2)));
+      }
     }
   }
 };
