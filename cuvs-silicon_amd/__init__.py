@@ -372,8 +372,8 @@ def _heads(ctx: "Context", x, what: str, layered: bool = False):
     Returns (view, layers, layer stride)."""
     shape = x.shape
     if len(shape) == 3:
-        tokens, heads, dim = shape
         layers, layer = 1, 0
+        tokens, heads, dim = shape
     elif layered and len(shape) == 4:
         layers, tokens, heads, dim = shape
         layer = None
@@ -390,16 +390,18 @@ def _heads(ctx: "Context", x, what: str, layered: bool = False):
             raise ValueError(f"{what} must be on the context's device")
         if x.requires_grad:
             _no_gradient(what)
-        *first, by_token, by_head, step = x.stride()
+        if layer is None:
+            layer, by_token, by_head, step = x.stride()
+        else:
+            by_token, by_head, step = x.stride()
         if step != 1 and dim > 1:
             raise ValueError(f"{what}: the last axis must be contiguous")
         ptr = x.data_ptr()
-        if layer is None:
-            layer = first[0]
     else:
         raise ValueError(f"{what} must be a DeviceArray or a torch tensor")
-    kind = _HEAD_TYPES.get(x.dtype)
-    return Heads(ptr, tokens, by_token, by_head, heads, dim, _head_type(x.dtype) if kind is None else kind), layers, layer
+    dtype = x.dtype
+    kind = _HEAD_TYPES[dtype] if dtype in _HEAD_TYPES else _head_type(dtype)
+    return Heads(ptr, tokens, by_token, by_head, heads, dim, kind), layers, layer
 
 
 def _lse(ctx: "Context", lse, heads: int, tokens: int):
@@ -459,9 +461,9 @@ def _norm(ctx: "Context", weight, heads, eps: float, what: str):
 
 
 def _scores(ctx: "Context", cap: float, slopes, heads: int):
-    """The cvs_scores of a call, None where scores stay as they are."""
+    """The cvs_scores of a call."""
     if slopes is None:
-        return ScoreOptions(cap, None) if cap else None
+        return ScoreOptions(cap, None)
     return ScoreOptions(cap, _vector(ctx, slopes, "slopes", heads, ("float32",))[0])
 
 
@@ -639,7 +641,7 @@ class Context:
         it is not 0, and lose slopes[head] (float32) times their distance."""
         hq, hk, hv, ho = (_heads(self, x, w)[0] for x, w in ((q, "q"), (k, "k"), (v, "v"), (out, "out")))
         hl = _lse(self, lse, hq.heads, hq.tokens)
-        sc = _scores(self, cap, slopes, hq.heads)
+        sc = _scores(self, cap, slopes, hq.heads) if cap or slopes is not None else None
         after = self._behind_torch(q, k, v, out, lse, slopes)
         _check(load().cvs_prompt_attention_scored_async(self.handle, plan.handle, hq, hk, hv, ho, hl, scale, sc))
         if after:
@@ -1215,7 +1217,7 @@ class KvCache:
         slopes as in prompt_attention_async."""
         hq, ho = _heads(self.ctx, q, "q")[0], _heads(self.ctx, out, "out")[0]
         hl = _lse(self.ctx, lse, hq.heads, hq.tokens)
-        sc = _scores(self.ctx, cap, slopes, hq.heads)
+        sc = _scores(self.ctx, cap, slopes, hq.heads) if cap or slopes is not None else None
         after = self.ctx._behind_torch(q, out, lse, slopes)
         _check(load().cvs_kv_attention_scored_async(self.handle, plan.handle, layer, hq, ho, hl, scale, sc))
         if after:

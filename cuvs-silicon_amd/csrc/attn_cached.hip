@@ -357,7 +357,7 @@ extern "C" int cvs_kv_attention_scored_async(cvs_kv_cache* cache, cvs_kv_plan* p
                        reinterpret_cast<const int32_t*>(blob + plan->at_pages),
                        reinterpret_cast<const int32_t*>(blob + plan->at_limits),
                        reinterpret_cast<const int32_t*>(blob + plan->at_rows), view_of(q), view_of(out), lse,
-                       plan->tokens, cache->kv_heads, group, cache->dim, sc, part_o, part_ml, plan->slots};
+                       plan->tokens, cache->kv_heads, group, cache->dim, part_o, part_ml, plan->slots, sc};
     const int64_t blocks = int64_t(plan->workgroups) * cache->kv_heads;
     const bool is_bf = cache->type == CVS_BF16;
     if (sc.cap > 0.f || sc.slopes) launch_cached_scored(ctx, a, cache->nb, blocks, cache->type);

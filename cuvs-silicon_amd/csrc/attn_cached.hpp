@@ -53,10 +53,10 @@ struct CachedArgs {
   float* lse;
   int64_t q_tokens;
   int kv_heads, group, dim;
-  ScoreArgs scores;
   float* part_o;  // kv head, slot, 32 NB values
   float2* part_ml;
   int64_t slots;  // 0: write the output
+  ScoreArgs scores;
 };
 
 // Words of the plan: written before the kernel starts and never by it, which
