@@ -157,6 +157,7 @@ extern "C" int cvs_kv_append_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int l
     check_move(plan, layer, 1, k, v, true);
     if (rotary) check_rotary(rotary, ctx, cache->dim);
     if (positions && !rotary) fail(CVS_ERR_INVALID_ARGUMENT, "positions without a rotary");
+    check_positions(positions);
     AppendArgs a{};
     a.k_norm = norm_of(k_norm, cache->type, "k");
     if (q) {

@@ -111,6 +111,7 @@ void rotate(cvs_context* ctx, const cvs_rotary* rotary, const int64_t* positions
   if (rotary) check_rotary(rotary, ctx, first->head_dim);
   if (first->tokens == 0) return;
   if (rotary && !positions) fail(CVS_ERR_INVALID_ARGUMENT, "null positions");
+  if (rotary) check_positions(positions);
   a.positions = positions;
   a.tokens = first->tokens;
   a.turning.dim = first->head_dim;
@@ -165,6 +166,11 @@ void check_rotary(const cvs_rotary* rotary, const cvs_context* ctx, int dim) {
   if (rotary->dims > dim)
     fail(CVS_ERR_INVALID_ARGUMENT, "the rotary turns " + std::to_string(rotary->dims) + " channels, heads have " +
                                        std::to_string(dim));
+}
+
+void check_positions(const int64_t* positions) {
+  if (reinterpret_cast<uintptr_t>(positions) % 8 != 0)
+    fail(CVS_ERR_UNSUPPORTED, "positions must be aligned to 8 bytes");
 }
 
 void captured_rotary(const cvs_rotary* rotary) {

@@ -267,6 +267,8 @@ __device__ CVS_INLINE void ready_rows(const HeadLane<kLanes>& l, const Rows& a, 
 Norm norm_of(const cvs_head_norm* norm, int type, const char* what);
 // Checks that a rotary belongs to the context and fits heads of `dim`.
 void check_rotary(const cvs_rotary* rotary, const cvs_context* ctx, int dim);
+// Checks positions in device memory.
+void check_positions(const int64_t* positions);
 // Before a call with the rotary is launched: keeps its memory for the replays of a capture.
 void captured_rotary(const cvs_rotary* rotary);
 

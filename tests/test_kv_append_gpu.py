@@ -278,3 +278,24 @@ def test_graphs(cvs):
         del others, more, plan
         cache.close()
         ctx.close()
+
+
+def test_past_4_gib(tctx, cvs):
+    """A page whose place in the pool and whose tokens' positions are far."""
+    cache = tctx.kv_cache(1, 300, 4096, 8, 128, "bf16")
+    (s,) = cache.sequences(1)
+    n = 299 * 4096 + 7
+    cache.extend([s], [n])
+    cache.extend([s], [40])
+    q, k, v = (rand(i, 40, h, 128, dtype="bf16") for i, h in enumerate((16, 8, 8)))
+    plan, w = cache.plan([s], [40]), rand(5, 128, dtype="bf16")
+    out, ko, vo = torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    cache.append_async(plan, k, v, rotary=tctx.rotary(128, 500000.0), k_weight=w, q=q, q_out=out)
+    cache.read_async(plan, ko, vo)
+    f, at = cvs.rotary_frequencies(128, 500000.0), list(range(n, n + 40))
+    for x, got, weight in ((q, out, None), (k, ko, w)):
+        want, tol = ready(f64(x), "bf16", at, f, weight=None if weight is None else f64(weight), eps=1e-6)
+        assert_within(f64(got), want, tol, "past 4 GiB")
+    assert torch.equal(bits(vo), bits(v))
+    del plan
+    cache.close()

@@ -224,6 +224,8 @@ def test_refusals(tctx, cvs):
     view = cvs._heads(tctx, x, "x")[0]
     assert lib.cvs_rotate_async(tctx.handle, rotary.handle, None, view, view) == cvs.CVS_ERR_INVALID_ARGUMENT
     assert lib.cvs_rotate_async(tctx.handle, rotary.handle, at.data_ptr(), view, None) == cvs.CVS_ERR_INVALID_ARGUMENT
+    hout = cvs._heads(tctx, out, "out")[0]
+    assert lib.cvs_rotate_async(tctx.handle, rotary.handle, at.data_ptr() + 4, view, hout) == cvs.CVS_ERR_UNSUPPORTED
     h = ctypes.c_void_p()
     f = (ctypes.c_double * 32)()
     assert lib.cvs_rotary_create(tctx.handle, 64, 5, f, 1.0, ctypes.byref(h)) == cvs.CVS_ERR_INVALID_ARGUMENT
@@ -294,3 +296,32 @@ def test_graphs(cvs):
             torch.randn(1000, 1000, device="cuda").sum().item()
         del others
         c.close()
+
+
+def test_far_apart_rows(tctx, cvs):
+    """Rows that span more than 4 GiB, token by token and head by head."""
+    room = torch.empty(5 << 29, dtype=torch.float16, device="cuda")  # 5 GiB
+    for tokens, heads, strides in ((300, 3, (1 << 23, 64)), (5, 70, (64, 36 << 20))):
+        x = room.as_strided((tokens, heads, 64), (*strides, 1))
+        x.copy_(rand(1, tokens, heads, 64, dtype="fp16"))
+        at = torch.arange(9, 9 + tokens, device="cuda")
+        for interleaved in (False, True):
+            apart = check(tctx, cvs, x, at, "fp16", 64, interleaved)
+            check(tctx, cvs, apart, at, "fp16", 64, interleaved, out=x)
+            x.copy_(rand(1, tokens, heads, 64, dtype="fp16"))
+
+
+def test_tiny_and_large_heads(tctx):
+    """Norms of values whose squares leave the range of fp16, and are as small as fp32 holds; zeros keep their sign."""
+    for dtype, sizes in (("fp16", (2.0 ** -24, 1e-4, 6e4)), ("bf16", (1e-17, 1e-10, 1e15))):
+        for size in sizes:
+            x = (rand(1, 6, 3, 64, dtype="bf16").float().sign() * size).to(TORCH[dtype])
+            w, out = torch.ones(64, dtype=TORCH[dtype], device="cuda"), torch.zeros_like(x)
+            tctx.norm_rotate_async(None, None, x, out, q_weight=w, eps=0.0)
+            want, tol = ready(f64(x), dtype, weight=f64(w))
+            assert_within(f64(out), want, tol, f"{dtype} {size}")
+    x = torch.zeros(2, 1, 64, dtype=torch.float16, device="cuda")
+    x[1] = -0.0
+    out = torch.full_like(x, 7.0)
+    tctx.rotate_async(tctx.rotary(32), places([3, 4]), x, out)
+    assert torch.equal(bits(out[..., 32:]), bits(x[..., 32:]))
