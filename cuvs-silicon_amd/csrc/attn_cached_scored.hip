@@ -1,4 +1,9 @@
-// Attention over a paged cache with capped scores, a bias by distance, or both: the kernels of attn_cached.hpp.
+// Attention over a paged cache with capped scores, a bias by distance, or both:
+// the kernels of attn_cached.hpp.
+//
+// Bounds: the memory, as with plain scores: 48 sequences of 100 to 6,000 tokens,
+// 32/8 heads of 128, bf16, cap 30, 104 us = 6.2 TB/s (plain 103).  One sequence of
+// 777 tokens, 16/4 heads of 64, biased: 7.6 us, latency.
 #include "attn_cached.hpp"
 
 namespace cvs {

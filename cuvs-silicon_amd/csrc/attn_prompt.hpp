@@ -149,6 +149,8 @@ struct PromptSource {
   __device__ CVS_INLINE u32x4 hide(u32x4 v, int, int, int) { return v; }  // past the sequence's end are zeros
 };
 
+// Capped and biased scores leave a SIMD a wave less where heads are small: with the registers of plain ones they spill in
+// the loop (64 passages of heads of 64, biased: 114 us, 51 so).
 template <bool kBf, int NB, int KS, typename Scoring>
 __global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 3 ? (Scoring::kPlain ? 3 : 2) : (Scoring::kPlain ? 4 : 3)) void prompt_attn_kernel(const PromptArgs a) {
   typedef PromptSource<NB> Source;

@@ -9,6 +9,11 @@
 // where they change places, in the factors' room; values go straight from their
 // rows to the pool (kv_tiles.hpp).  All of a wave's loads are under way before
 // the factors are made.
+//
+// Bounds: prompts the memory (24 of up to 2,000 tokens, 20/4 heads of 80, bf16,
+// normed: 41 us, 5.0 TB/s read and write, inputs in the last-level cache), steps a
+// chain of loads, factors and two barriers (a token of each of 64 sequences, 32/8
+// heads of 128, normed: 7.6 us; of one, 16/4 heads of 64: 5.2 us).
 #include <algorithm>
 #include <cstring>
 

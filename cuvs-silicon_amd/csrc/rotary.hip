@@ -8,7 +8,15 @@
 // The sum of squares goes over those lanes, a channel's partner comes from its
 // own piece, from the lane that has it, or, where the halves are no whole pieces
 // apart, through LDS.  Rows are read kAhead at a time, the first of them before
-// the factors are made.  Bound by the memory.
+// the factors are made.
+//
+// Bounds: long prompts the memory (12,000 tokens, 32/8 heads of 128, bf16, normed
+// and rotated: 53 us with inputs from memory, 4.6 TB/s read and write, where a
+// copy by the vendor's library reaches 4.9; 41 us with inputs still in the
+// last-level cache; the vector unit is busy 54% of the cycles then).  With cosines
+// and sines in LDS, and weights applied to each row, it took 74 us.  Few tokens a
+// chain of loads, the factors and a barrier: 2.9 us for one token of 16 heads of
+// 64, 4.7 us for 48 of 40 heads of 128, normed.
 #include <algorithm>
 #include <cmath>
 #include <cstring>

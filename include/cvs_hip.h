@@ -629,8 +629,9 @@ int cvs_kv_cache_compact(cvs_kv_cache* cache, int64_t* out_live);
  * (extended, truncated, freed, or moved by compaction).
  *
  * HIP graphs: calls of cvs_prompt_attention_async, cvs_kv_write_async,
- * cvs_kv_read_async and cvs_kv_attention_async can be captured, the last once
- * the same call has been made before (its workspace is there then).  The memory
+ * cvs_kv_read_async and cvs_kv_attention_async (and of both attentions with
+ * scores) can be captured, attention over the cache once the same call has been
+ * made before (its workspace is there then).  The memory
  * of their plans and workspace stays as it is until the context or cache is
  * destroyed, also when the plans are destroyed or larger calls follow.  Replays
  * belong in order with the context's stream, and end when one of the plans'
@@ -709,7 +710,8 @@ int cvs_rotary_frequencies(int dims, double base, const cvs_rotary_scaling* scal
 /* Rotary positions of a model: dims (even, up to CVS_ATTN_MAX_DIM) channels of
  * each head, dims / 2 host frequencies (of cvs_rotary_frequencies or any
  * others from -1024 to 1024), and the factor of all that is rotated.  Made once
- * for all layers and calls of its context. */
+ * for all layers and calls of its context; not while its stream is captured.
+ * What a captured call uses of it stays until the context's end. */
 typedef struct cvs_rotary cvs_rotary;
 int cvs_rotary_create(cvs_context* ctx, int dims, int layout, const double* radians, float magnitude,
                       cvs_rotary** out_rotary);
