@@ -52,17 +52,19 @@ ScoreArgs score_args(const cvs_scores* scores, float scale, int dim) {
     fail(CVS_ERR_UNSUPPORTED, "slopes must be aligned to 4 bytes");
   a.slopes = scores->slopes;
   if (scores->cap == 0.f) return a;
+  // u = ratio * s.  A cap that is larger still would be applied where a product's square has left the range of fp32, and
+  // be off by its own last places there, far more than the score.
+  const double ratio = double(a.c) / (double(scores->cap) * double(kLog2e)), y = ratio * ratio;
+  if (scores->cap < 1e-30f || ratio < 1e-18)
+    fail(CVS_ERR_UNSUPPORTED, "cap must be from 1e-30 to 1e18 times the scale");
   a.cap = scores->cap * kLog2e;
-  if (!(a.cap >= 1e-30f) || std::isinf(a.cap)) fail(CVS_ERR_UNSUPPORTED, "cap must be from 1e-30 to 2e38");
-  // u = ratio * s.  P's coefficients for s^2 leave the range of fp32 where the ratio is large; all scores are then large
-  // beside the cap.
-  const double ratio = double(a.c) / double(a.cap), y = ratio * ratio;
   a.twice = float(std::min(2.0 * ratio * double(kLog2e), 1e38));
+  // P's coefficients for s^2 leave the range of fp32 where the ratio is large; all scores are then large beside the cap.
   if (ratio > 1e4) {
     a.largest_y = -1.f;
     return a;
   }
-  a.largest_y = float(std::min(0.25 / y, 1e37));
+  a.largest_y = float(0.25 / y);
   const double fit[3] = {-3.332826464e-01, 1.320671470e-01, -4.478946771e-02};
   double power = double(a.c);
   for (int i = 0; i < 3; ++i) {

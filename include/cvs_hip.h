@@ -561,7 +561,7 @@ int cvs_prompt_plan_create_prefix(cvs_context* ctx, const int64_t* q_lengths, co
                                   cvs_prompt_plan** out_plan);
 
 /* What becomes of a score x = scale * q . k: cap * tanh(x / cap) where cap is
- * not 0 (finite, 1e-30 to 2e38), then less slopes[h] times the distance |p - j|
+ * not 0 (1e-30 to 1e18 scale), then less slopes[h] times the distance |p - j|
  * of the key's place j from the query's, p = i + k_length - q_length in a
  * prompt and the token's place in its sequence in a cache.  slopes: device
  * memory, a finite float for each query head, or null.  Both are in fp32; a

@@ -113,7 +113,7 @@ def test_caps_of_any_size(tctx, dtype, cap, spread):
     check(tctx, q, k, v, lengths, None, dtype, True, cap, torch.tensor([0.3, 0.0, 2.0, 1e-3], device="cuda"))
 
 
-@pytest.mark.parametrize("cap", [1e-30, 1e-9, 1e20, 2e38])
+@pytest.mark.parametrize("cap", [1e-30, 1e-9, 1e6, 0.99e12])
 @pytest.mark.parametrize("scale", [None, 1e-6, 1e4])
 def test_caps_at_the_ends(tctx, cap, scale):
     """A cap that flattens every score, one that changes none."""
@@ -182,6 +182,22 @@ def test_infinite_products_are_capped(tctx, kind):
     k[11, :, 5], k[50, 1, 7] = float("inf"), float("-inf")
     q[..., 5] = q[..., 5].abs() + 0.1
     check(tctx, q, k, v, [80], None, "bf16", False, *options(kind, 4, cap=3.0))
+
+
+def test_products_beyond_fp32s_squares(tctx):
+    """Products whose squares are infinite are at the cap, whatever it is: they share, and those far below have nothing."""
+    q = torch.full((3, 1, 64), 2.0 ** 33, dtype=torch.bfloat16, device="cuda")
+    k = torch.zeros(5, 1, 64, dtype=torch.bfloat16, device="cuda")
+    k[:, :, 0] = torch.tensor([1.0, 2.0 ** 40, 2.0 ** 41, -2.0 ** 41, 2.0 ** 41], device="cuda")[:, None]
+    v, out = rand(1, 5, 1, 64, dtype="bf16"), torch.zeros_like(q)
+    plan = tctx.prompt_plan([3], 1, 1, [5], causal=False)
+    for cap, share in ((2.0 ** 55, [0, 1 / 3, 1 / 3, 0, 1 / 3]), (4.0, [1 / 3, 1 / 3, 1 / 3, 0, 0])):
+        if cap == 4.0:
+            k[4, :, 0] = -1.0
+        tctx.prompt_attention_async(plan, q, k, v, out, cap=cap)
+        # Beside them are weights of e^-8 at most (a cap of 4: every score is 4 or -4).
+        want = sum(w * f64(v)[i, 0] for i, w in enumerate(share))
+        assert np.abs(f64(out)[:, 0] - want).max() < 2.0 ** -7 * (1 + np.abs(f64(v)).max())
 
 
 def test_rows_depend_on_themselves_alone(tctx):
@@ -386,8 +402,9 @@ def test_refusals(tctx, cvs):
         torch.cuda.synchronize()
         assert (out == 2).all(), "nothing is written by a refused call"
 
-    for cap in (-1.0, float("nan"), float("inf"), 1e-31, 3e38):
+    for cap in (-1.0, float("nan"), float("inf"), 1e-31, 3e38, 1.1e18 / 8):
         refused("cap", cap=cap)
+    refused("cap", cap=1.1e12, scale=1e-6)
     refused("slopes must be 4", slopes=slopes[:2])
     refused("slopes must be 4", slopes=slopes.double())
     refused("slopes must be 4", slopes=slopes[:, None])
