@@ -129,12 +129,13 @@ void rotate(cvs_context* ctx, const cvs_rotary* rotary, const int64_t* positions
     a.turning.turns = rotary->turns.as<uint64_t>();
     a.turning.magnitude = rotary->magnitude;
   }
-  // A workgroup makes its tokens' cosines once for all of its rows, about 128.  Where tokens are few it takes one, and
-  // their heads are spread over more workgroups, down to 16 rows each.
+  // A workgroup makes its tokens' factors once for all of its rows, about 128.  Fewer tokens are spread over two
+  // workgroups a compute unit, queries' and keys' by their heads, and few ones' heads over more, down to 16 rows each.
+  const int64_t all = int64_t(a.part[0].heads) + a.part[1].heads;
   int64_t blocks = 0;
   for (Part& p : a.part) {
     if (!p.heads) continue;
-    const int64_t least = 2 * ctx->compute_units;
+    const int64_t least = std::max<int64_t>(1, 2 * ctx->compute_units * p.heads / all);
     p.per_block = int(std::clamp<int64_t>(std::min<int64_t>(128 / p.heads, a.tokens / least), 1, kTokens));
     const int64_t groups = (a.tokens + p.per_block - 1) / p.per_block;
     const int64_t fit = std::clamp<int64_t>(least / groups, 1, (p.heads + 15) / 16);
