@@ -341,7 +341,7 @@ __device__ CVS_INLINE void many_rows(const Work<kBf, NB>& w, int wave, char* lds
   const Scoring scoring = scoring_of<Scoring>(w.a, r, key0);
   const int tiles = (it.tiles + 1) / 2, open = max(0, min(it.min_limit - key0, keys)) / 64;
   std::conditional_t<Scoring::kDown, FromTheMiddle, Ascending> order;
-  if constexpr (Scoring::kDown) order.top = tiles;
+  if constexpr (Scoring::kDown) order.top = order.before = tiles;  // open tiles lie before all rows
   attend_tiles<kBf, NB, 2 * NB>(st, q, src, tiles, open, it.min_limit < it.max_limit, min(r.limit - key0, keys), scoring,
                                 order, bad);
   const float l = both_sum(st.l);

@@ -146,7 +146,9 @@ __device__ CVS_INLINE float largest(const f32x16& s, float c) {
 //   them in models whose scores stay within half of the cap, takes five
 //   instructions a score more than a plain one and no exponential;
 //
-//   bias: minus log2(e) slope |place - key|, by the row's place and slope.
+//   bias: minus log2(e) slope |place - key|, by the row's place and slope: linear
+//   in the key where all of a tile's keys lie on one side of all rows, one
+//   instruction a score, two elsewhere.
 struct ScoreArgs {
   float c;
   float cap;            // log2(e) C
@@ -174,20 +176,23 @@ struct Scores {
     if constexpr (!kCap) return a.c;
     else return __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, a.a[2], a.a[1]), a.a[0]), a.c);
   }
-  // Score r of a lane's 16 less `base`, up to the cap's small scores; far: the place less that of r = 0.
-  __device__ CVS_INLINE float less(float s, float base, float far, int r) const {
-    const float x = __builtin_fmaf(s, factor(s * s), -base);
-    return biased(x, far, r);
+  // What is added to a product's score r of a lane's 16: rise (r's place) + from.  In a tile that lies before all of a
+  // wave's rows, or behind them, the bias is linear in the key, and one instruction a score.
+  static __device__ CVS_INLINE float added(float from, float rise, int r) {
+    if constexpr (kBias) return __builtin_fmaf(rise, float(8 * (r / 4) + r % 4), from);
+    else return from;
+  }
+  // Score r plus `from`, up to the cap's small scores.
+  __device__ CVS_INLINE float score(float s, float from, float rise, int r) const {
+    return __builtin_fmaf(s, factor(s * s), added(from, rise, r));
   }
   // The same, of any score.  one: 1, which the compiler does not know: it would keep what this has in common with
-  // `less`, 16 registers of it, for a pass that hardly ever comes.
-  __device__ CVS_INLINE float any_less(float s, float base, float far, int r, float one) const {
-    const float t = s * one, y = s * t;
-    float x = __builtin_fmaf(t, factor(y), -base);
-    if constexpr (kCap) {
-      x = y <= a.largest_y ? x : large(t) - base;
-    }
-    return biased(x, far * one, r);
+  // `score`, 16 registers of it, for a pass that hardly ever comes.
+  __device__ CVS_INLINE float any_score(float s, float from, float rise, int r, float one) const {
+    const float t = s * one, y = s * t, add = added(from, rise * one, r);
+    const float x = __builtin_fmaf(t, factor(y), add);
+    if constexpr (kCap) return y <= a.largest_y ? x : large(t) + add;
+    else return x;
   }
   // Products of keys key + 8 (r / 4) + r % 4 to scores, in place: for `probabilities` with a c of 1.
   __device__ CVS_INLINE void finish(f32x16& s, int key) const {
@@ -206,15 +211,14 @@ struct Scores {
       }
     }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = biased(x[r], far, r);
+    for (int r = 0; r < 16; ++r) {
+      if constexpr (kBias) s[r] = __builtin_fmaf(-slope, __builtin_fabsf(far - float(8 * (r / 4) + r % 4)), x[r]);
+      else s[r] = x[r];
+    }
   }
   __device__ CVS_INLINE float large(float s) const {
     const float e = 1.f + __builtin_amdgcn_exp2f(s * a.twice);
     return __builtin_fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(e), a.cap);
-  }
-  __device__ CVS_INLINE float biased(float x, float far, int r) const {
-    if constexpr (kBias) return __builtin_fmaf(-slope, __builtin_fabsf(far - float(8 * (r / 4) + r % 4)), x);
-    else return x;
   }
 };
 // A call's scores, checked; cap 0 for none.
@@ -227,13 +231,15 @@ void pick_scores(const ScoreArgs& a, const Go& go) {
   else go(std::common_type<Scores<true, false>>{});
 }
 
-// The order in which a row's tiles are taken: ascending, or from tile `top` - 1 down to 0 and then up from `top`.
+// The order in which a row's tiles are taken: ascending, or from tile `top` - 1
+// down to 0 and then up from `top`; tiles below `before` lie before the places of
+// all rows, those from `top` on behind them.
 struct Ascending {
-  static constexpr int top = 0;
+  static constexpr int top = 0, before = 0;
   __device__ CVS_INLINE int operator()(int step) const { return step; }
 };
 struct FromTheMiddle {
-  int top;
+  int top, before;
   __device__ CVS_INLINE int operator()(int step) const { return step < top ? top - 1 - step : step; }
 };
 
@@ -299,22 +305,25 @@ __device__ CVS_INLINE void probabilities(f32x16& s, RowState<NB>& st, float c) {
 }
 
 // `probabilities` of products s of capped or biased scores of keys key + 8 (r /
-// 4) + r % 4.  Where all are P's, and nothing has to rise, one pass does, in one
+// 4) + r % 4, which lie before the row's place (behind it: `behind`).  Where all are P's, and nothing has to rise, one pass does, in one
 // block with the matrix products before it; else the scores are taken once more,
 // larger ones by their exponential.  Which of the two is used changes no bit of
 // a row whose own scores are small.
 template <bool kBf, int NB, typename Scoring>
-__device__ CVS_INLINE void scored_probabilities(f32x16& s, RowState<NB>& st, const Scoring& sc, int key) {
-  const float far = Scoring::kBias ? float(sc.place - key) : 0.f;
+__device__ CVS_INLINE void scored_probabilities(f32x16& s, RowState<NB>& st, const Scoring& sc, int key, bool behind) {
+  const float rise = Scoring::kBias ? (behind ? -sc.slope : sc.slope) : 0.f;
+  auto from = [&](float base) CVS_INLINE {
+    return Scoring::kBias ? __builtin_fmaf(rise, float(key - sc.place), -base) : -base;
+  };
   f32x16 p;
   float sum;
   {
-    const float base = st.m == -INFINITY ? 0.f : st.m;
+    const float f = from(st.m == -INFINITY ? 0.f : st.m);
     float part[2] = {0.f, 0.f}, top = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       if constexpr (Scoring::kCap) top = fmaxf(top, s[r] * s[r]);
-      p[r] = __builtin_amdgcn_exp2f(sc.less(s[r], base, far, r));
+      p[r] = __builtin_amdgcn_exp2f(sc.score(s[r], f, rise, r));
       part[r & 1] += p[r];
     }
     sum = part[0] + part[1];
@@ -327,13 +336,13 @@ __device__ CVS_INLINE void scored_probabilities(f32x16& s, RowState<NB>& st, con
   }
   float most;
   auto pass = [&]() CVS_INLINE {
-    const float base = st.m == -INFINITY ? 0.f : st.m;
+    const float base = st.m == -INFINITY ? 0.f : st.m, f = from(base);
     float one = 1.f, part[2] = {0.f, 0.f};
     asm volatile("" : "+s"(one));
     most = -INFINITY;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const float x = sc.any_less(s[r], base, far, r, one);
+      const float x = sc.any_score(s[r], f, rise, r, one);
       most = fmaxf(most, x);
       p[r] = __builtin_amdgcn_exp2f(x);
       part[r & 1] += p[r];
@@ -344,16 +353,16 @@ __device__ CVS_INLINE void scored_probabilities(f32x16& s, RowState<NB>& st, con
   const float base = pass();
   const bool over = !(sum <= kMost<kBf>) || st.m == -INFINITY;
   if (__ballot(over)) {
-    const float rise = both_max(most) + base - kLift<kBf>;
+    const float m = both_max(most) + base - kLift<kBf>;
     const uint32_t either = uint32_t(over) | xor_lanes(uint32_t(over), 32);
-    const bool raise = either != 0 && rise > st.m;
-    const float alpha = raise ? __builtin_amdgcn_exp2f(st.m - rise) : 1.f;
+    const bool raise = either != 0 && m > st.m;
+    const float alpha = raise ? __builtin_amdgcn_exp2f(st.m - m) : 1.f;
     st.l *= alpha;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) st.o[b][r] *= alpha;
-    st.m = raise ? rise : st.m;
+    st.m = raise ? m : st.m;
     pass();  // from the scores again: less the m of before they have its last place
   }
   st.l += sum;
@@ -431,7 +440,7 @@ __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[KS], 
   };
   auto soften = [&](int n, int h, auto masked) CVS_INLINE {
     if constexpr (Scoring::kPlain || masked) probabilities<kBf>(s[h], st, scoring.c);
-    else scored_probabilities<kBf>(s[h], st, scoring, 64 * order(n) + 32 * h + 4 * half);
+    else scored_probabilities<kBf>(s[h], st, scoring, 64 * order(n) + 32 * h + 4 * half, n >= order.top);
 #pragma unroll
     for (int k = 0; k < 2; ++k) p[h][k] = prob_operand<kBf>(s[h], k);
   };
@@ -475,8 +484,10 @@ __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[KS], 
     steps(open_tiles, std::false_type{});
     steps(tiles, std::true_type{});
   } else {
-    // Masked tiles come first, down to the open ones, and last; a step behind a masked one still adds its values.
-    const int first = order.top > open_tiles ? order.top - open_tiles + 1 : 0, last = max(order.top, open_tiles);
+    // Masked tiles come first, with those that lie neither before all rows nor behind them, and last; a step behind a
+    // masked one still adds its values.
+    const int sure = min(open_tiles, order.before);
+    const int first = order.top > sure ? order.top - sure + 1 : 0, last = max(order.top, open_tiles);
     for (int masked = min(first, tiles), open = min(last, tiles);; masked = open = tiles) {
       steps(masked, std::true_type{});
       steps(open, std::false_type{});

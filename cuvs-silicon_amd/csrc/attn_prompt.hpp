@@ -196,9 +196,10 @@ __global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 3 ? (Scoring::kPlain ? 3 :
     if (Scoring::kDown && place < 0) shift = slope * float(place);
     const Scoring scoring{a.scores, slope, max(place, 0)};
     if constexpr (Scoring::kDown) {
+      const int place0 = it.k_len - it.q_len + it.row0 / a.group;  // of the first row
       const int last = it.k_len - it.q_len + (min(it.row0 + kRows, rows) - 1) / a.group;
       attend_tiles<kBf, NB, KS>(st, q, src, tiles, open, mixed, limit, scoring,
-                                FromTheMiddle{min(max(last, 0) / kKeys + 1, tiles)}, bad);
+                                FromTheMiddle{min(max(last, 0) / kKeys + 1, tiles), (max(place0, 0) + 1) / kKeys}, bad);
     } else {
       attend_tiles<kBf, NB, KS>(st, q, src, tiles, open, mixed, limit, scoring, Ascending{}, bad);
     }
