@@ -18,7 +18,11 @@ training) stands in for a model; what matters is the order of the calls:
 5. Half of the sequences end and the cache is compacted; each answer is checked
    against the whole prompt run through prompt attention from scratch.
 
-Run: python examples/answer_over_passages.py
+Positions are added to the tokens' embeddings, or (positions="rotary") turn
+the queries and keys, whose heads are normed first: of a prompt in one pass
+before its attention, of new tokens on their way into the cache.
+
+Run: python examples/answer_over_passages.py [rotary]
 """
 from __future__ import annotations
 
@@ -46,7 +50,8 @@ def load_package():
 class Model:
     """Layers of grouped-head attention with residuals; random weights."""
 
-    def __init__(self, seed, vocab=1000, width=512, layers=3, heads=8, kv_heads=2, dim=64, dtype=torch.float16):
+    def __init__(self, seed, vocab=1000, width=512, layers=3, heads=8, kv_heads=2, dim=64, dtype=torch.float16,
+                 added=True):
         g = torch.Generator(device="cuda").manual_seed(seed)
 
         def weight(*shape):
@@ -58,8 +63,12 @@ class Model:
         self.out = [weight(heads * dim, width) for _ in range(layers)]
         half = torch.arange(width // 2, device="cuda") / (width // 2)
         self.frequencies = 1e-4 ** half
+        self.added = added
+        self.q_norm, self.k_norm = (torch.ones(dim, dtype=dtype, device="cuda") for _ in "qk")
 
     def embed(self, ids, positions):
+        if not self.added:
+            return self.tokens[ids]
         angle = positions[:, None].float() * self.frequencies
         return self.tokens[ids] + torch.cat([angle.sin(), angle.cos()], dim=1).to(self.tokens.dtype)
 
@@ -84,20 +93,32 @@ def packed_positions(lengths, first=0):
     return torch.cat([torch.arange(first, first + n, device="cuda") for n in lengths])
 
 
-def main(passages=200, found=8, questions=12, steps=16, seed=1, quiet=False):
+def main(passages=200, found=8, questions=12, steps=16, seed=1, quiet=False, positions="added"):
     say = (lambda *a: None) if quiet else print
     cvs = load_package()
     # A context on torch's stream: its calls and torch's run in order, and nothing is waited for in between.
     ctx = cvs.Context(0, stream=torch.cuda.current_stream().cuda_stream)
-    model = Model(seed)
+    model = Model(seed, added=positions == "added")
+    rotary = ctx.rotary(model.dim) if positions == "rotary" else None
+
+    def prompt(plan, places):
+        """A prompt's attention: its queries and keys normed and turned in place, if the model has them so."""
+        def attend(layer, q, k, v, out):
+            if rotary:
+                ctx.norm_rotate_async(rotary, places, q, q, k, k, model.q_norm, model.k_norm)
+            ctx.prompt_attention_async(plan, q, k, v, out)
+        return attend
+
+    def run(ids, places, attend):
+        return model.run(ids, places, attend(places))
+
     g = torch.Generator().manual_seed(seed)
     lengths = torch.randint(20, 200, (passages,), generator=g).tolist()
     texts = [torch.randint(1000, (n,), generator=g).cuda() for n in lengths]
 
     # 1. The passages' vectors.
     plan = ctx.prompt_plan(lengths, model.heads, model.kv_heads, causal=False)
-    x = model.run(torch.cat(texts), packed_positions(lengths),
-                  lambda layer, q, k, v, out: ctx.prompt_attention_async(plan, q, k, v, out))
+    x = run(torch.cat(texts), packed_positions(lengths), lambda places: prompt(plan, places))
     owner = torch.repeat_interleave(torch.arange(passages, device="cuda"), torch.tensor(lengths, device="cuda"))
     vectors = torch.zeros(passages, model.width, device="cuda").index_add_(0, owner, x.float())
     vectors /= torch.tensor(lengths, device="cuda")[:, None]
@@ -120,11 +141,15 @@ def main(passages=200, found=8, questions=12, steps=16, seed=1, quiet=False):
     rows = cache.plan([root], [len(prefix)])
     plan = ctx.prompt_plan([len(prefix)], model.heads, model.kv_heads)
 
-    def first_time(layer, q, k, v, out):
-        ctx.prompt_attention_async(plan, q, k, v, out)
-        cache.write_async(rows, k, v, layer=layer)
+    def first_time(places):
+        attend = prompt(plan, places)
 
-    model.run(prefix, packed_positions([len(prefix)]), first_time)
+        def and_keep(layer, q, k, v, out):
+            attend(layer, q, k, v, out)
+            cache.write_async(rows, k, v, layer=layer)
+        return and_keep
+
+    run(prefix, packed_positions([len(prefix)]), first_time)
 
     # 4. The questions, then their answers.
     own = [torch.randint(1000, (n,), generator=g).cuda() for n in asked]
@@ -137,11 +162,15 @@ def main(passages=200, found=8, questions=12, steps=16, seed=1, quiet=False):
         rows = cache.plan(sequences, new, heads=model.heads)
 
         def over_cache(layer, q, k, v, out):
-            cache.write_async(rows, k, v, layer=layer)
+            if rotary:  # at the tokens' places in their sequences, which the plan knows
+                cache.append_async(rows, k, v, layer=layer, rotary=rotary, k_weight=model.k_norm, q=q, q_out=q,
+                                   q_weight=model.q_norm)
+            else:
+                cache.write_async(rows, k, v, layer=layer)
             cache.attention_async(rows, q, out, layer=layer)
 
-        positions = torch.cat([torch.arange(s, s + n, device="cuda") for s, n in zip(start, new)])
-        x = model.run(last, positions, over_cache)
+        places = torch.cat([torch.arange(s, s + n, device="cuda") for s, n in zip(start, new)])
+        x = run(last, places, lambda _: over_cache)
         ends = torch.tensor(new, device="cuda").cumsum(0) - 1
         answer_logits.append(model.logits(x[ends]))
         last = answer_logits[-1].argmax(1)
@@ -158,8 +187,7 @@ def main(passages=200, found=8, questions=12, steps=16, seed=1, quiet=False):
     for i in range(questions):
         whole = torch.cat([prefix, history[i][:-1]])
         plan = ctx.prompt_plan([len(whole)], model.heads, model.kv_heads)
-        x = model.run(whole, packed_positions([len(whole)]),
-                      lambda layer, q, k, v, out: ctx.prompt_attention_async(plan, q, k, v, out))
+        x = run(whole, packed_positions([len(whole)]), lambda places: prompt(plan, places))
         want = model.logits(x[len(prefix) + asked[i] - 1:])
         got = torch.stack([l[i] for l in answer_logits])
         worst = max(worst, ((got - want).norm() / want.norm()).item())
@@ -173,4 +201,4 @@ def main(passages=200, found=8, questions=12, steps=16, seed=1, quiet=False):
 
 
 if __name__ == "__main__":
-    main()
+    main(positions="rotary" if "rotary" in sys.argv[1:] else "added")
