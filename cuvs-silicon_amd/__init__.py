@@ -460,6 +460,15 @@ def _norm(ctx: "Context", weight, heads, eps: float, what: str):
     return HeadNorm(ptr, FP32 if kind == "float32" else heads.type, eps)
 
 
+def _open(rotary):
+    """The handle of a rotary, None without one: a closed one's is none as well, but it is no call without rotation."""
+    if rotary is None:
+        return None
+    if rotary.handle is None:
+        raise ValueError("the rotary is closed")
+    return rotary.handle
+
+
 def _scores(ctx: "Context", cap: float, slopes, heads: int):
     """The cvs_scores of a call."""
     if slopes is None:
@@ -676,11 +685,10 @@ class Context:
         if hq is None and hk is None:
             raise ValueError("neither q nor k")
         at = None
-        if rotary is not None:
+        if positions is not None:
             at = _vector(self, positions, "positions", (hq or hk).tokens, ("int64",))[0]
         after = self._behind_torch(q, q_out, k, k_out, q_weight, k_weight, positions)
-        _check(load().cvs_norm_rotate_async(self.handle, None if rotary is None else rotary.handle, at, hq, hqo, nq,
-                                            hk, hko, nk))
+        _check(load().cvs_norm_rotate_async(self.handle, _open(rotary), at, hq, hqo, nq, hk, hko, nk))
         if after:
             after()
 
@@ -1204,8 +1212,7 @@ class KvCache:
         hq, hqo, nq = _ready(self.ctx, q, q_out, q_weight, eps, "q")
         at = None if positions is None else _vector(self.ctx, positions, "positions", hk.tokens, ("int64",))[0]
         after = self.ctx._behind_torch(k, v, q, q_out, k_weight, q_weight, positions)
-        _check(load().cvs_kv_append_async(self.handle, plan.handle, layer, None if rotary is None else rotary.handle, at,
-                                          hk, nk, hv, hq, hqo, nq))
+        _check(load().cvs_kv_append_async(self.handle, plan.handle, layer, _open(rotary), at, hk, nk, hv, hq, hqo, nq))
         if after:
             after()
 

@@ -117,9 +117,10 @@ void rotate(cvs_context* ctx, const cvs_rotary* rotary, const int64_t* positions
   }
   if (!first) fail(CVS_ERR_INVALID_ARGUMENT, "neither q nor k");
   if (rotary) check_rotary(rotary, ctx, first->head_dim);
+  if (positions && !rotary) fail(CVS_ERR_INVALID_ARGUMENT, "positions without a rotary");
+  check_positions(positions);
   if (first->tokens == 0) return;
   if (rotary && !positions) fail(CVS_ERR_INVALID_ARGUMENT, "null positions");
-  if (rotary) check_positions(positions);
   a.positions = positions;
   a.tokens = first->tokens;
   a.turning.dim = first->head_dim;

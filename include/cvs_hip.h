@@ -733,7 +733,7 @@ int cvs_rotate_async(cvs_context* ctx, const cvs_rotary* rotary, const int64_t* 
 
 /* Queries and keys of the same tokens, normed and rotated in one pass.  q or k
  * (with its output and norm), either norm, and rotary (with positions) may be
- * null.  Outputs as in cvs_rotate_async. */
+ * null.  Outputs as in cvs_rotate_async, and each apart from all else. */
 int cvs_norm_rotate_async(cvs_context* ctx, const cvs_rotary* rotary, const int64_t* positions, const cvs_heads* q,
                           const cvs_heads* q_out, const cvs_head_norm* q_norm, const cvs_heads* k,
                           const cvs_heads* k_out, const cvs_head_norm* k_norm);
@@ -743,7 +743,8 @@ int cvs_norm_rotate_async(cvs_context* ctx, const cvs_rotary* rotary, const int6
  * cvs_kv_write_async would write them, and its queries q, normed and rotated,
  * to q_out.  Token t is at positions[t] (device memory, in the plan's order),
  * or, where positions is null, at its place in its sequence.  rotary, either
- * norm, and q (with its output and norm) may be null; q_out may be q itself.
+ * norm, and q (with its output and norm) may be null; q_out may be q itself and
+ * must not share memory with anything else.
  * q has any number of heads, a plan's with query heads its number.  Device
  * memory; enqueued on the context stream; can be captured like
  * cvs_kv_write_async. */

@@ -69,3 +69,11 @@ def test_arrays_the_binding_refuses(cvs):
     for x in (at(0, (64,), np.float16), at(0, (63,), np.float32), at(0, (64,), np.float64)):
         with pytest.raises(ValueError, match="w must be 64 elements"):
             cvs._norm(ctx, x, heads, 1e-6, "w")
+
+
+def test_a_closed_rotary_is_not_none(cvs):
+    """A closed rotary's handle is None, which C takes for a call without rotation."""
+    assert cvs._open(None) is None
+    assert cvs._open(types.SimpleNamespace(handle=5)) == 5
+    with pytest.raises(ValueError, match="closed"):
+        cvs._open(types.SimpleNamespace(handle=None))

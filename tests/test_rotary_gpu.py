@@ -325,3 +325,28 @@ def test_tiny_and_large_heads(tctx):
     out = torch.full_like(x, 7.0)
     tctx.rotate_async(tctx.rotary(32), places([3, 4]), x, out)
     assert torch.equal(bits(out[..., 32:]), bits(x[..., 32:]))
+
+
+def test_positions_and_their_rotary(cvs, tctx):
+    """A closed rotary, and positions that nothing would use, are refused rather than passed over."""
+    x = rand(1, 5, 4, 64, dtype="fp16")
+    out, at = torch.full_like(x, 7.0), torch.arange(5, device="cuda")
+    w = torch.ones(64, dtype=torch.float16, device="cuda")
+    closed = tctx.rotary(64)
+    closed.close()
+    cache = tctx.kv_cache(1, 4, 32, 4, 64, "fp16")
+    seqs = cache.sequences(1)
+    cache.extend(seqs, [5])
+    plan = cache.plan(seqs, [5])
+    for match, call in (
+            ("null rotary", lambda: tctx.rotate_async(closed, at, x, out)),
+            ("closed", lambda: tctx.norm_rotate_async(closed, at, x, out, q_weight=w)),
+            ("closed", lambda: tctx.norm_rotate_async(closed, None, x, out, q_weight=w)),
+            ("closed", lambda: cache.append_async(plan, x, x, rotary=closed, q=x, q_out=out)),
+            ("without a rotary", lambda: tctx.norm_rotate_async(None, at, x, out, q_weight=w)),
+            ("null positions", lambda: tctx.norm_rotate_async(tctx.rotary(64), None, x, out, q_weight=w))):
+        with pytest.raises(ValueError, match=match):
+            call()
+        torch.cuda.synchronize()
+        assert (out == 7).all(), "a refused call wrote"
+    cache.close()
