@@ -3,15 +3,15 @@
 // normed and rotated, in one launch.
 //
 // A workgroup takes one tile of up to 32 tokens: a wave for each of up to 4 kv
-// heads, or some query heads by all of them.  Its threads first make the factors
-// of the tile's tokens, a pair of channels each, for all heads (rotary.hpp).  A
-// wave's keys are normed and rotated as rows of pieces on their way to LDS,
-// where they change places, in the factors' room; values go straight from their
-// rows to the pool (kv_tiles.hpp).  All of a wave's loads are under way before
-// the factors are made.
+// heads; or, by all of its waves, query heads of some of the tokens.  Its
+// threads first make the factors of these tokens, a pair of channels each, for
+// all heads (rotary.hpp).  A wave's keys are normed and rotated as rows of
+// pieces on their way to LDS, where they change places, in the factors' room;
+// values go straight from their rows to the pool (kv_tiles.hpp).  All of a
+// wave's loads of keys and values are under way before the factors are made.
 //
 // Bounds: prompts the memory (24 of up to 2,000 tokens, 20/4 heads of 80, bf16,
-// normed: 41 us, 5.0 TB/s read and write, inputs in the last-level cache), steps a
+// normed: 38 us, 5.0 TB/s read and write, inputs in the last-level cache), steps a
 // chain of loads, factors and two barriers (a token of each of 64 sequences, 32/8
 // heads of 128, normed: 7.6 us; of one, 16/4 heads of 64: 5.2 us).
 #include <algorithm>
@@ -33,7 +33,8 @@ struct AppendArgs {
   Turning turning;
   int n_spans, page_tiles, by_tile;
   int kv_heads, kv_groups;         // workgroups of a tile's kv heads
-  int q_heads, q_chunk, q_chunks;  // and of its query heads
+  int q_parts;                     // of its query tokens,
+  int q_heads, q_chunk, q_chunks;  // and of their heads
   uint32_t q_magic, q_last_magic;  // of a chunk's heads, and of the last one's
   int kv_blocks;
   int at_rows;  // in LDS, of kChannels' rows
@@ -47,12 +48,20 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a, const S
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool queries = int(blockIdx.x) >= a.kv_blocks;
-  const int block = queries ? blockIdx.x - a.kv_blocks : blockIdx.x, each = queries ? a.q_chunks : a.kv_groups;
-  const int part = block % each, n = block / each;
+  const int block = queries ? blockIdx.x - a.kv_blocks : blockIdx.x, each = queries ? a.q_parts * a.q_chunks : a.kv_groups;
+  int part = block % each;
+  const int n = block / each;
   const int at = a.by_tile ? n % a.n_spans : n / a.page_tiles, tile = a.by_tile ? n / a.n_spans : n % a.page_tiles;
   const Span sp = a.spans ? a.spans[at] : inl.s[at];
-  const int lo = max(sp.begin() - 32 * tile, 0), hi = min(sp.end() - 32 * tile, 32);
+  int lo = max(sp.begin() - 32 * tile, 0), hi = min(sp.end() - 32 * tile, 32);
   if (lo >= hi) return;
+  if (queries && a.q_parts > 1) {
+    const int of = part / a.q_chunks, all = hi - lo, from = lo;
+    part -= of * a.q_chunks;
+    lo = from + all * of / a.q_parts;
+    hi = from + all * (of + 1) / a.q_parts;
+    if (lo == hi) return;
+  }
   const int64_t row = int64_t(sp.row0) + 32 * tile - sp.begin();  // of the tile's token 0
 
   const HeadLane<kLanes> l(a.turning.dim, a.turning.half);
@@ -204,7 +213,7 @@ extern "C" int cvs_kv_append_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int l
     a.turning.dim = cache->dim;
     a.kv_heads = cache->kv_heads;
     a.kv_groups = (cache->kv_heads + 3) / 4;
-    const int waves = (cache->kv_heads + a.kv_groups - 1) / a.kv_groups;
+    int waves = (cache->kv_heads + a.kv_groups - 1) / a.kv_groups;
     const int64_t tiles = int64_t(a.n_spans) * a.page_tiles;
     int64_t blocks = tiles * a.kv_groups;
     if (blocks <= kMaxBlocks) a.kv_blocks = int(blocks);
@@ -212,16 +221,22 @@ extern "C" int cvs_kv_append_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int l
       a.q = view_of(q);
       a.q_out = view_of(q_out);
       a.q_heads = q->heads;
-      // All heads by one workgroup, which makes a tile's factors once, or, where that leaves compute units without one,
-      // down to 16 rows each.
+      // A tile's queries by workgroups of some of its tokens and all heads, about 32 KB of them (tiles whole: 24 prompts of
+      // up to 2,000 tokens, 32/8 heads of 128, normed, take 134 us instead of 123), or, where that leaves compute units
+      // without one, of fewer heads, down to 16 rows each.
       const int64_t fill = std::max<int64_t>(1, plan->tokens / tiles), filled = (plan->tokens + fill - 1) / fill;
-      const int64_t fit = std::clamp<int64_t>(2 * ctx->compute_units / filled, 1, (q->heads * fill + 15) / 16);
+      a.q_parts = int(std::clamp<int64_t>(q->heads * fill * cache->dim / 16384, 1, fill));
+      const int64_t fit = std::clamp<int64_t>(2 * ctx->compute_units / (filled * a.q_parts), 1,
+                                              (q->heads * fill / a.q_parts + 15) / 16);
       a.q_chunk = int(std::min<int64_t>((q->heads + fit - 1) / fit, 1024));
       if (!rows_near(a.q, a.q_chunk) || !rows_near(a.q_out, a.q_chunk)) a.q_chunk = 1;
       a.q_chunks = (q->heads + a.q_chunk - 1) / a.q_chunk;
+      // A wave for each 16 rows, however few the kv heads are: with one of those, the prompts above take 84 us, and 150
+      // with one wave.
+      waves = int(std::clamp<int64_t>((a.q_chunk * fill / a.q_parts + 15) / 16, waves, 4));
       a.q_magic = magic_of(a.q_chunk);
       a.q_last_magic = magic_of(q->heads - (a.q_chunks - 1) * a.q_chunk);
-      blocks += tiles * a.q_chunks;
+      blocks += tiles * a.q_parts * a.q_chunks;
     }
     if (blocks > kMaxBlocks) fail(CVS_ERR_UNSUPPORTED, "too many tokens");
     Spans inl;

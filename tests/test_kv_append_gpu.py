@@ -130,6 +130,12 @@ def test_many_sequences(tctx, cvs, page):
     check(tctx, cvs, [3, 500], [2000, 777], 5, 5, 64, 64, "bf16", page=page)
 
 
+@pytest.mark.parametrize("heads,kv,dim,dims", [(40, 5, 128, 128), (32, 1, 64, 24), (63, 1, 80, 80), (24, 2, 128, 22)])
+def test_query_parts(tctx, cvs, heads, kv, dim, dims):
+    """Tiles whose queries several workgroups share by their tokens, tiles of fewer tokens than workgroups among them."""
+    check(tctx, cvs, [0, 7, 31, 64, 3], [333, 95, 1, 3, 640], heads, kv, dim, dims, "bf16", dims == 128, page=64)
+
+
 def test_a_long_sequence(tctx, cvs):
     """Positions past 100,000 from the cache's own places."""
     cache = tctx.kv_cache(1, 1001, 128, 1, 64, "bf16")
