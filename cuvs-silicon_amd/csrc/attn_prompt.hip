@@ -55,21 +55,35 @@ ScoreArgs score_args(const cvs_scores* scores, float scale, int dim) {
   // u = ratio * s.  A cap that is larger still would be applied where a product's square has left the range of fp32, and
   // be off by its own last places there, far more than the score.
   const double ratio = double(a.c) / (double(scores->cap) * double(kLog2e)), y = ratio * ratio;
-  if (scores->cap < 1e-30f || ratio < 1e-18)
-    fail(CVS_ERR_UNSUPPORTED, "cap must be from 1e-30 to 1e18 times the scale");
+  if (scores->cap < 1e-30f || scores->cap > 1e38f || ratio < 1e-18)
+    fail(CVS_ERR_UNSUPPORTED, "cap must be from 1e-30 to 1e38 and at most 1e18 times the scale");
   a.cap = scores->cap * kLog2e;
   a.twice = float(std::min(2.0 * ratio * double(kLog2e), 1e38));
-  // P's coefficients for s^2 leave the range of fp32 where the ratio is large; all scores are then large beside the cap.
-  if (ratio > 1e4) {
-    a.largest_y = -1.f;
-    return a;
+  // P's coefficients are c ratio^2, ratio^4 and ratio^6 times these.  All have to be normal numbers of fp32: of a cap far
+  // above the scale (from 9e5 times it on, for a scale of 1/8) the last ones would be rounded to few bits or to 0.  Then a
+  // P of fewer terms, tanh's series, goes up to a |u| where the first term that it leaves out is below 2^-21, and larger
+  // scores are the exponential's.  Of a scale so far above the cap that a coefficient is infinite, all are.
+  struct Terms {
+    double largest_u, of[3];
+  };
+  constexpr Terms kinds[] = {{0.5, {-3.332826464e-01, 1.320671470e-01, -4.478946771e-02}},
+                             {0.125, {-1.0 / 3.0, 2.0 / 15.0, 0.0}},     // less 17/315 u^6
+                             {0.03125, {-1.0 / 3.0, 0.0, 0.0}},          // 2/15 u^4
+                             {0.0009765625, {0.0, 0.0, 0.0}}};           // u^2 / 3
+  for (const Terms& k : kinds) {
+    double power = double(a.c);
+    bool all = true;
+    for (int i = 0; i < 3; ++i) {
+      power *= y;
+      a.a[i] = float(k.of[i] * power);
+      all &= k.of[i] == 0.0 || std::isnormal(a.a[i]) || std::isinf(a.a[i]);
+    }
+    a.largest_y = float(k.largest_u * k.largest_u / y);
+    if (all) break;
   }
-  a.largest_y = float(0.25 / y);
-  const double fit[3] = {-3.332826464e-01, 1.320671470e-01, -4.478946771e-02};
-  double power = double(a.c);
-  for (int i = 0; i < 3; ++i) {
-    power *= y;
-    a.a[i] = float(fit[i] * power);
+  if (ratio > 1e4 || std::isinf(a.a[2])) {
+    a.a[0] = a.a[1] = a.a[2] = 0.f;
+    a.largest_y = -1.f;
   }
   return a;
 }
