@@ -156,6 +156,7 @@ struct ScoreArgs {
   float twice;          // log2(e) 2 scale / C
   float largest_y;      // of P's range; -1: P is not used
   float a[3];           // P's coefficients behind c
+  int apart;            // scores may pass 2^24: they are finished before their row's m is taken off (attend_tiles)
   const float* slopes;  // of the heads, natural units; null: none
 };
 struct PlainScores {
@@ -408,6 +409,7 @@ __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[KS], 
                                         int open_tiles, bool mixed, int limit, const Scoring& scoring,
                                         const Order& order, bool& bad) {
   const int half = __lane_id() >> 5;
+  int unmasked_tiles = open_tiles;
   f32x16 s[2];    // scores of a tile's two halves
   u32x4 p[2][2];  // and their probabilities
   auto scores = [&](int n, int h) CVS_INLINE {
@@ -474,6 +476,12 @@ __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[KS], 
     mask(0, 0);
     st.m = largest(s[0], scoring.c) - kLift<kBf>;
   }
+  // Steps of open tiles take m off in the multiply-add that makes a score.  What the rounded m lacks of its own score
+  // passes 1 where scores pass 2^24, and from 2^31 on makes the exponential infinite, or leaves the row nothing: calls whose
+  // cap allows such scores take masked steps, which round a score first.
+  if constexpr (!Scoring::kPlain) {
+    if (Scoring::kCap && scoring.a.apart) unmasked_tiles = 0;
+  }
   int n = 0;
   auto steps = [&](int end, auto masked) CVS_INLINE {
     for (; n < end; ++n) step(n, masked, std::false_type{});
@@ -482,13 +490,13 @@ __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[KS], 
   // a branch would split the blocks that overlap products and exponentials; it is there a masked one, of any tile.
   if constexpr (!Scoring::kPlain) step(n++, std::true_type{}, std::true_type{});
   if constexpr (!Scoring::kDown) {
-    steps(open_tiles, std::false_type{});
+    steps(unmasked_tiles, std::false_type{});
     steps(tiles, std::true_type{});
   } else {
     // Masked tiles come first, with those that lie neither before all rows nor behind them, and last; a step behind a
     // masked one still adds its values.
-    const int sure = min(open_tiles, order.before);
-    const int first = order.top > sure ? order.top - sure + 1 : 0, last = max(order.top, open_tiles);
+    const int sure = min(unmasked_tiles, order.before);
+    const int first = order.top > sure ? order.top - sure + 1 : 0, last = max(order.top, unmasked_tiles);
     for (int masked = min(first, tiles), open = min(last, tiles);; masked = open = tiles) {
       steps(masked, std::true_type{});
       steps(open, std::false_type{});

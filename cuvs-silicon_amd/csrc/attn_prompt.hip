@@ -85,6 +85,7 @@ ScoreArgs score_args(const cvs_scores* scores, float scale, int dim) {
     a.a[0] = a.a[1] = a.a[2] = 0.f;
     a.largest_y = -1.f;
   }
+  a.apart = a.cap >= 16777216.f;
   return a;
 }
 

@@ -25,6 +25,23 @@ def tctx(cvs):
     c.close()
 
 
+def check(ctx, scale, cap, steep):
+    """SHARES of the cap, a key alone and many."""
+    heads, kv, n = 4, 2, len(SHARES)
+    v = rand(3, 400, kv, 64, dtype="bf16")
+    slopes = None if steep is None else torch.full((heads,), steep, device="cuda")
+    for keys in (1, 400):
+        q, k = products(scale, cap, heads, kv, keys)
+        out, lse = torch.full_like(q, 7.0), torch.full((heads, n), 7.0, device="cuda")
+        plan = ctx.prompt_plan([n], heads, kv, [keys], causal=False)
+        ctx.prompt_attention_async(plan, q, k, v[:keys], out, lse, scale, cap, slopes)
+        want, tol, l, l_tol = scored(f64(q), f64(k), f64(v[:keys]), np.full(n, keys), "bf16", scale, cap,
+                                     None if slopes is None else f64(slopes), np.arange(n) + keys - n)
+        assert_within(f64(lse), l, l_tol, f"{keys} keys")
+        assert_within(f64(out), want, tol, f"{keys} keys")
+    return f64(out), f64(lse), f64(v)
+
+
 def products(scale, cap, heads, kv, keys):
     """Queries and keys whose products, each of one channel, are SHARES of cap / scale."""
     whole = cap / scale
@@ -42,18 +59,19 @@ def products(scale, cap, heads, kv, keys):
 @pytest.mark.parametrize("steep", [None, 1e-3])
 def test_caps_of_any_size_beside_the_scale(tctx, scale, cap, steep):
     """Every share of the cap keeps the bound, whatever the cap, in masked tiles and in others."""
-    heads, kv, n = 4, 2, len(SHARES)
-    v = rand(3, 400, kv, 64, dtype="bf16")
-    slopes = None if steep is None else torch.full((heads,), steep, device="cuda")
-    for keys in (1, 400):
-        q, k = products(scale, cap, heads, kv, keys)
-        out, lse = torch.full_like(q, 7.0), torch.full((heads, n), 7.0, device="cuda")
-        plan = tctx.prompt_plan([n], heads, kv, [keys], causal=False)
-        tctx.prompt_attention_async(plan, q, k, v[:keys], out, lse, scale, cap, slopes)
-        want, tol, l, l_tol = scored(f64(q), f64(k), f64(v[:keys]), np.full(n, keys), "bf16", scale, cap,
-                                     None if slopes is None else f64(slopes), np.arange(n) + keys - n)
-        assert_within(f64(lse), l, l_tol, f"{keys} keys")
-        assert_within(f64(out), want, tol, f"{keys} keys")
+    check(tctx, scale, cap, steep)
+
+
+@pytest.mark.parametrize("scale,cap", [(0.125, 1e8), (0.125, 1e9), (0.125, 1e12), (0.125, 1e17), (1e12, 1e9),
+                                       (1e18, 2e14), (1e21, 1e38), (2e38, 2e35)])
+def test_scores_beyond_2_to_the_24(tctx, scale, cap):
+    """Scores whose last place is more than 1: the same ones of a row still share evenly, whatever their size."""
+    out, lse, v = check(tctx, scale, cap, None)
+    even = v.mean(0).repeat(2, axis=0)
+    # Weights of 1 are exact, as are their sums: the sums of values and the quotient, in 32 bits, and the output's rounding.
+    room = 400 * 2.0 ** -24 * np.abs(v).mean(0).repeat(2, axis=0) + 2.0 ** -8 * np.abs(even) * 1.01
+    assert (np.abs(out - even) <= room).all()
+    check(tctx, scale, cap, 1e-3)
 
 
 def test_larger_products_have_no_smaller_scores(tctx):
