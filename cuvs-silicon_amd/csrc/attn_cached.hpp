@@ -235,7 +235,7 @@ __device__ CVS_INLINE void few_rows(const Work<kBf, NB>& w, int wave, char* lds)
         if (it.min_limit < it.max_limit) bad |= clean<kBf>(vf);
       }
       if (i == wave) st.m = largest(s, scoring.c) - kLift<kBf>;
-      probabilities<kBf>(s, st, scoring.c);
+      probabilities<kBf, !Scoring::kPlain>(s, st, scoring.c);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const u32x4 pr = prob_operand<kBf>(s, h);

@@ -268,14 +268,20 @@ struct FromTheMiddle {
 // a lift of 0, 8 or 10 where scores are spread by 1, and 162, 170 or 176 us where
 // they are spread by 2.6 (natural units).  A tile that sums to more than kMost
 // has a probability above kMost / 16 > 2^(kLift + 1), so its row does rise.
+//
+// Scores that pass kFar are rounded before m is taken off: in one multiply-add,
+// what m, a rounded score, lacks of its own passes 1 there, and from 2^31 on would
+// make the exponential infinite, or leave the row nothing.  (Finished scores are
+// rounded already.)  Nor has m a lift there, which could be rounded to twice itself.
+constexpr float kFar = 16777216.f;
 template <bool kBf>
 constexpr float kLift = kBf ? 0.f : 8.f;
 template <bool kBf>
 constexpr float kMost = kBf ? 4096.f : 65504.f;
-template <bool kBf, int NB>
+template <bool kBf, bool kFinished, int NB>
 __device__ CVS_INLINE void probabilities(f32x16& s, RowState<NB>& st, float c) {
   f32x16 p;
-  auto exponentials = [&]() CVS_INLINE {
+  auto exponentials = [&](float c) CVS_INLINE {
     const float base = st.m == -INFINITY ? 0.f : st.m;
     float sum[2] = {0.f, 0.f};
 #pragma unroll
@@ -285,10 +291,10 @@ __device__ CVS_INLINE void probabilities(f32x16& s, RowState<NB>& st, float c) {
     }
     return sum[0] + sum[1];
   };
-  float sum = exponentials();
-  const bool over = !(sum <= kMost<kBf>) || st.m == -INFINITY;
+  float sum = exponentials(c);
+  const bool over = !(sum <= kMost<kBf>) || (kFinished ? st.m == -INFINITY : !(__builtin_fabsf(st.m) < kFar));
   if (__ballot(over)) {
-    const float top = largest(s, c) - kLift<kBf>;
+    const float most = largest(s, c), top = __builtin_fabsf(most) < kFar ? most - kLift<kBf> : most;
     // Either of the row's two lanes (exchanged by all lanes, before any condition); the other rows stay as they are, so
     // that a row's result depends on itself alone.
     const uint32_t either = uint32_t(over) | xor_lanes(uint32_t(over), 32);
@@ -300,7 +306,10 @@ __device__ CVS_INLINE void probabilities(f32x16& s, RowState<NB>& st, float c) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) st.o[b][r] *= alpha;
     st.m = raise ? top : st.m;
-    sum = exponentials();
+    const bool far = !kFinished && !(__builtin_fabsf(st.m) < kFar);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = far ? s[r] * c : s[r];
+    sum = exponentials(far ? 1.f : c);
   }
   st.l += sum;
   s = p;
@@ -329,7 +338,7 @@ __device__ CVS_INLINE void scored_probabilities(f32x16& s, RowState<NB>& st, con
       part[r & 1] += p[r];
     }
     sum = part[0] + part[1];
-    const bool over = !(sum <= kMost<kBf>) | (st.m == -INFINITY), large = Scoring::kCap & !(top <= sc.a.largest_y);
+    const bool over = !(sum <= kMost<kBf>) | !(__builtin_fabsf(st.m) < kFar), large = Scoring::kCap & !(top <= sc.a.largest_y);
     if (__ballot(over | large) == 0) {
       st.l += sum;
       s = p;
@@ -353,9 +362,24 @@ __device__ CVS_INLINE void scored_probabilities(f32x16& s, RowState<NB>& st, con
     return base;
   };
   const float base = pass();
-  const bool over = !(sum <= kMost<kBf>) || st.m == -INFINITY;
+  const bool over = !(sum <= kMost<kBf>) || !(__builtin_fabsf(st.m) < kFar);
   if (__ballot(over)) {
-    const float m = both_max(most) + base - kLift<kBf>;
+    float m = both_max(most) + base - kLift<kBf>;
+    // Rows whose scores pass kFar, or did so far: biased ones (of capped ones there are none here).
+    const bool far = Scoring::kBias && !(fmaxf(__builtin_fabsf(m), __builtin_fabsf(base)) < kFar);
+    const bool any_far = __ballot(far) != 0;
+    if (any_far) {
+      float one = 1.f, top = -INFINITY;
+      asm volatile("" : "+s"(one));
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = sc.any_score(s[r], from(0.f), rise, r, one);
+        top = fmaxf(top, x);
+        s[r] = far ? x : s[r];
+      }
+      top = both_max(top);
+      m = far ? top : m;
+    }
     const uint32_t either = uint32_t(over) | xor_lanes(uint32_t(over), 32);
     const bool raise = either != 0 && m > st.m;
     const float alpha = raise ? __builtin_amdgcn_exp2f(st.m - m) : 1.f;
@@ -366,6 +390,15 @@ __device__ CVS_INLINE void scored_probabilities(f32x16& s, RowState<NB>& st, con
       for (int r = 0; r < 16; ++r) st.o[b][r] *= alpha;
     st.m = raise ? m : st.m;
     pass();  // from the scores again: less the m of before they have its last place
+    if (any_far) {
+      float part[2] = {0.f, 0.f};
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        p[r] = far ? __builtin_amdgcn_exp2f(s[r] - (st.m == -INFINITY ? 0.f : st.m)) : p[r];
+        part[r & 1] += p[r];
+      }
+      sum = part[0] + part[1];
+    }
   }
   st.l += sum;
   s = p;
@@ -442,7 +475,7 @@ __device__ CVS_INLINE void attend_tiles(RowState<NB>& st, const u32x4 (&q)[KS], 
       if (8 * (r / 4) + r % 4 >= seen) s[h][r] = -INFINITY;
   };
   auto soften = [&](int n, int h, auto masked) CVS_INLINE {
-    if constexpr (Scoring::kPlain || masked) probabilities<kBf>(s[h], st, scoring.c);
+    if constexpr (Scoring::kPlain || masked) probabilities<kBf, !Scoring::kPlain>(s[h], st, scoring.c);
     else scored_probabilities<kBf>(s[h], st, scoring, 64 * order(n) + 32 * h + 4 * half, n >= order.top);
 #pragma unroll
     for (int k = 0; k < 2; ++k) p[h][k] = prob_operand<kBf>(s[h], k);
