@@ -182,7 +182,7 @@ struct Tiles {
 template <typename Scoring>
 __device__ CVS_INLINE Scoring scoring_of(const CachedArgs& a, const Row& r, int key0) {
   if constexpr (Scoring::kPlain) return {a.scores.c};
-  else return {a.scores, Scoring::kDown ? a.scores.slopes[r.head] * kLog2e : 0.f, r.limit - 1 - key0};
+  else return {a.scores, Scoring::kDown ? slope_log2(a.scores.slopes[r.head]) : 0.f, r.limit - 1 - key0};
 }
 
 // Up to 32 rows: the waves share the tiles.

@@ -223,6 +223,13 @@ struct Scores {
     return __builtin_fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(e), a.cap);
   }
 };
+// A head's slope in log2 units, from -kSteepest to kSteepest natural ones: of those a key a token nearer has all the weight
+// already, and their products with 2^31 tokens are numbers of 32 bits (with a slope of 3e38 a row's own key, 0 tokens away,
+// was at 0 times infinity).
+constexpr float kSteepest = 1e28f;
+__device__ CVS_INLINE float slope_log2(float slope) {
+  return (slope > kSteepest ? kSteepest : slope < -kSteepest ? -kSteepest : slope) * kLog2e;
+}
 // A call's scores, checked; cap 0 for none.
 ScoreArgs score_args(const cvs_scores* scores, float scale, int dim);
 // Calls go with the type of a call's capped or biased scores (a std::common_type of it).

@@ -192,7 +192,7 @@ __global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 3 ? (Scoring::kPlain ? 3 :
   } else {
     // Rows before the first key count from it, so that distances are as exact for them as for others.
     const int place = it.k_len - it.q_len + tok;
-    const float slope = Scoring::kDown ? a.scores.slopes[head] * kLog2e : 0.f;
+    const float slope = Scoring::kDown ? slope_log2(a.scores.slopes[head]) : 0.f;
     if (Scoring::kDown && place < 0) shift = slope * float(place);
     const Scoring scoring{a.scores, slope, max(place, 0)};
     if constexpr (Scoring::kDown) {

@@ -564,9 +564,9 @@ int cvs_prompt_plan_create_prefix(cvs_context* ctx, const int64_t* q_lengths, co
  * not 0 (1e-30 to 1e38, and at most 1e18 scale), then less slopes[h] times the
  * distance |p - j| of the key's place j from the query's, p = i + k_length -
  * q_length in a prompt and the token's place in its sequence in a cache.
- * slopes: device memory, a finite float for each query head, or null.  Both are
- * in fp32; a capped score is off by at most 2^-20 of itself and 2^-22 of the
- * cap. */
+ * slopes: device memory, a finite float for each query head, or null; those
+ * beyond 1e28 and -1e28 count as these.  Both are in fp32; a capped score is off
+ * by at most 2^-20 of itself and 2^-22 of the cap. */
 typedef struct cvs_scores {
   float cap;
   const float* slopes;

@@ -8,7 +8,7 @@ import torch
 
 from attention_oracle import assert_within, f64
 from scored_oracle import scored
-from test_kv_cache_gpu import rand
+from test_kv_cache_gpu import Filled, bits, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -120,3 +120,53 @@ def test_caps_beyond_32_bits_are_refused(tctx):
             tctx.prompt_attention_async(plan, q, k, v, out, cap=cap, scale=1e25)
     torch.cuda.synchronize()
     assert (out == 2).all()
+
+
+STEEP = [1e20, 1e28, 1e33, 1e37, 2.4e38, 3.4028234e38]
+
+
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_the_steepest_slopes(tctx, dtype, cap):
+    """Of any finite slope a row has its nearest key alone, of a negative one its farthest."""
+    slopes = torch.tensor(STEEP + [-s for s in STEEP], device="cuda")
+    heads, kv = len(slopes), 1
+    # Rows before the first key, tiles that end at a row's place, a row alone behind whole tiles, many rows.
+    for ql, kl in ((300, 300), (1, 64), (1, 128), (64, 192), (70, 40), (1, 777), (130, 700)):
+        q, k, v = (rand(i, n, h, 64, dtype=dtype) for i, n, h in ((1, ql, heads), (2, kl, kv), (3, kl, kv)))
+        out, lse = torch.zeros_like(q), torch.zeros(heads, ql, device="cuda")
+        tctx.prompt_attention_async(tctx.prompt_plan([ql], heads, kv, [kl], prefixes=[min(kl, 20)]), q, k, v, out, lse,
+                                    cap=cap, slopes=slopes)
+        place = torch.arange(ql, device="cuda") + kl - ql
+        seen = torch.maximum(place + 1, torch.tensor(min(kl, 20), device="cuda")).clamp(max=kl)
+        near = place.clamp(min=0)
+        far = torch.where(place >= seen - 1 - place, 0, seen - 1)
+        alone = place * 2 != seen - 1  # not as far from the first key as from the last
+        for h in range(heads):
+            at = near if slopes[h] > 0 else far
+            rows = alone if slopes[h] < 0 else torch.ones_like(alone)
+            assert torch.equal(bits(out[:, h][rows]), bits(v[at, 0][rows])), (ql, kl, slopes[h].item())
+        want = -slopes.double().clamp(-1e28, 1e28)[:, None] * torch.stack(
+            [(place - (near if s > 0 else far)).abs().double() for s in slopes])
+        assert ((lse.double() - want).abs() <= 2.0 ** -21 * want.abs() + 30.0).all(), (ql, kl)
+
+
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("new", [1, 3, 80])
+def test_the_steepest_slopes_over_the_cache(tctx, cap, new):
+    slopes = torch.tensor(STEEP + [-s for s in STEEP], device="cuda")
+    f = Filled(tctx, 1, 400, 32, 1, 64, "fp16", 3)
+    seqs = f.new(4)
+    lengths = [64, 100, 777, 9000]
+    f.append(seqs, lengths)
+    here = [min(new, n) for n in lengths]
+    q = rand(9, sum(here), len(slopes), 64, dtype="fp16")
+    out, start = torch.zeros_like(q), 0
+    f.cache.attention_async(f.cache.plan(seqs, here, heads=len(slopes)), q, out, cap=cap, slopes=slopes)
+    for s, n, m in zip(seqs, here, lengths):
+        v = f.held[s][1][0, :, 0]
+        for h in range(len(slopes)):
+            want = v[m - n:] if slopes[h] > 0 else v[:1].expand(n, 64)
+            assert torch.equal(bits(out[start:start + n, h]), bits(want)), (m, slopes[h].item())
+        start += n
+    f.cache.close()
