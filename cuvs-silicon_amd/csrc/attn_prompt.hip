@@ -39,6 +39,7 @@ void check_rows_apart(const cvs_heads* x, const char* what, int64_t layers, int6
 float scale_log2(float scale, int dim) {
   if (!(scale >= 0.f) || std::isinf(scale))
     fail(CVS_ERR_INVALID_ARGUMENT, "scale must be finite and positive, or 0 for 1 / sqrt(head_dim)");
+  if (scale > 2e38f) fail(CVS_ERR_UNSUPPORTED, "scale must be at most 2e38");  // log2(e) times it is a number of 32 bits
   return (scale == 0.f ? 1.f / std::sqrt(float(dim)) : scale) * kLog2e;
 }
 

@@ -547,7 +547,7 @@ int cvs_prompt_plan_create(cvs_context* ctx, const int64_t* q_lengths, const int
 int cvs_prompt_plan_destroy(cvs_prompt_plan* plan);
 
 /* Attention of a plan's batch.  q, out: the plan's query tokens x heads; k,
- * v: its key tokens x kv_heads.  scale: finite and positive, or 0 for 1 /
+ * v: its key tokens x kv_heads.  scale: positive, up to 2e38, or 0 for 1 /
  * sqrt(head_dim).  lse (may be null): heads x query tokens floats.  Device
  * memory; enqueued on the context stream. */
 int cvs_prompt_attention_async(cvs_context* ctx, const cvs_prompt_plan* plan, const cvs_heads* q, const cvs_heads* k,

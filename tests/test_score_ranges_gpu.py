@@ -170,3 +170,29 @@ def test_the_steepest_slopes_over_the_cache(tctx, cap, new):
             assert torch.equal(bits(out[start:start + n, h]), bits(want)), (m, slopes[h].item())
         start += n
     f.cache.close()
+
+
+def test_scales_beyond_32_bits_are_refused(tctx):
+    """log2(e) times the scale has to be a number of 32 bits, or products of 0 would be NaN."""
+    q = torch.zeros(3, 1, 64, dtype=torch.bfloat16, device="cuda")
+    q[1:, :, 3] = 2.0 ** -130
+    k = q + 0.0
+    v, out = rand(1, 3, 1, 64, dtype="bf16"), torch.full_like(q, 2.0)
+    plan = tctx.prompt_plan([3], 1, 1)
+    f = Filled(tctx, 1, 2, 32, 1, 64, "bf16")
+    (s,) = f.new()
+    f.append([s], [3])
+    step = f.cache.plan([s], [3], heads=1)
+    for scale in (2.01e38, 2.4e38, 3.4028234e38):
+        for options in ({}, {"cap": 5.0}):
+            with pytest.raises(ValueError, match="scale must be at most"):
+                tctx.prompt_attention_async(plan, q, k, v, out, scale=scale, **options)
+            with pytest.raises(ValueError, match="scale must be at most"):
+                f.cache.attention_async(step, q, out, scale=scale, **options)
+    torch.cuda.synchronize()
+    assert (out == 2).all()
+    tctx.prompt_attention_async(plan, q, k, v, out, scale=2e38)
+    want = torch.cumsum(v.float(), 0) / torch.arange(1, 4, device="cuda")[:, None, None]
+    assert (out.float() - want).abs().max() <= 2.0 ** -7 * v.float().abs().max()
+    del step
+    f.cache.close()
