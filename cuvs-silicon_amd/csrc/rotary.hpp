@@ -156,7 +156,10 @@ __device__ CVS_INLINE u32x4 ready(u32x4 x, const HeadLane<kLanes>& l, const floa
 #pragma unroll
     for (int m = 1; m < kLanes; m <<= 1) sum += xor_lanes_f(sum, m);
     const float root = inverse_root(__builtin_fmaf(sum, l.inv_dim, eps));
+    // Before the factors: a product of them and a large channel could be infinite, and 0 times that is NaN.
     inv = normed ? root : 1.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= inv;
   }
   if constexpr (kPairs == kNeighbours) {
     // Whole pairs are in or out.
@@ -170,6 +173,10 @@ __device__ CVS_INLINE u32x4 ready(u32x4 x, const HeadLane<kLanes>& l, const floa
       px[k] = l.turned ? w : 0;
     }
     unpack8<kBf>(px, g);
+    if constexpr (kNorm) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[e] *= inv;
+    }
   } else {
     // The row's pieces side by side.
     *scratch = x;
@@ -179,7 +186,7 @@ __device__ CVS_INLINE u32x4 ready(u32x4 x, const HeadLane<kLanes>& l, const floa
     for (int e = 0; e < 8; ++e) {
       const int c = 8 * l.piece + e;
       const float v = to_float<kBf>(row[c < l.half ? c + l.half : c < 2 * l.half ? c - l.half : c]);
-      g[e] = c < 2 * l.half ? v : 0.f;
+      g[e] = c < 2 * l.half ? (kNorm ? v * inv : v) : 0.f;
     }
     wave_lds_ready();  // read before the next row's pieces are written
   }
@@ -191,7 +198,6 @@ __device__ CVS_INLINE u32x4 ready(u32x4 x, const HeadLane<kLanes>& l, const floa
     for (int k = 0; k < 4; ++k) {
       const int e = 4 * i + k;
       o[e] = __builtin_fmaf(f[e], a[k], g[e] * b[k]);
-      if constexpr (kNorm) o[e] *= inv;
     }
   }
   return pack8<kBf>(o);
