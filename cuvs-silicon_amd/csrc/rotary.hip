@@ -89,6 +89,20 @@ void launch(cvs_context* ctx, const RotateArgs& a, Pairs pairs, bool norm, dim3 
   else launch<kBf, 4>(ctx, a, pairs, norm, grid);
 }
 
+// The part of a turn that a position adds, in units of 2^-64 modulo whole turns, rounded: the radians' 53 bits times 1 / 2 pi
+// in 128, of which the whole turns of 1024 radians take 8.
+uint64_t turns_of(double radians) {
+  constexpr uint64_t hi = 0x28be60db9391054aull, lo = 0x7f09d5f47d4d3770ull;  // 2^128 / 2 pi
+  int exponent;
+  const uint64_t m = uint64_t(std::ldexp(std::frexp(std::abs(radians), &exponent), 53));
+  const int shift = 53 - exponent;  // radians = m 2^-shift; 42 and more, as they are at most 1024
+  if (shift > 120) return 0;
+  typedef unsigned __int128 u128;
+  const u128 product = u128(m) * hi + (u128(m) * lo >> 64);  // m / 2 pi in units of 2^-64: 118 bits at most
+  const uint64_t turns = uint64_t((product + (u128(1) << (shift - 1))) >> shift);
+  return radians < 0 ? -turns : turns;
+}
+
 // Checks and launches; q or k may be null.
 void rotate(cvs_context* ctx, const cvs_rotary* rotary, const int64_t* positions, const cvs_heads* const (&in)[2],
             const cvs_heads* const (&out)[2], const cvs_head_norm* const (&norm)[2], const char* const (&names)[2]) {
@@ -245,11 +259,7 @@ int cvs_rotary_create(cvs_context* ctx, int dims, int layout, const double* radi
     for (int i = 0; i < dims / 2; ++i) {
       if (!(std::abs(radians[i]) <= 1024.0))
         fail(CVS_ERR_UNSUPPORTED, "frequencies must be from -1024 to 1024 radians a position");
-      // 64 bits of the part behind the point; a long double has them for all that is less than a turn.
-      constexpr long double two_pi = 6.283185307179586476925286766559L;
-      const long double t = static_cast<long double>(radians[i]) / two_pi;
-      const long double part = (t - std::floor(t)) * 18446744073709551616.0L;
-      turns.push_back(part >= 18446744073709551615.0L ? 0 : uint64_t(std::llroundl(part / 2) * 2));
+      turns.push_back(turns_of(radians[i]));
     }
     need_no_capture(ctx, "a rotary cannot be made");
     auto r = std::make_unique<cvs_rotary>();

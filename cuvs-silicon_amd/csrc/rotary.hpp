@@ -8,7 +8,7 @@
 // all in fp32, rounded once.  A frequency is held as the turns that a position
 // adds, in units of 2^-64 modulo whole turns, and the angle is the integer
 // product of both modulo 2^64: what is left of a turn is off by at most
-// |p| 2^-63 turns however many whole ones there are, where p f in fp32 would be
+// |p| 2^-64 turns however many whole ones there are, where p f in fp32 would be
 // off by 0.004 radians at position 100,000.
 #pragma once
 
@@ -29,7 +29,8 @@ namespace attn {
 // cos and sin of `phase` / 2^64 turns: the nearest quarter turn is taken off,
 // and the rest, at most pi / 4, goes through polynomials fitted to sin(t) / t
 // and cos(t) over that range (weighted least squares, errors of 1.8e-9 and
-// 1e-10 before rounding; a float holds the rest to 2^-25 of it).
+// 1e-10 before rounding; a float holds the rest to 2^-25 of it).  The rest's
+// lower 32 bits are left out, 2^-32 turns or 1.5e-9 radians at most.
 __device__ CVS_INLINE float2 cos_sin(uint64_t phase) {
   const uint64_t quarter = (phase + (uint64_t(1) << 61)) >> 62;
   const int32_t rest = int32_t(uint32_t((phase - (quarter << 62)) >> 32));

@@ -679,12 +679,12 @@ int cvs_kv_attention_scored_async(cvs_kv_cache* cache, cvs_kv_plan* plan, int la
  *   y_b = m (n_b cos t + n_a sin t)          `dims` channels; y = n elsewhere
  *
  * with t = position * frequency of the pair and m the magnitude.  Everything
- * is in fp32 and rounded once; t is exact modulo whole turns (2^-63 turns a
- * position), so far positions are as precise as near ones.  Positions are 64
- * bit, may be negative (the inverse rotation) and may repeat.  Squares whose
- * sum passes the range of fp32 make their head's norm infinite, and the head 0;
- * those below its range count as 0, so that heads of such channels alone need
- * an eps that is not 0. */
+ * is in fp32 and rounded once; t is exact modulo whole turns (2^-64 turns a
+ * position and 2^-32 in all), so far positions are as precise as near ones.
+ * Positions are 64 bit, may be negative (the inverse rotation) and may repeat.
+ * Squares whose sum passes the range of fp32 make their head's norm infinite,
+ * and the head 0; those below its range count as 0, so that heads of such
+ * channels alone need an eps that is not 0. */
 
 #define CVS_ROTARY_HALVES 0     /* pair i: channels i and i + dims / 2 */
 #define CVS_ROTARY_NEIGHBOURS 1 /* pair i: channels 2 i and 2 i + 1 */
