@@ -26,8 +26,9 @@
 // 96 run four and three workgroups.
 //
 // Bounds: long prompts with heads of 128 the matrix cores (busy 61% of the
-// cycles, the vector unit 52%: 12,000 causal tokens, 32/8 heads, bf16, in
-// 1.03 ms = 1.14 PFLOP/s, 0.80 of the vendor's plain product).  Prompts with
+// cycles, the vector unit 52%: 12,000 causal tokens, 32/8 heads, bf16, in 1.03
+// to 1.05 ms from box to box = 1.13 PFLOP/s, 0.80 of the vendor's plain product).
+// Prompts with
 // smaller heads no one unit: 64 passages of 40 to 512 tokens, 12 heads of 64,
 // take 45 us with the vector unit busy 51% of the cycles (193 instructions a
 // 64-key step, 32 exponentials among them), the matrix cores 27%, the waves 27%
@@ -150,7 +151,8 @@ struct PromptSource {
 };
 
 // Capped and biased scores leave a SIMD a wave less where heads are small: with the registers of plain ones they spill in
-// the loop (64 passages of heads of 64, biased: 114 us, 51 so).
+// the loop (64 passages of heads of 64, biased: 114 us, 51 so).  A few are spilled all the same: 2 for heads of 64 with
+// both, 5 (biased) and 7 (both) for heads of 128; two to four of them come back in a step.
 template <bool kBf, int NB, int KS, typename Scoring>
 __global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 3 ? (Scoring::kPlain ? 3 : 2) : (Scoring::kPlain ? 4 : 3)) void prompt_attn_kernel(const PromptArgs a) {
   typedef PromptSource<NB> Source;
