@@ -143,9 +143,9 @@ __device__ CVS_INLINE float largest(const f32x16& s, float c) {
 //   weighted to an even relative error: 6e-7), with the powers of scale / C in
 //   its coefficients (of lower degree, up to a smaller |u|, where those would
 //   leave the range of fp32: score_args); above, C (1 - 2 / (1 + e^2u)), off by
-//   its last places, 2^-22 C, which is as much beside the score.  A tile with no |u| above 1/2, all of
-//   them in models whose scores stay within half of the cap, takes five
-//   instructions a score more than a plain one and no exponential;
+//   its last places, 2^-22 C, which is as much beside the score.  A tile with no
+//   |u| above 1/2, all of them in models whose scores stay within half of the cap,
+//   takes five instructions a score more than a plain one and no exponential;
 //
 //   bias: minus log2(e) slope |place - key|, by the row's place and slope: linear
 //   in the key where all of a tile's keys lie on one side of all rows, one

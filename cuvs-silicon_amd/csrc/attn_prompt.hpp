@@ -27,14 +27,13 @@
 //
 // Bounds: long prompts with heads of 128 the matrix cores (busy 61% of the
 // cycles, the vector unit 52%: 12,000 causal tokens, 32/8 heads, bf16, in 1.03
-// to 1.05 ms from box to box = 1.13 PFLOP/s, 0.80 of the vendor's plain product).
-// Prompts with
-// smaller heads no one unit: 64 passages of 40 to 512 tokens, 12 heads of 64,
-// take 45 us with the vector unit busy 51% of the cycles (193 instructions a
-// 64-key step, 32 exponentials among them), the matrix cores 27%, the waves 27%
-// of their time waiting, and 146 MB fetched for 88 MB of inputs: row blocks
-// that share keys run on different XCDs, each with an L2 of its own.  Short
-// prompts each workgroup's first loads.
+// to 1.05 ms from card to card = 1.13 PFLOP/s, 0.80 of the vendor's plain
+// product).  Prompts with smaller heads no one unit: 64 passages of 40 to 512
+// tokens, 12 heads of 64, take 45 us with the vector unit busy 51% of the cycles
+// (193 instructions a 64-key step, 32 exponentials among them), the matrix cores
+// 27%, the waves 27% of their time waiting, and 146 MB fetched for 88 MB of
+// inputs: row blocks that share keys run on different XCDs, each with an L2 of
+// its own.  Short prompts each workgroup's first loads.
 #pragma once
 
 #include "attn_common.hpp"
